@@ -59,6 +59,11 @@ extern "C" {
 #define OVFQ_TYPE_Q5_0 6
 #define OVFQ_TYPE_Q5_K 13
 
+/* Plain element types (ggml's ids), for what is kept unquantized: low-rank adapters. */
+#define OVFQ_TYPE_F32 0
+#define OVFQ_TYPE_F16 1
+#define OVFQ_TYPE_BF16 30
+
 /* Block geometry. */
 #define OVFQ_QK 256          /* elements per K-quant super-block (RT/Q4KWeight.cs:26) */
 #define OVFQ_Q4K_BYTES 144   /* RT/Q4KWeight.cs:29 */
@@ -68,6 +73,7 @@ extern "C" {
 
 typedef struct ovfq_ctx ovfq_ctx;
 typedef struct ovfq_weight ovfq_weight;
+typedef struct ovfq_adapters ovfq_adapters;
 
 /* ------------------------------------------------------------------------------------------------ context */
 
@@ -260,6 +266,107 @@ OVFQ_API int ovfq_project_multi_dev(ovfq_ctx* ctx, int count, const ovfq_weight*
 OVFQ_API int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights,
                                                  const int8_t* quants, const float* scales, const int16_t* bsums,
                                                  int rows, const float* const* biases, float* const* ys);
+
+/* ------------------------------------------------------------------------------------ low-rank adapters */
+
+/* Adapters of one projection weight, for requests that share the quantized weight and each bring their own low-rank
+ * update (the reference trains and applies such adapters one at a time, Sources/Main/LanguageModels/LoRA/): `slots`
+ * places, each empty or holding A [rank][input_size], B [output_size][rank] and a scale, with rank <= max_rank, kept
+ * in `type` (OVFQ_TYPE_F32, _F16 or _BF16; the tensors of a GGUF adapter file, lora_a and lora_b, lie in memory like this).
+ * All memory is allocated here: slots * max_rank * (input_size + output_size) values, max_rank rounded up to a
+ * multiple of 8. A set belongs to its context like a weight. input_size % 32 == 0. */
+#define OVFQ_MAX_ADAPTER_SLOTS 4096
+#define OVFQ_MAX_ADAPTER_RANK 256
+OVFQ_API int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_size, int slots, int max_rank,
+                                  ovfq_adapters** out);
+OVFQ_API int ovfq_adapters_destroy(ovfq_adapters* set);
+/* Puts an adapter into `slot` (replacing what is there): a [rank][input_size] and b [output_size][rank] in the set's type,
+ * scale usually alpha / rank. In order with the context's other work: calls enqueued before see the old adapter, later
+ * ones, replays of graphs captured earlier among them, the new one. Returns when the copy is done; not for a stream
+ * that is being captured (OVFQ_ERR_STATE). */
+OVFQ_API int ovfq_adapters_load(ovfq_adapters* set, int slot, const void* a, const void* b, int rank, float scale);
+/* As ovfq_adapters_load, from device memory. */
+OVFQ_API int ovfq_adapters_load_dev(ovfq_adapters* set, int slot, const void* a, const void* b, int rank, float scale);
+/* Empties `slot`: rows that name it get no adapter. */
+OVFQ_API int ovfq_adapters_unload(ovfq_adapters* set, int slot);
+/* Any out pointer may be NULL. byte_count: device bytes of the set. */
+OVFQ_API int ovfq_adapters_info(const ovfq_adapters* set, int* type, int* input_size, int* output_size, int* slots,
+                                int* max_rank, size_t* byte_count);
+
+/* ovfq_project_multi with each row's adapter added: for weight i and row m with s = row_slots[m],
+ *   ys[i][m] = (biases[i] +) W_i q(x[m]) + scale_s B_s (A_s x[m])
+ * where (A_s, B_s, scale_s) is slot s of sets[i]; x is not quantised in the second term, and its products and sums are fp32. A
+ * row whose slot is negative, past the set or empty gets the projection alone (bit-identical to ovfq_project_multi), and
+ * so does every row of a weight whose sets[i] is NULL. row_slots [rows] is read on the device at each call, so one captured
+ * graph serves any assignment. Sets of one call share a type; each has its weight's sizes. At most 4 weights. Host
+ * pointers, synchronous. */
+OVFQ_API int ovfq_project_adapters(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights,
+                                   const ovfq_adapters* const* sets, const float* x, int rows, const int* row_slots,
+                                   const float* const* biases, float* const* ys);
+/* As ovfq_project_adapters, with device pointers (enqueued on the context's stream). */
+OVFQ_API int ovfq_project_adapters_dev(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights,
+                                       const ovfq_adapters* const* sets, const float* x, int rows,
+                                       const int* row_slots, const float* const* biases, float* const* ys);
+
+/* ------------------------------------------------------------------------- norms around the residual sum */
+
+#define OVFQ_NORM_RMS 0   /* v / sqrt(mean(v^2) + eps) * weight (+ bias)                              */
+#define OVFQ_NORM_LAYER 1 /* (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias        */
+typedef struct ovfq_norm {
+    int kind;
+    float eps;           /* finite, not negative */
+    const float* weight; /* [k]; NULL: ones */
+    const float* bias;   /* [k]; NULL: none */
+} ovfq_norm;
+
+#define OVFQ_GATE_NONE 0
+#define OVFQ_GATE_CHANNEL 1 /* gate [k]: one factor for each channel            */
+#define OVFQ_GATE_ROW 2     /* gate [rows]: one factor for each row             */
+#define OVFQ_GATE_FULL 3    /* gate [rows][k]                                   */
+
+/* The step between two blocks, over `rows` rows of k values in one launch (the reference runs its steps one by one on the
+ * host, RT/CachedTransformerBlock.cs:205):
+ *   t = post(y)            the norm after the block that gave y (NULL: t = y)
+ *   h_out = residual + scale * gate * t   (residual NULL: without it; gate by gate_mode)
+ *   x_out = pre(h_out)     the norm before the next block (NULL: no x_out)
+ * h_out may be NULL when only x_out is wanted (residual, post and gate NULL: a plain norm). Per-head norms are rows of head_dim.
+ * h_out may be the residual plane or the y plane itself, x_out the y plane or, with h_out NULL, the residual plane; planes
+ * must not overlap otherwise. Sums are fp32. Host pointers, synchronous. */
+OVFQ_API int ovfq_residual_norm(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k,
+                                const ovfq_norm* post, const float* gate, int gate_mode, float scale,
+                                const ovfq_norm* pre, float* h_out, float* x_out);
+/* As ovfq_residual_norm; y, residual, gate, the norms' weights and biases and the outputs are device pointers, the ovfq_norm
+ * structures themselves lie in host memory and are read during the call. */
+OVFQ_API int ovfq_residual_norm_dev(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k,
+                                    const ovfq_norm* post, const float* gate, int gate_mode, float scale,
+                                    const ovfq_norm* pre, float* h_out, float* x_out);
+
+/* ---------------------------------------------------------------------- verification of drafted tokens */
+
+/* Speculative decoding's check of drafted tokens, from the LM head's logits and given random numbers. `requests` requests
+ * share logits [rows][vocab]: request r's rows are row_offsets[r] .. row_offsets[r + 1] - 1, the target's answers after its
+ * last token and after each of its n_r = (its rows) - 1 drafted tokens, so there are drafts = rows - requests of those, draft
+ * i of request r at index row_offsets[r] - r + i of draft_tokens, accept_uniforms and draft_probs [drafts][vocab] (the
+ * distributions that they were drawn from; NULL: drafted with certainty). With p = softmax(logits / temperature[r]) in
+ * fp64 (temperature NULL: 1; not in (0, inf): all of p on the first of the largest logits):
+ *   draft x is accepted while accept_uniform * q(x) < p(x);
+ *   the first one refused is replaced by a draw from max(p - q, 0) (from p, where that is all zero), or, with none refused,
+ *   one more token is drawn from the last row's p: the lowest token whose running sum passes final_uniforms[r] times the total.
+ * accepted[r] is the number of drafts kept; tokens [rows] holds, from row_offsets[r] on, those and the drawn token, then -1.
+ * Logits of -inf or NaN have no probability; a row without a finite largest logit refuses its draft, and draws -1. A draft
+ * outside the vocabulary is refused. Negative or NaN draft probabilities count as 0. */
+OVFQ_API int ovfq_verify_drafts(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests,
+                                const int* row_offsets, const int* draft_tokens, const float* draft_probs,
+                                const float* temperature, const float* accept_uniforms, const float* final_uniforms,
+                                int* accepted, int* tokens);
+/* As ovfq_verify_drafts, with device pointers (enqueued on the context's stream). The host form refuses offsets that do not
+ * start at 0, grow by at least 1 and end at rows; here a request whose offsets do not grow or leave the rows gets
+ * accepted -1 and leaves `tokens` as it was, and rows of no request are left as they were. Offsets of different requests
+ * must not overlap. */
+OVFQ_API int ovfq_verify_drafts_dev(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests,
+                                    const int* row_offsets, const int* draft_tokens, const float* draft_probs,
+                                    const float* temperature, const float* accept_uniforms,
+                                    const float* final_uniforms, int* accepted, int* tokens);
 
 /* ---------------------------------------------------------------------------- per-head attention output */
 

@@ -24,11 +24,27 @@ TYPE_Q4_K = 12
 TYPE_Q6_K = 14
 TYPE_Q5_0 = 6
 TYPE_Q5_K = 13
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 30
+MAX_ADAPTER_SLOTS = 4096
+MAX_ADAPTER_RANK = 256
 
 vp = ctypes.c_void_p
 ci = ctypes.c_int
 sz = ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
+
+cf = ctypes.c_float
+
+
+class NormStruct(ctypes.Structure):
+    """ovfq_norm."""
+
+    _fields_ = [("kind", ci), ("eps", cf), ("weight", vp), ("bias", vp)]
+
+
+NP = ctypes.POINTER(NormStruct)
 
 # name -> (restype, argtypes). Every symbol include/ovfq.h declares.
 SIGNATURES = {
@@ -80,6 +96,18 @@ SIGNATURES = {
     "ovfq_project_heads_q8_0": (ci, [vp, ci, PP, vp, ci, vp, vp]),
     "ovfq_project_heads_q8_0_dev": (ci, [vp, ci, PP, vp, ci, vp, vp]),
     "ovfq_project_multi_prequantized_dev": (ci, [vp, ci, PP, vp, vp, vp, ci, PP, PP]),
+    "ovfq_adapters_create": (ci, [vp, ci, ci, ci, ci, ci, PP]),
+    "ovfq_adapters_destroy": (ci, [vp]),
+    "ovfq_adapters_load": (ci, [vp, ci, vp, vp, ci, cf]),
+    "ovfq_adapters_load_dev": (ci, [vp, ci, vp, vp, ci, cf]),
+    "ovfq_adapters_unload": (ci, [vp, ci]),
+    "ovfq_adapters_info": (ci, [vp] + [ctypes.POINTER(ci)] * 5 + [ctypes.POINTER(sz)]),
+    "ovfq_project_adapters": (ci, [vp, ci, PP, PP, vp, ci, vp, PP, PP]),
+    "ovfq_project_adapters_dev": (ci, [vp, ci, PP, PP, vp, ci, vp, PP, PP]),
+    "ovfq_residual_norm": (ci, [vp, vp, vp, ci, ci, NP, vp, ci, cf, NP, vp, vp]),
+    "ovfq_residual_norm_dev": (ci, [vp, vp, vp, ci, ci, NP, vp, ci, cf, NP, vp, vp]),
+    "ovfq_verify_drafts": (ci, [vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "ovfq_verify_drafts_dev": (ci, [vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp]),
     "ovfq_quantize_weight_q4k_dev": (ci, [vp, vp, ci, ci, vp]),
     "ovfq_quantize_weight_q6k_dev": (ci, [vp, vp, ci, ci, vp]),
     "ovfq_quantize_weight_q8_0_dev": (ci, [vp, vp, ci, ci, vp, vp]),

@@ -5,6 +5,7 @@
 // buffers for the synchronous entry points, and dispatch to the kernels in quant.hip / project.hip.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -59,6 +60,8 @@ struct ovfq_ctx {
     DevBuf act_q, act_s, act_b, x_stage, y_stage, y2_stage, bias_stage;
     // Routed-MoE scratch (plan, gate/up/intermediate/expert outputs, host staging), carved from one buffer.
     DevBuf moe;
+    // Adapter products, verification sums, and the host staging of those calls and of the norms, carved from one buffer.
+    DevBuf step;
     // Page-locked host arenas of the host-pointer entry points (hipHostMalloc): inputs go up, outputs come down.
     DevBuf h_up, h_down;
     // Scratch buffers replaced by larger ones. A HIP graph captured from _dev calls keeps the addresses it
@@ -67,6 +70,7 @@ struct ovfq_ctx {
     size_t retired_bytes = 0;
     // Live weights created on this context (ovfq_ctx_destroy refuses while any remain).
     int live_weights = 0;
+    int live_adapters = 0;  // the same for adapter sets
 };
 
 // One device allocation holding every expert sliced from a 3-D GGUF expert tensor; the last expert weight
@@ -86,6 +90,24 @@ struct ovfq_weight {
     size_t nbytes = 0;       // resident bytes (blocks + scales)
     void* mfma = nullptr;    // MFMA-ready copy (ovfq_weight_prepare_mfma), or NULL
     SharedPlane* shared = nullptr; // set for expert slices: blocks/scales point into shared->p
+};
+
+// The adapters of one weight (ovfq_adapters_create): fixed slots in one allocation. A [slots][max_rank][in], then B
+// [slots][out * rank_pad(max_rank)], then the slots' ranks and scales.
+struct ovfq_adapters {
+    ovfq_ctx* ctx = nullptr;
+    int type = 0;
+    int in = 0;
+    int out = 0;
+    int slots = 0;
+    int max_rank = 0;
+    char* a = nullptr;
+    char* b = nullptr;
+    ovfq::AdapterSlot* info = nullptr;
+    size_t nbytes = 0;
+    size_t elem() const { return type == OVFQ_TYPE_F32 ? 4 : 2; }
+    size_t a_slot() const { return (size_t)max_rank * in * elem(); }
+    size_t b_slot() const { return (size_t)out * ovfq::rank_pad(max_rank) * elem(); }
 };
 
 namespace {
@@ -584,10 +606,12 @@ int ovfq_ctx_destroy(ovfq_ctx* c) {
         // A weight locks its context when destroyed, so the context must outlive every weight made on it.
         if (c->live_weights > 0)
             return fail(OVFQ_ERR_STATE, "context still owns %d weight(s): destroy them first", c->live_weights);
+        if (c->live_adapters > 0)
+            return fail(OVFQ_ERR_STATE, "context still owns %d adapter set(s): destroy them first", c->live_adapters);
         (void)hipSetDevice(c->device);
         (void)hipStreamSynchronize(c->stream);
         DevBuf* bufs[] = {&c->act_q,   &c->act_s,   &c->act_b,      &c->x_stage,
-                          &c->y_stage, &c->y2_stage, &c->bias_stage, &c->moe};
+                          &c->y_stage, &c->y2_stage, &c->bias_stage, &c->moe, &c->step};
         for (DevBuf* b : bufs)
             if (b->p) (void)hipFree(b->p);
         for (void* p : c->retired) (void)hipFree(p);
@@ -638,7 +662,7 @@ int ovfq_ctx_scratch_bytes(ovfq_ctx* c, size_t* live, size_t* retired) {
     if (!c) return fail(OVFQ_ERR_NULL, "ctx is NULL");
     std::lock_guard<std::mutex> lk(c->mu);
     const DevBuf* bufs[] = {&c->act_q, &c->act_s, &c->act_b, &c->x_stage, &c->y_stage, &c->y2_stage, &c->bias_stage,
-                            &c->moe};
+                            &c->moe,   &c->step};
     size_t n = 0;
     for (const DevBuf* b : bufs) n += b->cap;
     if (live) *live = n;
@@ -995,9 +1019,39 @@ int ovfq_quantize_q8_0_dev(ovfq_ctx* ctx, const float* x, int rows, int k, int8_
 
 // ---------------------------------------------------------------------------------------- projections
 
-// Shared body of the fused (same activation) projections: count weights, one quantisation, one launch.
+// The adapters of a projection call: a set or NULL for each weight, and each row's slot.
+struct AdapterCall {
+    const ovfq_adapters* const* sets;
+    const int* row_slots;
+};
+
+// The rows' adapters added to a projection's outputs yd.
+static int apply_adapters(ovfq_ctx* ctx, int count, const ovfq_adapters* const* sets, const int* row_slots, const float* x,
+                          int rows, int in, float* low, float* const* yd) {
+    ovfq::AdapterArgs a{};
+    int jobs = 0, type = 0;
+    for (int i = 0; i < count; i++) {
+        const ovfq_adapters* s = sets[i];
+        if (!s) continue;
+        type = s->type;
+        a.job[jobs++] = ovfq::AdapterJob{s->a,     s->b,        s->info,
+                                         low,      yd[i],       s->slots,
+                                         s->max_rank, ovfq::rank_pad(s->max_rank), s->out};
+        low += (size_t)rows * s->max_rank;
+    }
+    if (!jobs) return OVFQ_OK;
+    a.x = x;
+    a.row_slots = row_slots;
+    a.rows = rows;
+    a.in = in;
+    HIP_TRY(ovfq::launch_adapters(a, type, jobs, ctx->stream));
+    return OVFQ_OK;
+}
+
+// Shared body of the fused (same activation) projections: count weights, one quantisation, one launch, and the rows' adapters
+// where the call has them.
 static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, const float* x, int rows,
-                        const float* const* biases, float* const* ys, bool host) {
+                        const float* const* biases, float* const* ys, bool host, const AdapterCall* ad = nullptr) {
     if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
     if (count < 1 || count > ovfq::kMaxJobs) return fail(OVFQ_ERR_RANGE, "count (%d) must be in [1, 4]", count);
     if (!ws || !ys) return fail(OVFQ_ERR_NULL, "weights / outputs array is NULL");
@@ -1015,8 +1069,38 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     if (!host && (rc = check_dev_align(x, "input"))) return rc;
     const int in = ws[0]->in;
     if ((rc = check_plane(rows, in, "activation"))) return rc;
+    size_t low = 0;  // low-rank products of the rows
+    if (ad) {
+        if (!ad->sets) return fail(OVFQ_ERR_NULL, "adapter set array is NULL");
+        if (!ad->row_slots) return fail(OVFQ_ERR_NULL, "row_slots is NULL");
+        if (!host && (rc = check_dev_align(ad->row_slots, "row_slots"))) return rc;
+        const ovfq_adapters* first = nullptr;
+        for (int i = 0; i < count; i++) {
+            const ovfq_adapters* s = ad->sets[i];
+            if (!s) continue;
+            if (s->ctx != ctx) return fail(OVFQ_ERR_SIZE, "adapter set %d belongs to another context", i);
+            if (s->in != in || s->out != ws[i]->out)
+                return fail(OVFQ_ERR_SIZE, "adapter set %d is for %d x %d, its weight %d x %d", i, s->out, s->in, ws[i]->out, in);
+            if (first && s->type != first->type) return fail(OVFQ_ERR_TYPE, "the adapter sets of a call must share a type");
+            if (!first) first = s;
+            low += (size_t)rows * s->max_rank;
+        }
+    }
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
+    float* low_d = nullptr;
+    int* slots_d = ad ? const_cast<int*>(ad->row_slots) : nullptr;
+    if (ad) {
+        auto carve = [&](Carver& c) {
+            low_d = c.take<float>(low * 4);
+            if (host) slots_d = c.take<int>((size_t)rows * 4);
+        };
+        Carver sizing{nullptr};
+        carve(sizing);
+        if ((rc = ensure(ctx, ctx->step, sizing.used))) return rc;
+        Carver c{static_cast<char*>(ctx->step.p)};
+        carve(c);
+    }
     const float* xd = x;
     const float* bd[ovfq::kMaxJobs] = {nullptr, nullptr, nullptr, nullptr};
     float* yd[ovfq::kMaxJobs];
@@ -1033,6 +1117,7 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
         if ((rc = ensure(ctx, ctx->y_stage, ytotal * 4))) return rc;
         if (btotal && (rc = ensure(ctx, ctx->bias_stage, btotal * 4))) return rc;
         if ((rc = io.up(ctx->x_stage.p, x, (size_t)rows * in * 4))) return rc;
+        if (ad && (rc = io.up(slots_d, ad->row_slots, (size_t)rows * 4))) return rc;
         xd = (const float*)ctx->x_stage.p;
         size_t boff = 0;
         for (int i = 0; i < count; i++) {
@@ -1062,6 +1147,7 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
         if ((rc = quantize_into_scratch(ctx, ws[0]->type, xd, rows, in, &act, tiled))) return rc;
         if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, act))) return rc;
     }
+    if (ad && (rc = apply_adapters(ctx, count, ad->sets, slots_d, xd, rows, in, low_d, yd))) return rc;
     if (host) {
         for (int i = 0; i < count; i++)
             if ((rc = io.down(ys[i], yd[i], (size_t)rows * ws[i]->out * 4))) return rc;
@@ -1245,6 +1331,340 @@ int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const ovfq_wei
     HIP_TRY(hipSetDevice(ctx->device));
     if ((rc = launch_projection(ctx, ws, count, biases, ys, rows, ovfq::ActQ{q, s, b}))) return rc;
     return ok();
+}
+
+// ---------------------------------------------------------------------------------------- low-rank adapters
+
+int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_size, int slots, int max_rank,
+                         ovfq_adapters** out) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    if (!out) return fail(OVFQ_ERR_NULL, "out is NULL");
+    if (type != OVFQ_TYPE_F32 && type != OVFQ_TYPE_F16 && type != OVFQ_TYPE_BF16)
+        return fail(OVFQ_ERR_TYPE, "unsupported adapter type %d", type);
+    if (input_size <= 0) return fail(OVFQ_ERR_RANGE, "inputSize (%d) must be positive", input_size);
+    if (output_size <= 0) return fail(OVFQ_ERR_RANGE, "outputSize (%d) must be positive", output_size);
+    if (input_size % 32) return fail(OVFQ_ERR_SIZE, "inputSize (%d) must be a multiple of 32", input_size);
+    if (slots <= 0 || slots > OVFQ_MAX_ADAPTER_SLOTS)
+        return fail(OVFQ_ERR_RANGE, "slots (%d) must be in [1, %d]", slots, OVFQ_MAX_ADAPTER_SLOTS);
+    if (max_rank <= 0 || max_rank > OVFQ_MAX_ADAPTER_RANK)
+        return fail(OVFQ_ERR_RANGE, "max_rank (%d) must be in [1, %d]", max_rank, OVFQ_MAX_ADAPTER_RANK);
+    // a slot's planes are addressed with 32-bit byte offsets
+    if ((int64_t)max_rank * input_size * 4 >= (int64_t)1 << 31 ||
+        (int64_t)ovfq::rank_pad(max_rank) * output_size * 4 >= (int64_t)1 << 31)
+        return fail(OVFQ_ERR_SIZE, "an adapter of rank %d for %d x %d is too large", max_rank, output_size, input_size);
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    ovfq_adapters* s = new ovfq_adapters();
+    s->ctx = ctx;
+    s->type = type;
+    s->in = input_size;
+    s->out = output_size;
+    s->slots = slots;
+    s->max_rank = max_rank;
+    auto carve = [&](Carver& c) {
+        s->a = c.take<char>((size_t)slots * s->a_slot());
+        s->b = c.take<char>((size_t)slots * s->b_slot());
+        s->info = c.take<ovfq::AdapterSlot>((size_t)slots * sizeof(ovfq::AdapterSlot));
+    };
+    Carver sizing{nullptr};
+    carve(sizing);
+    s->nbytes = sizing.used;
+    void* p = nullptr;
+    hipError_t e = hipMalloc(&p, s->nbytes);
+    if (e == hipSuccess) {
+        Carver c{static_cast<char*>(p)};
+        carve(c);
+        for (int i = 0; i < slots && e == hipSuccess; i++) e = ovfq::launch_adapter_slot(s->info, i, 0, 0.0f, ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    }
+    if (e != hipSuccess) {
+        if (p) (void)hipFree(p);
+        const size_t n = s->nbytes;
+        delete s;
+        return fail(OVFQ_ERR_HIP, "adapter set of %zu B: %s", n, hipGetErrorString(e));
+    }
+    ctx->live_adapters++;
+    *out = s;
+    return ok();
+}
+
+int ovfq_adapters_destroy(ovfq_adapters* s) {
+    if (!s) return fail(OVFQ_ERR_NULL, "adapter set is NULL");
+    {
+        std::lock_guard<std::mutex> lk(s->ctx->mu);
+        (void)hipSetDevice(s->ctx->device);
+        (void)hipStreamSynchronize(s->ctx->stream);
+        (void)hipFree(s->a);  // the allocation's first piece
+        s->ctx->live_adapters--;
+    }
+    delete s;
+    return ok();
+}
+
+// No work of an adapter's load goes into a captured graph: it copies from the caller's memory and waits.
+static int check_not_capturing(ovfq_ctx* ctx, const char* what) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(OVFQ_ERR_STATE, "%s while the context's stream is captured", what);
+    return OVFQ_OK;
+}
+
+static int adapters_load_impl(ovfq_adapters* s, int slot, const void* a, const void* b, int rank, float scale, bool host) {
+    if (!s) return fail(OVFQ_ERR_NULL, "adapter set is NULL");
+    if (!a || !b) return fail(OVFQ_ERR_NULL, "a / b is NULL");
+    if (slot < 0 || slot >= s->slots) return fail(OVFQ_ERR_RANGE, "slot %d out of range [0, %d)", slot, s->slots);
+    if (rank <= 0 || rank > s->max_rank) return fail(OVFQ_ERR_RANGE, "rank (%d) must be in [1, %d]", rank, s->max_rank);
+    if (!host && (!aligned(a, s->elem()) || !aligned(b, s->elem())))
+        return fail(OVFQ_ERR_SIZE, "a and b must be aligned to their elements");
+    ovfq_ctx* ctx = s->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    int rc = check_not_capturing(ctx, "an adapter cannot be loaded");
+    if (rc) return rc;
+    const size_t b_bytes = (size_t)s->out * rank * s->elem();
+    const void* b_dev = b;
+    void* staged = nullptr;
+    hipError_t e = hipSuccess;
+    if (host) {
+        e = hipMalloc(&staged, b_bytes);
+        if (e == hipSuccess) e = hipMemcpyAsync(staged, b, b_bytes, hipMemcpyHostToDevice, ctx->stream);
+        b_dev = staged;
+    }
+    if (e == hipSuccess)
+        e = hipMemcpyAsync(s->a + (size_t)slot * s->a_slot(), a, (size_t)rank * s->in * s->elem(),
+                           host ? hipMemcpyHostToDevice : hipMemcpyDeviceToDevice, ctx->stream);
+    if (e == hipSuccess)
+        e = ovfq::launch_adapter_pad(b_dev, s->b + (size_t)slot * s->b_slot(), s->out, rank, (int)s->elem(), ctx->stream);
+    if (e == hipSuccess) e = ovfq::launch_adapter_slot(s->info, slot, rank, scale, ctx->stream);
+    const hipError_t done = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = done;
+    if (staged) (void)hipFree(staged);
+    if (e != hipSuccess) return fail(OVFQ_ERR_HIP, "adapter upload failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ovfq_adapters_load(ovfq_adapters* set, int slot, const void* a, const void* b, int rank, float scale) {
+    return adapters_load_impl(set, slot, a, b, rank, scale, true);
+}
+
+int ovfq_adapters_load_dev(ovfq_adapters* set, int slot, const void* a, const void* b, int rank, float scale) {
+    return adapters_load_impl(set, slot, a, b, rank, scale, false);
+}
+
+int ovfq_adapters_unload(ovfq_adapters* s, int slot) {
+    if (!s) return fail(OVFQ_ERR_NULL, "adapter set is NULL");
+    if (slot < 0 || slot >= s->slots) return fail(OVFQ_ERR_RANGE, "slot %d out of range [0, %d)", slot, s->slots);
+    std::lock_guard<std::mutex> lk(s->ctx->mu);
+    HIP_TRY(hipSetDevice(s->ctx->device));
+    int rc = check_not_capturing(s->ctx, "an adapter cannot be unloaded");
+    if (rc) return rc;
+    HIP_TRY(ovfq::launch_adapter_slot(s->info, slot, 0, 0.0f, s->ctx->stream));
+    return ok();
+}
+
+int ovfq_adapters_info(const ovfq_adapters* s, int* type, int* input_size, int* output_size, int* slots, int* max_rank,
+                       size_t* byte_count) {
+    if (!s) return fail(OVFQ_ERR_NULL, "adapter set is NULL");
+    if (type) *type = s->type;
+    if (input_size) *input_size = s->in;
+    if (output_size) *output_size = s->out;
+    if (slots) *slots = s->slots;
+    if (max_rank) *max_rank = s->max_rank;
+    if (byte_count) *byte_count = s->nbytes;
+    return ok();
+}
+
+int ovfq_project_adapters(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights, const ovfq_adapters* const* sets,
+                          const float* x, int rows, const int* row_slots, const float* const* biases, float* const* ys) {
+    const AdapterCall ad{sets, row_slots};
+    return project_impl(ctx, count, weights, x, rows, biases, ys, true, &ad);
+}
+
+int ovfq_project_adapters_dev(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights,
+                              const ovfq_adapters* const* sets, const float* x, int rows, const int* row_slots,
+                              const float* const* biases, float* const* ys) {
+    const AdapterCall ad{sets, row_slots};
+    return project_impl(ctx, count, weights, x, rows, biases, ys, false, &ad);
+}
+
+// ---------------------------------------------------------------------------------------- norms
+
+static int check_norm(const ovfq_norm* n, const char* which, bool host) {
+    if (!n) return OVFQ_OK;
+    if (n->kind != OVFQ_NORM_RMS && n->kind != OVFQ_NORM_LAYER)
+        return fail(OVFQ_ERR_RANGE, "%s norm: kind %d is neither OVFQ_NORM_RMS nor OVFQ_NORM_LAYER", which, n->kind);
+    if (!(n->eps >= 0.0f) || std::isinf(n->eps)) return fail(OVFQ_ERR_RANGE, "%s norm: eps must be finite and not negative", which);
+    if (!host && (rc_align(n->weight) || rc_align(n->bias)))
+        return fail(OVFQ_ERR_SIZE, "%s norm: device pointers must be 4-byte aligned", which);
+    return OVFQ_OK;
+}
+
+static int norm_impl(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k, const ovfq_norm* post,
+                     const float* gate, int gate_mode, float scale, const ovfq_norm* pre, float* h_out, float* x_out,
+                     bool host) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    if (!y) return fail(OVFQ_ERR_NULL, "y is NULL");
+    if (rows <= 0) return fail(OVFQ_ERR_RANGE, "rows (%d) must be positive", rows);
+    if (k <= 0) return fail(OVFQ_ERR_RANGE, "k (%d) must be positive", k);
+    int rc;
+    if ((rc = check_plane(rows, k, "activation"))) return rc;
+    if ((rc = check_norm(post, "post", host)) || (rc = check_norm(pre, "pre", host))) return rc;
+    if (gate_mode < OVFQ_GATE_NONE || gate_mode > OVFQ_GATE_FULL) return fail(OVFQ_ERR_RANGE, "unknown gate_mode %d", gate_mode);
+    if ((gate != nullptr) != (gate_mode != OVFQ_GATE_NONE))
+        return fail(OVFQ_ERR_NULL, gate ? "a gate without a gate_mode" : "gate is NULL");
+    if ((pre != nullptr) != (x_out != nullptr))
+        return fail(OVFQ_ERR_NULL, pre ? "x_out is NULL" : "x_out without a pre norm");
+    if (!pre && !h_out) return fail(OVFQ_ERR_NULL, "h_out is NULL and there is no pre norm");
+    if (h_out && h_out == x_out) return fail(OVFQ_ERR_SIZE, "h_out and x_out are the same plane");
+    if (h_out && x_out && x_out == residual) return fail(OVFQ_ERR_SIZE, "x_out is the residual plane beside an h_out");
+    if (!host && (rc_align(y) || rc_align(residual) || rc_align(gate) || rc_align(h_out) || rc_align(x_out)))
+        return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    ovfq::NormArgs a{};
+    a.rows = rows;
+    a.k = k;
+    a.gate_mode = gate_mode;
+    a.scale = scale;
+    a.has_post = post != nullptr;
+    a.has_pre = pre != nullptr;
+    const ovfq_norm none{};
+    const ovfq_norm &po = post ? *post : none, &pr = pre ? *pre : none;
+    const float* in[7] = {y, residual, gate, po.weight, po.bias, pr.weight, pr.bias};
+    const size_t plane = (size_t)rows * k * 4, row = (size_t)k * 4;
+    HostIO io(ctx);
+    float *hd = h_out, *xd = x_out;
+    if (host) {
+        const size_t bytes[7] = {plane, plane,
+                                 gate_mode == OVFQ_GATE_FULL ? plane : gate_mode == OVFQ_GATE_ROW ? (size_t)rows * 4 : row,
+                                 row,   row,
+                                 row,   row};
+        float* dev[7];
+        auto carve = [&](Carver& c) {
+            for (int i = 0; i < 7; i++) dev[i] = in[i] ? c.take<float>(bytes[i]) : nullptr;
+            if (h_out) hd = c.take<float>(plane);
+            if (x_out) xd = c.take<float>(plane);
+        };
+        Carver sizing{nullptr};
+        carve(sizing);
+        if ((rc = ensure(ctx, ctx->step, sizing.used))) return rc;
+        Carver c{static_cast<char*>(ctx->step.p)};
+        carve(c);
+        for (int i = 0; i < 7; i++) {
+            if (in[i] && (rc = io.up(dev[i], in[i], bytes[i]))) return rc;
+            in[i] = dev[i];
+        }
+    }
+    a.y = in[0];
+    a.h = in[1];
+    a.gate = in[2];
+    a.post = ovfq::NormSide{in[3], in[4], po.eps, po.kind == OVFQ_NORM_LAYER};
+    a.pre = ovfq::NormSide{in[5], in[6], pr.eps, pr.kind == OVFQ_NORM_LAYER};
+    a.h_out = hd;
+    a.x_out = xd;
+    HIP_TRY(ovfq::launch_residual_norm(a, ctx->stream));
+    if (host && ((h_out && (rc = io.down(h_out, hd, plane))) || (x_out && (rc = io.down(x_out, xd, plane))) ||
+                 (rc = io.finish())))
+        return rc;
+    return ok();
+}
+
+int ovfq_residual_norm(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k, const ovfq_norm* post,
+                       const float* gate, int gate_mode, float scale, const ovfq_norm* pre, float* h_out, float* x_out) {
+    return norm_impl(ctx, y, residual, rows, k, post, gate, gate_mode, scale, pre, h_out, x_out, true);
+}
+
+int ovfq_residual_norm_dev(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k, const ovfq_norm* post,
+                           const float* gate, int gate_mode, float scale, const ovfq_norm* pre, float* h_out,
+                           float* x_out) {
+    return norm_impl(ctx, y, residual, rows, k, post, gate, gate_mode, scale, pre, h_out, x_out, false);
+}
+
+// ---------------------------------------------------------------------------------------- drafted tokens
+
+static int verify_impl(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests, const int* row_offsets,
+                       const int* draft_tokens, const float* draft_probs, const float* temperature,
+                       const float* accept_uniforms, const float* final_uniforms, int* accepted, int* tokens, bool host) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    if (!logits || !row_offsets || !final_uniforms) return fail(OVFQ_ERR_NULL, "logits / row_offsets / final_uniforms is NULL");
+    if (!accepted || !tokens) return fail(OVFQ_ERR_NULL, "accepted / tokens is NULL");
+    int rc;
+    if ((rc = check_rows(rows))) return rc;
+    if (vocab <= 0) return fail(OVFQ_ERR_RANGE, "vocab (%d) must be positive", vocab);
+    if (requests <= 0) return fail(OVFQ_ERR_RANGE, "requests (%d) must be positive", requests);
+    if (requests > rows) return fail(OVFQ_ERR_SIZE, "%d requests need as many rows at least, got %d", requests, rows);
+    const int drafts = rows - requests;
+    if (drafts && (!draft_tokens || !accept_uniforms)) return fail(OVFQ_ERR_NULL, "draft_tokens / accept_uniforms is NULL");
+    if ((rc = check_plane(rows, vocab, "logits"))) return rc;
+    if (host) {
+        bool good = row_offsets[0] == 0 && row_offsets[requests] == rows;
+        for (int r = 0; r < requests; r++) good = good && row_offsets[r] < row_offsets[r + 1];
+        if (!good) return fail(OVFQ_ERR_SIZE, "row_offsets must start at 0, grow by at least 1 and end at rows (%d)", rows);
+    } else if (rc_align(logits) || rc_align(row_offsets) || rc_align(draft_tokens) || rc_align(draft_probs) ||
+               rc_align(temperature) || rc_align(accept_uniforms) || rc_align(final_uniforms) || rc_align(accepted) ||
+               rc_align(tokens)) {
+        return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    }
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    ovfq::VerifyArgs a{};
+    a.rows = rows;
+    a.vocab = vocab;
+    a.requests = requests;
+    a.drafts = drafts;
+    a.pieces = (vocab + ovfq::kVerifyPiece - 1) / ovfq::kVerifyPiece;
+    const size_t R = (size_t)rows, Q = (size_t)requests, D = (size_t)drafts, V = (size_t)vocab;
+    const void* in[7] = {logits, row_offsets, draft_tokens, draft_probs, temperature, accept_uniforms, final_uniforms};
+    const size_t bytes[7] = {R * V * 4, (Q + 1) * 4, D * 4, D * V * 4, Q * 4, D * 4, Q * 4};
+    void* dev[7];
+    int *acc = accepted, *tok = tokens;
+    auto carve = [&](Carver& c) {
+        a.stats = c.take<ovfq::VerifyStat>(R * a.pieces * sizeof(ovfq::VerifyStat));
+        a.parts = c.take<double>(Q * a.pieces * 2 * sizeof(double));
+        a.pick = c.take<ovfq::VerifyPick>(Q * sizeof(ovfq::VerifyPick));
+        if (!host) return;
+        for (int i = 0; i < 7; i++) dev[i] = in[i] ? c.take<char>(bytes[i]) : nullptr;
+        acc = c.take<int>(Q * 4);
+        tok = c.take<int>(R * 4);
+    };
+    Carver sizing{nullptr};
+    carve(sizing);
+    if ((rc = ensure(ctx, ctx->step, sizing.used))) return rc;
+    Carver c{static_cast<char*>(ctx->step.p)};
+    carve(c);
+    HostIO io(ctx);
+    if (host) {
+        for (int i = 0; i < 7; i++) {
+            if (in[i] && bytes[i] && (rc = io.up(dev[i], in[i], bytes[i]))) return rc;
+            in[i] = dev[i];
+        }
+    }
+    a.logits = (const float*)in[0];
+    a.row_offsets = (const int*)in[1];
+    a.draft_tokens = (const int*)in[2];
+    a.draft_probs = (const float*)in[3];
+    a.temperature = (const float*)in[4];
+    a.accept_uniforms = (const float*)in[5];
+    a.final_uniforms = (const float*)in[6];
+    a.accepted = acc;
+    a.tokens = tok;
+    HIP_TRY(ovfq::launch_verify_drafts(a, ctx->stream));
+    if (host && ((rc = io.down(accepted, acc, Q * 4)) || (rc = io.down(tokens, tok, R * 4)) || (rc = io.finish()))) return rc;
+    return ok();
+}
+
+int ovfq_verify_drafts(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests, const int* row_offsets,
+                       const int* draft_tokens, const float* draft_probs, const float* temperature,
+                       const float* accept_uniforms, const float* final_uniforms, int* accepted, int* tokens) {
+    return verify_impl(ctx, logits, rows, vocab, requests, row_offsets, draft_tokens, draft_probs, temperature,
+                       accept_uniforms, final_uniforms, accepted, tokens, true);
+}
+
+int ovfq_verify_drafts_dev(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests, const int* row_offsets,
+                           const int* draft_tokens, const float* draft_probs, const float* temperature,
+                           const float* accept_uniforms, const float* final_uniforms, int* accepted, int* tokens) {
+    return verify_impl(ctx, logits, rows, vocab, requests, row_offsets, draft_tokens, draft_probs, temperature,
+                       accept_uniforms, final_uniforms, accepted, tokens, false);
 }
 
 // ---------------------------------------------------------------------------------------- per-head Q8_0 Wo

@@ -1,0 +1,245 @@
+// norm.hip — the step between two blocks of a transformer in one pass over the rows:
+//   t = post(y);  h' = h + scale * gate * t;  x = pre(h')
+// with RMS or layer norms: n(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias, the means over the row, no mean
+// subtracted and no bias in the RMS form. Sums, variances and the two planes are fp32; layer norms take the squares of the
+// deviations from the mean, so a large common offset loses nothing.
+//
+// Bound: HBM for many rows (each input element is read once and each output written once; a row stays in registers between its
+// two norms), launch and two dependent reductions for one. A group of kT threads owns a row: 16 to 64 lanes for rows of up to
+// 1024 elements (several rows a workgroup, sums by lane exchanges alone), a workgroup of up to 1024 threads for rows of up to
+// 16384, and past that a workgroup that reads the row once per step.
+#include "ovfq_device.h"
+#include "ovfq_launch.h"
+
+namespace ovfq {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+__device__ __forceinline__ f32x4 ldf4(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(f32x4, ld4(r, off));
+}
+
+// Sum over the kT threads that own a row; every one of them receives it. kT > 64: `red` holds a float per wave, in two halves
+// that successive sums of a row alternate between (one barrier a sum).
+template <int kT>
+__device__ __forceinline__ float group_sum(float v, float* red, int& turn) {
+#pragma unroll
+    for (int off = (kT < 64 ? kT : 64) / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    if constexpr (kT > 64) {
+        constexpr int kW = kT / 64;
+        float* half = red + kW * (turn & 1);
+        turn++;
+        if ((threadIdx.x & 63) == 0) half[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kW; i++) v += half[i];
+    }
+    return v;
+}
+
+// The norm of one row of k elements held as kNV four-element pieces a thread; elements past the row are zero and stay out of
+// the sums.
+template <int kT, int kNV>
+__device__ __forceinline__ void norm_row(f32x4 (&v)[kNV], const f32x4 (&w)[kNV], const f32x4 (&b)[kNV], const NormSide& n,
+                                         int k, int t, float* red, int& turn) {
+    const float inv_k = 1.0f / (float)k;
+    if (n.layer) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kNV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s += v[i][c];
+        const float mean = group_sum<kT>(s, red, turn) * inv_k;
+#pragma unroll
+        for (int i = 0; i < kNV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[i][c] = 4 * (t + i * kT) + c < k ? v[i][c] - mean : 0.0f;
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kNV; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) s = fmaf(v[i][c], v[i][c], s);
+    const float var = group_sum<kT>(s, red, turn) * inv_k;
+    const float r = 1.0f / sqrtf(var + n.eps);
+#pragma unroll
+    for (int i = 0; i < kNV; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            v[i][c] *= r;
+            if (n.weight) v[i][c] *= w[i][c];
+            if (n.bias) v[i][c] += b[i][c];
+        }
+}
+
+template <int kT, int kNV>
+__device__ __forceinline__ void load_side(const NormSide& n, int k, int t, f32x4 (&w)[kNV], f32x4 (&b)[kNV]) {
+    const __amdgpu_buffer_rsrc_t wr = make_rsrc(n.weight, n.weight ? (uint32_t)k * 4 : 0u);
+    const __amdgpu_buffer_rsrc_t br = make_rsrc(n.bias, n.bias ? (uint32_t)k * 4 : 0u);
+#pragma unroll
+    for (int i = 0; i < kNV; i++) w[i] = ldf4(wr, 16u * (uint32_t)(t + i * kT));
+    if (n.bias) {
+#pragma unroll
+        for (int i = 0; i < kNV; i++) b[i] = ldf4(br, 16u * (uint32_t)(t + i * kT));
+    }
+}
+
+template <int kT, int kNV>
+__device__ __forceinline__ void store_row(float* p, const f32x4 (&v)[kNV], int k, int t) {
+#pragma unroll
+    for (int i = 0; i < kNV; i++) {
+        const int e = 4 * (t + i * kT);
+        if (e + 4 <= k) {
+            __builtin_memcpy(p + e, &v[i], 16);  // a row starts on any 4-byte boundary
+        } else {
+#pragma unroll
+            for (int c = 0; c < 3; c++)
+                if (e + c < k) p[e + c] = v[i][c];
+        }
+    }
+}
+
+// Rows of up to 4 * kT * kNV elements. Everything that the row needs is loaded before its first sum.
+template <int kT, int kNV>
+__global__ __launch_bounds__(kT < 256 ? 256 : kT) void residual_norm_kernel(const NormArgs a) {
+    constexpr int kRows = kT < 256 ? 256 / kT : 1;  // rows a workgroup
+    __shared__ float red[kT > 64 ? 2 * (kT / 64) : 1];
+    const int t = kRows > 1 ? (int)threadIdx.x % kT : (int)threadIdx.x;
+    const int64_t row0 = (int64_t)blockIdx.x * kRows;
+    const int sub = kRows > 1 ? (int)threadIdx.x / kT : 0;
+    const int64_t row = row0 + sub;
+    const int k = a.k;
+    int turn = 0;
+    // one resource over the workgroup's rows: what is past a row's end is masked below, what is past the last row reads zeros
+    const int64_t left = a.rows - row0 < kRows ? a.rows - row0 : kRows;
+    const uint32_t bytes = (uint32_t)left * (uint32_t)k * 4;
+    const uint32_t base = (uint32_t)sub * (uint32_t)k * 4;
+    f32x4 v[kNV], h[kNV], g[kNV], pw[kNV], pb[kNV], qw[kNV], qb[kNV];
+    auto load_plane = [&](const float* p, f32x4(&d)[kNV]) {
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(p + row0 * k, bytes);
+#pragma unroll
+        for (int i = 0; i < kNV; i++) d[i] = ldf4(r, base + 16u * (uint32_t)(t + i * kT));
+    };
+    load_plane(a.y, v);
+    if (a.h) load_plane(a.h, h);
+    if (a.has_post) load_side<kT, kNV>(a.post, k, t, pw, pb);
+    float g_row = a.scale;
+    if (a.gate_mode == kGateFull) {
+        load_plane(a.gate, g);
+    } else if (a.gate_mode == kGateChannel) {
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.gate, (uint32_t)k * 4);
+#pragma unroll
+        for (int i = 0; i < kNV; i++) g[i] = ldf4(r, 16u * (uint32_t)(t + i * kT));
+    } else if (a.gate_mode == kGateRow) {
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.gate + row0, (uint32_t)left * 4);
+        g_row *= as_float(ld1(r, (uint32_t)sub * 4));
+    }
+    if (a.has_pre) load_side<kT, kNV>(a.pre, k, t, qw, qb);
+#pragma unroll
+    for (int i = 0; i < kNV; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (4 * (t + i * kT) + c >= k) v[i][c] = 0.0f;
+    if (a.has_post) norm_row<kT, kNV>(v, pw, pb, a.post, k, t, red, turn);
+    if (a.gate_mode == kGateFull || a.gate_mode == kGateChannel) {
+#pragma unroll
+        for (int i = 0; i < kNV; i++) v[i] *= g[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kNV; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float s = v[i][c] * g_row;
+            v[i][c] = 4 * (t + i * kT) + c < k ? (a.h ? h[i][c] + s : s) : 0.0f;
+        }
+    const bool live = row < a.rows;
+    if (a.h_out && live) store_row<kT, kNV>(a.h_out + row * k, v, k, t);
+    if (!a.has_pre) return;
+    norm_row<kT, kNV>(v, qw, qb, a.pre, k, t, red, turn);
+    if (live) store_row<kT, kNV>(a.x_out + row * k, v, k, t);
+}
+
+// Rows past 16384 elements: a workgroup of 1024 reads its row once per sum and once more for x (from the caches, where a row of
+// that length still lies). h_out may be the h plane and x_out the y plane: each element is read by the thread that writes it,
+// and the last step reads h' back from h_out where there is one.
+__global__ __launch_bounds__(1024) void residual_norm_long_kernel(const NormArgs a) {
+    __shared__ float red[32];
+    const int64_t row = blockIdx.x;
+    const int k = a.k, t = threadIdx.x;
+    const float* y = a.y + row * k;
+    const float* h = a.h ? a.h + row * k : nullptr;
+    float* ho = a.h_out ? a.h_out + row * k : nullptr;
+    const float inv_k = 1.0f / (float)k;
+    int turn = 0;
+    auto stats = [&](const NormSide& n, auto&& at, float& mean, float& r) {
+        mean = 0.0f;
+        if (n.layer) {
+            float s = 0.0f;
+            for (int e = t; e < k; e += 1024) s += at(e);
+            mean = group_sum<1024>(s, red, turn) * inv_k;
+        }
+        float s = 0.0f;
+        for (int e = t; e < k; e += 1024) {
+            const float d = at(e) - mean;
+            s = fmaf(d, d, s);
+        }
+        r = 1.0f / sqrtf(group_sum<1024>(s, red, turn) * inv_k + n.eps);
+    };
+    auto apply = [](const NormSide& n, float v, int e, float mean, float r) {
+        v = (v - mean) * r;
+        if (n.weight) v *= n.weight[e];
+        return n.bias ? v + n.bias[e] : v;
+    };
+    float pm = 0.0f, pr = 1.0f;
+    if (a.has_post) stats(a.post, [&](int e) { return y[e]; }, pm, pr);
+    const float g_row = a.gate_mode == kGateRow ? a.scale * a.gate[row] : a.scale;
+    auto sum_at = [&](int e) {
+        float v = a.has_post ? apply(a.post, y[e], e, pm, pr) : y[e];
+        if (a.gate_mode == kGateFull) v *= a.gate[row * k + e];
+        if (a.gate_mode == kGateChannel) v *= a.gate[e];
+        v *= g_row;
+        return h ? h[e] + v : v;
+    };
+    if (ho)
+        for (int e = t; e < k; e += 1024) ho[e] = sum_at(e);
+    if (!a.has_pre) return;
+    float* x = a.x_out + row * k;
+    float xm, xr;
+    if (ho) {  // an element is read back by the thread that wrote it
+        stats(a.pre, [&](int e) { return ho[e]; }, xm, xr);
+        for (int e = t; e < k; e += 1024) x[e] = apply(a.pre, ho[e], e, xm, xr);
+    } else {
+        stats(a.pre, sum_at, xm, xr);
+        for (int e = t; e < k; e += 1024) x[e] = apply(a.pre, sum_at(e), e, xm, xr);
+    }
+}
+
+template <int kT, int kNV>
+hipError_t launch(const NormArgs& a, hipStream_t st) {
+    constexpr int kRows = kT < 256 ? 256 / kT : 1;
+    hipLaunchKernelGGL((residual_norm_kernel<kT, kNV>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
+                       dim3(kT < 256 ? 256 : kT), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_residual_norm(const NormArgs& a, hipStream_t st) {
+    const int k = a.k;
+    if (k <= 64) return launch<16, 1>(a, st);
+    if (k <= 128) return launch<32, 1>(a, st);
+    if (k <= 256) return launch<64, 1>(a, st);
+    if (k <= 512) return launch<64, 2>(a, st);
+    if (k <= 1024) return launch<64, 4>(a, st);
+    if (k <= 2048) return launch<256, 2>(a, st);
+    if (k <= 4096) return launch<256, 4>(a, st);
+    if (k <= 8192) return launch<512, 4>(a, st);
+    if (k <= 16384) return launch<1024, 4>(a, st);
+    hipLaunchKernelGGL(residual_norm_long_kernel, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace ovfq

@@ -224,6 +224,87 @@ hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int 
 hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int planes, bool heads, int plane_in, int n_out,
                            int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st);
 
+// Low-rank adapters beside a projection (adapters.hip). A set keeps its adapters in fixed slots of one type: A [slots][max_rank]
+// [in] and, slot by slot, B rows of rank_pad(rank) values (b_stride = rank_pad(max_rank) of them a row at most).
+enum AdapterType { kAdapterF32 = 0, kAdapterF16 = 1, kAdapterBF16 = 30 };
+struct AdapterSlot {
+    int rank;  // 0: nothing loaded
+    float scale;
+};
+struct AdapterJob {
+    const void* a;
+    const void* b;
+    const AdapterSlot* info;  // [slots]
+    float* low;               // scratch [rows][max_rank]
+    float* y;                 // [rows][out], added to
+    int slots, max_rank, b_stride, out;
+};
+struct AdapterArgs {
+    AdapterJob job[kMaxJobs];
+    const float* x;  // [rows][in]
+    const int* row_slots;
+    int rows, in;
+};
+__host__ __device__ constexpr int rank_pad(int rank) { return (rank + 7) & ~7; }
+// Adds every row's adapter to the outputs of `jobs` projections of x (sets of one type).
+hipError_t launch_adapters(const AdapterArgs& a, int type, int jobs, hipStream_t st);
+hipError_t launch_adapter_slot(AdapterSlot* info, int slot, int rank, float scale, hipStream_t st);
+// B [out][rank] (elem bytes a value) into a slot's padded rows.
+hipError_t launch_adapter_pad(const void* src, void* dst, int out, int rank, int elem, hipStream_t st);
+
+// Norms around a residual sum (norm.hip): h_out = h + scale * gate * post(y), x_out = pre(h_out).
+enum GateMode { kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3 };
+struct NormSide {
+    const float* weight;  // [k], or NULL: ones
+    const float* bias;    // [k], or NULL
+    float eps;
+    int layer;  // layer norm, else RMS
+};
+struct NormArgs {
+    const float* y;
+    const float* h;     // may be NULL
+    const float* gate;  // [k], [rows] or [rows][k] by gate_mode
+    float* h_out;       // may be NULL
+    float* x_out;       // set with has_pre
+    int64_t rows;
+    int k;
+    int gate_mode;
+    float scale;
+    int has_post, has_pre;
+    NormSide post, pre;
+};
+hipError_t launch_residual_norm(const NormArgs& a, hipStream_t st);
+
+// Verification of drafted tokens (verify.hip); the scratch planes stats [rows][pieces], parts [requests][pieces][2] and pick
+// [requests] are written by the launch.
+constexpr int kVerifyPiece = 8192;  // tokens a workgroup
+struct VerifyStat {
+    float max;   // largest logit
+    int at;      // its first token (greedy requests)
+    double sum;  // sum of exp((logit - max) / temperature)
+};
+struct VerifyPick {
+    int row;    // the row to draw from, -1: no such request
+    int draft;  // the refused draft, -1: none
+    VerifyStat stat;
+};
+struct VerifyArgs {
+    const float* logits;         // [rows][vocab]
+    const int* row_offsets;      // [requests + 1]
+    const int* draft_tokens;     // [drafts]
+    const float* draft_probs;    // [drafts][vocab] or NULL
+    const float* temperature;    // [requests] or NULL
+    const float* accept_uniforms;  // [drafts]
+    const float* final_uniforms;   // [requests]
+    int* accepted;               // [requests]
+    int* tokens;                 // [rows]
+    VerifyStat* stats;
+    double* parts;
+    VerifyPick* pick;
+    int rows, vocab, requests, drafts, pieces;
+};
+hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st);
+
 // GGUF Q8_0 (34-byte blocks) -> int8 quant plane + f32 scale plane.
 hipError_t launch_q8_0_deinterleave(const void* gguf, int64_t n_blocks, int8_t* q, float* s, hipStream_t st);
 // GGUF Q5_0 (22-byte blocks of 32) or Q5_K (176-byte super-blocks) -> resident Q8_0 planes: decoded and requantised

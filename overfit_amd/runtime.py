@@ -156,6 +156,31 @@ class Context:
         held until the callable is dropped."""
         return BoundMulti(self, weights, x, ys, biases, rows)
 
+    def bind_adapters_dev(self, weights, adapters, x, row_slots, ys, biases=None, rows=1):
+        """`step.project_adapters` on device tensors with its arguments converted once (see bind_multi_dev)."""
+        from .step import _adapters_call
+
+        return _device_call(_adapters_call(weights, adapters, x, row_slots, rows, biases, ys)[0])
+
+    def bind_residual_norm_dev(self, y, rows, residual=None, post=None, gate=None, gate_axis=None, scale=1.0, pre=None,
+                               h_out=None, x_out=None):
+        """`step.residual_norm` on device tensors with its arguments converted once; h_out or x_out is given."""
+        from .step import _norm_call
+
+        if h_out is None and x_out is None:
+            raise ValueError("a prepared call needs its outputs")
+        return _device_call(_norm_call(y, rows, residual, post, gate, gate_axis, scale, pre, h_out, x_out, self, False)[0])
+
+    def bind_verify_drafts_dev(self, logits, vocab, row_offsets, draft_tokens, accept_uniforms, final_uniforms,
+                               draft_probs=None, temperature=None, accepted=None, tokens=None):
+        """`step.verify_drafts` on device tensors with its arguments converted once; accepted and tokens are given."""
+        from .step import _verify_call
+
+        if accepted is None or tokens is None:
+            raise ValueError("a prepared call needs its outputs")
+        return _device_call(_verify_call(logits, vocab, row_offsets, draft_tokens, accept_uniforms, final_uniforms,
+                                         draft_probs, temperature, accepted, tokens, self)[0])
+
     def project_multi_prequantized_dev(self, weights, q, s, b, ys, biases=None, rows=1):
         n = len(weights)
         W = (ctypes.c_void_p * n)(*[w.handle.value for w in weights])
@@ -195,6 +220,26 @@ class BoundMulti:
         rc = self._fn(*self._args)
         if rc:
             self._ctx.check(rc)
+
+
+class BoundCall:
+    """A prepared call of a library function: its converted arguments, and what they point into."""
+
+    __slots__ = ("_ctx", "_fn", "_args", "_keep")
+
+    def __init__(self, ctx, fn, args, keep):
+        self._ctx, self._fn, self._args, self._keep = ctx, fn, args, keep
+
+    def __call__(self):
+        rc = self._fn(*self._args)
+        if rc:
+            self._ctx.check(rc)
+
+
+def _device_call(call):
+    if not call._fn.__name__.endswith("_dev"):
+        raise OverfitArgumentError("a prepared _dev call takes device tensors")
+    return call
 
 
 _default = {}
