@@ -274,9 +274,11 @@ OVFQ_API int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const
  * places, each empty or holding A [rank][input_size], B [output_size][rank] and a scale, with rank <= max_rank, kept
  * in `type` (OVFQ_TYPE_F32, _F16 or _BF16; the tensors of a GGUF adapter file, lora_a and lora_b, lie in memory like this).
  * All memory is allocated here: slots * max_rank * (input_size + output_size) values, max_rank rounded up to a
- * multiple of 8. A set belongs to its context like a weight. input_size % 32 == 0. */
+ * multiple of 4. A set belongs to its context like a weight. input_size % 32 == 0, at most OVFQ_MAX_ADAPTER_INPUT, and
+ * max_rank times either size below 2^28. */
 #define OVFQ_MAX_ADAPTER_SLOTS 4096
 #define OVFQ_MAX_ADAPTER_RANK 256
+#define OVFQ_MAX_ADAPTER_INPUT (1 << 20)
 OVFQ_API int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_size, int slots, int max_rank,
                                   ovfq_adapters** out);
 OVFQ_API int ovfq_adapters_destroy(ovfq_adapters* set);

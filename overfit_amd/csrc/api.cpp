@@ -1025,29 +1025,6 @@ struct AdapterCall {
     const int* row_slots;
 };
 
-// The rows' adapters added to a projection's outputs yd.
-static int apply_adapters(ovfq_ctx* ctx, int count, const ovfq_adapters* const* sets, const int* row_slots, const float* x,
-                          int rows, int in, float* low, float* const* yd) {
-    ovfq::AdapterArgs a{};
-    int jobs = 0, type = 0;
-    for (int i = 0; i < count; i++) {
-        const ovfq_adapters* s = sets[i];
-        if (!s) continue;
-        type = s->type;
-        a.job[jobs++] = ovfq::AdapterJob{s->a,     s->b,        s->info,
-                                         low,      yd[i],       s->slots,
-                                         s->max_rank, ovfq::rank_pad(s->max_rank), s->out};
-        low += (size_t)rows * s->max_rank;
-    }
-    if (!jobs) return OVFQ_OK;
-    a.x = x;
-    a.row_slots = row_slots;
-    a.rows = rows;
-    a.in = in;
-    HIP_TRY(ovfq::launch_adapters(a, type, jobs, ctx->stream));
-    return OVFQ_OK;
-}
-
 // Shared body of the fused (same activation) projections: count weights, one quantisation, one launch, and the rows' adapters
 // where the call has them.
 static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, const float* x, int rows,
@@ -1069,30 +1046,37 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     if (!host && (rc = check_dev_align(x, "input"))) return rc;
     const int in = ws[0]->in;
     if ((rc = check_plane(rows, in, "activation"))) return rc;
-    size_t low = 0;  // low-rank products of the rows
+    ovfq::AdapterArgs aa{};
+    int ad_jobs = 0, ad_job_of[ovfq::kMaxJobs], ad_type = 0;
     if (ad) {
         if (!ad->sets) return fail(OVFQ_ERR_NULL, "adapter set array is NULL");
         if (!ad->row_slots) return fail(OVFQ_ERR_NULL, "row_slots is NULL");
         if (!host && (rc = check_dev_align(ad->row_slots, "row_slots"))) return rc;
-        const ovfq_adapters* first = nullptr;
+        int max_rank = 0;
         for (int i = 0; i < count; i++) {
             const ovfq_adapters* s = ad->sets[i];
             if (!s) continue;
             if (s->ctx != ctx) return fail(OVFQ_ERR_SIZE, "adapter set %d belongs to another context", i);
             if (s->in != in || s->out != ws[i]->out)
                 return fail(OVFQ_ERR_SIZE, "adapter set %d is for %d x %d, its weight %d x %d", i, s->out, s->in, ws[i]->out, in);
-            if (first && s->type != first->type) return fail(OVFQ_ERR_TYPE, "the adapter sets of a call must share a type");
-            if (!first) first = s;
-            low += (size_t)rows * s->max_rank;
+            if (ad_jobs && s->type != ad_type) return fail(OVFQ_ERR_TYPE, "the adapter sets of a call must share a type");
+            ad_type = s->type;
+            max_rank = s->max_rank > max_rank ? s->max_rank : max_rank;
+            ad_job_of[ad_jobs] = i;
+            aa.job[ad_jobs++] = ovfq::AdapterJob{s->a, s->b, s->info, nullptr, nullptr, s->slots, s->max_rank,
+                                                 ovfq::rank_pad(s->max_rank), s->out};
         }
+        aa.rows = rows;
+        aa.in = in;
+        if (ad_jobs) ovfq::plan_adapters(aa, ad_jobs, max_rank);
     }
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
-    float* low_d = nullptr;
     int* slots_d = ad ? const_cast<int*>(ad->row_slots) : nullptr;
     if (ad) {
-        auto carve = [&](Carver& c) {
-            low_d = c.take<float>(low * 4);
+        auto carve = [&](Carver& c) {  // the jobs' products, and the staged slots of a host call
+            for (int i = 0; i < ad_jobs; i++)
+                aa.job[i].low = c.take<float>((size_t)aa.shares * rows * aa.low_stride * 4);
             if (host) slots_d = c.take<int>((size_t)rows * 4);
         };
         Carver sizing{nullptr};
@@ -1147,7 +1131,12 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
         if ((rc = quantize_into_scratch(ctx, ws[0]->type, xd, rows, in, &act, tiled))) return rc;
         if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, act))) return rc;
     }
-    if (ad && (rc = apply_adapters(ctx, count, ad->sets, slots_d, xd, rows, in, low_d, yd))) return rc;
+    if (ad_jobs) {
+        aa.x = xd;
+        aa.row_slots = slots_d;
+        for (int i = 0; i < ad_jobs; i++) aa.job[i].y = yd[ad_job_of[i]];
+        HIP_TRY(ovfq::launch_adapters(aa, ad_type, ad_jobs, ctx->stream));
+    }
     if (host) {
         for (int i = 0; i < count; i++)
             if ((rc = io.down(ys[i], yd[i], (size_t)rows * ws[i]->out * 4))) return rc;
@@ -1348,9 +1337,11 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
         return fail(OVFQ_ERR_RANGE, "slots (%d) must be in [1, %d]", slots, OVFQ_MAX_ADAPTER_SLOTS);
     if (max_rank <= 0 || max_rank > OVFQ_MAX_ADAPTER_RANK)
         return fail(OVFQ_ERR_RANGE, "max_rank (%d) must be in [1, %d]", max_rank, OVFQ_MAX_ADAPTER_RANK);
-    // a slot's planes are addressed with 32-bit byte offsets
-    if ((int64_t)max_rank * input_size * 4 >= (int64_t)1 << 31 ||
-        (int64_t)ovfq::rank_pad(max_rank) * output_size * 4 >= (int64_t)1 << 31)
+    // the kernels address a slot's planes, and 16 rows of x, with 32-bit byte offsets that leave room for out-of-range ones
+    if (input_size > OVFQ_MAX_ADAPTER_INPUT)
+        return fail(OVFQ_ERR_SIZE, "inputSize (%d) above %d", input_size, OVFQ_MAX_ADAPTER_INPUT);
+    if ((int64_t)max_rank * input_size * 4 >= (int64_t)1 << 30 ||
+        (int64_t)ovfq::rank_pad(max_rank) * output_size * 4 >= (int64_t)1 << 30)
         return fail(OVFQ_ERR_SIZE, "an adapter of rank %d for %d x %d is too large", max_rank, output_size, input_size);
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
@@ -1374,7 +1365,7 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
     if (e == hipSuccess) {
         Carver c{static_cast<char*>(p)};
         carve(c);
-        for (int i = 0; i < slots && e == hipSuccess; i++) e = ovfq::launch_adapter_slot(s->info, i, 0, 0.0f, ctx->stream);
+        e = ovfq::launch_adapter_slots(s->info, 0, slots, 0, 0.0f, ctx->stream);
         if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     }
     if (e != hipSuccess) {
@@ -1435,7 +1426,7 @@ static int adapters_load_impl(ovfq_adapters* s, int slot, const void* a, const v
                            host ? hipMemcpyHostToDevice : hipMemcpyDeviceToDevice, ctx->stream);
     if (e == hipSuccess)
         e = ovfq::launch_adapter_pad(b_dev, s->b + (size_t)slot * s->b_slot(), s->out, rank, (int)s->elem(), ctx->stream);
-    if (e == hipSuccess) e = ovfq::launch_adapter_slot(s->info, slot, rank, scale, ctx->stream);
+    if (e == hipSuccess) e = ovfq::launch_adapter_slots(s->info, slot, 1, rank, scale, ctx->stream);
     const hipError_t done = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) e = done;
     if (staged) (void)hipFree(staged);
@@ -1458,7 +1449,7 @@ int ovfq_adapters_unload(ovfq_adapters* s, int slot) {
     HIP_TRY(hipSetDevice(s->ctx->device));
     int rc = check_not_capturing(s->ctx, "an adapter cannot be unloaded");
     if (rc) return rc;
-    HIP_TRY(ovfq::launch_adapter_slot(s->info, slot, 0, 0.0f, s->ctx->stream));
+    HIP_TRY(ovfq::launch_adapter_slots(s->info, slot, 1, 0, 0.0f, s->ctx->stream));
     return ok();
 }
 

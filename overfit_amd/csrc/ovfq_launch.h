@@ -235,7 +235,7 @@ struct AdapterJob {
     const void* a;
     const void* b;
     const AdapterSlot* info;  // [slots]
-    float* low;               // scratch [rows][max_rank]
+    float* low;               // scratch [shares][rows][low_stride]
     float* y;                 // [rows][out], added to
     int slots, max_rank, b_stride, out;
 };
@@ -244,11 +244,16 @@ struct AdapterArgs {
     const float* x;  // [rows][in]
     const int* row_slots;
     int rows, in;
+    // set by plan_adapters
+    int low_stride;  // ranks of a scratch row: the largest max_rank, in whole tiles of 16
+    int shares;      // workgroups that divide the inputs of a product
+    int slot_ways;   // workgroups that divide the distinct slots of a row tile
 };
-__host__ __device__ constexpr int rank_pad(int rank) { return (rank + 7) & ~7; }
+__host__ __device__ constexpr int rank_pad(int rank) { return (rank + 3) & ~3; }
+void plan_adapters(AdapterArgs& a, int jobs, int max_rank);
 // Adds every row's adapter to the outputs of `jobs` projections of x (sets of one type).
 hipError_t launch_adapters(const AdapterArgs& a, int type, int jobs, hipStream_t st);
-hipError_t launch_adapter_slot(AdapterSlot* info, int slot, int rank, float scale, hipStream_t st);
+hipError_t launch_adapter_slots(AdapterSlot* info, int first, int count, int rank, float scale, hipStream_t st);
 // B [out][rank] (elem bytes a value) into a slot's padded rows.
 hipError_t launch_adapter_pad(const void* src, void* dst, int out, int rank, int elem, hipStream_t st);
 
