@@ -1,14 +1,14 @@
 // adapters.hip — low-rank adapters of many requests beside a shared projection: for every activation row m with an adapter
 // slot s, y[m] += scale_s * B_s (A_s x[m]), A_s [rank][in], B_s [out][rank].
 //
-// Two launches: the rows' products A_s x[m] into scratch planes (shrink), then B_s times them into the outputs (expand). Both
-// are matrix products over 16-row tiles of the activation on fp32 MFMA (16x16x4), whatever the adapters are kept in: products
-// and sums are fp32 like the projection's tail, and at ranks of 8 to 64 the matrix pipe is not what bounds them. What a tile's
-// rows do not share is handled by slot: a tile's distinct slots are found with wave ballots (a prompt's tile has one or two, a
-// decode step's up to 16), each is multiplied with the whole tile, and its results go to its own rows only, by selection and
-// not by a zero factor, so that infinities in one request's adapter stay out of the others' rows.
+// Two steps: the rows' products A_s x[m] into scratch planes (shrink), in one launch with the quantisation of the activation
+// where the projection has one, then B_s times them (expand), in the epilogue of the projection kernels that take adapters and
+// in a launch of its own behind the others (adapter_tile.h). Products and sums are fp32 like the projection's tail, whatever the
+// adapters are kept in.
 #include <type_traits>
 
+#include "act_quant.h"
+#include "adapter_tile.h"
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
 
@@ -18,21 +18,29 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-// Four or eight consecutive adapter values at byte `off` of a resource, widened to fp32 (exact).
-template <int kType>
-__device__ __forceinline__ void load_values(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4& v) {
-    if constexpr (kType == kAdapterF32) {
-        v = __builtin_bit_cast(f32x4, ld4(r, off));
-    } else {
-        const u32x2 raw = ld2(r, off);
-        const uint32_t lo = raw.x, hi = raw.y;
-        if constexpr (kType == kAdapterF16)
-            v = f32x4{half_lo(lo), half_hi(lo), half_lo(hi), half_hi(hi)};
-        else
-            v = f32x4{as_float(lo << 16), as_float(lo & 0xffff0000u), as_float(hi << 16), as_float(hi & 0xffff0000u)};
-    }
+// fp32 operands of bf16 MFMA: a value is the sum of three bf16 parts (8 significant bits each, cut off, so every part and rest is
+// exact), and the products of parts are exact in fp32. Eight consecutive values of a lane, two to a dword.
+struct Parts {
+    u32x4 part[3];
+};
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ float cut(float v) { return as_float(__builtin_bit_cast(uint32_t, v) & 0xffff0000u); }
+template <int kParts>
+__device__ __forceinline__ void split_pair(float v0, float v1, int i, u32x4 (&part)[3]) {
+    part[0][i] = upper_halves(v0, v1);
+    const float r0 = v0 - cut(v0), r1 = v1 - cut(v1);
+    part[1][i] = upper_halves(r0, r1);
+    if constexpr (kParts == 3) part[2][i] = upper_halves(r0 - cut(r0), r1 - cut(r1));
 }
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// A lane's eight values of a piece of A, at byte `off` of the resource.
 template <int kType>
 struct Raw8 {
     u32x4 v[kType == kAdapterF32 ? 2 : 1];
@@ -41,195 +49,223 @@ template <int kType>
 __device__ __forceinline__ Raw8<kType> load_raw8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     Raw8<kType> x;
     x.v[0] = ld4(r, off);
-    if constexpr (kType == kAdapterF32) x.v[1] = ld4(r, off + 16);
+    if constexpr (kType == kAdapterF32) x.v[1] = ld4(r, off + 1024);
     return x;
 }
+
+// acc += x w over 32 inputs, the small products first. bf16 adapters are their own part (three MFMAs), fp16 ones (11 bits)
+// two parts (six, every product exact), fp32 ones three: of their nine products the three that are 2^-24 of the whole or less are
+// left out.
 template <int kType>
-__device__ __forceinline__ void widen8(const Raw8<kType>& x, float (&f)[8]) {
-    const uint32_t w[4] = {x.v[0].x, x.v[0].y, x.v[0].z, x.v[0].w};
-    if constexpr (kType == kAdapterF32) {
-        const uint32_t u[4] = {x.v[1].x, x.v[1].y, x.v[1].z, x.v[1].w};
+__device__ __forceinline__ f32x4 multiply(const Parts& x, const Raw8<kType>& w, f32x4 acc) {
+    if constexpr (kType == kAdapterBF16) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f[i] = as_float(w[i]);
-            f[4 + i] = as_float(u[i]);
-        }
+        for (int p = 2; p >= 0; p--) acc = mfma_bf16(x.part[p], w.v[0], acc);
     } else {
+        u32x4 part[3];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            f[2 * i] = kType == kAdapterF16 ? half_lo(w[i]) : as_float(w[i] << 16);
-            f[2 * i + 1] = kType == kAdapterF16 ? half_hi(w[i]) : as_float(w[i] & 0xffff0000u);
+            if constexpr (kType == kAdapterF16) {
+                const uint32_t u = w.v[0][i];
+                split_pair<2>(half_lo(u), half_hi(u), i, part);
+            } else {
+                const uint32_t u0 = w.v[i >> 1][2 * (i & 1)], u1 = w.v[i >> 1][2 * (i & 1) + 1];
+                split_pair<3>(as_float(u0), as_float(u1), i, part);
+            }
+        }
+        if constexpr (kType == kAdapterF16) {
+#pragma unroll
+            for (int p = 2; p >= 0; p--) acc = mfma_bf16(x.part[p], part[1], acc);
+#pragma unroll
+            for (int p = 2; p >= 0; p--) acc = mfma_bf16(x.part[p], part[0], acc);
+        } else {
+            acc = mfma_bf16(x.part[2], part[0], acc);
+            acc = mfma_bf16(x.part[0], part[2], acc);
+            acc = mfma_bf16(x.part[1], part[1], acc);
+            acc = mfma_bf16(x.part[1], part[0], acc);
+            acc = mfma_bf16(x.part[0], part[1], acc);
+            acc = mfma_bf16(x.part[0], part[0], acc);
         }
     }
+    return acc;
 }
 
-constexpr int kElem(int type) { return type == kAdapterF32 ? 4 : 2; }
-
-// The slots of a tile's 16 rows, row m0 + (lane & 15) in each of a wave's four 16-lane groups; -1 for a row without an adapter
-// (past the rows, no such slot, nothing loaded there).
-__device__ __forceinline__ int tile_slots(const AdapterJob& j, const int* row_slots, int m0, int rows) {
-    const int m = m0 + (int)(threadIdx.x & 15);
-    const int s = m < rows ? row_slots[m] : -1;
-    return s >= 0 && s < j.slots && j.info[s].rank > 0 ? s : -1;
-}
-
-// Calls f(slot, rows) for the tile's distinct slots number first, first + step, ...: wave-uniform, `rows` with a bit for each
-// of the tile's rows that have the slot.
-template <class F>
-__device__ __forceinline__ void for_slots(int slot, int first, int step, F f) {
-    uint32_t left = (uint32_t)__ballot(slot >= 0) & 0xffffu;
-    for (int u = 0; left; u++) {
-        const int s = __builtin_amdgcn_readlane(slot, __builtin_ctz(left));
-        const uint32_t mine = (uint32_t)__ballot(slot == s) & 0xffffu;
-        left &= ~mine;
-        if (u >= first && (u - first) % step == 0) f(s, mine);
+// A_s x for one 16-row tile, kNV rank tiles (16 ranks of one of the jobs each; two jobs share the loads of x) and a share of
+// the inputs: grid (way of the tile's distinct slots + ways * row tile, rank tile group + groups * share). Its waves divide the
+// share, 128 inputs a round, and add their sums in LDS; the shares of several workgroups stay apart in the scratch planes and are
+// added, in order, where they are used. Rows of the grid after these quantise the activation.
+//
+// Bound by latencies: the slots, then A and x, then the sums, behind a launch of 3 to 4.5 us. Three things were taken out of that
+// chain (18.7 us at 331 rows of q/k/v and rank 32, of which the products were less than one). Operands loaded where they lie, a
+// lane's 16 or 32 bytes of its own row, are 64 pieces an instruction: A is kept in operand order, and x goes through LDS, two
+// rows' 512 bytes an instruction in, a lane's own 32 bytes out. A slot's rank, another dependent load, is waited for before A
+// only past the first 16 ranks. And the workgroup's place comes from the grid and from the host, not from divisions.
+constexpr int kShrinkWaves = 4, kRound = 128, kXRow = kRound + 4;
+template <int kType, int kNV>
+__global__ __launch_bounds__(64 * kShrinkWaves, 3) void adapter_shrink_kernel(const AdapterArgs a, const ActQuantJob quant) {
+    const int shrink_rows = a.groups * a.shares;
+    if ((int)blockIdx.y >= shrink_rows) {
+        quantize_part(quant, (int64_t)((int)blockIdx.y - shrink_rows) * gridDim.x + blockIdx.x);
+        return;
     }
-}
-
-// A_s x for one 16-row tile, kNT tiles of 16 ranks and a share of the inputs: grid ((row tile, distinct slot), (job, rank group),
-// input share). The waves of a workgroup divide the share, 32 inputs a step (a lane of an operand holds eight consecutive ones,
-// which the eight MFMAs of a step take in turn, so every load is 16 bytes), and add their sums in LDS; the shares of several
-// workgroups stay apart in the scratch planes and the expanding kernel adds them, in order.
-constexpr int kShrinkWaves = 8;
-template <int kType, int kNT>
-__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(const AdapterArgs a) {
-    __shared__ f32x4 red[kShrinkWaves][kNT][64];
-    const int groups = (a.low_stride + 16 * kNT - 1) / (16 * kNT);
-    const AdapterJob j = a.job[blockIdx.y / groups];
-    const int r0 = (int)(blockIdx.y % groups) * 16 * kNT;
-    const int m0 = (int)(blockIdx.x / a.slot_ways) * 16;
+    if ((int)blockIdx.x >= a.shrink_x) return;
+    // x of the waves' rounds; their sums afterwards
+    __shared__ __align__(16) float lds[kShrinkWaves][16 * kXRow];
+    static_assert(kNV * 256 <= 16 * kXRow, "sums of a wave");
+    const int per_job = a.low_stride / 16;
+    int v0 = (int)blockIdx.y, share = 0;
+    while (v0 >= a.groups) {
+        v0 -= a.groups;
+        share++;
+    }
+    v0 *= kNV;
+    const int m0 = ((int)blockIdx.x >> a.way_shift) * 16, way = (int)blockIdx.x & ((1 << a.way_shift) - 1);
     const int wave = wave_id(), lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int chunks = a.in / 32;
-    const int each = (chunks + kShrinkWaves * a.shares - 1) / (kShrinkWaves * a.shares);
-    const int c0 = ((int)blockIdx.z * kShrinkWaves + wave) * each, c1 = min(c0 + each, chunks);
+    const int m = m0 + l16;
+    const int slot = m < a.rows ? a.row_slots[m] : -1;  // of row m0 + l16 in each 16-lane group
+    const int c0 = (share * kShrinkWaves + wave) * a.each, c1 = min(c0 + a.each, a.in / 32);
     const __amdgpu_buffer_rsrc_t xr =
         make_rsrc(a.x + (int64_t)m0 * a.in, (uint32_t)min(16, a.rows - m0) * (uint32_t)a.in * 4u);
-    const int slot = tile_slots(j, a.row_slots, m0, a.rows);
-    for_slots(slot, (int)blockIdx.x % a.slot_ways, a.slot_ways, [&](int s, uint32_t mine) {
-        const int rank = j.info[s].rank;
-        if (r0 >= rank) return;  // the same for every wave of the workgroup
-        const __amdgpu_buffer_rsrc_t ar = make_rsrc(static_cast<const char*>(j.a) + (int64_t)s * j.max_rank * a.in * kElem(kType),
-                                                    (uint32_t)rank * (uint32_t)a.in * kElem(kType));
-        // rows of other slots are not fetched (an offset past the resource reads zeros)
-        const uint32_t x0 = mine >> l16 & 1 ? (uint32_t)l16 * (uint32_t)a.in * 4u + (uint32_t)g * 32u : 0xf0000000u;
-        const uint32_t a0 = (uint32_t)(r0 + l16) * (uint32_t)a.in * kElem(kType) + (uint32_t)g * 8u * kElem(kType);
-        f32x4 acc[kNT];
+    struct Tile {
+        const char* a;
+        const AdapterSlot* info;
+        float* low;
+        AdapterRow* row;
+        int slots, max_rank, r0;
+    } tl[kNV];
+    bool first_ranks = false;
 #pragma unroll
-        for (int t = 0; t < kNT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr int kAhead = kNT == 4 ? 2 : 4;  // steps whose loads go out together
-        for (int c = c0; c < c1; c += kAhead) {
-            u32x4 xv[kAhead][2];
-            Raw8<kType> av[kAhead][kNT];
-#pragma unroll
-            for (int p = 0; p < kAhead; p++) {
-                // past the share: offsets past the resources, zeros (ovfq_adapters_create keeps a slot below 2^30 bytes)
-                const bool live = c + p < c1;
-                const uint32_t ka = live ? (uint32_t)(c + p) * 32u * kElem(kType) : 0x80000000u;
-                const uint32_t kx = live ? (uint32_t)(c + p) * 128u : 0x80000000u;
-#pragma unroll
-                for (int t = 0; t < kNT; t++)
-                    av[p][t] = load_raw8<kType>(ar, a0 + ka + (uint32_t)t * 16u * (uint32_t)a.in * kElem(kType));
-                xv[p][0] = ld4(xr, x0 + kx);
-                xv[p][1] = ld4(xr, x0 + kx + 16u);
-            }
-#pragma unroll
-            for (int p = 0; p < kAhead; p++) {
-                const float x[8] = {as_float(xv[p][0].x), as_float(xv[p][0].y), as_float(xv[p][0].z), as_float(xv[p][0].w),
-                                    as_float(xv[p][1].x), as_float(xv[p][1].y), as_float(xv[p][1].z), as_float(xv[p][1].w)};
-#pragma unroll
-                for (int t = 0; t < kNT; t++) {
-                    float w[8];
-                    widen8<kType>(av[p][t], w);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w[i], acc[t], 0, 0, 0);
-                }
-            }
+    for (int t = 0; t < kNV; t++) {
+        int job = 0, r = v0 + t;
+        while (r >= per_job) {
+            r -= per_job;
+            job++;
         }
-        __syncthreads();  // the last slot's sums have been read
-#pragma unroll
-        for (int t = 0; t < kNT; t++) red[wave][t][lane] = acc[t];
-        __syncthreads();
-        for (int t = wave; t < kNT; t += kShrinkWaves) {
-            f32x4 v = red[0][t][lane];
-#pragma unroll
-            for (int w = 1; w < kShrinkWaves; w++) v += red[w][t][lane];
-            // lane (g, l16) holds rows 4 g .. 4 g + 3 of rank r0 + 16 t + l16
-            const int r = r0 + 16 * t + l16;
-            float* low = j.low + ((int64_t)blockIdx.z * a.rows + m0 + 4 * g) * a.low_stride + r;
-            if (r < a.low_stride) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (mine >> (4 * g + i) & 1) low[(int64_t)i * a.low_stride] = v[i];
-            }
-        }
-    });
-}
-
-// The products of one slot for a 16-row tile and kT tiles of 16 outputs: acc[t] (lane (g, l16): rows 4 g .. 4 g + 3, output
-// n0 + 16 t + l16) = sum_r low[m][r] B[n][r], 16 ranks a step.
-template <int kType, int kT>
-__device__ __forceinline__ void expand_slot(const AdapterArgs& a, const AdapterJob& j, int s, int m0, int n0, f32x4 (&acc)[kT]) {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int pad = rank_pad(j.info[s].rank);
-    const __amdgpu_buffer_rsrc_t br =
-        make_rsrc(static_cast<const char*>(j.b) + (int64_t)s * j.out * j.b_stride * kElem(kType),
-                  (uint32_t)j.out * (uint32_t)pad * kElem(kType));
-    const int left = min(16, a.rows - m0);
-#pragma unroll
-    for (int t = 0; t < kT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int r = 0; r < pad; r += 16) {
-        const int at = r + 4 * g;  // this lane's four ranks
-        f32x4 b[kT], low = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < kT; t++) {
-            const uint32_t off = (uint32_t)(n0 + 16 * t + l16) * (uint32_t)pad * kElem(kType) + (uint32_t)at * kElem(kType);
-            load_values<kType>(br, at < pad && n0 + 16 * t + l16 < j.out ? off : 0xf0000000u, b[t]);
-        }
-        for (int sh = 0; sh < a.shares; sh++) {
-            const __amdgpu_buffer_rsrc_t lr = make_rsrc(j.low + ((int64_t)sh * a.rows + m0) * a.low_stride,
-                                                        (uint32_t)left * (uint32_t)a.low_stride * 4u);
-            low += __builtin_bit_cast(f32x4, ld4(lr, at < pad ? (uint32_t)(l16 * a.low_stride + at) * 4u : 0xf0000000u));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int t = 0; t < kT; t++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[i], b[t][i], acc[t], 0, 0, 0);
+        const AdapterJob j = adapter_job(a, job < a.jobs ? job : 0);
+        tl[t] = Tile{static_cast<const char*>(j.a), j.info, j.low, j.row, job < a.jobs ? j.slots : 0, j.max_rank, r * 16};
+        first_ranks = first_ranks || (tl[t].slots && !r);
     }
-}
-
-// grid (row tiles, output tiles, jobs): a wave per 16 rows x 64 outputs.
-template <int kType>
-__global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
-    constexpr int kT = 4;
-    const AdapterJob j = a.job[blockIdx.z];
-    const int m0 = (int)blockIdx.x * 16, n0 = ((int)blockIdx.y * 4 + wave_id()) * 16 * kT;
-    if (n0 >= j.out) return;
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int slot = tile_slots(j, a.row_slots, m0, a.rows);
-    const uint32_t any = (uint32_t)__ballot(slot >= 0) & 0xffffu;
-    if (!any) return;
-    f32x4 y[kT];
-    float* yp = j.y + (int64_t)(m0 + 4 * g) * j.out + n0 + l16;
+    // What the rows have of the sets; this workgroup writes it down for the kernels that expand if it is the first of its rows.
+    AdapterSlot info[kNV];
 #pragma unroll
-    for (int t = 0; t < kT; t++)
+    for (int t = 0; t < kNV; t++) info[t] = slot >= 0 && slot < tl[t].slots ? tl[t].info[slot] : AdapterSlot{0, 0.0f};
+    uint32_t left = (uint32_t)__ballot(slot >= 0) & 0xffffu;
+    float* xs = lds[wave];
+    for (int u = 0; left; u++) {
+        const int first = __builtin_ctz(left);
+        const int s = __builtin_amdgcn_readlane(slot, first);
+        const uint32_t mine = (uint32_t)__ballot(slot == s) & 0xffffu;
+        left &= ~mine;
+        if ((u & ((1 << a.way_shift) - 1)) != way) continue;
+        // (the same for every wave of the workgroup)
+        if (!first_ranks) {
+            bool any = false;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (any >> (4 * g + i) & 1 && n0 + 16 * t + l16 < j.out) y[t][i] = yp[(int64_t)i * j.out + 16 * t];
-    for_slots(slot, 0, 1, [&](int s, uint32_t mine) {
-        f32x4 acc[kT];
-        expand_slot<kType, kT>(a, j, s, m0, n0, acc);
-        const float scale = j.info[s].scale;
+            for (int t = 0; t < kNV; t++) any = any || tl[t].r0 < __builtin_amdgcn_readlane(info[t].rank, first);
+            if (!any) continue;
+        }
+        constexpr uint32_t kAbsent = 0xf0000000u;  // past every resource: reads zeros
+        __amdgpu_buffer_rsrc_t ar[kNV];
 #pragma unroll
-        for (int t = 0; t < kT; t++)
+        for (int t = 0; t < kNV; t++) {
+            const bool in = s < tl[t].slots && tl[t].r0 < tl[t].max_rank;
+            const int64_t size = adapter_a_slot(a.in, tl[t].max_rank) * adapter_elem(kType);
+            ar[t] = make_rsrc(tl[t].a + (in ? s * size + (int64_t)tl[t].r0 * a.in * adapter_elem(kType) : 0),
+                              in ? 16u * (uint32_t)a.in * adapter_elem(kType) : 0u);
+        }
+        f32x4 acc[kNV];
+#pragma unroll
+        for (int t = 0; t < kNV; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        u32x4 xv[8];
+        Raw8<kType> av[4][kNV];
+        auto load_a = [&](int c, int p) {
+#pragma unroll
+            for (int t = 0; t < kNV; t++)
+                av[p][t] = load_raw8<kType>(ar[t], c + p < c1 ? (uint32_t)(c + p) * (512u * adapter_elem(kType)) + 16u * (uint32_t)lane
+                                                              : kAbsent);
+        };
+        auto load_x = [&](int c) {  // rows of other slots are not fetched
+            const int k = c * 32 + 4 * (lane & 31);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = 2 * i + (lane >> 5);
+                xv[i] = ld4(xr, (mine >> r & 1) && k < c1 * 32 ? ((uint32_t)r * (uint32_t)a.in + (uint32_t)k) * 4u : kAbsent);
+            }
+        };
+        load_x(c0);
+#pragma unroll
+        for (int p = 0; p < 4; p++) load_a(c0, p);
+        __syncthreads();  // the last slot's sums have been read
+        for (int c = c0; c < c1; c += 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                *reinterpret_cast<u32x4*>(xs + (2 * i + (lane >> 5)) * kXRow + 4 * (lane & 31)) = xv[i];
+            wave_sync();
+            const bool more = c + 4 < c1;
+            if (more) load_x(c + 4);
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(xs + l16 * kXRow + 32 * p + 8 * g);
+                const f32x4 hi = *reinterpret_cast<const f32x4*>(xs + l16 * kXRow + 32 * p + 8 * g + 4);
+                Parts x;
+                split_pair<3>(lo[0], lo[1], 0, x.part);
+                split_pair<3>(lo[2], lo[3], 1, x.part);
+                split_pair<3>(hi[0], hi[1], 2, x.part);
+                split_pair<3>(hi[2], hi[3], 3, x.part);
+#pragma unroll
+                for (int t = 0; t < kNV; t++) acc[t] = multiply<kType>(x, av[p][t], acc[t]);
+                if (more) load_a(c + 4, p);
+            }
+            wave_sync();
+        }
+        // (the wave's own words: its x is used up)
+#pragma unroll
+        for (int t = 0; t < kNV; t++) *reinterpret_cast<f32x4*>(xs + t * 256 + 4 * lane) = acc[t];
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < kNV; t++) {
+            if (wave != t || tl[t].r0 >= __builtin_amdgcn_readlane(info[t].rank, first)) continue;
+            f32x4 v = *reinterpret_cast<const f32x4*>(lds[0] + t * 256 + 4 * lane);
+#pragma unroll
+            for (int w = 1; w < kShrinkWaves; w++) v += *reinterpret_cast<const f32x4*>(lds[w] + t * 256 + 4 * lane);
+            // lane (g, l16) holds rows 4 g .. 4 g + 3 of rank r0 + l16
+            float* low = tl[t].low + ((int64_t)share * a.rows + m0 + 4 * g) * a.low_stride + tl[t].r0 + l16;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (mine >> (4 * g + i) & 1) y[t][i] = fmaf(acc[t][i], scale, y[t][i]);
-    });
+                if (mine >> (4 * g + i) & 1) low[(int64_t)i * a.low_stride] = v[i];
+        }
+    }
 #pragma unroll
-    for (int t = 0; t < kT; t++)
+    for (int t = 0; t < kNV; t++)
+        if (tl[t].slots && !tl[t].r0 && !share && !way && wave == kShrinkWaves - 1 - t && lane < 16 && m < a.rows)
+            tl[t].row[m] = AdapterRow{info[t].rank > 0 ? (uint32_t)slot << 16 | (uint32_t)rank_pad(info[t].rank) : 0u, info[t].scale};
+}
+
+// Outputs that a projection kernel without adapters has written: grid (row tiles, output tiles, jobs), a wave per 16 rows x 64
+// outputs.
+__global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
+    constexpr int kN = 4;
+    const AdapterJob j = adapter_job(a, (int)blockIdx.z);
+    __shared__ float low[AdapterTiles<1, kN>::kLds];
+    const int m0 = (int)blockIdx.x * 16, n0 = ((int)blockIdx.y * 4 + wave_id()) * 16 * kN;
+    if (!j.slots || (int)blockIdx.y * 64 * kN >= j.out) return;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    AdapterTiles<1, kN> tiles;
+    tiles.load(a, j, m0);
+    const uint32_t any = (uint32_t)__ballot((tiles.key[0] & 0xffffu) != 0) & 0xffffu;
+    float y[1][kN][4];
+    float* yp = j.y + (int64_t)(m0 + 4 * g) * j.out + n0 + l16;
+#pragma unroll
+    for (int c = 0; c < kN; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (any >> (4 * g + i) & 1 && n0 + 16 * t + l16 < j.out) yp[(int64_t)i * j.out + 16 * t] = y[t][i];
+            if (any >> (4 * g + i) & 1 && n0 + 16 * c + l16 < j.out) y[0][c][i] = yp[(int64_t)i * j.out + 16 * c];
+    tiles.add(a, j, m0, n0, y, low, 256);
+#pragma unroll
+    for (int c = 0; c < kN; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (any >> (4 * g + i) & 1 && n0 + 16 * c + l16 < j.out) yp[(int64_t)i * j.out + 16 * c] = y[0][c][i];
 }
 
 __global__ __launch_bounds__(256) void adapter_slot_kernel(AdapterSlot* info, int first, int count, int rank, float scale) {
@@ -237,59 +273,79 @@ __global__ __launch_bounds__(256) void adapter_slot_kernel(AdapterSlot* info, in
     if (i < count) info[first + i] = AdapterSlot{rank, scale};
 }
 
-// B [out][rank] -> rows of rank_pad(rank) values, zeros past the rank. T: the values' storage width.
+// A and B into operand order; T: the values' storage width. A: values i = ((tile, chunk, half), lane, e), E = 16 / sizeof(T) values
+// a lane and half; B: ((output tile, rank step), lane, four ranks).
 template <class T>
-__global__ __launch_bounds__(256) void adapter_pad_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t n, int rank,
-                                                          int pad) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t row = i / pad;
-    const int r = (int)(i - row * pad);
-    dst[i] = r < rank ? src[row * rank + r] : T(0);
+__global__ __launch_bounds__(256) void adapter_pack_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __restrict__ pa,
+                                                           T* __restrict__ pb, int in, int out, int rank) {
+    constexpr int E = 16 / sizeof(T), kHalves = 8 / E;
+    const int steps = adapter_tiles16(rank);
+    const int64_t na = (int64_t)steps * 16 * in, nb = (int64_t)adapter_tiles16(out) * steps * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < na + nb; i += (int64_t)gridDim.x * 256) {
+        if (i < na) {
+            const int e = (int)(i % E), lane = (int)(i / E % 64);
+            const int64_t piece = i / (E * 64);
+            const int half = (int)(piece % kHalves), c = (int)(piece / kHalves % (in / 32)), t = (int)(piece / kHalves / (in / 32));
+            const int r = 16 * t + (lane & 15), k = 32 * c + 8 * (lane >> 4) + E * half + e;
+            pa[i] = r < rank ? a[(int64_t)r * in + k] : T(0);
+        } else {
+            const int64_t q = i - na;
+            const int e = (int)(q & 3), lane = (int)(q >> 2 & 63);
+            const int64_t piece = q >> 8;
+            const int64_t n = piece / steps * 16 + (lane & 15);
+            const int r = (int)(piece % steps) * 16 + 4 * (lane >> 4) + e;
+            pb[q] = r < rank && n < out ? b[n * rank + r] : T(0);
+        }
+    }
 }
 
 template <int kType>
-hipError_t launch_apply(const AdapterArgs& a, int jobs, hipStream_t st) {
-    int out = 0;
-    for (int i = 0; i < jobs; i++) out = a.job[i].out > out ? a.job[i].out : out;
-    const unsigned tiles = (unsigned)((a.rows + 15) / 16);
-    const auto shrink = [&](auto nt) {
-        constexpr int kNT = decltype(nt)::value;
-        const unsigned groups = (unsigned)((a.low_stride + 16 * kNT - 1) / (16 * kNT));
-        hipLaunchKernelGGL((adapter_shrink_kernel<kType, kNT>), dim3(tiles * (unsigned)a.slot_ways, (unsigned)jobs * groups, (unsigned)a.shares),
-                           dim3(64 * kShrinkWaves), 0, st, a);
-    };
-    if (a.rows <= 64 || a.low_stride <= 16)
-        shrink(std::integral_constant<int, 1>{});
-    else if (a.low_stride <= 32)
-        shrink(std::integral_constant<int, 2>{});
+hipError_t launch_shrink(const AdapterArgs& a, const ActQuantJob& quant, hipStream_t st) {
+    // quantising parts fill rows of their own behind the others, at least 64 workgroups wide
+    const int64_t parts = quant.parts(), want = parts < 64 ? parts : 64, x = a.shrink_x > want ? a.shrink_x : want;
+    const dim3 grid((unsigned)x, (unsigned)(a.groups * a.shares + (parts + x - 1) / x)), wg(64 * kShrinkWaves);
+    if (a.rank_tiles == 1)
+        hipLaunchKernelGGL((adapter_shrink_kernel<kType, 1>), grid, wg, 0, st, a, quant);
     else
-        shrink(std::integral_constant<int, 4>{});
-    hipLaunchKernelGGL(adapter_expand_kernel<kType>, dim3(tiles, (unsigned)((out + 255) / 256), (unsigned)jobs), dim3(256), 0, st,
-                       a);
+        hipLaunchKernelGGL((adapter_shrink_kernel<kType, 2>), grid, wg, 0, st, a, quant);
     return hipGetLastError();
 }
 
 }  // namespace
 
-void plan_adapters(AdapterArgs& a, int jobs, int max_rank) {
+void plan_adapters(AdapterArgs& a, int max_rank) {
     a.low_stride = (max_rank + 15) & ~15;
-    const int tiles = (a.rows + 15) / 16;
-    const int nt = a.rows <= 64 || a.low_stride <= 16 ? 1 : a.low_stride <= 32 ? 2 : 4;
-    const int wgs = tiles * jobs * ((a.low_stride + 16 * nt - 1) / (16 * nt));
-    const int most = (a.in / 32 + 4 * kShrinkWaves - 1) / (4 * kShrinkWaves);  // four steps a wave at least
+    int slots = 1;
+    for (int i = 0; i < a.jobs; i++) slots = a.job[i].slots > slots ? a.job[i].slots : slots;
+    const int tiles = (a.rows + 15) / 16, all = a.jobs * (a.low_stride / 16);
+    constexpr int kMostShares = 4;
+    // two rank tiles beside each other where that leaves 128 workgroups
+    a.rank_tiles = all > 1 && tiles * ((all + 1) / 2) * kMostShares >= 128 ? 2 : 1;
+    a.groups = (all + a.rank_tiles - 1) / a.rank_tiles;
+    const int wgs = tiles * a.groups;
+    const int most = (a.in / 32 + 4 * kShrinkWaves - 1) / (4 * kShrinkWaves);  // a round a wave at least
     a.shares = (256 + wgs - 1) / wgs;
     if (a.shares > most) a.shares = most;
-    int slots = 1;
-    for (int i = 0; i < jobs; i++) slots = a.job[i].slots > slots ? a.job[i].slots : slots;
-    a.slot_ways = a.rows > 64 ? 2 : a.rows < 16 ? a.rows : 16;
-    if (a.slot_ways > slots) a.slot_ways = slots;
+    if (a.shares > kMostShares) a.shares = kMostShares;
+    a.each = (a.in / 32 + kShrinkWaves * a.shares - 1) / (kShrinkWaves * a.shares);
+    // a workgroup for each of a tile's slots at a few rows, which may all differ; one in all at many
+    a.way_shift = 0;
+    while (a.rows <= 64 && a.way_shift < 4 && 1 << a.way_shift < slots && 1 << a.way_shift < a.rows) a.way_shift++;
+    a.shrink_x = tiles << a.way_shift;
 }
 
-hipError_t launch_adapters(const AdapterArgs& a, int type, int jobs, hipStream_t st) {
-    if (type == kAdapterF32) return launch_apply<kAdapterF32>(a, jobs, st);
-    if (type == kAdapterF16) return launch_apply<kAdapterF16>(a, jobs, st);
-    return launch_apply<kAdapterBF16>(a, jobs, st);
+hipError_t launch_adapters_shrink(const AdapterArgs& a, const ActQuantJob& quant, hipStream_t st) {
+    if (a.type == kAdapterF32) return launch_shrink<kAdapterF32>(a, quant, st);
+    if (a.type == kAdapterF16) return launch_shrink<kAdapterF16>(a, quant, st);
+    return launch_shrink<kAdapterBF16>(a, quant, st);
+}
+
+hipError_t launch_adapters_expand(const AdapterArgs& a, hipStream_t st) {
+    int out = 0;
+    for (int i = 0; i < a.jobs; i++) out = a.job[i].slots && a.job[i].out > out ? a.job[i].out : out;
+    hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)((a.rows + 15) / 16), (unsigned)((out + 255) / 256), (unsigned)a.jobs),
+                       dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_adapter_slots(AdapterSlot* info, int first, int count, int rank, float scale, hipStream_t st) {
@@ -298,16 +354,16 @@ hipError_t launch_adapter_slots(AdapterSlot* info, int first, int count, int ran
     return hipGetLastError();
 }
 
-hipError_t launch_adapter_pad(const void* src, void* dst, int out, int rank, int elem, hipStream_t st) {
-    const int pad = rank_pad(rank);
-    const int64_t n = (int64_t)out * pad;
-    const dim3 grid((unsigned)((n + 255) / 256));
-    if (elem == 4)
-        hipLaunchKernelGGL(adapter_pad_kernel<uint32_t>, grid, dim3(256), 0, st, (const uint32_t*)src, (uint32_t*)dst, n, rank,
-                           pad);
+hipError_t launch_adapter_pack(const void* a, const void* b, void* a_slot, void* b_slot, int type, int in, int out, int rank,
+                               hipStream_t st) {
+    const int64_t n = adapter_a_slot(in, rank) + adapter_b_slot(out, rank);
+    const dim3 grid((unsigned)((n + 1023) / 1024 < 4096 ? (n + 1023) / 1024 : 4096));
+    if (type == kAdapterF32)
+        hipLaunchKernelGGL(adapter_pack_kernel<uint32_t>, grid, dim3(256), 0, st, (const uint32_t*)a, (const uint32_t*)b,
+                           (uint32_t*)a_slot, (uint32_t*)b_slot, in, out, rank);
     else
-        hipLaunchKernelGGL(adapter_pad_kernel<uint16_t>, grid, dim3(256), 0, st, (const uint16_t*)src, (uint16_t*)dst, n, rank,
-                           pad);
+        hipLaunchKernelGGL(adapter_pack_kernel<uint16_t>, grid, dim3(256), 0, st, (const uint16_t*)a, (const uint16_t*)b,
+                           (uint16_t*)a_slot, (uint16_t*)b_slot, in, out, rank);
     return hipGetLastError();
 }
 

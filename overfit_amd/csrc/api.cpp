@@ -92,8 +92,8 @@ struct ovfq_weight {
     SharedPlane* shared = nullptr; // set for expert slices: blocks/scales point into shared->p
 };
 
-// The adapters of one weight (ovfq_adapters_create): fixed slots in one allocation. A [slots][max_rank][in], then B
-// [slots][out * rank_pad(max_rank)], then the slots' ranks and scales.
+// The adapters of one weight (ovfq_adapters_create): fixed slots in one allocation, A of every slot in operand order, then B,
+// then the slots' ranks and scales.
 struct ovfq_adapters {
     ovfq_ctx* ctx = nullptr;
     int type = 0;
@@ -105,9 +105,9 @@ struct ovfq_adapters {
     char* b = nullptr;
     ovfq::AdapterSlot* info = nullptr;
     size_t nbytes = 0;
-    size_t elem() const { return type == OVFQ_TYPE_F32 ? 4 : 2; }
-    size_t a_slot() const { return (size_t)max_rank * in * elem(); }
-    size_t b_slot() const { return (size_t)out * ovfq::rank_pad(max_rank) * elem(); }
+    size_t elem() const { return (size_t)ovfq::adapter_elem(type); }
+    size_t a_slot() const { return (size_t)ovfq::adapter_a_slot(in, max_rank) * elem(); }
+    size_t b_slot() const { return (size_t)ovfq::adapter_b_slot(out, max_rank) * elem(); }
 };
 
 namespace {
@@ -297,41 +297,73 @@ int quantize_q8_tiled_into_scratch(ovfq_ctx* c, const float* x_dev, int rows, in
     return OVFQ_OK;
 }
 
-// Quantises `rows` activation rows of length `in` for weight type `type` into the context scratch.
-int quantize_into_scratch(ovfq_ctx* c, int type, const float* x_dev, int rows, int in, ovfq::ActQ* act,
-                          bool tiled = false) {
+// Scratch for `rows` activation rows of length `in` quantised for weight type `type`, and the job that writes it.
+int plan_quantize(ovfq_ctx* c, int type, const float* x_dev, int rows, int in, ovfq::ActQ* act, ovfq::ActQuantJob* job,
+                  bool tiled) {
+    using Job = ovfq::ActQuantJob;
     const size_t n = (size_t)rows * in;
     int rc;
-    if (tiled && type == OVFQ_TYPE_Q8_0) return quantize_q8_tiled_into_scratch(c, x_dev, rows, 1, in, act);
-    if (tiled) {
+    *job = Job{};
+    job->x = x_dev;
+    if (tiled && type == OVFQ_TYPE_Q8_0) {
+        const size_t recs = ovfq::q8_tiled_records(rows, 1, in);
+        if ((rc = ensure(c, c->act_q, recs * ovfq::kQ8TiledQ)) ||
+            (rc = ensure(c, c->act_s, recs * ovfq::kQ8TiledS * sizeof(float))))
+            return rc;
+        job->kind = Job::kQ80Tiled;
+        job->n_blocks = (int64_t)(n / OVFQ_Q8_BLOCK);
+        job->per_row = in / OVFQ_Q8_BLOCK;
+        *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, nullptr, nullptr, true};
+    } else if (tiled) {
         const size_t recs = (size_t)ovfq::tiled_subs(rows) * (size_t)(in / OVFQ_QK);
         if ((rc = ensure(c, c->act_q, recs * ovfq::kTiledQ)) || (rc = ensure(c, c->act_s, recs * ovfq::kTiledS)) ||
             (rc = ensure(c, c->act_b, recs * ovfq::kTiledB)))
             return rc;
-        *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, nullptr, (const uint16_t*)c->act_b.p, true};
-        HIP_TRY(ovfq::launch_quantize_q8k_tiled(type, x_dev, rows, in, (int8_t*)c->act_q.p, (float*)c->act_s.p,
-                                                (uint16_t*)c->act_b.p, c->stream));
-        return OVFQ_OK;
-    }
-    rc = ensure(c, c->act_q, n);
-    if (rc) return rc;
-    if (type == OVFQ_TYPE_Q8_0) {
-        rc = ensure(c, c->act_s, n / 32 * sizeof(float));
-        if (rc) return rc;
-        HIP_TRY(ovfq::launch_quantize_q8_0(x_dev, (int64_t)(n / 32), (int8_t*)c->act_q.p, (float*)c->act_s.p,
-                                           c->stream));
+        job->kind = Job::kQ8KTiled;
+        job->n_blocks = (int64_t)(n / OVFQ_QK);
+        job->per_row = in / OVFQ_QK;
+        job->q6 = type == OVFQ_TYPE_Q6_K;
+        job->bh = (uint16_t*)c->act_b.p;
+        *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, nullptr, job->bh, true};
+    } else if (type == OVFQ_TYPE_Q8_0) {
+        if ((rc = ensure(c, c->act_q, n)) || (rc = ensure(c, c->act_s, n / 32 * sizeof(float)))) return rc;
+        job->kind = Job::kQ80;
+        job->n_blocks = (int64_t)(n / OVFQ_Q8_BLOCK);
         *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, nullptr};
     } else {
-        rc = ensure(c, c->act_s, n / 256 * sizeof(float));
-        if (rc) return rc;
         // the int16 bsums, then the same sums as fp16 (read by the tiled Q4_K kernels)
-        rc = ensure(c, c->act_b, n / 16 * 2 * sizeof(int16_t));
-        if (rc) return rc;
-        int16_t* b = (int16_t*)c->act_b.p;
-        uint16_t* bh = (uint16_t*)(b + n / 16);
-        HIP_TRY(ovfq::launch_quantize_q8k(x_dev, (int64_t)(n / 256), (int8_t*)c->act_q.p, (float*)c->act_s.p, b,
-                                          c->stream, bh));
-        *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, b, bh};
+        if ((rc = ensure(c, c->act_q, n)) || (rc = ensure(c, c->act_s, n / 256 * sizeof(float))) ||
+            (rc = ensure(c, c->act_b, n / 16 * 2 * sizeof(int16_t))))
+            return rc;
+        job->kind = Job::kQ8K;
+        job->n_blocks = (int64_t)(n / OVFQ_QK);
+        job->b = (int16_t*)c->act_b.p;
+        job->bh = (uint16_t*)(job->b + n / 16);
+        *act = ovfq::ActQ{(const int8_t*)c->act_q.p, (const float*)c->act_s.p, job->b, job->bh};
+    }
+    job->q = (int8_t*)c->act_q.p;
+    job->s = (float*)c->act_s.p;
+    return OVFQ_OK;
+}
+
+// Quantises `rows` activation rows of length `in` for weight type `type` into the context scratch.
+int quantize_into_scratch(ovfq_ctx* c, int type, const float* x_dev, int rows, int in, ovfq::ActQ* act,
+                          bool tiled = false) {
+    ovfq::ActQuantJob j;
+    const int rc = plan_quantize(c, type, x_dev, rows, in, act, &j, tiled);
+    if (rc) return rc;
+    switch (j.kind) {
+        case ovfq::ActQuantJob::kQ80Tiled:
+            HIP_TRY(ovfq::launch_quantize_q8_0_tiled(x_dev, rows, 1, in, j.q, j.s, c->stream));
+            break;
+        case ovfq::ActQuantJob::kQ8KTiled:
+            HIP_TRY(ovfq::launch_quantize_q8k_tiled(type, x_dev, rows, in, j.q, j.s, j.bh, c->stream));
+            break;
+        case ovfq::ActQuantJob::kQ80:
+            HIP_TRY(ovfq::launch_quantize_q8_0(x_dev, j.n_blocks, j.q, j.s, c->stream));
+            break;
+        default:
+            HIP_TRY(ovfq::launch_quantize_q8k(x_dev, j.n_blocks, j.q, j.s, j.b, c->stream, j.bh));
     }
     return OVFQ_OK;
 }
@@ -435,9 +467,11 @@ bool quantize_in_launch(const ovfq_ctx* c, int type, int in, int rows, int count
 }
 
 // One launch for `count` weights sharing an activation: either the fp32 activation x (quantised inside the
-// decode kernel) or an already-quantised `act`.
+// decode kernel) or an already-quantised `act`. ad: the rows' adapters, whose low-rank products are under way; *ad_done is set
+// where the launch adds them to the outputs itself.
 int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, const float* const* biases,
-                      float* const* ys, int rows, ovfq::ActQ act, const float* x = nullptr) {
+                      float* const* ys, int rows, ovfq::ActQ act, const float* x = nullptr,
+                      const ovfq::AdapterArgs* ad = nullptr, bool* ad_done = nullptr) {
     ovfq::ProjJob jobs[ovfq::kMaxJobs];
     for (int i = 0; i < count; i++) {
         jobs[i].w = static_cast<const uint8_t*>(ws[i]->blocks);
@@ -462,9 +496,10 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
         }
     } else if (act.tiled) {
         if (use_mid(c, in, rows, ws, count) == ovfq::MidKernel::kPanel)
-            HIP_TRY(ovfq::launch_project_panel(type, jobs, count, in, rows, act, c->stream));
+            HIP_TRY(ovfq::launch_project_panel(type, jobs, count, in, rows, act, c->stream, ad));
         else
-            HIP_TRY(ovfq::launch_project_split(type, jobs, count, in, rows, act, c->stream));
+            HIP_TRY(ovfq::launch_project_split(type, jobs, count, in, rows, act, c->stream, ad));
+        if (ad) *ad_done = true;
     } else if (type == OVFQ_TYPE_Q8_0) {
         // Batches that q8_mid.hip does not take (a caller's quantised activation, the fixed-scratch entry point, more than
         // 512 rows, what q8_mid_choice leaves, OVFQ_SPLIT=0). The int8-MFMA kernel from 8 rows; for inputs up to 8192 from 6
@@ -1047,7 +1082,7 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     const int in = ws[0]->in;
     if ((rc = check_plane(rows, in, "activation"))) return rc;
     ovfq::AdapterArgs aa{};
-    int ad_jobs = 0, ad_job_of[ovfq::kMaxJobs], ad_type = 0;
+    bool any_set = false;
     if (ad) {
         if (!ad->sets) return fail(OVFQ_ERR_NULL, "adapter set array is NULL");
         if (!ad->row_slots) return fail(OVFQ_ERR_NULL, "row_slots is NULL");
@@ -1059,24 +1094,29 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
             if (s->ctx != ctx) return fail(OVFQ_ERR_SIZE, "adapter set %d belongs to another context", i);
             if (s->in != in || s->out != ws[i]->out)
                 return fail(OVFQ_ERR_SIZE, "adapter set %d is for %d x %d, its weight %d x %d", i, s->out, s->in, ws[i]->out, in);
-            if (ad_jobs && s->type != ad_type) return fail(OVFQ_ERR_TYPE, "the adapter sets of a call must share a type");
-            ad_type = s->type;
+            if (any_set && s->type != aa.type) return fail(OVFQ_ERR_TYPE, "the adapter sets of a call must share a type");
+            any_set = true;
+            aa.type = s->type;
             max_rank = s->max_rank > max_rank ? s->max_rank : max_rank;
-            ad_job_of[ad_jobs] = i;
-            aa.job[ad_jobs++] = ovfq::AdapterJob{s->a, s->b, s->info, nullptr, nullptr, s->slots, s->max_rank,
-                                                 ovfq::rank_pad(s->max_rank), s->out};
+            aa.job[i] = ovfq::AdapterJob{s->a,    s->b,     s->info,     nullptr,
+                                         nullptr, nullptr,  s->slots,    s->max_rank,
+                                         s->out};
         }
+        aa.jobs = count;
         aa.rows = rows;
         aa.in = in;
-        if (ad_jobs) ovfq::plan_adapters(aa, ad_jobs, max_rank);
+        if (any_set) ovfq::plan_adapters(aa, max_rank);
     }
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
     int* slots_d = ad ? const_cast<int*>(ad->row_slots) : nullptr;
     if (ad) {
-        auto carve = [&](Carver& c) {  // the jobs' products, and the staged slots of a host call
-            for (int i = 0; i < ad_jobs; i++)
+        auto carve = [&](Carver& c) {  // the rows' adapters and products for each set, and the staged slots of a host call
+            for (int i = 0; i < count; i++) {
+                if (!aa.job[i].slots) continue;
+                aa.job[i].row = c.take<ovfq::AdapterRow>((size_t)rows * sizeof(ovfq::AdapterRow));
                 aa.job[i].low = c.take<float>((size_t)aa.shares * rows * aa.low_stride * 4);
+            }
             if (host) slots_d = c.take<int>((size_t)rows * 4);
         };
         Carver sizing{nullptr};
@@ -1121,22 +1161,31 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     }
     const bool tiled = use_mid(ctx, in, rows, ws, count) != ovfq::MidKernel::kNone ||
                        use_q8_mid(ctx, in, rows, ws, count);
+    bool ad_done = false;
+    const ovfq::AdapterArgs* ap = any_set ? &aa : nullptr;
+    if (any_set) {
+        aa.x = xd;
+        aa.row_slots = slots_d;
+        for (int i = 0; i < count; i++) aa.job[i].y = yd[i];
+    }
     if (!tiled && quantize_in_launch(ctx, ws[0]->type, in, rows, count,
                                      count == 2 && ws[0]->out == ws[1]->out ? ws[0]->out : 0)) {
         // Decode: the Q8_K quantisation happens inside the projection launch.
-        if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, ovfq::ActQ{nullptr, nullptr, nullptr}, xd)))
+        if (ap) HIP_TRY(ovfq::launch_adapters_shrink(aa, ovfq::ActQuantJob{}, ctx->stream));
+        if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, ovfq::ActQ{nullptr, nullptr, nullptr}, xd, ap, &ad_done)))
             return rc;
     } else {
         ovfq::ActQ act;
-        if ((rc = quantize_into_scratch(ctx, ws[0]->type, xd, rows, in, &act, tiled))) return rc;
-        if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, act))) return rc;
+        if (ap) {
+            ovfq::ActQuantJob job;
+            if ((rc = plan_quantize(ctx, ws[0]->type, xd, rows, in, &act, &job, tiled))) return rc;
+            HIP_TRY(ovfq::launch_adapters_shrink(aa, job, ctx->stream));
+        } else if ((rc = quantize_into_scratch(ctx, ws[0]->type, xd, rows, in, &act, tiled))) {
+            return rc;
+        }
+        if ((rc = launch_projection(ctx, ws, count, bd, yd, rows, act, nullptr, ap, &ad_done))) return rc;
     }
-    if (ad_jobs) {
-        aa.x = xd;
-        aa.row_slots = slots_d;
-        for (int i = 0; i < ad_jobs; i++) aa.job[i].y = yd[ad_job_of[i]];
-        HIP_TRY(ovfq::launch_adapters(aa, ad_type, ad_jobs, ctx->stream));
-    }
+    if (ap && !ad_done) HIP_TRY(ovfq::launch_adapters_expand(aa, ctx->stream));
     if (host) {
         for (int i = 0; i < count; i++)
             if ((rc = io.down(ys[i], yd[i], (size_t)rows * ws[i]->out * 4))) return rc;
@@ -1340,8 +1389,8 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
     // the kernels address a slot's planes, and 16 rows of x, with 32-bit byte offsets that leave room for out-of-range ones
     if (input_size > OVFQ_MAX_ADAPTER_INPUT)
         return fail(OVFQ_ERR_SIZE, "inputSize (%d) above %d", input_size, OVFQ_MAX_ADAPTER_INPUT);
-    if ((int64_t)max_rank * input_size * 4 >= (int64_t)1 << 30 ||
-        (int64_t)ovfq::rank_pad(max_rank) * output_size * 4 >= (int64_t)1 << 30)
+    if (ovfq::adapter_a_slot(input_size, max_rank) * 4 >= (int64_t)1 << 30 ||
+        ovfq::adapter_b_slot(output_size, max_rank) * 4 >= (int64_t)1 << 30)
         return fail(OVFQ_ERR_SIZE, "an adapter of rank %d for %d x %d is too large", max_rank, output_size, input_size);
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
@@ -1412,20 +1461,21 @@ static int adapters_load_impl(ovfq_adapters* s, int slot, const void* a, const v
     HIP_TRY(hipSetDevice(ctx->device));
     int rc = check_not_capturing(ctx, "an adapter cannot be loaded");
     if (rc) return rc;
-    const size_t b_bytes = (size_t)s->out * rank * s->elem();
-    const void* b_dev = b;
-    void* staged = nullptr;
+    const size_t a_bytes = (size_t)rank * s->in * s->elem(), b_bytes = (size_t)rank * s->out * s->elem();
+    const char *a_dev = static_cast<const char*>(a), *b_dev = static_cast<const char*>(b);
+    char* staged = nullptr;
     hipError_t e = hipSuccess;
     if (host) {
-        e = hipMalloc(&staged, b_bytes);
-        if (e == hipSuccess) e = hipMemcpyAsync(staged, b, b_bytes, hipMemcpyHostToDevice, ctx->stream);
-        b_dev = staged;
+        const size_t b_at = (a_bytes + 255) & ~size_t(255);
+        e = hipMalloc((void**)&staged, b_at + b_bytes);
+        if (e == hipSuccess) e = hipMemcpyAsync(staged, a, a_bytes, hipMemcpyHostToDevice, ctx->stream);
+        if (e == hipSuccess) e = hipMemcpyAsync(staged + b_at, b, b_bytes, hipMemcpyHostToDevice, ctx->stream);
+        a_dev = staged;
+        b_dev = staged + b_at;
     }
     if (e == hipSuccess)
-        e = hipMemcpyAsync(s->a + (size_t)slot * s->a_slot(), a, (size_t)rank * s->in * s->elem(),
-                           host ? hipMemcpyHostToDevice : hipMemcpyDeviceToDevice, ctx->stream);
-    if (e == hipSuccess)
-        e = ovfq::launch_adapter_pad(b_dev, s->b + (size_t)slot * s->b_slot(), s->out, rank, (int)s->elem(), ctx->stream);
+        e = ovfq::launch_adapter_pack(a_dev, b_dev, s->a + (size_t)slot * s->a_slot(), s->b + (size_t)slot * s->b_slot(), s->type,
+                                      s->in, s->out, rank, ctx->stream);
     if (e == hipSuccess) e = ovfq::launch_adapter_slots(s->info, slot, 1, rank, scale, ctx->stream);
     const hipError_t done = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) e = done;

@@ -22,6 +22,9 @@
 // the quantise launch, before / after: 24 rows 41.4 / 25.1 us, 64 rows 76.8 / 31.9; Q4_K 4096x4096 at 64 rows 23.5 / 14.1.
 #include <cstdlib>
 
+#include <type_traits>
+
+#include "adapter_tile.h"
 #include "kquant_mfma.h"
 #include "ovfq_launch.h"
 
@@ -121,9 +124,11 @@ struct SplitQ6K {
     }
 };
 
-template <class FS, int T, int W>
-__global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArgs a) {
+// AD: AdapterArgs, and the rows' adapters are added to the outputs, or NoAdapters.
+template <class FS, int T, int W, class AD>
+__global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArgs a, const AD ad) {
     using F = typename FS::F;
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
     constexpr bool kMin = F::kNumMfma == 3;
     constexpr int kOuts = T * 256;                         // outputs of the workgroup's tile
     constexpr int kPer = (kOuts + 64 * W - 1) / (64 * W);  // per thread in the ordered sum
@@ -132,6 +137,7 @@ __global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArg
     __shared__ __align__(16) uint8_t ring[3][W][kSlot];
     __shared__ __align__(16) float vals0[W][kOuts], vals1[W][kOuts];
     __shared__ __align__(16) float scl[W][64];
+    __shared__ __align__(16) float low_out[kAd ? kOuts : 4];  // the adapters' part of the outputs
 
     const int wave = wave_id();
     const int lane = threadIdx.x & 63;
@@ -280,6 +286,52 @@ __global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArg
     asm volatile("" ::: "memory");
     fetch(ring[1][wave], wave + W);
     fetch(ring[2][wave], wave + 2 * W);
+    // The adapters' part of the thread's outputs while the first weights are on their way, the low-rank products staged where the
+    // rounds' values come later; each thread's own LDS words keep its result.
+    uint32_t low_mine = 0;  // outputs that have one
+    if constexpr (kAd) {
+        const AdapterJob aj = adapter_job(ad, j);
+        if (aj.slots) {
+            constexpr int kPass = W == 8 ? 64 : 32;  // ranks that fit vals0
+            static_assert(16 * T * (kPass + 4) <= W * kOuts, "staged products");
+            AdapterRow row[kPer];
+            float part[kPer];
+            int most = 0;  // the largest padded rank of the workgroup's rows, the same for every wave
+#pragma unroll
+            for (int t = 0; t < T; t++) most = max(most, adapter_row(ad, aj, n0 + 16 * t + r16).pad());
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int idx = (int)threadIdx.x + 64 * W * i;
+                row[i] = adapter_row(ad, aj, idx < kOuts ? n0 + (idx >> 8) * 16 + (idx & 15) : ad.rows);
+                if (o0 + ((idx >> 4) & 15) >= n_out) row[i].key = 0;
+                part[i] = 0.0f;
+            }
+#pragma unroll
+            for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
+            most = __builtin_amdgcn_readfirstlane(most);
+            for (int r0 = 0; r0 < most; r0 += kPass) {
+                if (r0) adapter_barrier();
+                adapter_stage(ad, aj, n0, 16 * T, r0, kPass, &vals0[0][0], 64 * W);
+                adapter_barrier();
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const int idx = (int)threadIdx.x + 64 * W * i;
+                    if (row[i].pad() > r0)
+                        part[i] = adapter_dot(ad, aj, row[i], o0 + ((idx >> 4) & 15),
+                                              &vals0[0][0] + ((idx >> 8) * 16 + (idx & 15)) * (kPass + 4), r0, kPass, part[i]);
+                }
+            }
+            if (most) adapter_barrier();  // vals0 is the first round's next
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int idx = (int)threadIdx.x + 64 * W * i;
+                if (row[i].pad()) {
+                    low_out[idx] = part[i] * row[i].scale;
+                    low_mine |= 1u << i;
+                }
+            }
+        }
+    }
     const int rounds = (spr + W - 1) / W;
     // round 0 adds up zeros (a thread reads the places it writes here)
 #pragma unroll
@@ -307,28 +359,34 @@ __global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArg
     for (int i = 0; i < kPer; i++) {
         const int idx = (int)threadIdx.x + 64 * W * i;
         const int o = o0 + ((idx >> 4) & 15), n = n0 + (idx >> 8) * 16 + (idx & 15);
-        if (idx < kOuts && n < a.m_rows && o < n_out) y[(size_t)n * n_out + o] = bias ? bias[o] + sum[i] : sum[i];
+        float v = bias && o < n_out ? bias[o] + sum[i] : sum[i];
+        if constexpr (kAd) {
+            if (low_mine >> i & 1) v += low_out[idx];
+        }
+        if (idx < kOuts && n < a.m_rows && o < n_out) y[(size_t)n * n_out + o] = v;
     }
     __builtin_amdgcn_s_waitcnt(0);  // no DMA lands in LDS that another workgroup may have by then
 }
 
-template <class F, int W>
-static hipError_t launch_split_t(const PArgs& pa, int T, hipStream_t st) {
+template <class F, int W, class AD>
+static hipError_t launch_split_t(const PArgs& pa, int T, const AD& ad, hipStream_t st) {
     const dim3 grid((pa.o_tiles + 7) / 8 * 8 * pa.n_tiles), wg(64 * W);
     if (T == 1)
-        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 1, W>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 1, W, AD>), grid, wg, 0, st, pa, ad);
     else if (T == 2)
-        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 2, W>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 2, W, AD>), grid, wg, 0, st, pa, ad);
     else if (T == 3)
-        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 3, W>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 3, W, AD>), grid, wg, 0, st, pa, ad);
     else
-        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 4, W>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_split_kernel<F, 4, W, AD>), grid, wg, 0, st, pa, ad);
     return hipGetLastError();
 }
 
 template <int W>
-static hipError_t launch_split_w(int type, const PArgs& pa, int T, hipStream_t st) {
-    return type == 12 ? launch_split_t<SplitQ4K, W>(pa, T, st) : launch_split_t<SplitQ6K, W>(pa, T, st);
+static hipError_t launch_split_w(int type, const PArgs& pa, int T, const AdapterArgs* ad, hipStream_t st) {
+    if (ad) return type == 12 ? launch_split_t<SplitQ4K, W>(pa, T, *ad, st) : launch_split_t<SplitQ6K, W>(pa, T, *ad, st);
+    return type == 12 ? launch_split_t<SplitQ4K, W>(pa, T, NoAdapters{}, st)
+                      : launch_split_t<SplitQ6K, W>(pa, T, NoAdapters{}, st);
 }
 
 // ------------------------------------------------------------------------------------------ panel kernel
@@ -367,9 +425,11 @@ struct PanelArgs {
 // fp16 bsums), gathered through the pairs' rows into the same order in LDS.
 enum class Src { kDense, kGroups, kGather };
 
-template <class FS, int T, Src SRC>
-__global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelArgs args) {
+template <class FS, int T, Src SRC, class AD>
+__global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelArgs args, const AD ad) {
     using F = typename FS::F;
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    static_assert(!kAd || SRC == Src::kDense, "adapters are beside dense projections");
     constexpr bool kMin = F::kNumMfma == 3;
     constexpr bool GRP = SRC != Src::kDense;
     constexpr int W = 4;
@@ -393,6 +453,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
     const float* bias = nullptr;
     float* y;
     int n_out, o0, n0, m_end, sub0;  // output rows n0 .. m_end, activation tiles sub0 ..
+    [[maybe_unused]] int job = 0;
     if constexpr (GRP) {
         if (n_tile >= args.grp.tile_count[0]) return;
         const int te = args.grp.tiles[n_tile];
@@ -415,6 +476,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
         bias = a.job[j].bias;
         y = a.job[j].y;
         n_out = a.job[j].n_out;
+        job = j;
         o0 = (o_tile - a.job[j].tile0) * 64 + wave * 16;
         n0 = n_tile * 16 * T;
         m_end = min(n0 + 16 * T, a.m_rows);
@@ -570,6 +632,12 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
     stage(0, act0, bs0, sc0);
     asm volatile("" ::: "memory");
     fetch(1, 1);
+    [[maybe_unused]] AdapterTiles<T, 1> low;
+    [[maybe_unused]] AdapterJob aj;
+    if constexpr (kAd) {
+        aj = adapter_job(ad, job);
+        if (aj.slots) low.load(ad, aj, n0);
+    }
     int k = 0;
     auto next_slot = [](int i) { return i == 2 ? 0 : i + 1; };
     int sb = 0;
@@ -584,6 +652,25 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
     // y[n][o] = biasO + sum   (RT/Q4KDotKernel.cs:951, RT/Q6KDotKernel.cs:507)
     const int o = o0 + r16;
     const float bias_o = bias && o < n_out ? bias[o] : 0.0f;
+    if constexpr (kAd) {
+        if (aj.slots) {
+            float v[T][1][4];
+#pragma unroll
+            for (int s = 0; s < T; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[s][0][i] = bias ? bias_o + out[s][i] : out[s][i];
+            static_assert(T * 1024 >= AdapterTiles<T, 1>::kLds, "staged products");
+            // no prefetch is still on its way into the activation slots, and every wave is done with them
+            __builtin_amdgcn_s_waitcnt(0);
+            adapter_barrier();
+            low.add(ad, aj, n0, o0, v, reinterpret_cast<float*>(act0), 256);
+#pragma unroll
+            for (int s = 0; s < T; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[s][i] = v[s][0][i];
+            bias = nullptr;
+        }
+    }
 #pragma unroll
     for (int s = 0; s < T; s++)
 #pragma unroll
@@ -594,24 +681,24 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
     __builtin_amdgcn_s_waitcnt(0);  // no DMA lands in LDS that another workgroup may have by then
 }
 
-template <class FS>
-static hipError_t launch_panel_t(const PanelArgs& pa, int T, hipStream_t st) {
+template <class FS, class AD>
+static hipError_t launch_panel_t(const PanelArgs& pa, int T, const AD& ad, hipStream_t st) {
     const dim3 grid((pa.p.o_tiles + 7) / 8 * 8 * pa.p.n_tiles), wg(256);
     if (T == 1)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 1, Src::kDense>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 1, Src::kDense, AD>), grid, wg, 0, st, pa, ad);
     else if (T == 2)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 2, Src::kDense>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 2, Src::kDense, AD>), grid, wg, 0, st, pa, ad);
     else if (T == 3)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 3, Src::kDense>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 3, Src::kDense, AD>), grid, wg, 0, st, pa, ad);
     else if (T == 4)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 4, Src::kDense>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 4, Src::kDense, AD>), grid, wg, 0, st, pa, ad);
     else if constexpr (FS::F::kNumMfma == 3)  // Q4_K: two workgroups' LDS still fit a CU
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 5, Src::kDense>), grid, wg, 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<FS, 5, Src::kDense, AD>), grid, wg, 0, st, pa, ad);
     return hipGetLastError();
 }
 
-hipError_t launch_project_panel(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                                hipStream_t st) {
+hipError_t launch_project_panel(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                                const AdapterArgs* ad) {
     PanelArgs pa{};
     int tiles = 0;
     for (int i = 0; i < njobs; i++) {
@@ -630,7 +717,8 @@ hipError_t launch_project_panel(int type, const ProjJob* jobs, int njobs, int in
     int T;
     panel_cost(type, tiles, pa.p.subs, &T);
     pa.p.n_tiles = (pa.p.subs + T - 1) / T;
-    return type == 12 ? launch_panel_t<SplitQ4K>(pa, T, st) : launch_panel_t<SplitQ6K>(pa, T, st);
+    if (ad) return type == 12 ? launch_panel_t<SplitQ4K>(pa, T, *ad, st) : launch_panel_t<SplitQ6K>(pa, T, *ad, st);
+    return type == 12 ? launch_panel_t<SplitQ4K>(pa, T, NoAdapters{}, st) : launch_panel_t<SplitQ6K>(pa, T, NoAdapters{}, st);
 }
 
 hipError_t launch_mfma_grouped(int type, const GroupLaunch& L, const int* tiles, const int* tile_count,
@@ -661,13 +749,17 @@ hipError_t launch_mfma_grouped(int type, const GroupLaunch& L, const int* tiles,
     pa.grp.o_tiles1 = o1;
     const dim3 grid((pa.p.o_tiles + 7) / 8 * 8 * max_tiles);
     if (type == 12 && L.pair_row)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ4K, 4, Src::kGather>), grid, dim3(256), 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ4K, 4, Src::kGather, NoAdapters>), grid, dim3(256), 0, st, pa,
+                           NoAdapters{});
     else if (type == 12)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ4K, 4, Src::kGroups>), grid, dim3(256), 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ4K, 4, Src::kGroups, NoAdapters>), grid, dim3(256), 0, st, pa,
+                           NoAdapters{});
     else if (L.pair_row)
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ6K, 4, Src::kGather>), grid, dim3(256), 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ6K, 4, Src::kGather, NoAdapters>), grid, dim3(256), 0, st, pa,
+                           NoAdapters{});
     else
-        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ6K, 4, Src::kGroups>), grid, dim3(256), 0, st, pa);
+        hipLaunchKernelGGL((kquant_mfma_panel_kernel<SplitQ6K, 4, Src::kGroups, NoAdapters>), grid, dim3(256), 0, st, pa,
+                           NoAdapters{});
     return hipGetLastError();
 }
 
@@ -684,8 +776,8 @@ MidKernel mid_kernel(int type, int in, int rows, long tiles, int count, bool pre
     return mid_choice(type, in, rows, tiles, count, prepared);
 }
 
-hipError_t launch_project_split(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                                hipStream_t st) {
+hipError_t launch_project_split(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                                const AdapterArgs* ad) {
     PArgs pa{};
     int tiles = 0;
     for (int i = 0; i < njobs; i++) {
@@ -707,7 +799,7 @@ hipError_t launch_project_split(int type, const ProjJob* jobs, int njobs, int in
     // four waves: Q6_K 4096x14336 at 64 rows, 256 workgroups, 30.2 / 34.0 and at 96 rows, 512 workgroups, 47.5 / 40.6; Q4_K
     // 1024x14336 at 128 rows 25.9 / 30.7, 1024x1024 at 64 rows 8.5 / 7.1).
     const int w8 = pa.spr >= 8 && (long)tiles * pa.n_tiles <= 256;
-    return w8 ? launch_split_w<8>(type, pa, T, st) : launch_split_w<4>(type, pa, T, st);
+    return w8 ? launch_split_w<8>(type, pa, T, ad, st) : launch_split_w<4>(type, pa, T, ad, st);
 }
 
 }  // namespace ovfq

@@ -9,6 +9,7 @@
 namespace ovfq {
 
 constexpr int kMaxJobs = 4;
+struct AdapterArgs;  // projection launches that take one add the rows' adapters to their outputs
 constexpr int kMaxExperts = 64;
 
 // One output matrix of a (possibly fused) projection launch. Every job of a launch shares the activation.
@@ -75,10 +76,10 @@ hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in,
 // against `count` weights of `tiles` 16-row tiles in all (prepared: every one with its MFMA-ready copy).
 bool mid_enabled();  // false with OVFQ_SPLIT=0 (measurements): neither these kernels nor those of q8_mid.hip
 MidKernel mid_kernel(int type, int in, int rows, long tiles, int count, bool prepared);
-hipError_t launch_project_split(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                                hipStream_t st);
-hipError_t launch_project_panel(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                                hipStream_t st);
+hipError_t launch_project_split(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                                const AdapterArgs* ad = nullptr);
+hipError_t launch_project_panel(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                                const AdapterArgs* ad = nullptr);
 // Small-batch / grouped-expert K-quant projection. One or two matrices per expert (gate, up) of equal shape;
 // expert_off/pair_row (device arrays) select each expert's activation rows, or NULL for a single expert over
 // activation rows 0..rows-1 (outputs row-major [pairs][n_rows]).
@@ -224,38 +225,79 @@ hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int 
 hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int planes, bool heads, int plane_in, int n_out,
                            int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st);
 
-// Low-rank adapters beside a projection (adapters.hip). A set keeps its adapters in fixed slots of one type: A [slots][max_rank]
-// [in] and, slot by slot, B rows of rank_pad(rank) values (b_stride = rank_pad(max_rank) of them a row at most).
+// An activation to quantise in the launch of another kernel (act_quant.h), 256 threads a part.
+struct ActQuantJob {
+    enum Kind { kNone, kQ8K, kQ8KTiled, kQ80, kQ80Tiled };
+    int kind = kNone;
+    const float* x = nullptr;
+    int64_t n_blocks = 0;  // of 256 or 32 values
+    int per_row = 0;       // blocks of a row (tiled kinds)
+    int q6 = 0;            // kQ8KTiled: for a Q6_K weight
+    int8_t* q = nullptr;
+    float* s = nullptr;
+    int16_t* b = nullptr;
+    uint16_t* bh = nullptr;
+    int64_t parts() const { return kind == kNone ? 0 : kind <= kQ8KTiled ? (n_blocks + 15) / 16 : (n_blocks + 31) / 32; }
+};
+
+// Low-rank adapters beside a projection (adapters.hip). A set keeps its adapters in fixed slots of one type, in the order in which
+// the lanes (g, l16) of a wave take MFMA operands, so that a wave's load is one contiguous piece:
+//   A: for 16 ranks and 32 inputs, rank 16 t + l16, inputs 32 c + 8 g .. + 7 (fp32: two pieces of four inputs a lane);
+//   B: for 16 outputs and 16 ranks, output 16 t + l16, ranks 16 r + 4 g .. + 3; a slot has as many rank steps as its rank needs.
+// Values past the rank and the outputs are zeros.
 enum AdapterType { kAdapterF32 = 0, kAdapterF16 = 1, kAdapterBF16 = 30 };
 struct AdapterSlot {
     int rank;  // 0: nothing loaded
     float scale;
 };
+// What an activation row has of a set: the shrinking launch writes it for the kernels that expand.
+struct AdapterRow {
+    uint32_t key;  // slot << 16 | rank_pad(rank); 0 in the low half: no adapter
+    float scale;
+    __host__ __device__ int slot() const { return (int)(key >> 16); }
+    __host__ __device__ int pad() const { return (int)(key & 0xffffu); }
+};
 struct AdapterJob {
     const void* a;
     const void* b;
     const AdapterSlot* info;  // [slots]
+    AdapterRow* row;          // scratch [rows]
     float* low;               // scratch [shares][rows][low_stride]
     float* y;                 // [rows][out], added to
-    int slots, max_rank, b_stride, out;
+    int slots;                // 0: this weight has no adapters
+    int max_rank, out;
 };
 struct AdapterArgs {
-    AdapterJob job[kMaxJobs];
-    const float* x;  // [rows][in]
+    AdapterJob job[kMaxJobs];  // by weight of the call
+    const float* x;            // [rows][in]
     const int* row_slots;
-    int rows, in;
+    int type, jobs, rows, in;
     // set by plan_adapters
     int low_stride;  // ranks of a scratch row: the largest max_rank, in whole tiles of 16
+    int rank_tiles;  // tiles of 16 ranks, of all the jobs', a workgroup of the shrinking launch
+    int groups;      // of such
     int shares;      // workgroups that divide the inputs of a product
-    int slot_ways;   // workgroups that divide the distinct slots of a row tile
+    int each;        // chunks of 32 inputs a wave
+    int way_shift;   // log2 of the workgroups that divide the distinct slots of a row tile
+    int shrink_x;    // row tiles << way_shift
 };
 __host__ __device__ constexpr int rank_pad(int rank) { return (rank + 3) & ~3; }
-void plan_adapters(AdapterArgs& a, int jobs, int max_rank);
-// Adds every row's adapter to the outputs of `jobs` projections of x (sets of one type).
-hipError_t launch_adapters(const AdapterArgs& a, int type, int jobs, hipStream_t st);
+__host__ __device__ constexpr int adapter_elem(int type) { return type == kAdapterF32 ? 4 : 2; }
+__host__ __device__ constexpr int adapter_tiles16(int n) { return (n + 15) / 16; }
+// Values of a slot's A and B for the set's largest rank.
+__host__ __device__ constexpr int64_t adapter_a_slot(int in, int max_rank) { return (int64_t)adapter_tiles16(max_rank) * 16 * in; }
+__host__ __device__ constexpr int64_t adapter_b_slot(int out, int max_rank) {
+    return (int64_t)adapter_tiles16(out) * adapter_tiles16(max_rank) * 256;
+}
+void plan_adapters(AdapterArgs& a, int max_rank);
+// The rows' low-rank products, and in the same launch an activation's quantisation.
+hipError_t launch_adapters_shrink(const AdapterArgs& a, const ActQuantJob& quant, hipStream_t st);
+// B times them added to the jobs' outputs, for projection kernels that do not do it themselves.
+hipError_t launch_adapters_expand(const AdapterArgs& a, hipStream_t st);
 hipError_t launch_adapter_slots(AdapterSlot* info, int first, int count, int rank, float scale, hipStream_t st);
-// B [out][rank] (elem bytes a value) into a slot's padded rows.
-hipError_t launch_adapter_pad(const void* src, void* dst, int out, int rank, int elem, hipStream_t st);
+// a [rank][in] and b [out][rank] of a type into a slot's operand order.
+hipError_t launch_adapter_pack(const void* a, const void* b, void* a_slot, void* b_slot, int type, int in, int out, int rank,
+                               hipStream_t st);
 
 // Norms around a residual sum (norm.hip): h_out = h + scale * gate * post(y), x_out = pre(h_out).
 enum GateMode { kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3 };

@@ -22,6 +22,7 @@
 // 31.7 / 42.7 / 45.4 -> 11.5 / 14.5 / 19.3 / 20.3 / 34.2 / 42.8; 4096x14336 at 4 / 16 / 32 / 300 rows 51.2 / 81.7 / 95.3 / 131
 // -> 22.7 / 22.9 / 33.7 / 99.7; 14336x4096 at 16 / 64 / 512 rows 31.4 / 33.2 / 132 -> 20.7 / 30.1 / 122; per-head Wo of 32 x
 // 4096x128 at 8 / 16 / 64 / 300 rows 18.1 / 26.9 / 35.3 / 46.1 -> 11.8 / 12.0 / 22.0 / 36.3.
+#include "act_quant.h"
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
 
@@ -437,25 +438,10 @@ __global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------ quantiser
-// Q8DotKernel.Quantize (RT/Q8DotKernel.cs:42-91) of rows x (planes * plane_in) into the records above: eight lanes a block.
 __global__ __launch_bounds__(256) void quantize_q8_0_tiled_kernel(const float* __restrict__ x, int64_t n_blocks, int nb,
                                                                   int wnb, int gph, uint8_t* __restrict__ q,
                                                                   float* __restrict__ s) {
-    const int64_t wblk = ((int64_t)blockIdx.x * 4 + wave_id()) * 8;
-    const int lane = threadIdx.x & 63;
-    const int64_t blk = wblk + (lane >> 3);
-    if (wblk >= n_blocks) return;
-    const int sub = lane & 7;  // elements 4 sub .. 4 sub + 3
-    const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + wblk * 32, rsrc_bytes((uint64_t)n_blocks * 128, (uint64_t)wblk * 128));
-    const Q80Lane r = q8_0_quantize_lane(ld4(xr, lane * 16));
-    if (blk >= n_blocks) return;
-    const int64_t row = blk / nb;
-    const int b = (int)(blk - row * nb), plane = b / wnb, bp = b - plane * wnb;
-    const int64_t rec = (row >> 4) * ((int64_t)(nb / wnb) * gph) + plane * gph + bp / 4;
-    const int j = bp & 3, r16 = (int)(row & 15), g = sub >> 1;
-    uint8_t* dst = q + rec * 2048 + (j >> 1) * 1024 + (g * 16 + r16) * 16 + (j & 1) * 8 + (sub & 1) * 4;
-    *reinterpret_cast<uint32_t*>(dst) = r.packed;
-    if (sub == 0) s[rec * 64 + j * 16 + r16] = r.scale;
+    quantize_q8_0_tiled_part(blockIdx.x, x, n_blocks, nb, wnb, gph, q, s);
 }
 
 hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int plane_in, int8_t* q, float* s,
