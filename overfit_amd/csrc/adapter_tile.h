@@ -59,22 +59,49 @@ __device__ __forceinline__ AdapterRow adapter_row(const AdapterArgs& e, const Ad
     return AdapterRow{v.x, as_float(scale)};
 }
 
-// The low-rank products of `rows` (a multiple of 16) activation rows from m0 on, ranks r0 .. r0 + nr (16, 32 or 64 of them), their
-// shares added: into LDS rows of nr + 4 floats, by all threads of the workgroup. Rows past the launch's hold zeros.
-__device__ __forceinline__ void adapter_stage(const AdapterArgs& e, const AdapterJob& j, int m0, int rows, int r0, int nr,
-                                              float* lds, int threads) {
-    const int shift = nr == 16 ? 2 : nr == 32 ? 3 : 4;  // four-rank pieces of a row
-    const int64_t left = e.rows - m0;
-    const uint32_t bytes = (uint32_t)(left < rows ? left : rows) * (uint32_t)e.low_stride * 4u;
-    for (int q = threadIdx.x; q < rows << shift; q += threads) {
-        const int row = q >> shift, c = 4 * (q & ((1 << shift) - 1));
-        const uint32_t off = r0 + c < e.low_stride ? (uint32_t)(row * e.low_stride + r0 + c) * 4u : 0xf0000000u;
-        adapter_f32x4 v = adapter_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int sh = 0; sh < e.shares; sh++)
-            v += __builtin_bit_cast(adapter_f32x4, ld4(make_rsrc(j.low + ((int64_t)sh * e.rows + m0) * e.low_stride, bytes), off));
-        *reinterpret_cast<adapter_f32x4*>(lds + row * (nr + 4) + c) = v;
+// The low-rank products of kRows (a multiple of 16) activation rows from m0 on, ranks r0 .. r0 + kRanks, their shares added: into
+// LDS rows of kRanks + 4 floats, by the kThreads threads of the workgroup. Rows past the launch's hold zeros. In two steps, so
+// that other loads can go out between: every load of the first is in flight at once (four shares at a time).
+template <int kRows, int kRanks, int kThreads>
+struct AdapterStage {
+    static constexpr int kQuads = kRows * kRanks / 4, kPer = (kQuads + kThreads - 1) / kThreads;
+    u32x4 v[kPer][4];
+
+    __device__ __forceinline__ static uint32_t offset(const AdapterArgs& e, int i, int r0) {
+        const int q = (int)threadIdx.x + kThreads * i, row = q / (kRanks / 4), c = r0 + 4 * (q % (kRanks / 4));
+        return q < kQuads && c < e.low_stride ? (uint32_t)(row * e.low_stride + c) * 4u : 0xf0000000u;
     }
-}
+    __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, int m0, int r0, int sh0 = 0) {
+        const int64_t left = e.rows - m0;
+        const uint32_t bytes = (uint32_t)(left < kRows ? left : kRows) * (uint32_t)e.low_stride * 4u;
+#pragma unroll
+        for (int sh = 0; sh < 4; sh++) {
+            const __amdgpu_buffer_rsrc_t r =
+                make_rsrc(j.low + ((int64_t)(sh0 + sh) * e.rows + m0) * e.low_stride, sh0 + sh < e.shares ? bytes : 0u);
+#pragma unroll
+            for (int i = 0; i < kPer; i++) v[i][sh] = ld4(r, offset(e, i, r0));
+        }
+    }
+    __device__ __forceinline__ void store(const AdapterArgs& e, const AdapterJob& j, int m0, int r0, float* lds) {
+        adapter_f32x4 sum[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) sum[i] = adapter_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int sh0 = 0;;) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+#pragma unroll
+                for (int sh = 0; sh < 4; sh++) sum[i] += __builtin_bit_cast(adapter_f32x4, v[i][sh]);
+            sh0 += 4;
+            if (sh0 >= e.shares) break;
+            load(e, j, m0, r0, sh0);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int q = (int)threadIdx.x + kThreads * i;
+            if (q < kQuads) *reinterpret_cast<adapter_f32x4*>(lds + q / (kRanks / 4) * (kRanks + 4) + 4 * (q % (kRanks / 4))) = sum[i];
+        }
+    }
+};
 
 // The workgroup's LDS stores before, its loads after; DMAs into LDS stay in flight.
 __device__ __forceinline__ void adapter_barrier() {
@@ -92,25 +119,30 @@ __device__ __forceinline__ uint32_t adapter_b_at(int n, int r, int steps) {
     return ((uint32_t)((n >> 4) * steps + (r >> 4)) * 64u + (uint32_t)((r & 12) << 2) + (uint32_t)(n & 15)) * 4u;
 }
 
-// sum += sum_r low[r] B[slot][n][r] over the ranks r0 .. r0 + nr of one row and output; low: the row's staged products.
-// n < j.out, row.pad() > 0.
+// sum + sum_r low[r] B[slot][n][r] over the kRanks ranks from r0 on of one row and output, r0 below the row's; low: the row's
+// staged products. All of B's values are loaded before the first is used. n < j.out.
+template <int kRanks>
 __device__ __forceinline__ float adapter_dot(const AdapterArgs& e, const AdapterJob& j, AdapterRow row, int n, const float* low,
-                                             int r0, int nr, float sum) {
-    const int pad = row.pad(), end = min(pad - r0, nr), steps = adapter_tiles16(pad);
+                                             int r0, float sum) {
+    const int end = row.pad() - r0, steps = adapter_tiles16(row.pad());
     const char* b = adapter_b(e, j, row.slot());
-    for (int r = 0; r < end; r += 4) {
-        const char* at = b + (size_t)adapter_b_at(n, r0 + r, steps) * adapter_elem(e.type);
-        u32x4 w;
+    u32x4 w[kRanks / 4];
+#pragma unroll
+    for (int q = 0; q < kRanks / 4; q++) {
+        const char* at = b + (size_t)adapter_b_at(n, 4 * q < end ? r0 + 4 * q : r0, steps) * adapter_elem(e.type);
         if (e.type == kAdapterF32) {
-            w = *reinterpret_cast<const u32x4*>(at);
+            w[q] = *reinterpret_cast<const u32x4*>(at);
         } else {
             const u32x2 v = *reinterpret_cast<const u32x2*>(at);
-            w = u32x4{v.x, v.y, 0u, 0u};
+            w[q] = u32x4{v.x, v.y, 0u, 0u};
         }
-        const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(low + r);
-        const adapter_f32x4 f = adapter_widen4(e.type, w);
+    }
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum = fmaf(l[i], f[i], sum);
+    for (int q = 0; q < kRanks / 4; q++) {
+        const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(low + 4 * q);
+        const adapter_f32x4 f = adapter_widen4(e.type, w[q]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum = 4 * q < end ? fmaf(l[i], f[i], sum) : sum;
     }
     return sum;
 }
@@ -158,8 +190,9 @@ struct AdapterTiles {
     }
 
     // out[t][c][i] += scale * (B low) for the rows that have an adapter.
-    __device__ __forceinline__ void add(const AdapterArgs& e, const AdapterJob& j, int m0, int n0, float (&out)[T][kN][4], float* lds,
-                                        int threads) const {
+    template <int kThreads>
+    __device__ __forceinline__ void add(const AdapterArgs& e, const AdapterJob& j, int m0, int n0, float (&out)[T][kN][4],
+                                        float* lds) const {
         constexpr uint32_t kAbsent = 0xf0000000u;  // past every resource: reads zeros
         constexpr int kRow = kPass + 4;
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
@@ -172,6 +205,8 @@ struct AdapterTiles {
             most = max(most, (int)(key[t] & 0xffffu));
         }
         if (!any) return;
+        AdapterStage<16 * T, kPass, kThreads> staged;
+        staged.load(e, j, m0, 0);
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
         most = __builtin_amdgcn_readfirstlane(most);
@@ -191,8 +226,11 @@ struct AdapterTiles {
 #pragma unroll
                     for (int i = 0; i < 4; i++) sum[t][c][i] = 0.0f;
             for (int r0 = 0; r0 < most; r0 += kPass) {
-                if (r0) adapter_barrier();
-                adapter_stage(e, j, m0, 16 * T, r0, kPass, lds, threads);
+                if (r0) {
+                    adapter_barrier();
+                    staged.load(e, j, m0, r0);
+                }
+                staged.store(e, j, m0, r0, lds);
                 adapter_barrier();
 #pragma unroll
                 for (int t = 0; t < T; t++)
@@ -202,9 +240,11 @@ struct AdapterTiles {
                         const AdapterRow r{(uint32_t)__shfl((int)key[t], src, 64), 0.0f};
 #pragma unroll
                         for (int c = 0; c < kN; c++)
-                            if (r.pad() > r0 && n0 + 16 * c + l16 < j.out)
-                                sum[t][c][i] = adapter_dot(e, j, r, n0 + 16 * c + l16, lds + (16 * t + src) * kRow, r0, kPass,
-                                                           sum[t][c][i]);
+                            if (r.pad() > r0 && n0 + 16 * c + l16 < j.out) {
+                                const float* low = lds + (16 * t + src) * kRow;
+                                sum[t][c][i] = most <= r0 + 16 ? adapter_dot<16>(e, j, r, n0 + 16 * c + l16, low, r0, sum[t][c][i])
+                                                               : adapter_dot<32>(e, j, r, n0 + 16 * c + l16, low, r0, sum[t][c][i]);
+                            }
                     }
             }
 #pragma unroll
@@ -246,8 +286,11 @@ struct AdapterTiles {
                                                                        (uint32_t)adapter_elem(e.type)
                                                                  : kAbsent);
                     }
-            if (r0) adapter_barrier();
-            adapter_stage(e, j, m0, 16 * T, r0, kPass, lds, threads);
+            if (r0) {
+                adapter_barrier();
+                staged.load(e, j, m0, r0);
+            }
+            staged.store(e, j, m0, r0, lds);
             adapter_barrier();
 #pragma unroll
             for (int h = 0; h < kPass / 16; h++) {

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (any >> (4 * g + i) & 1 && n0 + 16 * c + l16 < j.out) y[0][c][i] = yp[(int64_t)i * j.out + 16 * c];
-    tiles.add(a, j, m0, n0, y, low, 256);
+    tiles.add<256>(a, j, m0, n0, y, low);
 #pragma unroll
     for (int c = 0; c < kN; c++)
 #pragma unroll
@@ -302,7 +302,10 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(const T* __restrict__
 template <int kType>
 hipError_t launch_shrink(const AdapterArgs& a, const ActQuantJob& quant, hipStream_t st) {
     // quantising parts fill rows of their own behind the others, at least 64 workgroups wide
-    const int64_t parts = quant.parts(), want = parts < 64 ? parts : 64, x = a.shrink_x > want ? a.shrink_x : want;
+    const int64_t parts = quant.parts(), want = parts < 64 ? parts : 64, least = a.shrink_x > want ? a.shrink_x : want;
+    // Consecutive workgroups go to the 8 XCDs in turn. Many row tiles: a multiple of 8, so that a tile's workgroups run on one XCD
+    // and share its L2's copy of x; few: an odd number, so that they spread over all.
+    const int64_t x = a.rows > 64 ? (least + 7) / 8 * 8 : least | 1;
     const dim3 grid((unsigned)x, (unsigned)(a.groups * a.shares + (parts + x - 1) / x)), wg(64 * kShrinkWaves);
     if (a.rank_tiles == 1)
         hipLaunchKernelGGL((adapter_shrink_kernel<kType, 1>), grid, wg, 0, st, a, quant);
@@ -318,7 +321,7 @@ void plan_adapters(AdapterArgs& a, int max_rank) {
     int slots = 1;
     for (int i = 0; i < a.jobs; i++) slots = a.job[i].slots > slots ? a.job[i].slots : slots;
     const int tiles = (a.rows + 15) / 16, all = a.jobs * (a.low_stride / 16);
-    constexpr int kMostShares = 4;
+    const int kMostShares = a.rows <= 32 ? 8 : 4;
     // two rank tiles beside each other where that leaves 128 workgroups
     a.rank_tiles = all > 1 && tiles * ((all + 1) / 2) * kMostShares >= 128 ? 2 : 1;
     a.groups = (all + a.rank_tiles - 1) / a.rank_tiles;
@@ -328,9 +331,10 @@ void plan_adapters(AdapterArgs& a, int max_rank) {
     if (a.shares > most) a.shares = most;
     if (a.shares > kMostShares) a.shares = kMostShares;
     a.each = (a.in / 32 + kShrinkWaves * a.shares - 1) / (kShrinkWaves * a.shares);
-    // a workgroup for each of a tile's slots at a few rows, which may all differ; one in all at many
+    // a workgroup for each of a tile's slots at a few rows, which may all differ; two at many, for the tiles where one request
+    // ends and the next begins
     a.way_shift = 0;
-    while (a.rows <= 64 && a.way_shift < 4 && 1 << a.way_shift < slots && 1 << a.way_shift < a.rows) a.way_shift++;
+    while (a.way_shift < (a.rows <= 64 ? 4 : 1) && 1 << a.way_shift < slots && 1 << a.way_shift < a.rows) a.way_shift++;
     a.shrink_x = tiles << a.way_shift;
 }
 
