@@ -1,11 +1,9 @@
 // adapter_tile.h — B times the rows' low-rank products, for the epilogues of the projection kernels and for the launch that
 // adds adapters to finished outputs (adapters.hip). Products and sums are fp32 whatever the adapters are kept in.
 //
-// Rows share a multiplication only where they share the slot. Tiles of one or two slots (a prompt's) go over fp32 MFMA
-// (16x16x4): each slot is multiplied with the whole tile and its results go to its own rows only, by selection and not by a
-// zero factor, so that an infinity in one request's adapter stays out of the others' rows. Tiles of more slots (a decode
-// step's) go output by output: a lane loads the row of B that its output's slot names, so all loads are in flight at once,
-// where a walk over 16 slots waited for each.
+// Rows share a multiplication only where they share the slot: a tile's slots are taken in turn, each multiplied over fp32 MFMA
+// (16x16x4) with all rows of the tile, and its results go to its own rows only, by selection and not by a zero factor, so that an
+// infinity in one request's adapter stays out of the others' rows.
 #pragma once
 
 #include "ovfq_device.h"
@@ -71,9 +69,13 @@ struct AdapterStage {
         const int q = (int)threadIdx.x + kThreads * i, row = q / (kRanks / 4), c = r0 + 4 * (q % (kRanks / 4));
         return q < kQuads && c < e.low_stride ? (uint32_t)(row * e.low_stride + c) * 4u : 0xf0000000u;
     }
+    // The bytes of the products from row m0 on, 0 where m0 is past the rows: loads past them read zeros.
+    __device__ __forceinline__ static uint32_t held(const AdapterArgs& e, int m0) {
+        const int left = e.rows - m0;
+        return (uint32_t)(left < 0 ? 0 : left < kRows ? left : kRows) * (uint32_t)e.low_stride * 4u;
+    }
     __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, int m0, int r0, int sh0 = 0) {
-        const int64_t left = e.rows - m0;
-        const uint32_t bytes = (uint32_t)(left < kRows ? left : kRows) * (uint32_t)e.low_stride * 4u;
+        const uint32_t bytes = held(e, m0);
 #pragma unroll
         for (int sh = 0; sh < 4; sh++) {
             const __amdgpu_buffer_rsrc_t r =
@@ -99,6 +101,26 @@ struct AdapterStage {
         for (int i = 0; i < kPer; i++) {
             const int q = (int)threadIdx.x + kThreads * i;
             if (q < kQuads) *reinterpret_cast<adapter_f32x4*>(lds + q / (kRanks / 4) * (kRanks + 4) + 4 * (q % (kRanks / 4))) = sum[i];
+        }
+    }
+    // load() and store() in fewer registers: a quad at a time.
+    __device__ __forceinline__ static void fill(const AdapterArgs& e, const AdapterJob& j, int m0, int r0, float* lds) {
+        const uint32_t bytes = held(e, m0);
+#pragma unroll 1
+        for (int i = 0; i < kPer; i++) {
+            const int q = (int)threadIdx.x + kThreads * i;
+            adapter_f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int sh0 = 0; sh0 < e.shares; sh0 += 4) {
+                u32x4 v[4];
+#pragma unroll
+                for (int sh = 0; sh < 4; sh++)
+                    v[sh] = ld4(make_rsrc(j.low + ((int64_t)(sh0 + sh) * e.rows + m0) * e.low_stride, sh0 + sh < e.shares ? bytes : 0u),
+                                offset(e, i, r0));
+#pragma unroll
+                for (int sh = 0; sh < 4; sh++) sum += __builtin_bit_cast(adapter_f32x4, v[sh]);
+            }
+            if (q < kQuads) *reinterpret_cast<adapter_f32x4*>(lds + q / (kRanks / 4) * (kRanks + 4) + 4 * (q % (kRanks / 4))) = sum;
         }
     }
 };
@@ -149,15 +171,14 @@ __device__ __forceinline__ float adapter_dot(const AdapterArgs& e, const Adapter
 
 // The adapters' part of a wave's outputs in the MFMA result layout: T tiles of 16 rows from m0 on and kN tiles of 16 outputs
 // from n0 on, lane (g, l16) holding rows 4 g .. 4 g + 3 of output l16 of each. All waves of the workgroup share the rows and call
-// load() and add() together.
-template <int T, int kN>
+// load() and add() together. kPass: ranks staged at a time. kAhead: slots whose B values are loaded together.
+template <int T, int kN, int kPass = 32, int kAhead = 1>
 struct AdapterTiles {
     uint32_t key[T];  // of row m0 + 16 t + l16
     float scale[T];
 
     // LDS floats that add() wants
-    static constexpr int kPass = 32;  // ranks staged at a time
-    static constexpr int kLds = 16 * T * (kPass + 4);
+    static constexpr int kRow = kPass + 4, kScale = 16 * T * kRow, kLds = kScale + 16 * T;
 
     __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, int m0) {
 #pragma unroll
@@ -168,34 +189,47 @@ struct AdapterTiles {
         }
     }
 
-    // Takes the next slot out of `left`: its rows of each tile, its key and scale; no rows if none is left.
-    __device__ __forceinline__ void take(uint32_t (&left)[T], uint32_t (&rows)[T], uint32_t& k, float& s) const {
-        bool found = false;
-        k = 0;
-        s = 0.0f;
+    // Takes the next slot out of `left`: its rows of each tile, and its key; no rows and 0 if none is left.
+    __device__ __forceinline__ uint32_t take(uint32_t (&left)[T], uint32_t (&rows)[T]) const {
+        uint32_t k = 0;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            if (!k && left[t]) k = (uint32_t)__builtin_amdgcn_readlane((int)key[t], __builtin_ctz(left[t]));
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            if (!found && left[t]) {
-                const int l = __builtin_ctz(left[t]);
-                k = (uint32_t)__builtin_amdgcn_readlane((int)key[t], l);
-                s = as_float((uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint32_t, scale[t]), l));
-                found = true;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < T; t++) {
-            rows[t] = found ? (uint32_t)__ballot(key[t] == k) & left[t] : 0u;
+            rows[t] = (uint32_t)__ballot(key[t] == k) & left[t];
             left[t] &= ~rows[t];
         }
+        return k;
     }
 
-    // out[t][c][i] += scale * (B low) for the rows that have an adapter.
+    // The lane's B values of ranks r0 .. r0 + kPass and the outputs from n0 on; zeros past the slot's ranks.
+    __device__ __forceinline__ static void load_b(const AdapterArgs& e, const AdapterJob& j, uint32_t k, int n0, int r0,
+                                                  u32x4 (&raw)[kPass / 16][kN]) {
+        constexpr uint32_t kAbsent = 0xf0000000u;  // past every resource: reads zeros
+        const int lane = threadIdx.x & 63, pad = (int)(k & 0xffffu), steps = adapter_tiles16(pad);
+        const __amdgpu_buffer_rsrc_t br = make_rsrc(adapter_b(e, j, (int)(k >> 16)),
+                                                    (uint32_t)(adapter_tiles16(j.out) * steps * 256 * adapter_elem(e.type)));
+#pragma unroll
+        for (int h = 0; h < kPass / 16; h++)
+#pragma unroll
+            for (int c = 0; c < kN; c++) {
+                const int at = r0 + 16 * h + 4 * (lane >> 4);  // this lane's four ranks
+                raw[h][c] = adapter_load4(e.type, br,
+                                          at < pad ? adapter_b_at(n0 + 16 * c + (lane & 15), at, steps) * (uint32_t)adapter_elem(e.type)
+                                                   : kAbsent);
+            }
+    }
+
+    // out[t][c][i] += scale * (B low) for the rows that have an adapter. The products of all rows with a slot's B go on from the
+    // sums, and the slot's own rows keep them.
     template <int kThreads>
     __device__ __forceinline__ void add(const AdapterArgs& e, const AdapterJob& j, int m0, int n0, float (&out)[T][kN][4],
                                         float* lds) const {
-        constexpr uint32_t kAbsent = 0xf0000000u;  // past every resource: reads zeros
-        constexpr int kRow = kPass + 4;
+        using Stage = AdapterStage<16 * T, kPass, kThreads>;
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+        Stage staged;
+        staged.load(e, j, m0, 0);
         uint32_t left[T], any = 0;
         int most = 0;  // the largest padded rank
 #pragma unroll
@@ -205,127 +239,110 @@ struct AdapterTiles {
             most = max(most, (int)(key[t] & 0xffffu));
         }
         if (!any) return;
-        AdapterStage<16 * T, kPass, kThreads> staged;
-        staged.load(e, j, m0, 0);
+        uint32_t k[kAhead], rows[kAhead][T];
+        u32x4 raw[kAhead][kPass / 16][kN];
+        auto next = [&](int r0) {  // the next slots' rows, keys and B values
+#pragma unroll
+            for (int b = 0; b < kAhead; b++) {
+                k[b] = take(left, rows[b]);
+                if (k[b]) load_b(e, j, k[b], n0, r0, raw[b]);
+            }
+        };
+        next(0);
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
         most = __builtin_amdgcn_readfirstlane(most);
-        uint32_t rows[2][T], k2[2];
-        float s2[2];
-        take(left, rows[0], k2[0], s2[0]);
-        take(left, rows[1], k2[1], s2[1]);
-        any = 0;
+        staged.store(e, j, m0, 0, lds);
+        if (threadIdx.x < 16) {
 #pragma unroll
-        for (int t = 0; t < T; t++) any |= left[t];
-        if (any) {  // more than two slots: output by output
-            float sum[T][kN][4];
+            for (int t = 0; t < T; t++) lds[kScale + 16 * t + l16] = scale[t];
+        }
+        adapter_f32x4 sum[T][kN];
 #pragma unroll
-            for (int t = 0; t < T; t++)
+        for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int c = 0; c < kN; c++)
+            for (int c = 0; c < kN; c++) sum[t][c] = adapter_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int r0 = 0;;) {
+            adapter_barrier();
+#pragma unroll 1
+            while (k[0]) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sum[t][c][i] = 0.0f;
-            for (int r0 = 0; r0 < most; r0 += kPass) {
-                if (r0) {
-                    adapter_barrier();
-                    staged.load(e, j, m0, r0);
-                }
-                staged.store(e, j, m0, r0, lds);
-                adapter_barrier();
+                for (int b = 0; b < kAhead; b++) {
+                    const int ranks = (int)(k[b] & 0xffffu) - r0;
+                    if (ranks <= 0) break;  // no slot
+                    adapter_f32x4 w[kPass / 16][kN];
 #pragma unroll
-                for (int t = 0; t < T; t++)
+                    for (int h = 0; h < kPass / 16; h++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int src = 4 * g + i;
-                        const AdapterRow r{(uint32_t)__shfl((int)key[t], src, 64), 0.0f};
+                        for (int c = 0; c < kN; c++) w[h][c] = adapter_widen4(e.type, raw[b][h][c]);
+#pragma unroll
+                    for (int t = 0; t < T; t++) {
+                        if (!rows[b][t]) continue;
+                        adapter_f32x4 acc[kN];
+#pragma unroll
+                        for (int c = 0; c < kN; c++) acc[c] = sum[t][c];
+#pragma unroll
+                        for (int h = 0; h < kPass / 16; h++) {
+                            if (16 * h >= ranks) continue;
+                            const adapter_f32x4 low =
+                                *reinterpret_cast<const adapter_f32x4*>(lds + (16 * t + l16) * kRow + 16 * h + 4 * g);
+#pragma unroll
+                            for (int c = 0; c < kN; c++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[i], w[h][c][i], acc[c], 0, 0, 0);
+                        }
 #pragma unroll
                         for (int c = 0; c < kN; c++)
-                            if (r.pad() > r0 && n0 + 16 * c + l16 < j.out) {
-                                const float* low = lds + (16 * t + src) * kRow;
-                                sum[t][c][i] = most <= r0 + 16 ? adapter_dot<16>(e, j, r, n0 + 16 * c + l16, low, r0, sum[t][c][i])
-                                                               : adapter_dot<32>(e, j, r, n0 + 16 * c + l16, low, r0, sum[t][c][i]);
-                            }
-                    }
-            }
-#pragma unroll
-            for (int t = 0; t < T; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t k = (uint32_t)__shfl((int)key[t], 4 * g + i, 64);
-                    const float s = __shfl(scale[t], 4 * g + i, 64);
-#pragma unroll
-                    for (int c = 0; c < kN; c++)
-                        if (k & 0xffffu) out[t][c][i] = fmaf(sum[t][c][i], s, out[t][c][i]);
-                }
-            return;
-        }
-        adapter_f32x4 acc[2][T][kN];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int t = 0; t < T; t++)
-#pragma unroll
-                for (int c = 0; c < kN; c++) acc[b][t][c] = adapter_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int pad[2] = {(int)(k2[0] & 0xffffu), (int)(k2[1] & 0xffffu)};
-        __amdgpu_buffer_rsrc_t br[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-            br[b] = make_rsrc(adapter_b(e, j, (int)(k2[b] >> 16)),
-                              (uint32_t)(adapter_tiles16(j.out) * adapter_tiles16(pad[b]) * 256 * adapter_elem(e.type)));
-        for (int r0 = 0; r0 < most; r0 += kPass) {
-            u32x4 raw[2][kPass / 16][kN];
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int h = 0; h < kPass / 16; h++)
-#pragma unroll
-                    for (int c = 0; c < kN; c++) {
-                        const int n = n0 + 16 * c + l16, at = r0 + 16 * h + 4 * g;  // this lane's four ranks
-                        raw[b][h][c] = adapter_load4(e.type, br[b],
-                                                     at < pad[b] ? adapter_b_at(n, at, adapter_tiles16(pad[b])) *
-                                                                       (uint32_t)adapter_elem(e.type)
-                                                                 : kAbsent);
-                    }
-            if (r0) {
-                adapter_barrier();
-                staged.load(e, j, m0, r0);
-            }
-            staged.store(e, j, m0, r0, lds);
-            adapter_barrier();
-#pragma unroll
-            for (int h = 0; h < kPass / 16; h++) {
-                if (r0 + 16 * h >= most) break;
-                adapter_f32x4 low[T];
-#pragma unroll
-                for (int t = 0; t < T; t++)
-                    low[t] = *reinterpret_cast<const adapter_f32x4*>(lds + (16 * t + l16) * kRow + 16 * h + 4 * g);
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    if (r0 + 16 * h >= pad[b]) continue;
-#pragma unroll
-                    for (int c = 0; c < kN; c++) {
-                        const adapter_f32x4 w = adapter_widen4(e.type, raw[b][h][c]);
-#pragma unroll
-                        for (int t = 0; t < T; t++) {
-                            if (!rows[b][t]) continue;
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                acc[b][t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[t][i], w[i], acc[b][t][c], 0, 0, 0);
-                        }
+                                if (rows[b][t] >> (4 * g + i) & 1) sum[t][c][i] = acc[c][i];
                     }
                 }
+                next(r0);
             }
+            r0 += kPass;
+            if (r0 >= most) break;
+#pragma unroll
+            for (int t = 0; t < T; t++) left[t] = (uint32_t)__ballot((int)(key[t] & 0xffffu) > r0) & 0xffffu;
+            next(r0);
+            adapter_barrier();
+            Stage::fill(e, j, m0, r0, lds);
         }
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int t = 0; t < T; t++) {
+            const adapter_f32x4 s = *reinterpret_cast<const adapter_f32x4*>(lds + kScale + 16 * t + 4 * g);
+            const uint32_t has = (uint32_t)__ballot((key[t] & 0xffffu) != 0);
 #pragma unroll
-            for (int t = 0; t < T; t++)
+            for (int c = 0; c < kN; c++)
 #pragma unroll
-                for (int c = 0; c < kN; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (rows[b][t] >> (4 * g + i) & 1) out[t][c][i] = fmaf(acc[b][t][c][i], s2[b], out[t][c][i]);
+                for (int i = 0; i < 4; i++)
+                    if (has >> (4 * g + i) & 1) out[t][c][i] = fmaf(sum[t][c][i], s[i], out[t][c][i]);
+        }
     }
 };
+
+// add() for out[T][4] and one output tile, kBy row tiles at a time (the registers that T at once would take).
+template <int T, int kBy, int kPass, int kThreads>
+__device__ __forceinline__ void adapter_add(const AdapterArgs& e, const AdapterJob& j, int m0, int n0, float (&out)[T][4], float* lds) {
+    static_assert(T % kBy == 0, "whole groups of tiles");
+#pragma unroll
+    for (int t0 = 0; t0 < T; t0 += kBy) {
+        AdapterTiles<kBy, 1, kPass> tiles;
+        tiles.load(e, j, m0 + 16 * t0);
+        float v[kBy][1][4];
+#pragma unroll
+        for (int t = 0; t < kBy; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[t][0][i] = out[t0 + t][i];
+        if (t0) adapter_barrier();  // the last tiles' products have been read
+        tiles.template add<kThreads>(e, j, m0 + 16 * t0, n0, v, lds);
+#pragma unroll
+        for (int t = 0; t < kBy; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[t0 + t][i] = v[t][0][i];
+    }
+}
 
 }  // namespace ovfq

@@ -537,7 +537,8 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     } else if (use_gemv_rows(c, type, in, rows, count, pair_out)) {
         HIP_TRY(ovfq::launch_gemv_rows_kquant(type, jobs, count, in, rows, x, act, c->stream));
     } else if (use_tiled_mfma(c, type, jobs, count, in, rows)) {
-        HIP_TRY(ovfq::launch_project_mfma(type, jobs, count, in, rows, act, c->stream));
+        HIP_TRY(ovfq::launch_project_mfma(type, jobs, count, in, rows, act, c->stream, ad));
+        if (ad) *ad_done = true;
     } else if (small_mfma_enabled(rows) && ovfq::mfma_small_supported(type, in)) {
         // Few rows: 16-row MFMA tiles with super-block-parallel waves; a gate/up-shaped pair shares one launch.
         const bool pair = count == 2 && jobs[0].n_rows == jobs[1].n_rows;

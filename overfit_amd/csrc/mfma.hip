@@ -34,6 +34,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "adapter_tile.h"
 #include "kquant_mfma.h"
 #include "ovfq_launch.h"
 
@@ -142,8 +143,11 @@ struct PreW {
 };
 
 // ------------------------------------------------------------------------------------------ kernel
-template <class F, int NT, bool PRE, bool BH = false, bool GRP = false>
-__global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditional_t<GRP, MGroupArgs, MArgs> a) {
+// AD: AdapterArgs, and the rows' adapters are added to the outputs, or NoAdapters (in this kernel and the next three).
+template <class F, int NT, bool PRE, bool BH = false, bool GRP = false, class AD = NoAdapters>
+__global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditional_t<GRP, MGroupArgs, MArgs> a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    static_assert(!(kAd && GRP), "adapters are beside dense projections");
     static_assert(!(PRE && GRP), "grouped launches read the GGUF operands");
     constexpr int kSub = NT / 16;
     constexpr int kDma = NT / 16;  // 1 KiB (4-row) activation DMA chunks per wave per super-block
@@ -170,6 +174,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditio
     const float* bias = nullptr;
     float* y;
     int n_out, o0, n0, m_valid;
+    [[maybe_unused]] int job = 0;
     int pbeg = 0;  // grouped: the expert's first pair (output row of tile row 0 is pbeg + n0)
     if constexpr (GRP) {
         if (n_tile >= a.grp.tile_count[0]) return;
@@ -188,6 +193,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditio
 #pragma unroll
         for (int t = 1; t < kMaxJobs; t++)
             if (t < a.njobs && o_tile >= a.job[t].tile0) j = t;
+        job = j;
         wptr = a.job[j].w;
         preptr = a.job[j].pre;
         bias = a.job[j].bias;
@@ -417,8 +423,20 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditio
 
     // y[n][o] = biasO + sum   (RT/Q4KDotKernel.cs:951, RT/Q6KDotKernel.cs:507); grouped: output row pbeg + n
     const int o = o0 + r16;
+    float bias_o = bias && o < n_out ? bias[o] : 0.0f;
+    if constexpr (kAd) {
+        const AdapterJob aj = adapter_job(ad, job);
+        if (aj.slots) {
+#pragma unroll
+            for (int s = 0; s < kSub; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
+            bias_o = 0.0f;
+            static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act), "staged products");
+            adapter_add<kSub, 2, 32, 256>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
+        }
+    }
     if (o >= n_out) return;
-    const float bias_o = bias ? bias[o] : 0.0f;
 #pragma unroll
     for (int s = 0; s < kSub; s++)
 #pragma unroll
@@ -438,8 +456,9 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditio
 // are built (the pair's activation DMA in flight), a wait and a barrier publish the slots, the next pair's weights
 // are loaded, the MFMAs and tails run, a barrier frees both slots and publishes the odd values, the next pair's DMA is
 // issued, and the even wave adds the odd values.
-template <class F, bool BH>
-__global__ __launch_bounds__(512) void kquant_mfma_pair_kernel(const MArgs a) {
+template <class F, bool BH, class AD>
+__global__ __launch_bounds__(512) void kquant_mfma_pair_kernel(const MArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
     constexpr int NT = 64;
     constexpr int kSub = NT / 16;
     constexpr bool kMinF16 = F::kNumMfma == 3;
@@ -596,8 +615,20 @@ __global__ __launch_bounds__(512) void kquant_mfma_pair_kernel(const MArgs a) {
 
     // y[n][o] = biasO + sum   (RT/Q4KDotKernel.cs:951, RT/Q6KDotKernel.cs:507): the even waves hold the sums
     const int o = o0 + r16;
+    float bias_o = bias && o < n_out ? bias[o] : 0.0f;
+    if constexpr (kAd) {
+        const AdapterJob aj = adapter_job(ad, j);
+        if (aj.slots) {  // (the odd waves help to stage the products)
+#pragma unroll
+            for (int s = 0; s < kSub; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
+            bias_o = 0.0f;
+            static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act), "staged products");
+            adapter_add<kSub, 2, 32, 512>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
+        }
+    }
     if (par != 0 || o >= n_out) return;
-    const float bias_o = bias ? bias[o] : 0.0f;
 #pragma unroll
     for (int s = 0; s < kSub; s++)
 #pragma unroll
@@ -617,8 +648,9 @@ __global__ __launch_bounds__(512) void kquant_mfma_pair_kernel(const MArgs a) {
 // even waves add the odd values and compute the second half; a barrier; the even waves add the odd second-half
 // values. Each (row, output) is summed in ascending super-block order. The code is specialised per parity so that
 // every slot a wave reads or DMAs is a fixed LDS object (see the wide kernel).
-template <class F, bool BH>
-__global__ __launch_bounds__(512) void kquant_mfma_pairwide_kernel(const MArgs a) {
+template <class F, bool BH, class AD>
+__global__ __launch_bounds__(512) void kquant_mfma_pairwide_kernel(const MArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
     constexpr int NH = 64;
     constexpr int kSubH = NH / 16;
     constexpr bool kMinF16 = F::kNumMfma == 3;
@@ -814,8 +846,20 @@ __global__ __launch_bounds__(512) void kquant_mfma_pairwide_kernel(const MArgs a
 
     // y[n][o] = biasO + sum   (RT/Q4KDotKernel.cs:951, RT/Q6KDotKernel.cs:507): the even waves hold the sums
     const int o = o0 + r16;
+    float bias_o = bias && o < n_out ? bias[o] : 0.0f;
+    if constexpr (kAd) {
+        const AdapterJob aj = adapter_job(ad, j);
+        if (aj.slots) {  // (the odd waves help to stage the products)
+#pragma unroll
+            for (int s = 0; s < 2 * kSubH; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
+            bias_o = 0.0f;
+            static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act00), "staged products");
+            adapter_add<2 * kSubH, 2, 32, 512>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act00));
+        }
+    }
     if (par != 0 || o >= n_out) return;
-    const float bias_o = bias ? bias[o] : 0.0f;
 #pragma unroll
     for (int s = 0; s < 2 * kSubH; s++)
 #pragma unroll
@@ -834,8 +878,9 @@ __global__ __launch_bounds__(512) void kquant_mfma_pairwide_kernel(const MArgs a
 // computed; a barrier; the DMA of the next super-block's first half is issued into the slot the first half has left,
 // and the second half is computed; a barrier. BH: the activation's bsums are fp16 (the quantiser's second bsum
 // plane), read as the min MFMA's A operand without conversion.
-template <class F, bool BH>
-__global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a) {
+template <class F, bool BH, class AD>
+__global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
     constexpr int NH = 64;          // activation rows per half
     constexpr int kSubH = NH / 16;  // sub-tiles per half
     constexpr int kDma = NH / 16;   // 1 KiB DMA chunks per wave per half
@@ -998,8 +1043,23 @@ __global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a)
 
     // y[n][o] = biasO + sum   (RT/Q4KDotKernel.cs:951, RT/Q6KDotKernel.cs:507)
     const int o = o0 + r16;
+    float bias_o = bias && o < n_out ? bias[o] : 0.0f;
+    if constexpr (kAd) {
+        const AdapterJob aj = adapter_job(ad, j);
+        if (aj.slots) {
+#pragma unroll
+            for (int s = 0; s < 2 * kSubH; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
+            bias_o = 0.0f;
+            // All eight row tiles at once, so that their loads are one latency, and 16 ranks at a time, which fits the registers
+            // (gate/up at 512 rows, 512 x 4096 -> 2 x 14336 of Q4_K and ranks to 16: 184 us for the call, the projection alone 157,
+            // four tiles of 32 ranks 186, two 189; with a launch of their own behind the projection the adapters cost 54).
+            static_assert(AdapterTiles<8, 1, 16>::kLds * 4 <= (int)sizeof(act0), "staged products");
+            adapter_add<2 * kSubH, 8, 16, 256>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act0));
+        }
+    }
     if (o >= n_out) return;
-    const float bias_o = bias ? bias[o] : 0.0f;
 #pragma unroll
     for (int s = 0; s < 2 * kSubH; s++)
 #pragma unroll
@@ -1009,22 +1069,26 @@ __global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a)
         }
 }
 
-template <class F, int NT>
-static hipError_t launch_mfma(MArgs& ma, bool pre, hipStream_t st) {
+template <class F, int NT, class AD>
+static hipError_t launch_mfma(MArgs& ma, bool pre, const AD& ad, hipStream_t st) {
     ma.n_tiles = (ma.m_rows + NT - 1) / NT;
     const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
     if constexpr (F::kNumMfma == 2) {  // only Q6_K weights carry the MFMA-ready copy
         if (pre) {
-            hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, true>), dim3(grid), dim3(256), 0, st, ma);
+            hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, true, false, false, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
             return hipGetLastError();
         }
     } else {
         if (ma.bh) {  // Q4_K with the quantiser's fp16 bsums
-            hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, false, true>), dim3(grid), dim3(256), 0, st, ma);
+            hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, false, true, false, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
             return hipGetLastError();
         }
     }
-    hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, false>), dim3(grid), dim3(256), 0, st, ma);
+    // (the quantiser always writes those for a projection with adapters)
+    if constexpr (F::kNumMfma == 3 && std::is_same_v<AD, AdapterArgs>)
+        return hipErrorInvalidValue;
+    else
+        hipLaunchKernelGGL((kquant_mfma_kernel<F, NT, false, false, false, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
     return hipGetLastError();
 }
 
@@ -1096,9 +1160,9 @@ hipError_t launch_mfma_grouped_tiled(int type, const GroupLaunch& L, const int* 
     const dim3 grid((ma.o_tiles + 7) / 8 * 8 * max_tiles);
     constexpr int NT = kGroupedTileRows;
     if (type == 12)
-        hipLaunchKernelGGL((kquant_mfma_kernel<Q4KMfma, NT, false, false, true>), grid, dim3(256), 0, st, ma);
+        hipLaunchKernelGGL((kquant_mfma_kernel<Q4KMfma, NT, false, false, true>), grid, dim3(256), 0, st, ma, NoAdapters{});
     else
-        hipLaunchKernelGGL((kquant_mfma_kernel<Q6KMfma, NT, false, false, true>), grid, dim3(256), 0, st, ma);
+        hipLaunchKernelGGL((kquant_mfma_kernel<Q6KMfma, NT, false, false, true>), grid, dim3(256), 0, st, ma, NoAdapters{});
     return hipGetLastError();
 }
 
@@ -1122,8 +1186,52 @@ bool mfma_tiled_preferred(int type, int rows, int o_tiles, long out_rows) {
     return type != 14 || (long)rows * out_rows >= 448L * 1024;
 }
 
-hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                               hipStream_t st) {
+// The tiled kernels by their tile; with adapters a Q4_K launch has the fp16 bsums, and the wide kernel is Q4_K's.
+template <class AD>
+static hipError_t launch_mfma_tiles(int type, MArgs& ma, bool pre, const AD& ad, hipStream_t st) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    const int rows = ma.m_rows, nt = mfma_tile_rows(type, rows, ma.o_tiles);
+    if (kAd && type == 12 && !ma.bh) return hipErrorInvalidValue;
+    if (nt == kPairWideTile && !pre) {
+        ma.n_tiles = (rows + 127) / 128;
+        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
+        if (type == 12 && ma.bh)
+            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q4KMfma, true, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        else if (type != 12)
+            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q6KMfma, false, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        else if constexpr (!kAd)
+            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q4KMfma, false, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        return hipGetLastError();
+    }
+    if (nt == kPairTile && !pre) {
+        ma.n_tiles = (rows + 63) / 64;
+        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
+        if (type == 12 && ma.bh)
+            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q4KMfma, true, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        else if (type != 12)
+            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q6KMfma, false, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        else if constexpr (!kAd)
+            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q4KMfma, false, AD>), dim3(grid), dim3(512), 0, st, ma, ad);
+        return hipGetLastError();
+    }
+    if (nt == kWideTile && !pre) {
+        ma.n_tiles = (rows + 127) / 128;
+        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
+        if (type == 12 && ma.bh)
+            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q4KMfma, true, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
+        else if (type != 12)
+            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q6KMfma, false, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
+        else if constexpr (!kAd)
+            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q4KMfma, false, AD>), dim3(grid), dim3(256), 0, st, ma, ad);
+        return hipGetLastError();
+    }
+    if (type == 12)
+        return nt == 128 ? launch_mfma<Q4KMfma, 128>(ma, pre, ad, st) : launch_mfma<Q4KMfma, 64>(ma, pre, ad, st);
+    return nt == 128 ? launch_mfma<Q6KMfma, 128>(ma, pre, ad, st) : launch_mfma<Q6KMfma, 64>(ma, pre, ad, st);
+}
+
+hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                               const AdapterArgs* ad) {
     MArgs ma{};
     int tiles = 0;
     bool pre = true;  // the prepared variant when every weight of the launch has its MFMA-ready copy
@@ -1141,43 +1249,7 @@ hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in,
     ma.b = act.b;
     ma.bh = type == 12 ? act.bh : nullptr;
     if (type == 12 && !ma.b) return hipErrorInvalidValue;  // the Q4_K kernel reads the bsums
-    const int nt = mfma_tile_rows(type, rows, tiles);
-    if (nt == kPairWideTile && !pre) {
-        ma.n_tiles = (rows + 127) / 128;
-        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
-        if (type == 12 && ma.bh)
-            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q4KMfma, true>), dim3(grid), dim3(512), 0, st, ma);
-        else if (type == 12)
-            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q4KMfma, false>), dim3(grid), dim3(512), 0, st, ma);
-        else
-            hipLaunchKernelGGL((kquant_mfma_pairwide_kernel<Q6KMfma, false>), dim3(grid), dim3(512), 0, st, ma);
-        return hipGetLastError();
-    }
-    if (nt == kPairTile && !pre) {
-        ma.n_tiles = (rows + 63) / 64;
-        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
-        if (type == 12 && ma.bh)
-            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q4KMfma, true>), dim3(grid), dim3(512), 0, st, ma);
-        else if (type == 12)
-            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q4KMfma, false>), dim3(grid), dim3(512), 0, st, ma);
-        else
-            hipLaunchKernelGGL((kquant_mfma_pair_kernel<Q6KMfma, false>), dim3(grid), dim3(512), 0, st, ma);
-        return hipGetLastError();
-    }
-    if (nt == kWideTile && !pre) {
-        ma.n_tiles = (rows + 127) / 128;
-        const int grid = (ma.o_tiles + 7) / 8 * 8 * ma.n_tiles;
-        if (type == 12 && ma.bh)
-            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q4KMfma, true>), dim3(grid), dim3(256), 0, st, ma);
-        else if (type == 12)
-            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q4KMfma, false>), dim3(grid), dim3(256), 0, st, ma);
-        else
-            hipLaunchKernelGGL((kquant_mfma_wide_kernel<Q6KMfma, false>), dim3(grid), dim3(256), 0, st, ma);
-        return hipGetLastError();
-    }
-    if (type == 12)
-        return nt == 128 ? launch_mfma<Q4KMfma, 128>(ma, pre, st) : launch_mfma<Q4KMfma, 64>(ma, pre, st);
-    return nt == 128 ? launch_mfma<Q6KMfma, 128>(ma, pre, st) : launch_mfma<Q6KMfma, 64>(ma, pre, st);
+    return ad ? launch_mfma_tiles(type, ma, pre, *ad, st) : launch_mfma_tiles(type, ma, pre, NoAdapters{}, st);
 }
 
 // The 16 x 16 fp32 values of one super-block for the small-M kernel: MFMAs over the four 64-element chunks (A

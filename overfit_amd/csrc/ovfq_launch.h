@@ -68,8 +68,8 @@ bool mfma_supported(int type);
 bool mfma_tiled_preferred(int type, int rows, int o_tiles, long out_rows);
 // Rows from which the tiled kernel runs where the small-M kernel cannot (input sizes past 16384).
 constexpr int kMfmaMinRows = 32;
-hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act,
-                               hipStream_t st);
+hipError_t launch_project_mfma(int type, const ProjJob* jobs, int njobs, int in, int rows, ActQ act, hipStream_t st,
+                               const AdapterArgs* ad = nullptr);
 // Batched K-quant projections from operand-ordered planes (act.tiled), any rows and K, bit-identical to
 // launch_project_kquant (mfma_split.hip): the split kernel divides the contraction over the waves of a workgroup, the panel
 // kernel walks it with 64 weight rows a workgroup. mid_kernel: the automatic choice (mid_choice) for `rows` activation rows
