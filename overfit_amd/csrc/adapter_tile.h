@@ -345,4 +345,185 @@ __device__ __forceinline__ void adapter_add(const AdapterArgs& e, const AdapterJ
     }
 }
 
+// The adapters' part of a workgroup's 16 T rows x 16 outputs, its 64 W threads each taking the outputs threadIdx.x + 64 W i: output
+// (idx >> 4) & 15 of row (idx >> 8) * 16 + (idx & 15). Every output loads the row of B that its slot names, so that all loads are in
+// flight at once, however many slots the rows have. kLowPass: ranks staged at a time.
+template <int T, int W, int kLowPass>
+struct AdapterOuts {
+    static constexpr int kOuts = 256 * T, kPer = kOuts > 64 * W ? kOuts / (64 * W) : 1;
+    static constexpr int kLds = 16 * T * (kLowPass + 4);  // floats of `staged`
+    AdapterTiles<T, 1> rows;
+    AdapterStage<16 * T, kLowPass, 64 * W> stage;
+
+    __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, int m0) {
+        rows.load(e, j, m0);
+        stage.load(e, j, m0, 0);
+    }
+
+    // Leaves the thread's parts in out[idx] and returns which of its outputs have one. All waves; `staged` is free again after.
+    __device__ __forceinline__ uint32_t part(const AdapterArgs& e, const AdapterJob& j, int m0, int o0, float* staged, float* out) {
+        AdapterRow row[kPer];
+        float sum[kPer];
+        int most = 0;  // the largest padded rank of the workgroup's rows, the same for every wave
+#pragma unroll
+        for (int t = 0; t < T; t++) most = max(most, (int)(rows.key[t] & 0xffffu));
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
+        most = __builtin_amdgcn_readfirstlane(most);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {  // (a wave's outputs are of one row tile)
+            const int idx = (int)threadIdx.x + 64 * W * i;
+            row[i] = AdapterRow{0, 0.0f};
+#pragma unroll
+            for (int t = 0; t < T; t++)
+                if ((wave_id() + W * i) >> 2 == t) row[i] = AdapterRow{rows.key[t], rows.scale[t]};
+            if (o0 + ((idx >> 4) & 15) >= j.out) row[i].key = 0;
+            sum[i] = 0.0f;
+        }
+        for (int r0 = 0; r0 < most; r0 += kLowPass) {
+            if (r0) {
+                adapter_barrier();
+                stage.load(e, j, m0, r0);
+            }
+            stage.store(e, j, m0, r0, staged);
+            adapter_barrier();
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int idx = (int)threadIdx.x + 64 * W * i, n = o0 + ((idx >> 4) & 15);
+                const float* low = staged + ((idx >> 8) * 16 + (idx & 15)) * (kLowPass + 4);
+#pragma unroll
+                for (int h = 0; h < kLowPass; h += 32) {
+                    if (r0 + h >= most) break;  // the same for every wave
+                    if (row[i].pad() > r0 + h)
+                        sum[i] = most <= r0 + h + 16 ? adapter_dot<16>(e, j, row[i], n, low + h, r0 + h, sum[i])
+                                                     : adapter_dot<32>(e, j, row[i], n, low + h, r0 + h, sum[i]);
+                }
+            }
+        }
+        if (most) adapter_barrier();
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (!row[i].pad()) continue;
+            out[(int)threadIdx.x + 64 * W * i] = sum[i] * row[i].scale;
+            mine |= 1u << i;
+        }
+        return mine;
+    }
+};
+
+// The adapters' part of a decode kernel's outputs: output oi of a wave's item (weight row n, activation row m) has the L lanes
+// from L oi on, each with every L-th quad of the ranks. The rows' adapters are loaded at the start, a lane's first P quads of B
+// beside the item's weights; the launch's low-rank products wait in LDS, [job][row][low_stride].
+template <int L, int P, int kThreads>
+struct AdapterLanes {
+    uint32_t key[kMaxJobs];  // of the lane's activation row
+    float scale[kMaxJobs];
+    u32x4 part[8];  // a quad of the products, its shares
+
+    struct Item {
+        u32x4 b[P];
+    };
+
+    __device__ __forceinline__ void load_products(const AdapterArgs& e, int f) {
+        const int quads = e.rows * e.low_stride / 4;  // of a job and share; the jobs' planes are one behind the other
+        int j = 0;
+#pragma unroll
+        for (int i = 1; i < kMaxJobs; i++) j += f >= i * quads;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(e.job[0].low, (uint32_t)(e.jobs * e.shares * quads) * 16u);
+#pragma unroll
+        for (int sh = 0; sh < 8; sh++)
+            part[sh] = ld4(r, sh < e.shares && f < e.jobs * quads ? (uint32_t)((j * (e.shares - 1) + sh) * quads + f) * 16u : 0xf0000000u);
+    }
+    // m: the lane's activation row
+    __device__ __forceinline__ void load(const AdapterArgs& e, int m) {
+#pragma unroll
+        for (int j = 0; j < kMaxJobs; j++) {
+            const bool any = j < e.jobs && e.job[j].slots;
+            const u32x2 v = ld2(make_rsrc(any ? (const void*)e.job[j].row : (const void*)e.x, any ? (uint32_t)e.rows * 8u : 0u),
+                                (uint32_t)m * 8u);
+            const uint32_t s = v.y;
+            key[j] = v.x;
+            scale[j] = as_float(s);
+        }
+        load_products(e, (int)threadIdx.x);
+    }
+    // The products into LDS; the workgroup's barrier comes after.
+    __device__ __forceinline__ void stage(const AdapterArgs& e, float* low) {
+        const int quads = e.jobs * e.rows * e.low_stride / 4;
+        for (int f = (int)threadIdx.x;;) {
+            adapter_f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int sh = 0; sh < 8; sh++) sum += __builtin_bit_cast(adapter_f32x4, part[sh]);
+            if (f < quads) *reinterpret_cast<adapter_f32x4*>(low + 4 * f) = sum;
+            f += kThreads;
+            if (f - (int)threadIdx.x >= quads) break;  // the same for every thread
+            load_products(e, f);
+        }
+    }
+
+    __device__ __forceinline__ uint32_t key_of(int job) const {
+        uint32_t k = key[0];
+#pragma unroll
+        for (int i = 1; i < kMaxJobs; i++) k = job == i ? key[i] : k;
+        return k;
+    }
+    // Where the lane's quad q of output n lies in the B of slot `k`; a quad that is not there reads some of x, unused.
+    __device__ __forceinline__ static u32x4 quad(const AdapterArgs& e, const AdapterJob& j, uint32_t k, int n, int q, bool want) {
+        const int pad = (int)(k & 0xffffu);
+        const bool there = want && 4 * q < pad;
+        const char* at = there ? adapter_b(e, j, (int)(k >> 16)) + (size_t)adapter_b_at(n, 4 * q, adapter_tiles16(pad)) * adapter_elem(e.type)
+                               : reinterpret_cast<const char*>(e.x);
+        if (e.type == kAdapterF32) return *reinterpret_cast<const u32x4*>(at);
+        const u32x2 v = *reinterpret_cast<const u32x2*>(at);
+        return u32x4{v.x, v.y, 0u, 0u};
+    }
+    // Issues the loads of the lane's output n of weight `job`; always as many, so that the waits before them count on.
+    __device__ __forceinline__ void fetch(const AdapterArgs& e, int job, int n, bool want, Item& it) const {
+        const AdapterJob j = adapter_job(e, job);
+        const uint32_t k = key_of(job);
+        const int sub = (int)(threadIdx.x % L);
+#pragma unroll
+        for (int p = 0; p < P; p++) it.b[p] = quad(e, j, k, n, sub + L * p, want && n < j.out);
+    }
+    // y += scale * (B low) for output `lane` of the item; n, m: of the output that the lane works for.
+    __device__ __forceinline__ void add(const AdapterArgs& e, int job, int n, int m, const Item& it, const float* low, float& y) const {
+        const AdapterJob j = adapter_job(e, job);
+        const uint32_t k = key_of(job);
+        const int pad = (int)(k & 0xffffu), sub = (int)(threadIdx.x % L);
+        const bool live = pad && m < e.rows && n < j.out;
+        const float* mine = low + (size_t)(job * e.rows + (live ? m : 0)) * e.low_stride;
+        float sum = 0.0f;
+        auto more = [&](int q, u32x4 raw) {
+            if (!live || 4 * q >= pad) return;
+            const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(mine + 4 * q);
+            const adapter_f32x4 w = adapter_widen4(e.type, raw);
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum = fmaf(l[i], w[i], sum);
+        };
+#pragma unroll
+        for (int p = 0; p < P; p++) more(sub + L * p, it.b[p]);
+        for (int q0 = L * P; q0 < adapter_tiles16(j.max_rank) * 4; q0 += 4 * L) {
+            u32x4 raw[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++) raw[p] = quad(e, j, k, n, q0 + sub + L * p, live);
+#pragma unroll
+            for (int p = 0; p < 4; p++) more(q0 + sub + L * p, raw[p]);
+        }
+#pragma unroll
+        for (int off = L / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        float s = scale[0];
+#pragma unroll
+        for (int i = 1; i < kMaxJobs; i++) s = job == i ? scale[i] : s;
+        const int lane = (int)(threadIdx.x & 63), src = lane * L & 63;
+        const float delta = __shfl(sum * s, src, 64);
+        const bool has = __shfl((int)live, src, 64) != 0;
+        if (has) y += delta;
+    }
+};
+
+// The LDS that AdapterLanes' products take, and whether it is left beside `lds` bytes of the kernel's own.
+inline size_t adapter_lanes_lds(const AdapterArgs& e) { return (size_t)e.jobs * e.rows * e.low_stride * 4; }
+inline bool adapter_lanes_fit(const AdapterArgs& e, size_t lds) { return e.shares <= 8 && lds + adapter_lanes_lds(e) <= 65536; }
+
 }  // namespace ovfq

@@ -486,14 +486,27 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     const int pair_out = count == 2 && ws[0]->out == ws[1]->out ? ws[0]->out : 0;
     if (x && rows > 1 && !use_gemv_rows(c, type, in, rows, count, pair_out))
         return fail(OVFQ_ERR_SIZE, "in-launch quantisation of %d rows needs the multi-row decode kernel", rows);
+    // the adapters, for a kernel that adds them where `fits` says so
+    auto in_epilogue = [&](bool (*fits)(int, int, const ovfq::AdapterArgs&)) -> const ovfq::AdapterArgs* {
+        if (!ad || !fits(in, rows, *ad)) return nullptr;
+        *ad_done = true;
+        return ad;
+    };
     // Every kernel below reads either the fp32 input (decode kernels that quantise it) or the quantised activation.
     if (!x && (!act.q || !act.s)) return fail(OVFQ_ERR_NULL, "projection launch without a quantised activation");
     if (act.tiled && type == OVFQ_TYPE_Q8_0) {
         for (int i = 0; i < count; i++) {
             const int8_t* wq = reinterpret_cast<const int8_t*>(jobs[i].w);
+            ovfq::AdapterArgs one{};  // this weight's adapters
+            if (ad) {
+                one = *ad;
+                one.job[0] = ad->job[i];
+                one.jobs = 1;
+            }
             HIP_TRY(ovfq::launch_q8_0_mid(&wq, &jobs[i].ws, 1, false, in, jobs[i].n_rows, rows, jobs[i].bias, act.q, act.s,
-                                          jobs[i].y, c->stream));
+                                          jobs[i].y, c->stream, ad && ad->job[i].slots ? &one : nullptr));
         }
+        if (ad) *ad_done = true;
     } else if (act.tiled) {
         if (use_mid(c, in, rows, ws, count) == ovfq::MidKernel::kPanel)
             HIP_TRY(ovfq::launch_project_panel(type, jobs, count, in, rows, act, c->stream, ad));
@@ -527,15 +540,16 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
         const bool q8_rows = gemv_enabled() && ovfq::q8_0_gemv_rows_supported(in, rows) && (rows == 1 || q8_choice);
         if (x && !q8_rows) return fail(OVFQ_ERR_SIZE, "in-launch Q8_0 quantisation needs the decode kernel");
         if (q8_rows)
-            HIP_TRY(ovfq::launch_q8_0_gemv(jobs, count, in, rows, x, act, c->stream));
+            HIP_TRY(ovfq::launch_q8_0_gemv(jobs, count, in, rows, x, act, c->stream, in_epilogue(ovfq::q8_0_gemv_adapters)));
         else if (q8_mfma && ovfq::q8_0_mfma_supported(in, rows))
             HIP_TRY(ovfq::launch_project_q8_0_mfma(jobs, count, in, rows, act, c->stream));
         else
             HIP_TRY(ovfq::launch_project_q8_0(jobs, count, in, rows, act, c->stream));
     } else if (rows == 1 && gemv_enabled() && ovfq::gemv_supported(in)) {
-        HIP_TRY(ovfq::launch_gemv_kquant(type, jobs, count, in, x, act, c->stream));
+        HIP_TRY(ovfq::launch_gemv_kquant(type, jobs, count, in, x, act, c->stream, ad));
+        if (ad) *ad_done = true;
     } else if (use_gemv_rows(c, type, in, rows, count, pair_out)) {
-        HIP_TRY(ovfq::launch_gemv_rows_kquant(type, jobs, count, in, rows, x, act, c->stream));
+        HIP_TRY(ovfq::launch_gemv_rows_kquant(type, jobs, count, in, rows, x, act, c->stream, in_epilogue(ovfq::gemv_rows_adapters)));
     } else if (use_tiled_mfma(c, type, jobs, count, in, rows)) {
         HIP_TRY(ovfq::launch_project_mfma(type, jobs, count, in, rows, act, c->stream, ad));
         if (ad) *ad_done = true;
@@ -1113,10 +1127,13 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     int* slots_d = ad ? const_cast<int*>(ad->row_slots) : nullptr;
     if (ad) {
         auto carve = [&](Carver& c) {  // the rows' adapters and products for each set, and the staged slots of a host call
-            for (int i = 0; i < count; i++) {
-                if (!aa.job[i].slots) continue;
-                aa.job[i].row = c.take<ovfq::AdapterRow>((size_t)rows * sizeof(ovfq::AdapterRow));
-                aa.job[i].low = c.take<float>((size_t)aa.shares * rows * aa.low_stride * 4);
+            const size_t plane = (size_t)aa.shares * rows * aa.low_stride;
+            if (any_set) {  // (the weights without a set have a plane too: the decode kernels read all of them in one)
+                float* low = c.take<float>(count * plane * 4);
+                for (int i = 0; i < count; i++) {
+                    aa.job[i].low = low + i * plane;
+                    if (aa.job[i].slots) aa.job[i].row = c.take<ovfq::AdapterRow>((size_t)rows * sizeof(ovfq::AdapterRow));
+                }
             }
             if (host) slots_d = c.take<int>((size_t)rows * 4);
         };

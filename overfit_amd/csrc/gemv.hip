@@ -17,6 +17,7 @@
 #include <cstdlib>
 #include <type_traits>
 
+#include "adapter_tile.h"
 #include "kquant_blocks.h"
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
@@ -141,8 +142,11 @@ __device__ __forceinline__ void stage_activation(const GArgs& a, uint8_t* lq, in
 
 // kMulti: the launch has several jobs (fused projections); with one, no job lookup is needed. W: waves per
 // workgroup (the activation prologue is paid once per workgroup, its quantisation spread over the W waves).
-template <class F, int R, bool kMulti, int W>
-__global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
+// AD: AdapterArgs, and the row's adapter is added to the outputs, or NoAdapters.
+template <class F, int R, bool kMulti, int W, class AD>
+__global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    using Lanes = AdapterLanes<64 / R, 1, 64 * W>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int spr = a.spr;
     uint8_t* lq = smem;
@@ -157,13 +161,20 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
     const int total = a.total_groups;
     const uint32_t row_bytes = (uint32_t)spr * F::kBytes;
     float* rw = red + wave * R * kRedStride;
+    [[maybe_unused]] float* low = red + W * R * kRedStride;
+    [[maybe_unused]] Lanes lanes;
+    if constexpr (kAd) lanes.load(ad, 0);
 
     // One work item = (row group g, 16-block chunk c): the weights of R rows plus, on a row group's last chunk,
-    // the bias of those rows.
-    struct Item {
+    // the bias of those rows and their adapters' values.
+    struct Plain {
         typename F::W w[R];
         uint32_t bias;
     };
+    struct Adapted : Plain {
+        typename Lanes::Item ad;
+    };
+    using Item = std::conditional_t<kAd, Adapted, Plain>;
 
     // Job fields and first row of row group g (wave-uniform). Every job field is read with a compile-time index
     // and chosen by select, so the table stays in scalar registers: indexing it with a run-time job number would
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
     // the same whether or not the item exists (past the end the resources have zero length, so the loads return 0
     // without touching memory): the compiler's wait counts then see a fixed number of younger loads and the prefetch
     // overlaps the current item's math.
-    auto load_item = [&](const Cur& jb, const WRes& wr, int c, bool valid, Item& it) {
+    auto load_item = [&](const Cur& jb, const WRes& wr, int c, bool valid, Item& it, [[maybe_unused]] int job) {
         const int row0 = jb.row0;
         const uint32_t sb = (uint32_t)(c * 16 + q);
 #pragma unroll
@@ -225,6 +236,16 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
         const uint32_t bbytes = (uint32_t)__builtin_amdgcn_readfirstlane(want_bias ? jb.n_rows * 4 : 0);
         const __amdgpu_buffer_rsrc_t bsr = make_rsrc(bias, bbytes);
         it.bias = ld1(bsr, (uint32_t)(row0 + (lane < R ? lane : 0)) * 4);
+        if constexpr (kAd) lanes.fetch(ad, job, row0 + lane / (64 / R), valid && c == nchunks - 1, it.ad);
+    };
+    // the job of row group g
+    auto job_of = [&](int g) {
+        int j = 0;
+        if constexpr (kAd && kMulti) {
+#pragma unroll
+            for (int i = 1; i < kMaxJobs; i++) j += i < a.njobs && g >= a.job[i].g_begin;
+        }
+        return j;
     };
 
     int g = blockIdx.x * W + wave;
@@ -234,8 +255,9 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
     // weights, bound the start of the first item).
     stage_activation<F, W>(a, lq, lb, ls, wave, lane, [&] {
         const Cur c0 = locate(g < total ? g : 0);
-        load_item(c0, bind(c0, g < total), 0, g < total, ia);
+        load_item(c0, bind(c0, g < total), 0, g < total, ia, job_of(g < total ? g : 0));
     });
+    if constexpr (kAd) lanes.stage(ad, low);
     __syncthreads();
     if (g >= total) return;
     Cur cj = locate(g);  // job record of row group g, looked up once per row group
@@ -258,7 +280,7 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
             nj = locate(more ? ng : 0);
             nw = bind(nj, more);
         }
-        load_item(nj, nw, nc, more, nxt);
+        load_item(nj, nw, nc, more, nxt, job_of(more ? ng : 0));
         const int sb = c * 16 + q;
         const bool live = sb < spr;
         if (c != a_chunk) {
@@ -274,8 +296,12 @@ __global__ __launch_bounds__(64 * W) void kquant_gemv_kernel(const GArgs a) {
         if (lane < R) acc = ordered_item_sum(acc, rw + lane * kRedStride);
         wave_sync();
         if (c == nchunks - 1) {
-            if (lane < R && cj.row0 + lane < cj.n_rows) {
-                // bias[o] + sum (RT/Q4KDotKernel.cs:473); no add at all without a bias
+            // bias[o] + sum (RT/Q4KDotKernel.cs:473); no add at all without a bias
+            if constexpr (kAd) {
+                float v = cj.bias ? as_float(cur.bias) + acc : acc;
+                lanes.add(ad, job_of(g), cj.row0 + lane / (64 / R), 0, cur.ad, low, v);
+                if (lane < R && cj.row0 + lane < cj.n_rows) cj.y[cj.row0 + lane] = v;
+            } else if (lane < R && cj.row0 + lane < cj.n_rows) {
                 cj.y[cj.row0 + lane] = cj.bias ? as_float(cur.bias) + acc : acc;
             }
             acc = 0.0f;
@@ -309,18 +335,19 @@ int cu_count() {
     return cus[dev];
 }
 
-template <class F, int R, int W>
-hipError_t launch_gemv_w(const GArgs& ga, int njobs, int wgs, hipStream_t st) {
-    const size_t lds = (size_t)((ga.spr * (kLdsSlot + 36) + 15) & ~15) + W * R * kRedStride * sizeof(float);
+template <class F, int R, int W, class AD>
+hipError_t launch_gemv_w(const GArgs& ga, int njobs, int wgs, const AD& ad, hipStream_t st) {
+    size_t lds = (size_t)((ga.spr * (kLdsSlot + 36) + 15) & ~15) + W * R * kRedStride * sizeof(float);
+    if constexpr (std::is_same_v<AD, AdapterArgs>) lds += adapter_lanes_lds(ad);
     if (njobs > 1)
-        hipLaunchKernelGGL((kquant_gemv_kernel<F, R, true, W>), dim3(wgs), dim3(64 * W), lds, st, ga);
+        hipLaunchKernelGGL((kquant_gemv_kernel<F, R, true, W, AD>), dim3(wgs), dim3(64 * W), lds, st, ga, ad);
     else
-        hipLaunchKernelGGL((kquant_gemv_kernel<F, R, false, W>), dim3(wgs), dim3(64 * W), lds, st, ga);
+        hipLaunchKernelGGL((kquant_gemv_kernel<F, R, false, W, AD>), dim3(wgs), dim3(64 * W), lds, st, ga, ad);
     return hipGetLastError();
 }
 
-template <class F, int R>
-hipError_t launch_gemv(GArgs& ga, const ProjJob* jobs, int njobs, hipStream_t st) {
+template <class F, int R, class AD>
+hipError_t launch_gemv(GArgs& ga, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
     int groups = 0;
     for (int i = 0; i < njobs; i++) {
         ga.job[i].g_begin = groups;
@@ -344,9 +371,9 @@ hipError_t launch_gemv(GArgs& ga, const ProjJob* jobs, int njobs, hipStream_t st
     const int cap = cu_count() * wg_per_cu;
     if (wgs > cap) wgs = cap;
     if constexpr (R != 4) {
-        if (W == 8) return launch_gemv_w<F, R, 8>(ga, njobs, wgs, st);
+        if (W == 8) return launch_gemv_w<F, R, 8>(ga, njobs, wgs, ad, st);
     }
-    return launch_gemv_w<F, R, 4>(ga, njobs, wgs, st);
+    return launch_gemv_w<F, R, 4>(ga, njobs, wgs, ad, st);
 }
 
 }  // namespace
@@ -374,8 +401,11 @@ struct RArgs {
     const int16_t* b;
 };
 
-template <class F, int R>
-__global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a) {
+template <class F, int R, class AD>
+__global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    constexpr int L = 64 / (kRowsMax * R);  // lanes of an output's adapter
+    using Lanes = AdapterLanes<L, 2, 256>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int spr = a.spr, rows = a.rows, slots = rows * spr;
     uint8_t* lq = smem;                                                      // [rows][spr] activation slots
@@ -390,10 +420,25 @@ __global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a) {
     const int total = a.total_groups;
     const uint32_t row_bytes = (uint32_t)spr * F::kBytes;
     float* rw = red + wave * (R * kRowsMax * kRedStride);
+    [[maybe_unused]] float* low = red + 4 * (R * kRowsMax * kRedStride);
+    [[maybe_unused]] const int ad_m = lane / (L * R), ad_r = lane / L % R;  // the output whose adapter the lane works for
+    [[maybe_unused]] Lanes lanes;
+    if constexpr (kAd) lanes.load(ad, ad_m);
 
-    struct Item {
+    struct Plain {
         typename F::W w[R];
         uint32_t bias;
+    };
+    struct Adapted : Plain {
+        typename Lanes::Item ad;
+    };
+    using Item = std::conditional_t<kAd, Adapted, Plain>;
+    // the job of row group g
+    auto job_of = [&](int g) {
+        int j = 0;
+#pragma unroll
+        for (int i = 1; i < kMaxJobs; i++) j += i < a.njobs && g >= a.job[i].g_begin;
+        return j;
     };
     struct Cur {
         const uint8_t* w;
@@ -433,6 +478,7 @@ __global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a) {
         const bool want_bias = valid && bias != nullptr && c == nchunks - 1;
         const __amdgpu_buffer_rsrc_t bsr = make_rsrc(bias, want_bias ? (uint32_t)jb.n_rows * 4 : 0u);
         it.bias = ld1(bsr, (uint32_t)(row0 + lane % R) * 4);
+        if constexpr (kAd) lanes.fetch(ad, job_of(valid ? g : 0), row0 + ad_r, valid && c == nchunks - 1, it.ad);
     };
 
     int g = blockIdx.x * 4 + wave;
@@ -510,6 +556,7 @@ __global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a) {
             }
         }
     }
+    if constexpr (kAd) lanes.stage(ad, low);
     __syncthreads();
     if (g >= total) return;
 
@@ -544,8 +591,12 @@ __global__ __launch_bounds__(256) void kquant_gemv_rows_kernel(const RArgs a) {
         if (c == nchunks - 1) {
             const Cur jb = locate(g);
             const int m = lane / R, r = lane % R;
-            if (lane < rows * R && jb.row0 + r < jb.n_rows) {
-                // bias[o] + sum (RT/Q4KDotKernel.cs:473); no add at all without a bias
+            // bias[o] + sum (RT/Q4KDotKernel.cs:473); no add at all without a bias
+            if constexpr (kAd) {
+                float v = jb.bias ? as_float(cur.bias) + acc : acc;
+                lanes.add(ad, job_of(g), jb.row0 + ad_r, ad_m, cur.ad, low, v);
+                if (lane < rows * R && jb.row0 + r < jb.n_rows) jb.y[(size_t)m * jb.n_rows + jb.row0 + r] = v;
+            } else if (lane < rows * R && jb.row0 + r < jb.n_rows) {
                 jb.y[(size_t)m * jb.n_rows + jb.row0 + r] = jb.bias ? as_float(cur.bias) + acc : acc;
             }
             acc = 0.0f;
@@ -572,8 +623,12 @@ bool gemv_rows_quantize_inside(int in, int rows) {
 
 namespace {
 
-template <class F, int R>
-hipError_t launch_gemv_rows(RArgs& ra, const ProjJob* jobs, int njobs, hipStream_t st) {
+size_t gemv_rows_lds(int slots, int R) {
+    return (size_t)((slots * (kLdsSlot + 36) + 15) & ~15) + 4 * R * kRowsMax * kRedStride * sizeof(float);
+}
+
+template <class F, int R, class AD>
+hipError_t launch_gemv_rows(RArgs& ra, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
     int groups = 0;
     for (int i = 0; i < njobs; i++) {
         ra.job[i].g_begin = groups;
@@ -587,17 +642,28 @@ hipError_t launch_gemv_rows(RArgs& ra, const ProjJob* jobs, int njobs, hipStream
     int wgs = (groups + 3) / 4;
     const int cap = cu_count() * wg_per_cu;
     if (wgs > cap) wgs = cap;
-    const int slots = ra.rows * ra.spr;
-    const size_t lds = (size_t)((slots * (kLdsSlot + 36) + 15) & ~15) + 4 * R * kRowsMax * kRedStride * sizeof(float);
-    hipLaunchKernelGGL((kquant_gemv_rows_kernel<F, R>), dim3(wgs), dim3(256), lds, st, ra);
+    size_t lds = gemv_rows_lds(ra.rows * ra.spr, R);
+    if constexpr (std::is_same_v<AD, AdapterArgs>) lds += adapter_lanes_lds(ad);
+    hipLaunchKernelGGL((kquant_gemv_rows_kernel<F, R, AD>), dim3(wgs), dim3(256), lds, st, ra, ad);
     return hipGetLastError();
+}
+
+template <class AD>
+hipError_t launch_gemv_rows_r(int type, int R, RArgs& ra, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
+    if (type == 12)
+        return R == 2 ? launch_gemv_rows<Q4K, 2>(ra, jobs, njobs, ad, st) : launch_gemv_rows<Q4K, 1>(ra, jobs, njobs, ad, st);
+    return R == 2 ? launch_gemv_rows<Q6K, 2>(ra, jobs, njobs, ad, st) : launch_gemv_rows<Q6K, 1>(ra, jobs, njobs, ad, st);
 }
 
 }  // namespace
 
+bool gemv_rows_adapters(int in, int rows, const AdapterArgs& ad) {
+    return gemv_rows_supported(in, rows) && adapter_lanes_fit(ad, gemv_rows_lds(rows * (in / kQK), 2));
+}
+
 hipError_t launch_gemv_rows_kquant(int type, const ProjJob* jobs, int njobs, int in, int rows, const float* x,
-                                   ActQ act, hipStream_t st) {
-    if (!gemv_rows_supported(in, rows)) return hipErrorInvalidValue;
+                                   ActQ act, hipStream_t st, const AdapterArgs* ad) {
+    if (!gemv_rows_supported(in, rows) || (ad && !gemv_rows_adapters(in, rows, *ad))) return hipErrorInvalidValue;
     RArgs ra{};
     for (int i = 0; i < kMaxJobs; i++) {
         if (i < njobs) {
@@ -615,8 +681,7 @@ hipError_t launch_gemv_rows_kquant(int type, const ProjJob* jobs, int njobs, int
     ra.b = act.b;
     static const int forced_r = env_int("OVFQ_GEMV_ROWS_R", 0);
     const int R = forced_r == 1 || forced_r == 2 ? forced_r : (ra.spr <= 16 ? 2 : 1);
-    if (type == 12) return R == 2 ? launch_gemv_rows<Q4K, 2>(ra, jobs, njobs, st) : launch_gemv_rows<Q4K, 1>(ra, jobs, njobs, st);
-    return R == 2 ? launch_gemv_rows<Q6K, 2>(ra, jobs, njobs, st) : launch_gemv_rows<Q6K, 1>(ra, jobs, njobs, st);
+    return ad ? launch_gemv_rows_r(type, R, ra, jobs, njobs, *ad, st) : launch_gemv_rows_r(type, R, ra, jobs, njobs, NoAdapters{}, st);
 }
 
 // Every workgroup of the decode kernel quantises the whole activation, for every input it takes (up to 64
@@ -628,8 +693,20 @@ bool gemv_quantize_inside(int in) {
     return in / kQK <= limit;
 }
 
+template <class AD>
+static hipError_t launch_gemv_r(int type, int R, GArgs& ga, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
+    if (type == 12) {
+        if (R == 4) return launch_gemv<Q4K, 4>(ga, jobs, njobs, ad, st);
+        if (R == 2) return launch_gemv<Q4K, 2>(ga, jobs, njobs, ad, st);
+        return launch_gemv<Q4K, 1>(ga, jobs, njobs, ad, st);
+    }
+    if (R == 4) return launch_gemv<Q6K, 4>(ga, jobs, njobs, ad, st);
+    if (R == 2) return launch_gemv<Q6K, 2>(ga, jobs, njobs, ad, st);
+    return launch_gemv<Q6K, 1>(ga, jobs, njobs, ad, st);
+}
+
 hipError_t launch_gemv_kquant(int type, const ProjJob* jobs, int njobs, int in, const float* x, ActQ act,
-                              hipStream_t st) {
+                              hipStream_t st, const AdapterArgs* ad) {
     GArgs ga{};
     for (int i = 0; i < kMaxJobs; i++) {
         if (i < njobs) {
@@ -650,14 +727,7 @@ hipError_t launch_gemv_kquant(int type, const ProjJob* jobs, int njobs, int in, 
     // is 7-11 % faster with one row per wave and three workgroups per CU (4096 rows 7.05 -> 6.29 us, 14336 rows
     // 14.3 -> 12.7 us; the 128256-row LM head 85.3 -> 84.3 us).
     if (R != 1 && R != 2 && R != 4) R = type == 12 && ga.spr <= 16 ? 2 : 1;
-    if (type == 12) {
-        if (R == 4) return launch_gemv<Q4K, 4>(ga, jobs, njobs, st);
-        if (R == 2) return launch_gemv<Q4K, 2>(ga, jobs, njobs, st);
-        return launch_gemv<Q4K, 1>(ga, jobs, njobs, st);
-    }
-    if (R == 4) return launch_gemv<Q6K, 4>(ga, jobs, njobs, st);
-    if (R == 2) return launch_gemv<Q6K, 2>(ga, jobs, njobs, st);
-    return launch_gemv<Q6K, 1>(ga, jobs, njobs, st);
+    return ad ? launch_gemv_r(type, R, ga, jobs, njobs, *ad, st) : launch_gemv_r(type, R, ga, jobs, njobs, NoAdapters{}, st);
 }
 
 }  // namespace ovfq

@@ -281,17 +281,13 @@ __global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArg
     // The adapters' part of the thread's outputs is computed while the first weights are on their way; the low-rank products are
     // staged where the rounds' values come later, and each thread's own LDS words keep its result. The rows' slots and the products
     // are loaded first: what is waited for later waits for the weights too.
-    constexpr int kLowPass = W == 8 ? 64 : 32;  // ranks that fit vals0
-    static_assert(16 * T * (kLowPass + 4) <= W * kOuts, "staged products");
+    using Low = AdapterOuts<T, W, W == 8 ? 64 : 32>;
+    static_assert(Low::kLds <= W * kOuts, "staged products");
     [[maybe_unused]] AdapterJob aj;
-    [[maybe_unused]] AdapterTiles<T, 1> low_key;
-    [[maybe_unused]] AdapterStage<16 * T, kLowPass, 64 * W> low_stage;
+    [[maybe_unused]] Low low;
     if constexpr (kAd) {
         aj = adapter_job(ad, j);
-        if (aj.slots) {
-            low_key.load(ad, aj, n0);
-            low_stage.load(ad, aj, n0, 0);
-        }
+        if (aj.slots) low.load(ad, aj, n0);
     }
 
     // Each wave's super-blocks: wave, wave + W, ...; weights three rounds ahead, activations one.
@@ -304,56 +300,7 @@ __global__ __launch_bounds__(64 * W, 2) void kquant_mfma_split_kernel(const PArg
     fetch(ring[2][wave], wave + 2 * W);
     uint32_t low_mine = 0;  // outputs of the thread that have an adapter
     if constexpr (kAd) {
-        if (aj.slots) {
-            AdapterRow row[kPer];
-            float part[kPer];
-            int most = 0;  // the largest padded rank of the workgroup's rows, the same for every wave
-#pragma unroll
-            for (int t = 0; t < T; t++) most = max(most, (int)(low_key.key[t] & 0xffffu));
-#pragma unroll
-            for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
-            most = __builtin_amdgcn_readfirstlane(most);
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {  // the thread's i-th output: row r16 of tile (wave + W i) / 4
-                const int tile = (wave + W * i) >> 2;
-                row[i] = AdapterRow{0, 0.0f};
-#pragma unroll
-                for (int t = 0; t < T; t++)
-                    if (tile == t) row[i] = AdapterRow{low_key.key[t], low_key.scale[t]};
-                if (o0 + (((int)threadIdx.x >> 4) & 15) >= n_out) row[i].key = 0;
-                part[i] = 0.0f;
-            }
-            float* staged = &vals0[0][0];
-            for (int r0 = 0; r0 < most; r0 += kLowPass) {
-                if (r0) {
-                    adapter_barrier();
-                    low_stage.load(ad, aj, n0, r0);
-                }
-                low_stage.store(ad, aj, n0, r0, staged);
-                adapter_barrier();
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int idx = (int)threadIdx.x + 64 * W * i;
-                    const float* low = staged + ((idx >> 8) * 16 + (idx & 15)) * (kLowPass + 4);
-#pragma unroll
-                    for (int h = 0; h < kLowPass; h += 32) {
-                        if (r0 + h >= most) break;  // the same for every wave
-                        if (row[i].pad() > r0 + h)
-                            part[i] = most <= r0 + h + 16 ? adapter_dot<16>(ad, aj, row[i], o0 + ((idx >> 4) & 15), low + h, r0 + h, part[i])
-                                                          : adapter_dot<32>(ad, aj, row[i], o0 + ((idx >> 4) & 15), low + h, r0 + h, part[i]);
-                    }
-                }
-            }
-            if (most) adapter_barrier();  // vals0 is the first round's next
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int idx = (int)threadIdx.x + 64 * W * i;
-                if (row[i].pad()) {
-                    low_out[idx] = part[i] * row[i].scale;
-                    low_mine |= 1u << i;
-                }
-            }
-        }
+        if (aj.slots) low_mine = low.part(ad, aj, n0, o0, &vals0[0][0], low_out);
     }
     const int rounds = (spr + W - 1) / W;
     // round 0 adds up zeros (a thread reads the places it writes here)

@@ -57,9 +57,11 @@ bool gemv_quantize_inside(int in);
 bool gemv_rows_supported(int in, int rows);
 bool gemv_rows_quantize_inside(int in, int rows);
 hipError_t launch_gemv_rows_kquant(int type, const ProjJob* jobs, int njobs, int in, int rows, const float* x,
-                                   ActQ act, hipStream_t st);
+                                   ActQ act, hipStream_t st, const AdapterArgs* ad = nullptr);
 hipError_t launch_gemv_kquant(int type, const ProjJob* jobs, int njobs, int in, const float* x, ActQ act,
-                              hipStream_t st);
+                              hipStream_t st, const AdapterArgs* ad = nullptr);
+// Whether the multi-row decode kernel has the LDS for these adapters' products beside its own.
+bool gemv_rows_adapters(int in, int rows, const AdapterArgs& ad);
 // Batched K-quant projection on int8 MFMA over 64-row weight tiles x 64/128-row activation tiles; bit-identical
 // to launch_project_kquant at any rows.
 bool mfma_supported(int type);
@@ -176,7 +178,8 @@ bool q8_0_gemv_supported(int in);
 bool q8_0_gemv_rows_supported(int in, int rows);
 bool q8_0_gemv_quantize_inside(int in);
 hipError_t launch_q8_0_gemv(const ProjJob* jobs, int njobs, int in, int rows, const float* x, ActQ act,
-                            hipStream_t st);
+                            hipStream_t st, const AdapterArgs* ad = nullptr);
+bool q8_0_gemv_adapters(int in, int rows, const AdapterArgs& ad);  // as gemv_rows_adapters
 // Q8_0 over several activation rows on int8 MFMA (one 16x16x32 MFMA per 32-element block), bit-identical to
 // launch_project_q8_0.
 bool q8_0_mfma_supported(int in, int rows);
@@ -223,7 +226,7 @@ bool q8_0_mid_supported(int planes, int plane_in, int rows);
 hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int plane_in, int8_t* q, float* s,
                                       hipStream_t st);
 hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int planes, bool heads, int plane_in, int n_out,
-                           int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st);
+                           int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st, const AdapterArgs* ad = nullptr);
 
 // An activation to quantise in the launch of another kernel (act_quant.h), 256 threads a part.
 struct ActQuantJob {

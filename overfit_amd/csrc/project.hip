@@ -16,6 +16,7 @@
 #include <cstdlib>
 #include <type_traits>
 
+#include "adapter_tile.h"
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
 #include "kquant_blocks.h"
@@ -297,8 +298,12 @@ constexpr int kQ8GemvQuantMaxIn = 8192;   // in-launch quantisation (every workg
 constexpr int kQ8Red = 68;                // floats per block-value row: 64 values, 16-byte aligned rows
 typedef float f32x4q __attribute__((ext_vector_type(4)));
 
-template <int R, bool kMulti>
-__global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
+// AD: AdapterArgs, and the rows' adapters are added to the outputs, or NoAdapters.
+template <int R, bool kMulti, class AD>
+__global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    constexpr int L = 64 / (kQ8GemvMaxRows * R);  // lanes of an output's adapter
+    using Lanes = AdapterLanes<L, 2, 256>;
     extern __shared__ __align__(16) uint8_t smem8[];
     const int K = a.in, nb = a.nb, M = a.m_rows;
     uint8_t* lq = smem8;                                          // [M][K] activation quants
@@ -310,11 +315,29 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
     const int stride = gridDim.x * 4;
     const int total = a.total_groups;
     float* rw = red + wave * R * kQ8GemvMaxRows * kQ8Red;
+    [[maybe_unused]] float* low = red + 4 * R * kQ8GemvMaxRows * kQ8Red;
+    // the output whose adapter the lane works for
+    [[maybe_unused]] const int ad_r = kAd ? lane / L / M : 0, ad_m = kAd ? lane / L - ad_r * M : 0;
+    [[maybe_unused]] Lanes lanes;
+    if constexpr (kAd) lanes.load(ad, ad_m);
 
-    struct Item {
+    struct Plain {
         u32x4 w[R][2];
         uint32_t ws[R];
         uint32_t bias;
+    };
+    struct Adapted : Plain {
+        typename Lanes::Item ad;
+    };
+    using Item = std::conditional_t<kAd, Adapted, Plain>;
+    // the job of row group g
+    auto job_of = [&](int g) {
+        int j = 0;
+        if constexpr (kMulti) {
+#pragma unroll
+            for (int i = 1; i < kMaxJobs; i++) j += i < a.njobs && g >= a.job[i].g_begin;
+        }
+        return j;
     };
     struct Cur {
         const int8_t* w;
@@ -343,7 +366,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
     };
     // Loads of item (row group of jb, chunk c); an invalid item reads through zero-length resources. Lanes past the
     // row's last block read the next row's bytes (or zeros past the group) and are not used.
-    auto load_item = [&](const Cur& jb, int c, bool valid, Item& it) {
+    auto load_item = [&](const Cur& jb, int c, bool valid, Item& it, [[maybe_unused]] int job) {
         const int rows = min(R, jb.n_rows - jb.row0);
         const __amdgpu_buffer_rsrc_t wr =
             make_rsrc(jb.w + (uint64_t)jb.row0 * K, valid ? (uint32_t)rows * (uint32_t)K : 0u);
@@ -360,6 +383,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
         const bool want_bias = valid && jb.bias != nullptr && c == nchunks - 1;
         const __amdgpu_buffer_rsrc_t bsr = make_rsrc(jb.bias, want_bias ? (uint32_t)jb.n_rows * 4u : 0u);
         it.bias = ld1(bsr, (uint32_t)(jb.row0 + (lane < R * M ? lane / M : 0)) * 4u);
+        if constexpr (kAd) lanes.fetch(ad, job, jb.row0 + ad_r, valid && c == nchunks - 1 && ad_r < R, it.ad);
     };
 
     int g = blockIdx.x * 4 + wave;
@@ -373,7 +397,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
         u32x4 xv[kPasses];
 #pragma unroll
         for (int p = 0; p < kPasses; p++) xv[p] = ld4(xr, (uint32_t)(p * 1024 + threadIdx.x * 4) * 4u);  // past K: 0
-        load_item(locate(g < total ? g : 0), 0, g < total, ia);
+        load_item(locate(g < total ? g : 0), 0, g < total, ia, kAd ? job_of(g < total ? g : 0) : 0);
 #pragma unroll
         for (int p = 0; p < kPasses; p++) {
             const Q80Lane r = q8_0_quantize_lane(xv[p]);  // every lane takes part
@@ -395,7 +419,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
         uint32_t sv[kQ8GemvMaxIn / 32 / 256];
 #pragma unroll
         for (int p = 0; p < kQ8GemvMaxIn / 32 / 256; p++) sv[p] = ld1(sr, (uint32_t)(p * 256 + threadIdx.x) * 4u);
-        load_item(locate(g < total ? g : 0), 0, g < total, ia);
+        load_item(locate(g < total ? g : 0), 0, g < total, ia, kAd ? job_of(g < total ? g : 0) : 0);
 #pragma unroll
         for (int p = 0; p < kPasses; p++) {
             const int i = p * 4096 + (int)threadIdx.x * 16;
@@ -407,6 +431,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
             if (i < M * nb) ls[i] = as_float(sv[p]);
         }
     }
+    if constexpr (kAd) lanes.stage(ad, low);
     __syncthreads();
     if (g >= total) return;
     Cur cj = locate(g);
@@ -421,7 +446,7 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
         const bool more = ng < total;
         Cur nj = cj;
         if (nc == 0) nj = locate(more ? ng : 0);
-        load_item(nj, nc, more, nxt);
+        load_item(nj, nc, more, nxt, kAd ? job_of(more ? ng : 0) : 0);
         const int blk = c * 64 + lane;
         const bool live = blk < nb;
         const int ab = live ? blk : 0;
@@ -464,8 +489,9 @@ __global__ __launch_bounds__(256) void q8_0_gemv_kernel(const Q8GArgs a) {
         wave_sync();
         if (c == nchunks - 1) {
             const int row = cj.row0 + lane / M, m = lane % M;
-            if (lane < R * M && row < cj.n_rows)
-                cj.y[(size_t)m * cj.n_rows + row] = cj.bias ? as_float(cur.bias) + acc : acc;
+            float v = cj.bias ? as_float(cur.bias) + acc : acc;
+            if constexpr (kAd) lanes.add(ad, job_of(g), cj.row0 + ad_r, ad_r < R ? ad_m : M, cur.ad, low, v);
+            if (lane < R * M && row < cj.n_rows) cj.y[(size_t)m * cj.n_rows + row] = v;
             acc = 0.0f;
         }
         g = ng;
@@ -496,8 +522,12 @@ int q8_cu_count() {
     return cus[dev];
 }
 
-template <int R>
-hipError_t launch_q8g(Q8GArgs& ga, const ProjJob* jobs, int njobs, hipStream_t st) {
+size_t q8g_lds(int rows, int in, int R) {
+    return (size_t)rows * in + 4 * (size_t)((rows * (in / 32) + 3) & ~3) + 4 * (size_t)4 * R * kQ8GemvMaxRows * kQ8Red;
+}
+
+template <int R, class AD>
+hipError_t launch_q8g(Q8GArgs& ga, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
     int groups = 0;
     for (int i = 0; i < njobs; i++) {
         ga.job[i].g_begin = groups;
@@ -512,18 +542,37 @@ hipError_t launch_q8g(Q8GArgs& ga, const ProjJob* jobs, int njobs, hipStream_t s
     int wgs = (groups + 3) / 4;
     const int cap = q8_cu_count() * wg_per_cu;
     if (wgs > cap) wgs = cap;
-    const size_t lds = (size_t)ga.m_rows * ga.in + 4 * (size_t)((ga.m_rows * ga.nb + 3) & ~3) +
-                       4 * (size_t)4 * R * kQ8GemvMaxRows * kQ8Red;
+    size_t lds = q8g_lds(ga.m_rows, ga.in, R);
+    if constexpr (std::is_same_v<AD, AdapterArgs>) lds += adapter_lanes_lds(ad);
     if (njobs > 1)
-        hipLaunchKernelGGL((q8_0_gemv_kernel<R, true>), dim3(wgs), dim3(256), lds, st, ga);
+        hipLaunchKernelGGL((q8_0_gemv_kernel<R, true, AD>), dim3(wgs), dim3(256), lds, st, ga, ad);
     else
-        hipLaunchKernelGGL((q8_0_gemv_kernel<R, false>), dim3(wgs), dim3(256), lds, st, ga);
+        hipLaunchKernelGGL((q8_0_gemv_kernel<R, false, AD>), dim3(wgs), dim3(256), lds, st, ga, ad);
     return hipGetLastError();
+}
+template <class AD>
+hipError_t launch_q8g_r(int R, Q8GArgs& ga, const ProjJob* jobs, int njobs, const AD& ad, hipStream_t st) {
+    if (R == 4) return launch_q8g<4>(ga, jobs, njobs, ad, st);
+    if (R == 1) return launch_q8g<1>(ga, jobs, njobs, ad, st);
+    return launch_q8g<2>(ga, jobs, njobs, ad, st);
+}
+
+int q8g_rows_per_wave() {
+    static const int forced_r = [] {
+        const char* v = getenv("OVFQ_Q8_GEMV_ROWS_PER_WAVE");
+        return v && *v ? atoi(v) : 0;
+    }();
+    return forced_r == 1 || forced_r == 2 || forced_r == 4 ? forced_r : 2;
 }
 }  // namespace
 
+bool q8_0_gemv_adapters(int in, int rows, const AdapterArgs& ad) {
+    return q8_0_gemv_rows_supported(in, rows) && adapter_lanes_fit(ad, q8g_lds(rows, in, q8g_rows_per_wave()));
+}
+
 hipError_t launch_q8_0_gemv(const ProjJob* jobs, int njobs, int in, int rows, const float* x, ActQ act,
-                            hipStream_t st) {
+                            hipStream_t st, const AdapterArgs* ad) {
+    if (ad && !q8_0_gemv_adapters(in, rows, *ad)) return hipErrorInvalidValue;
     if ((x && (rows != 1 || !q8_0_gemv_quantize_inside(in))) || !q8_0_gemv_rows_supported(in, rows))
         return hipErrorInvalidValue;
     Q8GArgs ga{};
@@ -541,14 +590,8 @@ hipError_t launch_q8_0_gemv(const ProjJob* jobs, int njobs, int in, int rows, co
     ga.x = x;
     ga.q = act.q;
     ga.s = act.s;
-    static const int forced_r = [] {
-        const char* v = getenv("OVFQ_Q8_GEMV_ROWS_PER_WAVE");
-        return v && *v ? atoi(v) : 0;
-    }();
-    const int R = forced_r == 1 || forced_r == 2 || forced_r == 4 ? forced_r : 2;
-    if (R == 4) return launch_q8g<4>(ga, jobs, njobs, st);
-    if (R == 1) return launch_q8g<1>(ga, jobs, njobs, st);
-    return launch_q8g<2>(ga, jobs, njobs, st);
+    const int R = q8g_rows_per_wave();
+    return ad ? launch_q8g_r(R, ga, jobs, njobs, *ad, st) : launch_q8g_r(R, ga, jobs, njobs, NoAdapters{}, st);
 }
 
 // ------------------------------------------------------------------------------------------ Q8_0 on int8 MFMA

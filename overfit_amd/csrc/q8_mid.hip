@@ -22,7 +22,10 @@
 // 31.7 / 42.7 / 45.4 -> 11.5 / 14.5 / 19.3 / 20.3 / 34.2 / 42.8; 4096x14336 at 4 / 16 / 32 / 300 rows 51.2 / 81.7 / 95.3 / 131
 // -> 22.7 / 22.9 / 33.7 / 99.7; 14336x4096 at 16 / 64 / 512 rows 31.4 / 33.2 / 132 -> 20.7 / 30.1 / 122; per-head Wo of 32 x
 // 4096x128 at 8 / 16 / 64 / 300 rows 18.1 / 26.9 / 35.3 / 46.1 -> 11.8 / 12.0 / 22.0 / 36.3.
+#include <type_traits>
+
 #include "act_quant.h"
+#include "adapter_tile.h"
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
 
@@ -166,9 +169,11 @@ struct Q8Cursor {
 // SIMD (a conversion takes twice the issue of a multiplication or addition: 60 against 111 lanes a clock and CU). 4096x4096 at 512
 // rows, 40.3 us: 30 were left with the DMAs taken out. Eight waves a workgroup, each with half the rows, were no faster (512 rows
 // 43.4; 64 rows 20.6 instead of 19.5), nor were more groups in flight.
-// J: blocks of a group that are computed (planes of fewer than four blocks).
-template <int T, bool kHeads, int J = 4>
-__global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a) {
+// J: blocks of a group that are computed (planes of fewer than four blocks). AD: AdapterArgs, and the rows' adapters (of job 0) are
+// added to the outputs, or NoAdapters.
+template <int T, bool kHeads, int J, class AD>
+__global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
     __shared__ __align__(16) uint8_t ring[3][4][kQ8Slot];
     __shared__ __align__(16) uint8_t act0[T * 2048], act1[T * 2048], act2[T * 2048];
     __shared__ __align__(16) uint32_t sc0[4 * 64], sc1[4 * 64], sc2[4 * 64];
@@ -269,6 +274,8 @@ __global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a) {
     stage(1, act1, sc1);
     asm volatile("" ::: "memory");
     fetch(1);
+    [[maybe_unused]] AdapterTiles<T, 1> low;
+    if constexpr (kAd) low.load(ad, ad.job[0], n0);
     int gi = 0;
     for (; gi + 2 < ng; gi += 3) {
         step(gi, 0, act0, sc0, act2, sc2);
@@ -277,13 +284,29 @@ __global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a) {
     }
     if (gi < ng) step(gi, 0, act0, sc0, act2, sc2);
     if (gi + 1 < ng) step(gi + 1, 1, act1, sc1, act0, sc0);
+    if constexpr (kAd) {
+        float v[T][1][4];
+#pragma unroll
+        for (int s = 0; s < T; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[s][0][i] = a.bias ? bias_o + acc[s][i] : acc[s][i];
+        static_assert(AdapterTiles<T, 1>::kLds * 4 <= (int)sizeof(ring), "staged products");
+        // no prefetch is still on its way into the weights' slots, and every wave is done with them
+        __builtin_amdgcn_s_waitcnt(0);
+        adapter_barrier();
+        low.template add<256>(ad, ad.job[0], n0, o0, v, reinterpret_cast<float*>(&ring[0][0][0]));
+#pragma unroll
+        for (int s = 0; s < T; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[s][i] = v[s][0][i];
+    }
 #pragma unroll
     for (int s = 0; s < T; s++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int n = n0 + s * 16 + 4 * g + i;
             if (n >= a.rows || o >= a.n_out) continue;
-            a.y[(size_t)n * a.n_out + o] = kHeads ? tot[s][i] : a.bias ? bias_o + acc[s][i] : acc[s][i];
+            a.y[(size_t)n * a.n_out + o] = kHeads ? tot[s][i] : a.bias && !kAd ? bias_o + acc[s][i] : acc[s][i];
         }
     __builtin_amdgcn_s_waitcnt(0);  // no DMA lands in LDS that another workgroup may have by then
 }
@@ -293,11 +316,14 @@ __global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a) {
 // workgroups as it has 16-row tiles, and W times the loads in flight of one that walks its groups in order. A round leaves
 // 4 W block values per output in LDS, which the workgroup's threads add up in order between two barriers. Bound by the
 // latency of a round (about 1.3 us, four rounds of 4096 inputs with eight waves), then by the LDS traffic of the values.
-template <int T, int W, bool kHeads>
-__global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a) {
+template <int T, int W, bool kHeads, class AD>
+__global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a, const AD ad) {
+    constexpr bool kAd = std::is_same_v<AD, AdapterArgs>;
+    using Low = AdapterOuts<T, W, 64>;
     constexpr int kOuts = 256 * T, kThreads = 64 * W, kPer = kOuts > kThreads ? kOuts / kThreads : 1;
     __shared__ __align__(16) uint8_t ring[3][W][kQ8Slot];
     __shared__ __align__(16) float vals[W][4][kOuts];
+    __shared__ __align__(16) float low_out[kAd ? kOuts : 4];  // the adapters' part of the outputs
     const int wave = wave_id();
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, r16 = lane & 15;
@@ -409,6 +435,9 @@ __global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a) {
         }
         barrier();  // the values are read: the next round may write
     };
+    // (before the weights, which what is waited for later would wait for too)
+    [[maybe_unused]] Low low;
+    if constexpr (kAd) low.load(ad, ad.job[0], n0);
     Act a0, a1;
     fetch(0);
     asm volatile("" ::: "memory");  // kLeft counts on this order
@@ -416,6 +445,12 @@ __global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a) {
     asm volatile("" ::: "memory");
     fetch(1);
     fetch(2);
+    // while the first weights are on their way; the products are staged where the rounds' values come later
+    [[maybe_unused]] uint32_t low_mine = 0;
+    if constexpr (kAd) {
+        static_assert(Low::kLds <= W * 4 * kOuts, "staged products");
+        low_mine = low.part(ad, ad.job[0], n0, o0, &vals[0][0][0], low_out);
+    }
     const int rounds = (ng + W - 1) / W;
     int k = 0;
     auto next_slot = [](int i) { return i == 2 ? 0 : i + 1; };
@@ -431,8 +466,13 @@ __global__ __launch_bounds__(64 * W, 2) void q8_0_split_kernel(const Q8Args a) {
     for (int p = 0; p < kPer; p++) {
         const int idx = (int)threadIdx.x + p * kThreads;
         const int o = o0 + ((idx >> 4) & 15), n = n0 + (idx >> 8) * 16 + (idx & 15);
-        if (idx < kOuts && o < a.n_out && n < a.rows)
-            a.y[(size_t)n * a.n_out + o] = kHeads ? tot[p] : a.bias ? a.bias[o] + sum[p] : sum[p];
+        if (idx < kOuts && o < a.n_out && n < a.rows) {
+            float v = kHeads ? tot[p] : a.bias ? a.bias[o] + sum[p] : sum[p];
+            if constexpr (kAd) {
+                if (low_mine >> p & 1) v += low_out[idx];
+            }
+            a.y[(size_t)n * a.n_out + o] = v;
+        }
     }
     __builtin_amdgcn_s_waitcnt(0);  // no DMA lands in LDS that another workgroup may have by then
 }
@@ -453,19 +493,19 @@ hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int 
     return hipGetLastError();
 }
 
-template <bool kHeads, int J>
-static hipError_t launch_panel_t(const Q8Args& a, int T, dim3 grid, hipStream_t st) {
+template <bool kHeads, int J, class AD>
+static hipError_t launch_panel_t(const Q8Args& a, int T, dim3 grid, const AD& ad, hipStream_t st) {
     if (T == 2)
-        hipLaunchKernelGGL((q8_0_panel_kernel<2, kHeads, J>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((q8_0_panel_kernel<2, kHeads, J, AD>), grid, dim3(256), 0, st, a, ad);
     else if (T == 3)
-        hipLaunchKernelGGL((q8_0_panel_kernel<3, kHeads, J>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((q8_0_panel_kernel<3, kHeads, J, AD>), grid, dim3(256), 0, st, a, ad);
     else
-        hipLaunchKernelGGL((q8_0_panel_kernel<4, kHeads, J>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((q8_0_panel_kernel<4, kHeads, J, AD>), grid, dim3(256), 0, st, a, ad);
     return hipGetLastError();
 }
 
-template <bool kHeads>
-static hipError_t launch_panel(Q8Args& a, hipStream_t st) {
+template <bool kHeads, class AD>
+static hipError_t launch_panel(Q8Args& a, const AD& ad, hipStream_t st) {
     a.o_tiles = (a.n_out + 63) / 64;
     // Rows of a workgroup: a CU's step takes about T + 0.84 (in 0.125 us) for each of its workgroups, and one unit more where
     // it has only one, whose waits nothing hides (4096x4096, us at T = 2 / 3 / 4: 128 rows 20.3 / 25.0 / 29.1, 160 rows 28.5 /
@@ -484,12 +524,12 @@ static hipError_t launch_panel(Q8Args& a, hipStream_t st) {
     const dim3 grid((a.o_tiles + 7) / 8 * 8 * a.n_tiles);
     const int wnb = a.in / 32;
     if constexpr (kHeads)
-        if (wnb < 4) return wnb < 3 ? launch_panel_t<true, 2>(a, T, grid, st) : launch_panel_t<true, 3>(a, T, grid, st);
-    return launch_panel_t<kHeads, 4>(a, T, grid, st);
+        if (wnb < 4) return wnb < 3 ? launch_panel_t<true, 2>(a, T, grid, ad, st) : launch_panel_t<true, 3>(a, T, grid, ad, st);
+    return launch_panel_t<kHeads, 4>(a, T, grid, ad, st);
 }
 
-template <bool kHeads>
-static hipError_t launch_mid(Q8Args& a, hipStream_t st) {
+template <bool kHeads, class AD>
+static hipError_t launch_mid(Q8Args& a, const AD& ad, hipStream_t st) {
     const int wnb = a.in / 32, ng = (kHeads ? a.planes : 1) * ((wnb + 3) / 4);
     // The split kernel while its workgroups fit the CUs at one each (eight waves; four where there are no more groups than
     // that), and up to 16 rows with four waves up to two each; then the panel kernel (MI355X, us, split of 8 / of 4 / panel:
@@ -501,18 +541,18 @@ static hipError_t launch_mid(Q8Args& a, hipStream_t st) {
     a.n_tiles = (a.subs + T - 1) / T;
     const long wgs = (long)((a.o_tiles + 7) / 8) * a.n_tiles * 8;  // as the busiest XCD has them (293x1088 at 370 rows, 228
                                                                    // workgroups, 36 on three XCDs: 14.5, panel 9.8)
-    if (wgs > 256 && (T == 2 || wgs > 512)) return launch_panel<kHeads>(a, st);
+    if (wgs > 256 && (T == 2 || wgs > 512)) return launch_panel<kHeads>(a, ad, st);
     const dim3 grid((a.o_tiles + 7) / 8 * 8 * a.n_tiles);
     if (wgs > 256 || ng <= 4) {
         if (T == 1)
-            hipLaunchKernelGGL((q8_0_split_kernel<1, 4, kHeads>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((q8_0_split_kernel<1, 4, kHeads, AD>), grid, dim3(256), 0, st, a, ad);
         else
-            hipLaunchKernelGGL((q8_0_split_kernel<2, 4, kHeads>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((q8_0_split_kernel<2, 4, kHeads, AD>), grid, dim3(256), 0, st, a, ad);
     } else {
         if (T == 1)
-            hipLaunchKernelGGL((q8_0_split_kernel<1, 8, kHeads>), grid, dim3(512), 0, st, a);
+            hipLaunchKernelGGL((q8_0_split_kernel<1, 8, kHeads, AD>), grid, dim3(512), 0, st, a, ad);
         else
-            hipLaunchKernelGGL((q8_0_split_kernel<2, 8, kHeads>), grid, dim3(512), 0, st, a);
+            hipLaunchKernelGGL((q8_0_split_kernel<2, 8, kHeads, AD>), grid, dim3(512), 0, st, a, ad);
     }
     return hipGetLastError();
 }
@@ -525,8 +565,9 @@ bool q8_0_mid_supported(int planes, int plane_in, int rows) {
 }
 
 hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int planes, bool heads, int plane_in, int n_out,
-                           int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st) {
-    if (planes < 1 || planes > kHeadsMax || (planes > 1 && !heads) || !q8_0_mid_supported(planes, plane_in, rows))
+                           int rows, const float* bias, const int8_t* q, const float* s, float* y, hipStream_t st,
+                           const AdapterArgs* ad) {
+    if (planes < 1 || planes > kHeadsMax || (planes > 1 && !heads) || (heads && ad) || !q8_0_mid_supported(planes, plane_in, rows))
         return hipErrorInvalidValue;
     Q8Args a{};
     for (int i = 0; i < planes; i++) {
@@ -542,7 +583,8 @@ hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int 
     a.subs = (rows + 15) / 16;
     a.q = q;
     a.s = s;
-    return heads ? launch_mid<true>(a, st) : launch_mid<false>(a, st);
+    if (heads) return launch_mid<true>(a, NoAdapters{}, st);
+    return ad ? launch_mid<false>(a, *ad, st) : launch_mid<false>(a, NoAdapters{}, st);
 }
 
 }  // namespace ovfq
