@@ -1679,8 +1679,10 @@ static int verify_impl(ovfq_ctx* ctx, const float* logits, int rows, int vocab, 
     int *acc = accepted, *tok = tokens;
     auto carve = [&](Carver& c) {
         a.stats = c.take<ovfq::VerifyStat>(R * a.pieces * sizeof(ovfq::VerifyStat));
-        a.parts = c.take<double>(Q * a.pieces * 2 * sizeof(double));
-        a.pick = c.take<ovfq::VerifyPick>(Q * sizeof(ovfq::VerifyPick));
+        if (draft_probs) {
+            a.parts = c.take<double>(Q * a.pieces * sizeof(double));
+            a.done = c.take<int>(Q * sizeof(int));
+        }
         if (!host) return;
         for (int i = 0; i < 7; i++) dev[i] = in[i] ? c.take<char>(bytes[i]) : nullptr;
         acc = c.take<int>(Q * 4);

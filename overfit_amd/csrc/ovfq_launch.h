@@ -325,18 +325,12 @@ struct NormArgs {
 };
 hipError_t launch_residual_norm(const NormArgs& a, hipStream_t st);
 
-// Verification of drafted tokens (verify.hip); the scratch planes stats [rows][pieces], parts [requests][pieces][2] and pick
-// [requests] are written by the launch.
+// Verification of drafted tokens (verify.hip); the scratch planes stats, parts and done are written by the launch.
 constexpr int kVerifyPiece = 8192;  // tokens a workgroup
 struct VerifyStat {
     float max;   // largest logit
     int at;      // its first token (greedy requests)
     double sum;  // sum of exp((logit - max) / temperature)
-};
-struct VerifyPick {
-    int row;    // the row to draw from, -1: no such request
-    int draft;  // the refused draft, -1: none
-    VerifyStat stat;
 };
 struct VerifyArgs {
     const float* logits;         // [rows][vocab]
@@ -349,8 +343,8 @@ struct VerifyArgs {
     int* accepted;               // [requests]
     int* tokens;                 // [rows]
     VerifyStat* stats;
-    double* parts;
-    VerifyPick* pick;
+    double* parts;  // [requests][pieces] and
+    int* done;      // [requests], where there are draft_probs
     int rows, vocab, requests, drafts, pieces;
 };
 hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st);

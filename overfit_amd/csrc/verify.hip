@@ -8,12 +8,14 @@
 // tokens together are then distributed as the target alone would draw them.
 //
 // Probabilities, totals and running sums are fp64: among 128256 running sums in fp32 a hundredth of all draws would land in
-// the rounding of a neighbour. Bound: reading the logits once (HBM), and the fp64 exponentials behind it.
+// the rounding of a neighbour. An exponential is a power of two, a table's 2^(j / 32) and a polynomial of the rest (table-driven
+// range reduction as Tang published it in 1989), to 2e-15 of its value.
 //
-// Three launches. (1) A workgroup per row and 8192 tokens: the largest logit and the sum of exponentials relative to it.
-// (2) A workgroup per request and 8192 tokens: the rows' sums joined, the drafts decided (every workgroup of a request repeats
-// this, it takes less than a launch), and the weights of its tokens in the row to draw from summed. (3) A workgroup per
-// request: the piece, then the token in it, where the running sum passes.
+// Two launches. (1) A workgroup per row and 8192 tokens: the largest logit and the sum of exponentials relative to it. (2) A
+// workgroup per request: a wave a row joins the row's sums and decides the draft, the first refused wins; the sums of the row to
+// draw from are its pieces' weights already (a one-hot q takes its token's away), so that only the piece that the draw falls into
+// is read again. With the drafts' distributions the weights are max(p - q, 0) of all tokens: then a workgroup per request and
+// piece, and the last of a request to finish, by a counter, draws.
 #include <cmath>
 
 #include "ovfq_device.h"
@@ -25,9 +27,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-constexpr int kPiece = kVerifyPiece;  // tokens a workgroup: 256 threads x 8 four-token loads
-constexpr int kThreads = 256;
-constexpr int kVecs = kPiece / (4 * kThreads);
+constexpr int kPiece = kVerifyPiece;
+constexpr int kThreads = 256;  // of the first launch: 8 four-token loads a thread
+constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64;
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -52,49 +54,88 @@ __device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : v;
 
 __device__ __forceinline__ bool is_greedy(float temperature) { return !(temperature > 0.0f && temperature < INFINITY); }
 
-// Tokens [lo, lo + kPiece) of a row of `vocab`: piece i of a thread is tokens lo + 4 (i * kThreads + t) on; past the row
-// `fill`.
-__device__ __forceinline__ void load_piece(const float* row, int vocab, int lo, int t, float fill, float (&v)[4 * kVecs]) {
+// 2^(j / 32), j < 32, by the first threads of the workgroup; a barrier comes before its use.
+__device__ __forceinline__ void fill_powers(double* powers) {
+    if (threadIdx.x < 32) powers[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 32));
+}
+
+// exp(x), x <= 0. x = n ln2 / 32 + r with |r| <= ln2 / 64, so that the Taylor polynomial of degree 5 is off by r^6 / 720 < 2.3e-15;
+// n comes out of the low bits of a sum with 1.5 * 2^52. kZero: values below the normal range are right (0 in the end), else they
+// are about 1e-304, which no sum with a 1 in it sees.
+template <bool kZero>
+__device__ __forceinline__ double negative_exp(double x, const double* powers) {
+    constexpr double kMagic = 6755399441055744.0, kPer = 46.16624130844682903, kStep = 0.02166084939249829091;  // 32 / ln2, ln2 / 32
+    x = fmax(x, kZero ? -800.0 : -700.0);
+    const double t = fma(x, kPer, kMagic);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double r = fma(-(t - kMagic), kStep, x);
+    double p = fma(r, 1.0 / 120, 1.0 / 24);
+    p = fma(r, p, 1.0 / 6);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0);
+    p *= powers[n & 31];
+    if constexpr (kZero) return ldexp(p, n >> 5);
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(n >> 5) << 52));
+}
+
+// Tokens [lo, lo + kPiece) of a row of `vocab`, four at a time: vector i of thread t is tokens lo + 4 (i * kT + t) on or, kRuns,
+// lo + 4 (kVecs t + i) on; past the row `fill`.
+template <int kT, bool kRuns>
+__device__ __forceinline__ int piece_at(int i) {
+    return 4 * (kRuns ? kPiece / (4 * kT) * (int)threadIdx.x + i : i * kT + (int)threadIdx.x);
+}
+template <int kT, bool kRuns>
+__device__ __forceinline__ void load_piece(const float* row, int vocab, int lo, float fill, float (&v)[kPiece / kT]) {
     const int n = min(kPiece, vocab - lo);
     const __amdgpu_buffer_rsrc_t r = make_rsrc(row + lo, (uint32_t)n * 4);
-    u32x4 raw[kVecs];
+    u32x4 raw[kPiece / (4 * kT)];
 #pragma unroll
-    for (int i = 0; i < kVecs; i++) raw[i] = ld4(r, 16u * (uint32_t)(i * kThreads + t));
+    for (int i = 0; i < kPiece / (4 * kT); i++) raw[i] = ld4(r, 4u * (uint32_t)piece_at<kT, kRuns>(i));
 #pragma unroll
-    for (int i = 0; i < kVecs; i++) {
+    for (int i = 0; i < kPiece / (4 * kT); i++) {
         const uint32_t a[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int c = 0; c < 4; c++) v[4 * i + c] = 4 * (i * kThreads + t) + c < n ? as_float(a[c]) : fill;
+        for (int c = 0; c < 4; c++) v[4 * i + c] = piece_at<kT, kRuns>(i) + c < n ? as_float(a[c]) : fill;
     }
 }
 
-// The request that owns `row` (its offsets in order and within the rows), or -1; every thread of the workgroup calls it.
-__device__ __forceinline__ int owner_of(const VerifyArgs& a, int row, int* shared) {
-    if (threadIdx.x == 0) *shared = -1;
-    __syncthreads();
-    for (int r = threadIdx.x; r < a.requests; r += kThreads) {
-        const int lo = a.row_offsets[r], hi = a.row_offsets[r + 1];
-        if (lo >= 0 && lo <= row && row < hi && hi <= a.rows) atomicMax(shared, r);
+// The request that owns `row` (its offsets in order and within the rows), or -1; the same for every lane of the wave.
+__device__ __forceinline__ int owner_of(const VerifyArgs& a, int row) {
+    int owner = -1;
+    for (int r0 = 0; r0 < a.requests; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        bool mine = false;
+        if (r < a.requests) {
+            const int lo = a.row_offsets[r], hi = a.row_offsets[r + 1];
+            mine = lo >= 0 && lo <= row && row < hi && hi <= a.rows;
+        }
+        const uint64_t at = __ballot(mine);
+        if (at) owner = r0 + 63 - __builtin_clzll(at);
     }
-    __syncthreads();
-    return *shared;
+    return owner;
 }
 
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs a) {
-    __shared__ int owner;
+    constexpr int kEach = kPiece / kThreads;
+    __shared__ double powers[32];
     __shared__ float wmax[4];
     __shared__ double wsum[4];
     __shared__ int wmin[4];
-    const int row = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x % a.pieces;
+    const int row = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x;
+    if (row >= a.rows) return;
     const int t = threadIdx.x, wave = t >> 6, lo = piece * kPiece;
-    float v[4 * kVecs];
-    load_piece(a.logits + (int64_t)row * a.vocab, a.vocab, lo, t, -INFINITY, v);
-    const int request = owner_of(a, row, &owner);
-    if (request < 0) return;
+    float v[kEach];
+    load_piece<kThreads, false>(a.logits + (int64_t)row * a.vocab, a.vocab, lo, -INFINITY, v);
+    fill_powers(powers);
+    if (a.done && !row && !piece)
+        for (int r = t; r < a.requests; r += kThreads) a.done[r] = 0;
+    const int request = owner_of(a, row);
+    if (request < 0) return;  // the whole workgroup
     const float temperature = a.temperature ? a.temperature[request] : 1.0f;
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4 * kVecs; i++) {
+    for (int i = 0; i < kEach; i++) {
         v[i] = clean(v[i]);
         m = fmaxf(m, v[i]);
     }
@@ -106,19 +147,19 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
     if (is_greedy(temperature)) {
         int at = 0x7fffffff;
 #pragma unroll
-        for (int i = 4 * kVecs - 1; i >= 0; i--)
-            if (v[i] == m) at = lo + 4 * ((i >> 2) * kThreads + t) + (i & 3);
+        for (int i = kEach - 1; i >= 0; i--)
+            if (v[i] == m) at = lo + piece_at<kThreads, false>(i >> 2) + (i & 3);
         at = wave_min(at);
         if ((t & 63) == 0) wmin[wave] = at;
         __syncthreads();
         out.at = min(min(wmin[0], wmin[1]), min(wmin[2], wmin[3]));
     } else if (m > -INFINITY && m < INFINITY) {
         const double inv = 1.0 / (double)temperature;
-        double s = 0.0;
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int i = 0; i < 4 * kVecs; i++) s += exp(((double)v[i] - (double)m) * inv);
-        s = wave_sum(s);
-        if ((t & 63) == 0) wsum[wave] = s;
+        for (int i = 0; i < kEach; i++) s[i & 3] += negative_exp<false>(((double)v[i] - (double)m) * inv, powers);
+        const double sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+        if ((t & 63) == 0) wsum[wave] = sum;
         __syncthreads();
         out.sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
     }
@@ -126,193 +167,245 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
 }
 
 // A row's pieces joined by one wave: the largest logit, its first token, and the sum of exponentials relative to it.
-__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv) {
+__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers) {
     const VerifyStat* s = a.stats + (int64_t)row * a.pieces;
     const int lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    for (int c = lane; c < a.pieces; c += 64) m = fmaxf(m, s[c].max);
+    const VerifyStat none{-INFINITY, 0x7fffffff, 0.0};
+    const VerifyStat first = lane < a.pieces ? s[lane] : none;
+    float m = first.max;
+    for (int c = 64 + lane; c < a.pieces; c += 64) m = fmaxf(m, s[c].max);
     m = wave_max(m);
-    int at = 0x7fffffff;
-    double sum = 0.0;
-    for (int c = lane; c < a.pieces; c += 64) {
-        if (s[c].max == m) at = min(at, s[c].at);
-        if (s[c].sum > 0.0) sum += s[c].sum * exp(((double)s[c].max - (double)m) * inv);
+    auto part = [&](const VerifyStat& v) { return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)m) * inv, powers) : 0.0; };
+    int at = first.max == m ? first.at : 0x7fffffff;
+    double sum = part(first);
+    for (int c = 64 + lane; c < a.pieces; c += 64) {
+        const VerifyStat v = s[c];
+        if (v.max == m) at = min(at, v.at);
+        sum += part(v);
     }
     return VerifyStat{m, wave_min(at), wave_sum(sum)};
 }
 
-// p of one token from its row's joined sums.
-__device__ __forceinline__ double prob(float logit, int token, const VerifyStat& s, bool greedy, double inv) {
-    if (greedy) return token == s.at ? 1.0 : 0.0;
-    return exp(((double)clean(logit) - (double)s.max) * inv) / s.sum;
-}
-
 __device__ __forceinline__ bool has_distribution(const VerifyStat& s) { return s.max > -INFINITY && s.max < INFINITY; }
 
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(const VerifyArgs a) {
-    __shared__ int refused;
-    __shared__ double wsum[4], wrest[4];
-    const int r = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x % a.pieces;
-    const int t = threadIdx.x, wave = t >> 6;
+// The sum over the workgroup, to every thread.
+__device__ __forceinline__ double block_sum(double v, double* shared) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kDrawWaves; w++) s += shared[w];
+    return s;
+}
+
+// The sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double u = __shfl_up(v, off, 64);
+        if (lane >= off) v += u;
+    }
+    return v;
+}
+
+// Bound by the chain of dependent reads: the offsets, the rows' sums and the drafts' values, the piece to draw from.
+template <bool kProbs>
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyArgs a) {
+    constexpr int kEach = kPiece / kDrawThreads;
+    __shared__ double powers[32], shared[kDrawWaves];
+    __shared__ int first, found, last;
+    __shared__ VerifyStat drawn;
+    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x;
+    if (r >= a.requests) return;
+    const int t = threadIdx.x, wave = wave_id(), lane = t & 63;
     const int row0 = a.row_offsets[r], end = a.row_offsets[r + 1];
-    if (row0 < 0 || end <= row0 || end > a.rows) {
-        if (piece == 0 && t == 0) {
-            a.accepted[r] = -1;
-            a.pick[r].row = -1;
-        }
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    fill_powers(powers);
+    if (row0 < 0 || end <= row0 || end > a.rows) {  // no such request
+        if (piece == 0 && t == 0) a.accepted[r] = -1;
         return;
     }
     const int n = end - row0 - 1;
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
     const bool greedy = is_greedy(temperature);
     const double inv = greedy ? 0.0 : 1.0 / (double)temperature;
-    if (t == 0) refused = n;
-    __syncthreads();
-    for (int i = wave; i < n; i += 4) {
-        const VerifyStat s = join_row(a, row0 + i, inv);
-        const int d = row0 - r + i;  // draft i of the request among all drafts
-        bool ok = false;
-        if (d >= 0 && d < a.drafts && has_distribution(s)) {
-            const int x = a.draft_tokens[d];
-            if (x >= 0 && x < a.vocab) {
-                const double p = prob(a.logits[(int64_t)(row0 + i) * a.vocab + x], x, s, greedy, inv);
-                const float q = a.draft_probs ? fmaxf(a.draft_probs[(int64_t)d * a.vocab + x], 0.0f) : 1.0f;
-                ok = (double)a.accept_uniforms[d] * (double)q < p;
-            }
-        }
-        if (!ok && (t & 63) == 0) atomicMin(&refused, i);
-    }
-    __syncthreads();
-    const int kept = refused;
-    const int row = row0 + kept;
-    const VerifyStat s = join_row(a, row, inv);
-    const int d = row0 - r + kept;
-    const bool rest = kept < n && d >= 0 && d < a.drafts;  // draw from max(p - q, 0)
-    if (piece == 0) {
-        if (t == 0) {
-            a.accepted[r] = kept;
-            a.pick[r] = VerifyPick{row, rest ? d : -1, s};
-        }
-        for (int i = t; i <= n; i += kThreads)
-            if (i != kept) a.tokens[row0 + i] = i < kept ? a.draft_tokens[row0 - r + i] : -1;
-    }
-    const int lo = piece * kPiece;
-    double sum = 0.0, left = 0.0;
-    if (has_distribution(s)) {
-        float v[4 * kVecs], q[4 * kVecs];
-        load_piece(a.logits + (int64_t)row * a.vocab, a.vocab, lo, t, -INFINITY, v);
-        const int x = rest && !a.draft_probs ? a.draft_tokens[d] : -1;
-        if (rest && a.draft_probs) load_piece(a.draft_probs + (int64_t)d * a.vocab, a.vocab, lo, t, 0.0f, q);
-#pragma unroll
-        for (int i = 0; i < 4 * kVecs; i++) {
-            const int token = lo + 4 * ((i >> 2) * kThreads + t) + (i & 3);
-            const double p = token < a.vocab ? prob(v[i], token, s, greedy, inv) : 0.0;
-            sum += p;
-            if (rest && a.draft_probs)
-                left += fmax(p - (double)fmaxf(q[i], 0.0f), 0.0);
-            else
-                left += token == x ? 0.0 : p;
-        }
-    }
-    sum = wave_sum(sum);
-    left = wave_sum(left);
-    if ((t & 63) == 0) {
-        wsum[wave] = sum;
-        wrest[wave] = left;
-    }
-    __syncthreads();
     if (t == 0) {
-        double* part = a.parts + 2 * ((int64_t)r * a.pieces + piece);
-        part[0] = (wrest[0] + wrest[1]) + (wrest[2] + wrest[3]);
-        part[1] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
-    }
-}
-
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyArgs a) {
-    __shared__ double run[kThreads];
-    __shared__ int found, last;
-    const int r = blockIdx.x, t = threadIdx.x;
-    const VerifyPick pk = a.pick[r];
-    if (pk.row < 0) return;
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-    const bool greedy = is_greedy(temperature);
-    const double inv = greedy ? 0.0 : 1.0 / (double)temperature;
-    const double* part = a.parts + 2 * (int64_t)r * a.pieces;
-    // the totals of both weights, and the piece that the draw falls into (every thread the same)
-    double total = 0.0, total_p = 0.0;
-    for (int c = 0; c < a.pieces; c++) {
-        total += part[2 * c];
-        total_p += part[2 * c + 1];
-    }
-    const bool rest = pk.draft >= 0 && total > 0.0;  // nothing left of p beside q: draw from p
-    if (!rest) total = total_p;
-    if (!(total > 0.0)) {  // no finite logit
-        if (t == 0) a.tokens[pk.row] = -1;
-        return;
-    }
-    const double target = (double)a.final_uniforms[r] * total;
-    double before = 0.0;
-    int piece = -1, some = 0;
-    double at_some = 0.0;
-    for (int c = 0; c < a.pieces && piece < 0; c++) {
-        const double w = part[2 * c + (rest ? 0 : 1)];
-        if (w > 0.0) {
-            some = c;
-            at_some = before;
-            if (before + w > target) piece = c;
-        }
-        before += w;
-    }
-    if (piece < 0) piece = some;  // rounding at the very end: the last token with a weight
-    before = at_some;
-    // 32 consecutive tokens a thread
-    constexpr int kEach = kPiece / kThreads;
-    const int lo = piece * kPiece + t * kEach;
-    const float* lg = a.logits + (int64_t)pk.row * a.vocab;
-    const float* q = rest && a.draft_probs ? a.draft_probs + (int64_t)pk.draft * a.vocab : nullptr;
-    const int x = rest && !a.draft_probs ? a.draft_tokens[pk.draft] : -1;
-    double w[kEach], mine = 0.0;
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int token = lo + i;
-        double p = 0.0;
-        if (token < a.vocab) {
-            p = prob(lg[token], token, pk.stat, greedy, inv);
-            if (q) p = fmax(p - (double)fmaxf(q[token], 0.0f), 0.0);
-            if (token == x) p = 0.0;
-        }
-        w[i] = p;
-        mine += p;
-    }
-    if (t == 0) {
+        first = n;
         found = 0x7fffffff;
         last = -1;
     }
-    run[t] = mine;
     __syncthreads();
-    double sum = before;
-    for (int i = 0; i < t; i++) sum += run[i];
-    int hit = 0x7fffffff, mine_last = -1;
+    // the first row that a wave does not keep; row n, behind the last draft, is none's to keep
+    int kept = 0x7fffffff;
+    VerifyStat s{};
+    for (int i = wave; i <= n; i += kDrawWaves) {
+        const int d = row0 - r + i;  // draft i of the request among all drafts
+        const bool draft = i < n && d >= 0 && d < a.drafts;
+        int x = -1;
+        float logit = 0.0f, q = 1.0f, u = 0.0f;
+        if (draft) {
+            x = a.draft_tokens[d];
+            u = a.accept_uniforms[d];
+            if (x >= 0 && x < a.vocab) {
+                logit = clean(a.logits[(int64_t)(row0 + i) * a.vocab + x]);
+                if (kProbs) q = fmaxf(a.draft_probs[(int64_t)d * a.vocab + x], 0.0f);
+            }
+        }
+        s = join_row(a, row0 + i, inv, powers);
+        bool ok = false;
+        if (x >= 0 && x < a.vocab && has_distribution(s)) {
+            const double p = greedy ? (x == s.at ? 1.0 : 0.0) : negative_exp<true>(((double)logit - (double)s.max) * inv, powers) / s.sum;
+            ok = (double)u * (double)q < p;
+        }
+        if (!ok) {
+            kept = i;
+            break;
+        }
+    }
+    if (kept < n && lane == 0) atomicMin(&first, kept);
+    __syncthreads();
+    if (kept == first && lane == 0) drawn = s;
+    kept = first;
+    __syncthreads();
+    s = drawn;
+    const int row = row0 + kept, d = row0 - r + kept;
+    if (piece == 0) {
+        if (t == 0) a.accepted[r] = kept;
+        for (int i = t; i <= n; i += kDrawThreads)
+            if (i != kept) a.tokens[row0 + i] = i < kept ? a.draft_tokens[row0 - r + i] : -1;
+    }
+    if (greedy || !has_distribution(s)) {  // without q's part of it the weight is on one token still
+        if (piece == 0 && t == 0) a.tokens[row] = has_distribution(s) ? s.at : -1;
+        return;
+    }
+    bool rest = kept < n && d >= 0 && d < a.drafts;  // draw from max(p - q, 0)
+    const double scale = 1.0 / s.sum;
+    const float* logits = a.logits + (int64_t)row * a.vocab;
+    const float* probs = kProbs && rest ? a.draft_probs + (int64_t)d * a.vocab : nullptr;
+    const int x = !kProbs && rest ? a.draft_tokens[d] : -1;
+    auto weight = [&](float logit, float q) {
+        const double p = negative_exp<true>(((double)clean(logit) - (double)s.max) * inv, powers) * scale;
+        return kProbs && rest ? fmax(p - (double)fmaxf(q, 0.0f), 0.0) : p;
+    };
+    double* parts = a.parts + (int64_t)r * a.pieces;
+    if (kProbs && rest) {
+        float v[kEach], q[kEach];
+        load_piece<kDrawThreads, false>(logits, a.vocab, piece * kPiece, -INFINITY, v);
+        load_piece<kDrawThreads, false>(probs, a.vocab, piece * kPiece, 0.0f, q);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) sum += weight(v[i], q[i]);
+        sum = block_sum(sum, shared);
+        // the last of the request's workgroups sees all parts: each is stored before its workgroup counts itself
+        if (t == 0) {
+            __hip_atomic_store(parts + piece, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            first = __hip_atomic_fetch_add(a.done + r, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (first != a.pieces - 1) return;
+    } else if (piece) {
+        return;
+    }
+    // The pieces' weights: the parts, or from the rows' sums, without the draft's own.
+    const VerifyStat* stats = a.stats + (int64_t)row * a.pieces;
+    double alone = -1.0;  // the weight of the draft's piece
+    auto of_piece = [&](int c) {
+        if (c >= a.pieces) return 0.0;
+        if (kProbs && rest) return __hip_atomic_load(parts + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (c == x / kPiece && alone >= 0.0) return alone;
+        const VerifyStat v = stats[c];
+        return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)s.max) * inv, powers) * scale : 0.0;
+    };
+    if (!kProbs && x >= 0 && x < a.vocab) {
+        const double all = of_piece(x / kPiece), left = all - weight(logits[x], 0.0f);
+        if (left > 1e-3 * all) {
+            alone = left;
+        } else {  // too little is left for a difference: the sum of the others
+            float v[kEach];
+            load_piece<kDrawThreads, false>(logits, a.vocab, x / kPiece * kPiece, -INFINITY, v);
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < kEach; i++)
+                sum += x / kPiece * kPiece + piece_at<kDrawThreads, false>(i >> 2) + (i & 3) == x ? 0.0 : weight(v[i], 0.0f);
+            alone = block_sum(sum, shared);
+        }
+    }
+    double total = 0.0;
+    auto add_up = [&] {
+        double sum = 0.0;
+        for (int c = lane; c < a.pieces; c += 64) sum += of_piece(c);
+        return wave_sum(sum);
+    };
+    total = add_up();
+    bool whole = false;
+    if (rest && !(total > 0.0)) {  // nothing left of p beside q: draw from p
+        rest = false;
+        whole = true;
+        alone = -1.0;
+        total = add_up();
+    }
+    const double target = (double)a.final_uniforms[r] * total;
+    // the piece in which the running sum passes (every wave the same)
+    double before = 0.0, some_before = 0.0;
+    int hit = -1, some = 0;
+    for (int c0 = 0; c0 < a.pieces && hit < 0; c0 += 64) {
+        const double w = of_piece(c0 + lane), upto = before + wave_scan(w);
+        const uint64_t any = __ballot(w > 0.0), over = __ballot(w > 0.0 && upto > target);
+        if (any) {
+            const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+            some = c0 + l;
+            const double prior = __shfl(upto, l ? l - 1 : 0, 64);
+            some_before = l ? prior : before;
+            if (over) hit = some;
+        }
+        before = __shfl(upto, 63, 64);
+    }
+    // rounding at the very end: the last token with a weight
+    const int lo = some * kPiece;
+    float v[kEach], q[kEach];
+    load_piece<kDrawThreads, true>(logits, a.vocab, lo, -INFINITY, v);
+    if (kProbs && rest) load_piece<kDrawThreads, true>(probs, a.vocab, lo, 0.0f, q);
+    double w[kEach], mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int token = lo + piece_at<kDrawThreads, true>(i >> 2) + (i & 3);
+        w[i] = token < a.vocab && (whole || token != x) ? weight(v[i], kProbs && rest ? q[i] : 0.0f) : 0.0;
+        mine += w[i];
+    }
+    const double upto = wave_scan(mine);
+    if (lane == 63) shared[wave] = upto;
+    __syncthreads();
+    double sum = some_before + (upto - mine);
+    for (int i = 0; i < wave; i++) sum += shared[i];
+    int at = 0x7fffffff, behind = -1;
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
         sum += w[i];
         if (w[i] > 0.0) {
-            if (sum > target && hit == 0x7fffffff) hit = lo + i;
-            mine_last = lo + i;
+            behind = lo + piece_at<kDrawThreads, true>(i >> 2) + (i & 3);
+            if (sum > target && at == 0x7fffffff) at = behind;
         }
     }
-    if (hit != 0x7fffffff) atomicMin(&found, hit);
-    if (mine_last >= 0) atomicMax(&last, mine_last);
+    if (at != 0x7fffffff) atomicMin(&found, at);
+    if (behind >= 0) atomicMax(&last, behind);
     __syncthreads();
-    if (t == 0) a.tokens[pk.row] = found != 0x7fffffff ? found : last;
+    if (t == 0) a.tokens[row] = found != 0x7fffffff ? found : last;
 }
 
 }  // namespace
 
 hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(verify_stats_kernel, dim3((unsigned)a.rows * (unsigned)a.pieces), dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL(verify_decide_kernel, dim3((unsigned)a.requests * (unsigned)a.pieces), dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)a.requests), dim3(kThreads), 0, st, a);
+    auto grid = [](int x, int n) {  // n in two dimensions
+        const unsigned y = (unsigned)(n < 65535 ? n : 65535);
+        return dim3((unsigned)x, y, ((unsigned)n + y - 1) / y);
+    };
+    hipLaunchKernelGGL(verify_stats_kernel, grid(a.pieces, a.rows), dim3(kThreads), 0, st, a);
+    if (a.draft_probs)
+        hipLaunchKernelGGL(verify_draw_kernel<true>, grid(a.pieces, a.requests), dim3(kDrawThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(verify_draw_kernel<false>, grid(1, a.requests), dim3(kDrawThreads), 0, st, a);
     return hipGetLastError();
 }
 
