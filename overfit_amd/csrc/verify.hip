@@ -31,22 +31,55 @@ constexpr int kPiece = kVerifyPiece;
 constexpr int kThreads = 256;  // of the first launch: 8 four-token loads a thread
 constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64;
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+// v of the lane that the DPP control names, `none` where there is no such lane: within 16 lanes (row_shr 1, 2, 4, 8), then the last
+// lane of the row before (row_bcast15) and of the 32 before (row_bcast31). Six steps scan a wave, some 10 cycles each, where a
+// shuffle goes through LDS.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t none) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, kCtrl, kRows, 0xf, false);
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double from_lane(double v) {  // + 0 where there is none
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = from_lane<kCtrl, kRows>((uint32_t)b, 0u), hi = from_lane<kCtrl, kRows>((uint32_t)(b >> 32), 0u);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane),
+                   hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+// The sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += from_lane<0x111, 0xf>(v);
+    v += from_lane<0x112, 0xf>(v);
+    v += from_lane<0x114, 0xf>(v);
+    v += from_lane<0x118, 0xf>(v);
+    v += from_lane<0x142, 0xa>(v);
+    v += from_lane<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) { return lane_of(wave_scan(v), 63); }
+
+template <class Op>
+__device__ __forceinline__ uint32_t wave_join(uint32_t v, uint32_t none, Op op) {
+    v = op(v, from_lane<0x111, 0xf>(v, none));
+    v = op(v, from_lane<0x112, 0xf>(v, none));
+    v = op(v, from_lane<0x114, 0xf>(v, none));
+    v = op(v, from_lane<0x118, 0xf>(v, none));
+    v = op(v, from_lane<0x142, 0xa>(v, none));
+    v = op(v, from_lane<0x143, 0xc>(v, none));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+    return as_float(wave_join(__builtin_bit_cast(uint32_t, v), 0xff800000u, [](uint32_t x, uint32_t y) {
+        return __builtin_bit_cast(uint32_t, fmaxf(as_float(x), as_float(y)));
+    }));
 }
-
 __device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
-    return v;
+    return (int)wave_join((uint32_t)v, 0x7fffffffu, [](uint32_t x, uint32_t y) { return (uint32_t)min((int)x, (int)y); });
 }
 
 // A NaN logit counts as -inf (the token has no probability).
@@ -116,7 +149,7 @@ __device__ __forceinline__ int owner_of(const VerifyArgs& a, int row) {
     return owner;
 }
 
-__global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void verify_stats_kernel(const VerifyArgs a) {
     constexpr int kEach = kPiece / kThreads;
     __shared__ double powers[32];
     __shared__ float wmax[4];
@@ -166,18 +199,18 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
     if (t == 0) a.stats[(int64_t)row * a.pieces + piece] = out;
 }
 
-// A row's pieces joined by one wave: the largest logit, its first token, and the sum of exponentials relative to it.
-__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers) {
+// A row's pieces joined by one wave: the largest logit, its first token, and the sum of exponentials relative to it. first: the
+// lane's piece; mine: its sum relative to the row's largest.
+__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers, const VerifyStat& first,
+                                               double& mine) {
     const VerifyStat* s = a.stats + (int64_t)row * a.pieces;
     const int lane = threadIdx.x & 63;
-    const VerifyStat none{-INFINITY, 0x7fffffff, 0.0};
-    const VerifyStat first = lane < a.pieces ? s[lane] : none;
     float m = first.max;
     for (int c = 64 + lane; c < a.pieces; c += 64) m = fmaxf(m, s[c].max);
     m = wave_max(m);
     auto part = [&](const VerifyStat& v) { return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)m) * inv, powers) : 0.0; };
     int at = first.max == m ? first.at : 0x7fffffff;
-    double sum = part(first);
+    double sum = mine = part(first);
     for (int c = 64 + lane; c < a.pieces; c += 64) {
         const VerifyStat v = s[c];
         if (v.max == m) at = min(at, v.at);
@@ -200,17 +233,6 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
     return s;
 }
 
-// The sum over the lanes up to this one.
-__device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double u = __shfl_up(v, off, 64);
-        if (lane >= off) v += u;
-    }
-    return v;
-}
-
 // Bound by the chain of dependent reads: the offsets, the rows' sums and the drafts' values, the piece to draw from.
 template <bool kProbs>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyArgs a) {
@@ -218,11 +240,12 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     __shared__ double powers[32], shared[kDrawWaves];
     __shared__ int first, found, last;
     __shared__ VerifyStat drawn;
+    __shared__ double pieces[64], chance;  // of the row to draw from: the first pieces' sums, and p of its draft
     const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x;
     if (r >= a.requests) return;
     const int t = threadIdx.x, wave = wave_id(), lane = t & 63;
     const int row0 = a.row_offsets[r], end = a.row_offsets[r + 1];
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f, final_u = a.final_uniforms[r];
     fill_powers(powers);
     if (row0 < 0 || end <= row0 || end > a.rows) {  // no such request
         if (piece == 0 && t == 0) a.accepted[r] = -1;
@@ -240,9 +263,12 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     // the first row that a wave does not keep; row n, behind the last draft, is none's to keep
     int kept = 0x7fffffff;
     VerifyStat s{};
+    double mine = 0.0, p = 0.0;
     for (int i = wave; i <= n; i += kDrawWaves) {
         const int d = row0 - r + i;  // draft i of the request among all drafts
         const bool draft = i < n && d >= 0 && d < a.drafts;
+        VerifyStat own{-INFINITY, 0x7fffffff, 0.0};
+        if (lane < a.pieces) own = a.stats[(int64_t)(row0 + i) * a.pieces + lane];
         int x = -1;
         float logit = 0.0f, q = 1.0f, u = 0.0f;
         if (draft) {
@@ -253,10 +279,11 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
                 if (kProbs) q = fmaxf(a.draft_probs[(int64_t)d * a.vocab + x], 0.0f);
             }
         }
-        s = join_row(a, row0 + i, inv, powers);
+        s = join_row(a, row0 + i, inv, powers, own, mine);
         bool ok = false;
+        p = 0.0;
         if (x >= 0 && x < a.vocab && has_distribution(s)) {
-            const double p = greedy ? (x == s.at ? 1.0 : 0.0) : negative_exp<true>(((double)logit - (double)s.max) * inv, powers) / s.sum;
+            p = greedy ? (x == s.at ? 1.0 : 0.0) : negative_exp<true>(((double)logit - (double)s.max) * inv, powers) / s.sum;
             ok = (double)u * (double)q < p;
         }
         if (!ok) {
@@ -266,7 +293,13 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     }
     if (kept < n && lane == 0) atomicMin(&first, kept);
     __syncthreads();
-    if (kept == first && lane == 0) drawn = s;
+    if (kept == first) {
+        pieces[lane] = mine;
+        if (lane == 0) {
+            drawn = s;
+            chance = p;
+        }
+    }
     kept = first;
     __syncthreads();
     s = drawn;
@@ -315,11 +348,12 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
         if (c >= a.pieces) return 0.0;
         if (kProbs && rest) return __hip_atomic_load(parts + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (c == x / kPiece && alone >= 0.0) return alone;
+        if (c < 64) return pieces[c] * scale;
         const VerifyStat v = stats[c];
         return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)s.max) * inv, powers) * scale : 0.0;
     };
     if (!kProbs && x >= 0 && x < a.vocab) {
-        const double all = of_piece(x / kPiece), left = all - weight(logits[x], 0.0f);
+        const double all = of_piece(x / kPiece), left = all - chance;
         if (left > 1e-3 * all) {
             alone = left;
         } else {  // too little is left for a difference: the sum of the others
@@ -332,13 +366,12 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
             alone = block_sum(sum, shared);
         }
     }
-    double total = 0.0;
     auto add_up = [&] {
-        double sum = 0.0;
-        for (int c = lane; c < a.pieces; c += 64) sum += of_piece(c);
+        double sum = of_piece(lane);
+        for (int c = 64 + lane; c < a.pieces; c += 64) sum += of_piece(c);
         return wave_sum(sum);
     };
-    total = add_up();
+    double total = add_up();
     bool whole = false;
     if (rest && !(total > 0.0)) {  // nothing left of p beside q: draw from p
         rest = false;
@@ -346,7 +379,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
         alone = -1.0;
         total = add_up();
     }
-    const double target = (double)a.final_uniforms[r] * total;
+    const double target = (double)final_u * total;
     // the piece in which the running sum passes (every wave the same)
     double before = 0.0, some_before = 0.0;
     int hit = -1, some = 0;
@@ -356,18 +389,18 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
         if (any) {
             const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
             some = c0 + l;
-            const double prior = __shfl(upto, l ? l - 1 : 0, 64);
-            some_before = l ? prior : before;
+            some_before = l ? lane_of(upto, l - 1) : before;
             if (over) hit = some;
         }
-        before = __shfl(upto, 63, 64);
+        before = lane_of(upto, 63);
     }
     // rounding at the very end: the last token with a weight
     const int lo = some * kPiece;
     float v[kEach], q[kEach];
     load_piece<kDrawThreads, true>(logits, a.vocab, lo, -INFINITY, v);
     if (kProbs && rest) load_piece<kDrawThreads, true>(probs, a.vocab, lo, 0.0f, q);
-    double w[kEach], mine = 0.0;
+    double w[kEach];
+    mine = 0.0;
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
         const int token = lo + piece_at<kDrawThreads, true>(i >> 2) + (i & 3);
