@@ -1678,7 +1678,7 @@ static int verify_impl(ovfq_ctx* ctx, const float* logits, int rows, int vocab, 
     void* dev[7];
     int *acc = accepted, *tok = tokens;
     auto carve = [&](Carver& c) {
-        a.stats = c.take<ovfq::VerifyStat>(R * a.pieces * sizeof(ovfq::VerifyStat));
+        a.stats = c.take<ovfq::VerifyStat>(R * a.pieces * 2 * sizeof(ovfq::VerifyStat));
         if (draft_probs) {
             a.parts = c.take<double>(Q * a.pieces * sizeof(double));
             a.done = c.take<int>(Q * sizeof(int));

@@ -326,7 +326,7 @@ struct NormArgs {
 hipError_t launch_residual_norm(const NormArgs& a, hipStream_t st);
 
 // Verification of drafted tokens (verify.hip); the scratch planes stats, parts and done are written by the launch.
-constexpr int kVerifyPiece = 8192;  // tokens a workgroup
+constexpr int kVerifyPiece = 4096;  // tokens whose sums are kept together
 struct VerifyStat {
     float max;   // largest logit
     int at;      // its first token (greedy requests)
@@ -342,7 +342,7 @@ struct VerifyArgs {
     const float* final_uniforms;   // [requests]
     int* accepted;               // [requests]
     int* tokens;                 // [rows]
-    VerifyStat* stats;
+    VerifyStat* stats;  // [rows][2 pieces]
     double* parts;  // [requests][pieces] and
     int* done;      // [requests], where there are draft_probs
     int rows, vocab, requests, drafts, pieces;

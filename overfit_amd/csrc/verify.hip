@@ -11,11 +11,11 @@
 // the rounding of a neighbour. An exponential is a power of two, a table's 2^(j / 32) and a polynomial of the rest (table-driven
 // range reduction as Tang published it in 1989), to 2e-15 of its value.
 //
-// Two launches. (1) A workgroup per row and 8192 tokens: the largest logit and the sum of exponentials relative to it. (2) A
+// Two launches. (1) A wave per row and 2048 tokens: the largest logit and the sum of exponentials relative to it. (2) A
 // workgroup per request: a wave a row joins the row's sums and decides the draft, the first refused wins; the sums of the row to
 // draw from are its pieces' weights already (a one-hot q takes its token's away), so that only the piece that the draw falls into
 // is read again. With the drafts' distributions the weights are max(p - q, 0) of all tokens: then a workgroup per request and
-// piece, and the last of a request to finish, by a counter, draws.
+// two pieces, and the last of a request to finish, by a counter, draws.
 #include <cmath>
 
 #include "ovfq_device.h"
@@ -28,7 +28,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 namespace {
 
 constexpr int kPiece = kVerifyPiece;
-constexpr int kThreads = 256;  // of the first launch: 8 four-token loads a thread
+constexpr int kHalf = kPiece / 2;  // a wave of the first launch
+constexpr int kThreads = 256;      // of the first launch
+constexpr int kSpan = 2;       // pieces a workgroup of the second sums up
 constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64;
 
 // v of the lane that the DPP control names, `none` where there is no such lane: within 16 lanes (row_shr 1, 2, 4, 8), then the last
@@ -112,24 +114,19 @@ __device__ __forceinline__ double negative_exp(double x, const double* powers) {
     return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(n >> 5) << 52));
 }
 
-// Tokens [lo, lo + kPiece) of a row of `vocab`, four at a time: vector i of thread t is tokens lo + 4 (i * kT + t) on or, kRuns,
-// lo + 4 (kVecs t + i) on; past the row `fill`.
-template <int kT, bool kRuns>
-__device__ __forceinline__ int piece_at(int i) {
-    return 4 * (kRuns ? kPiece / (4 * kT) * (int)threadIdx.x + i : i * kT + (int)threadIdx.x);
-}
-template <int kT, bool kRuns>
-__device__ __forceinline__ void load_piece(const float* row, int vocab, int lo, float fill, float (&v)[kPiece / kT]) {
-    const int n = min(kPiece, vocab - lo);
+// Tokens lo + 4 (i * kT + t) .. + 3, i < kN / 4, of a row of `vocab`; past the row `fill`.
+template <int kT, int kN>
+__device__ __forceinline__ void load_tokens(const float* row, int vocab, int lo, int t, float fill, float (&v)[kN]) {
+    const int n = min(kT * kN, vocab - lo);
     const __amdgpu_buffer_rsrc_t r = make_rsrc(row + lo, (uint32_t)n * 4);
-    u32x4 raw[kPiece / (4 * kT)];
+    u32x4 raw[kN / 4];
 #pragma unroll
-    for (int i = 0; i < kPiece / (4 * kT); i++) raw[i] = ld4(r, 4u * (uint32_t)piece_at<kT, kRuns>(i));
+    for (int i = 0; i < kN / 4; i++) raw[i] = ld4(r, 16u * (uint32_t)(i * kT + t));
 #pragma unroll
-    for (int i = 0; i < kPiece / (4 * kT); i++) {
+    for (int i = 0; i < kN / 4; i++) {
         const uint32_t a[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int c = 0; c < 4; c++) v[4 * i + c] = piece_at<kT, kRuns>(i) + c < n ? as_float(a[c]) : fill;
+        for (int c = 0; c < 4; c++) v[4 * i + c] = 4 * (i * kT + t) + c < n ? as_float(a[c]) : fill;
     }
 }
 
@@ -150,71 +147,80 @@ __device__ __forceinline__ int owner_of(const VerifyArgs& a, int row) {
 }
 
 __global__ __launch_bounds__(kThreads, 8) void verify_stats_kernel(const VerifyArgs a) {
-    constexpr int kEach = kPiece / kThreads;
+    constexpr int kEach = kHalf / 64;
     __shared__ double powers[32];
-    __shared__ float wmax[4];
-    __shared__ double wsum[4];
-    __shared__ int wmin[4];
-    const int row = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x;
+    const int row = (int)(blockIdx.z * gridDim.y + blockIdx.y), half = (int)blockIdx.x * (kThreads / 64) + wave_id();
+    const int lane = threadIdx.x & 63, lo = half * kHalf;
     if (row >= a.rows) return;
-    const int t = threadIdx.x, wave = t >> 6, lo = piece * kPiece;
-    float v[kEach];
-    load_piece<kThreads, false>(a.logits + (int64_t)row * a.vocab, a.vocab, lo, -INFINITY, v);
     fill_powers(powers);
-    if (a.done && !row && !piece)
-        for (int r = t; r < a.requests; r += kThreads) a.done[r] = 0;
-    const int request = owner_of(a, row);
-    if (request < 0) return;  // the whole workgroup
-    const float temperature = a.temperature ? a.temperature[request] : 1.0f;
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        v[i] = clean(v[i]);
-        m = fmaxf(m, v[i]);
-    }
-    m = wave_max(m);
-    if ((t & 63) == 0) wmax[wave] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    VerifyStat out{m, 0x7fffffff, 0.0};
-    if (is_greedy(temperature)) {
-        int at = 0x7fffffff;
+    if (a.done && !row && !blockIdx.x)
+        for (int r = threadIdx.x; r < a.requests; r += kThreads) a.done[r] = 0;
+    if (half >= 2 * a.pieces) return;
+    VerifyStat out{-INFINITY, 0x7fffffff, 0.0};
+    if (lo < a.vocab) {
+        float v[kEach];
+        load_tokens<64>(a.logits + (int64_t)row * a.vocab, a.vocab, lo, lane, -INFINITY, v);
+        const int request = owner_of(a, row);
+        if (request < 0) return;
+        const float temperature = a.temperature ? a.temperature[request] : 1.0f;
+        float m = -INFINITY;
 #pragma unroll
-        for (int i = kEach - 1; i >= 0; i--)
-            if (v[i] == m) at = lo + piece_at<kThreads, false>(i >> 2) + (i & 3);
-        at = wave_min(at);
-        if ((t & 63) == 0) wmin[wave] = at;
-        __syncthreads();
-        out.at = min(min(wmin[0], wmin[1]), min(wmin[2], wmin[3]));
-    } else if (m > -INFINITY && m < INFINITY) {
-        const double inv = 1.0 / (double)temperature;
-        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        for (int i = 0; i < kEach; i++) {
+            v[i] = clean(v[i]);
+            m = fmaxf(m, v[i]);
+        }
+        out.max = m = wave_max(m);
+        if (is_greedy(temperature)) {
+            int at = 0x7fffffff;
 #pragma unroll
-        for (int i = 0; i < kEach; i++) s[i & 3] += negative_exp<false>(((double)v[i] - (double)m) * inv, powers);
-        const double sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
-        if ((t & 63) == 0) wsum[wave] = sum;
-        __syncthreads();
-        out.sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+            for (int i = kEach - 1; i >= 0; i--)
+                if (v[i] == m) at = lo + 4 * ((i >> 2) * 64 + lane) + (i & 3);
+            out.at = wave_min(at);
+        } else if (m > -INFINITY && m < INFINITY) {
+            const double inv = 1.0 / (double)temperature;
+            double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int i = 0; i < kEach; i++) s[i & 3] += negative_exp<false>(((double)v[i] - (double)m) * inv, powers);
+            out.sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+        }
     }
-    if (t == 0) a.stats[(int64_t)row * a.pieces + piece] = out;
+    if (lane == 0) a.stats[(int64_t)row * 2 * a.pieces + half] = out;
+}
+
+struct Pair {
+    VerifyStat half[2];
+};
+__device__ __forceinline__ Pair load_pair(const VerifyArgs& a, int row, int piece) {
+    return *reinterpret_cast<const Pair*>(a.stats + ((int64_t)row * a.pieces + piece) * 2);
+}
+// A piece's sum relative to `most`.
+__device__ __forceinline__ double sum_of(const Pair& p, float most, double inv, const double* powers) {
+    double sum = 0.0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if (p.half[h].sum > 0.0) sum += p.half[h].sum * negative_exp<true>(((double)p.half[h].max - (double)most) * inv, powers);
+    return sum;
 }
 
 // A row's pieces joined by one wave: the largest logit, its first token, and the sum of exponentials relative to it. first: the
 // lane's piece; mine: its sum relative to the row's largest.
-__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers, const VerifyStat& first,
+__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers, const Pair& first,
                                                double& mine) {
-    const VerifyStat* s = a.stats + (int64_t)row * a.pieces;
     const int lane = threadIdx.x & 63;
-    float m = first.max;
-    for (int c = 64 + lane; c < a.pieces; c += 64) m = fmaxf(m, s[c].max);
-    m = wave_max(m);
-    auto part = [&](const VerifyStat& v) { return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)m) * inv, powers) : 0.0; };
-    int at = first.max == m ? first.at : 0x7fffffff;
-    double sum = mine = part(first);
+    float m = fmaxf(first.half[0].max, first.half[1].max);
     for (int c = 64 + lane; c < a.pieces; c += 64) {
-        const VerifyStat v = s[c];
-        if (v.max == m) at = min(at, v.at);
-        sum += part(v);
+        const Pair v = load_pair(a, row, c);
+        m = fmaxf(m, fmaxf(v.half[0].max, v.half[1].max));
+    }
+    m = wave_max(m);
+    auto first_of = [&](const Pair& p) { return p.half[0].max == m ? p.half[0].at : p.half[1].max == m ? p.half[1].at : 0x7fffffff; };
+    int at = first_of(first);
+    double sum = mine = sum_of(first, m, inv, powers);
+    for (int c = 64 + lane; c < a.pieces; c += 64) {
+        const Pair v = load_pair(a, row, c);
+        at = min(at, first_of(v));
+        sum += sum_of(v, m, inv, powers);
     }
     return VerifyStat{m, wave_min(at), wave_sum(sum)};
 }
@@ -237,11 +243,11 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 template <bool kProbs>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyArgs a) {
     constexpr int kEach = kPiece / kDrawThreads;
-    __shared__ double powers[32], shared[kDrawWaves];
+    __shared__ double powers[32], shared[kDrawWaves], totals[kSpan > kEach / 4 ? kSpan : kEach / 4][kDrawWaves];
     __shared__ int first, found, last;
     __shared__ VerifyStat drawn;
     __shared__ double pieces[64], chance;  // of the row to draw from: the first pieces' sums, and p of its draft
-    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x;
+    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), piece = (int)blockIdx.x * kSpan;
     if (r >= a.requests) return;
     const int t = threadIdx.x, wave = wave_id(), lane = t & 63;
     const int row0 = a.row_offsets[r], end = a.row_offsets[r + 1];
@@ -263,12 +269,13 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     // the first row that a wave does not keep; row n, behind the last draft, is none's to keep
     int kept = 0x7fffffff;
     VerifyStat s{};
-    double mine = 0.0, p = 0.0;
+    double mine = 0.0, p = 0.0;  // the lane's piece, and the draft's chance
     for (int i = wave; i <= n; i += kDrawWaves) {
         const int d = row0 - r + i;  // draft i of the request among all drafts
         const bool draft = i < n && d >= 0 && d < a.drafts;
-        VerifyStat own{-INFINITY, 0x7fffffff, 0.0};
-        if (lane < a.pieces) own = a.stats[(int64_t)(row0 + i) * a.pieces + lane];
+        const VerifyStat none{-INFINITY, 0x7fffffff, 0.0};
+        Pair own{{none, none}};
+        if (lane < a.pieces) own = load_pair(a, row0 + i, lane);
         int x = -1;
         float logit = 0.0f, q = 1.0f, u = 0.0f;
         if (draft) {
@@ -324,33 +331,47 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     };
     double* parts = a.parts + (int64_t)r * a.pieces;
     if (kProbs && rest) {
-        float v[kEach], q[kEach];
-        load_piece<kDrawThreads, false>(logits, a.vocab, piece * kPiece, -INFINITY, v);
-        load_piece<kDrawThreads, false>(probs, a.vocab, piece * kPiece, 0.0f, q);
-        double sum = 0.0;
+        float v[kSpan][kEach], q[kSpan][kEach];
 #pragma unroll
-        for (int i = 0; i < kEach; i++) sum += weight(v[i], q[i]);
-        sum = block_sum(sum, shared);
+        for (int h = 0; h < kSpan; h++) {  // (past the last piece: that one again, unused)
+            const int lo = min(piece + h, a.pieces - 1) * kPiece;
+            load_tokens<kDrawThreads>(logits, a.vocab, lo, t, -INFINITY, v[h]);
+            load_tokens<kDrawThreads>(probs, a.vocab, lo, t, 0.0f, q[h]);
+        }
+        double sum[kSpan];
+#pragma unroll
+        for (int h = 0; h < kSpan; h++) {
+            sum[h] = 0.0;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) sum[h] += weight(v[h][i], q[h][i]);
+            sum[h] = wave_sum(sum[h]);
+            if (lane == 0) totals[h][wave] = sum[h];
+        }
+        __syncthreads();
         // the last of the request's workgroups sees all parts: each is stored before its workgroup counts itself
         if (t == 0) {
-            __hip_atomic_store(parts + piece, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+            for (int h = 0; h < kSpan; h++) {
+                double all = 0.0;
+#pragma unroll
+                for (int o = 0; o < kDrawWaves; o++) all += totals[h][o];
+                if (piece + h < a.pieces) __hip_atomic_store(parts + piece + h, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
             first = __hip_atomic_fetch_add(a.done + r, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
-        if (first != a.pieces - 1) return;
+        if (first != (int)gridDim.x - 1) return;
     } else if (piece) {
         return;
     }
     // The pieces' weights: the parts, or from the rows' sums, without the draft's own.
-    const VerifyStat* stats = a.stats + (int64_t)row * a.pieces;
     double alone = -1.0;  // the weight of the draft's piece
     auto of_piece = [&](int c) {
         if (c >= a.pieces) return 0.0;
         if (kProbs && rest) return __hip_atomic_load(parts + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (c == x / kPiece && alone >= 0.0) return alone;
         if (c < 64) return pieces[c] * scale;
-        const VerifyStat v = stats[c];
-        return v.sum > 0.0 ? v.sum * negative_exp<true>(((double)v.max - (double)s.max) * inv, powers) * scale : 0.0;
+        return sum_of(load_pair(a, row, c), s.max, inv, powers) * scale;
     };
     if (!kProbs && x >= 0 && x < a.vocab) {
         const double all = of_piece(x / kPiece), left = all - chance;
@@ -358,11 +379,11 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
             alone = left;
         } else {  // too little is left for a difference: the sum of the others
             float v[kEach];
-            load_piece<kDrawThreads, false>(logits, a.vocab, x / kPiece * kPiece, -INFINITY, v);
+            load_tokens<kDrawThreads>(logits, a.vocab, x / kPiece * kPiece, t, -INFINITY, v);
             double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < kEach; i++)
-                sum += x / kPiece * kPiece + piece_at<kDrawThreads, false>(i >> 2) + (i & 3) == x ? 0.0 : weight(v[i], 0.0f);
+                sum += x / kPiece * kPiece + 4 * ((i >> 2) * kDrawThreads + t) + (i & 3) == x ? 0.0 : weight(v[i], 0.0f);
             alone = block_sum(sum, shared);
         }
     }
@@ -397,28 +418,41 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     // rounding at the very end: the last token with a weight
     const int lo = some * kPiece;
     float v[kEach], q[kEach];
-    load_piece<kDrawThreads, true>(logits, a.vocab, lo, -INFINITY, v);
-    if (kProbs && rest) load_piece<kDrawThreads, true>(probs, a.vocab, lo, 0.0f, q);
-    double w[kEach];
-    mine = 0.0;
+    load_tokens<kDrawThreads>(logits, a.vocab, lo, t, -INFINITY, v);
+    if (kProbs && rest) load_tokens<kDrawThreads>(probs, a.vocab, lo, t, 0.0f, q);
+    // four tokens a thread and stretch of 4 kDrawThreads
+    constexpr int kStretches = kEach / 4;
+    double w[kEach], fours[kStretches], upto[kStretches];
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-        const int token = lo + piece_at<kDrawThreads, true>(i >> 2) + (i & 3);
+        const int token = lo + 4 * ((i >> 2) * kDrawThreads + t) + (i & 3);
         w[i] = token < a.vocab && (whole || token != x) ? weight(v[i], kProbs && rest ? q[i] : 0.0f) : 0.0;
-        mine += w[i];
+        fours[i >> 2] = i & 3 ? fours[i >> 2] + w[i] : w[i];
     }
-    const double upto = wave_scan(mine);
-    if (lane == 63) shared[wave] = upto;
-    __syncthreads();
-    double sum = some_before + (upto - mine);
-    for (int i = 0; i < wave; i++) sum += shared[i];
-    int at = 0x7fffffff, behind = -1;
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        sum += w[i];
-        if (w[i] > 0.0) {
-            behind = lo + piece_at<kDrawThreads, true>(i >> 2) + (i & 3);
-            if (sum > target && at == 0x7fffffff) at = behind;
+    for (int i = 0; i < kStretches; i++) {
+        upto[i] = wave_scan(fours[i]);
+        if (lane == 63) totals[i][wave] = upto[i];
+    }
+    __syncthreads();
+    int at = 0x7fffffff, behind = -1;
+    double prior = some_before;
+#pragma unroll
+    for (int i = 0; i < kStretches; i++) {
+        double sum = prior + (upto[i] - fours[i]);
+#pragma unroll
+        for (int o = 0; o < kDrawWaves; o++) {
+            const double other = totals[i][o];
+            if (o < wave) sum += other;
+            prior += other;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            sum += w[4 * i + c];
+            if (w[4 * i + c] > 0.0) {
+                behind = lo + 4 * (i * kDrawThreads + t) + c;
+                if (sum > target && at == 0x7fffffff) at = behind;
+            }
         }
     }
     if (at != 0x7fffffff) atomicMin(&found, at);
@@ -434,9 +468,9 @@ hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st) {
         const unsigned y = (unsigned)(n < 65535 ? n : 65535);
         return dim3((unsigned)x, y, ((unsigned)n + y - 1) / y);
     };
-    hipLaunchKernelGGL(verify_stats_kernel, grid(a.pieces, a.rows), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(verify_stats_kernel, grid((2 * a.pieces + kThreads / 64 - 1) / (kThreads / 64), a.rows), dim3(kThreads), 0, st, a);
     if (a.draft_probs)
-        hipLaunchKernelGGL(verify_draw_kernel<true>, grid(a.pieces, a.requests), dim3(kDrawThreads), 0, st, a);
+        hipLaunchKernelGGL(verify_draw_kernel<true>, grid((a.pieces + kSpan - 1) / kSpan, a.requests), dim3(kDrawThreads), 0, st, a);
     else
         hipLaunchKernelGGL(verify_draw_kernel<false>, grid(1, a.requests), dim3(kDrawThreads), 0, st, a);
     return hipGetLastError();
