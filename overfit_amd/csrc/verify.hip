@@ -8,8 +8,9 @@
 // tokens together are then distributed as the target alone would draw them.
 //
 // Probabilities, totals and running sums are fp64: among 128256 running sums in fp32 a hundredth of all draws would land in
-// the rounding of a neighbour. An exponential is a power of two, a table's 2^(j / 32) and a polynomial of the rest (table-driven
-// range reduction as Tang published it in 1989), to 2e-15 of its value.
+// the rounding of a neighbour. An exponential is a power of two, a table's 2^(j / 128) and a polynomial of the rest (table-driven
+// range reduction as Tang published it in 1989): 14 instructions a token, where the library's exp() made the first launch take
+// 37.7 us on 240 rows of 128256 instead of 24.9 (4.9 TB/s, what a large copy reaches).
 //
 // Two launches. (1) A wave per row and 2048 tokens: the largest logit and the sum of exponentials relative to it. (2) A
 // workgroup per request: a wave a row joins the row's sums and decides the draft, the first refused wins; the sums of the row to
@@ -89,29 +90,41 @@ __device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : v;
 
 __device__ __forceinline__ bool is_greedy(float temperature) { return !(temperature > 0.0f && temperature < INFINITY); }
 
-// 2^(j / 32), j < 32, by the first threads of the workgroup; a barrier comes before its use.
-__device__ __forceinline__ void fill_powers(double* powers) {
-    if (threadIdx.x < 32) powers[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 32));
+// Exponentials of non-positive numbers. With z = x 128 / ln2 = n + f, n the nearest whole number, exp(x) = 2^(n / 128) 2^(f / 128);
+// the second factor is the Taylor polynomial of degree 3 of f ln2 / 128, |.| <= 0.0028, off by its fourth power / 24 < 2.5e-12. n
+// comes out of the low bits of a sum with 1.5 * 2^52. The table has 2^(j / 128), j < 128, less j << 13 in the high word, so that
+// n << 13 added to it puts the whole 2^(n / 128) together. (Running sums of 128256 probabilities that are off by 2.5e-12 each, now
+// up, now down, move a draw to a neighbour once in 10^8.)
+constexpr int kPowers = 128;
+constexpr double kMagic = 6755399441055744.0, kPer = 128 / 0.69314718055994530942;  // 1.5 * 2^52, 128 / ln2
+__device__ __forceinline__ void fill_powers(u32x2* powers) {  // a barrier comes before their use
+    const uint32_t j = threadIdx.x;
+    if (j >= (uint32_t)kPowers) return;
+    const u32x2 v = __builtin_bit_cast(u32x2, exp2((double)j * (1.0 / kPowers)));
+    powers[j] = u32x2{v.x, v.y - (j << 13)};
 }
-
-// exp(x), x <= 0. x = n ln2 / 32 + r with |r| <= ln2 / 64, so that the Taylor polynomial of degree 5 is off by r^6 / 720 < 2.3e-15;
-// n comes out of the low bits of a sum with 1.5 * 2^52. kZero: values below the normal range are right (0 in the end), else they
-// are about 1e-304, which no sum with a 1 in it sees.
-template <bool kZero>
-__device__ __forceinline__ double negative_exp(double x, const double* powers) {
-    constexpr double kMagic = 6755399441055744.0, kPer = 46.16624130844682903, kStep = 0.02166084939249829091;  // 32 / ln2, ln2 / 32
-    x = fmax(x, kZero ? -800.0 : -700.0);
+__device__ __forceinline__ double small_power(double f) {  // 2^(f / 128)
+    constexpr double c = 0.69314718055994530942 / 128;
+    return fma(f, fma(f, fma(f, c * c * c / 6, c * c / 2), c), 1.0);
+}
+__device__ __forceinline__ double whole_power(uint32_t n, const u32x2* powers) {  // 2^(n / 128) in the normal range
+    const u32x2 v = powers[n & (kPowers - 1)];
+    return __builtin_bit_cast(double, u32x2{v.x, v.y + (n << 13)});
+}
+__device__ __forceinline__ uint32_t low_word(double t) { return __builtin_bit_cast(u32x2, t).x; }
+// sum + exp(d per ln2 / 128), d <= 0; floor: the d of exp(-700), below which it is 1e-304, which no sum with a 1 in it sees.
+__device__ __forceinline__ double add_exp(double sum, double d, double per, double floor, const u32x2* powers) {
+    d = fmax(d, floor);
+    const double t = fma(d, per, kMagic);
+    const double f = fma(d, per, kMagic - t);
+    return fma(whole_power(low_word(t), powers), small_power(f), sum);
+}
+// exp(x), x <= 0, right below the normal range too: 0 in the end.
+__device__ __forceinline__ double negative_exp(double x, const u32x2* powers) {
+    x = fmax(x, -800.0);
     const double t = fma(x, kPer, kMagic);
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-    const double r = fma(-(t - kMagic), kStep, x);
-    double p = fma(r, 1.0 / 120, 1.0 / 24);
-    p = fma(r, p, 1.0 / 6);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0);
-    p *= powers[n & 31];
-    if constexpr (kZero) return ldexp(p, n >> 5);
-    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(n >> 5) << 52));
+    const uint32_t n = low_word(t);
+    return ldexp(whole_power(n & (kPowers - 1), powers) * small_power(fma(x, kPer, kMagic - t)), (int)n >> 7);
 }
 
 // Tokens lo + 4 (i * kT + t) .. + 3, i < kN / 4, of a row of `vocab`; past the row `fill`.
@@ -126,8 +139,12 @@ __device__ __forceinline__ void load_tokens(const float* row, int vocab, int lo,
     for (int i = 0; i < kN / 4; i++) {
         const uint32_t a[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int c = 0; c < 4; c++) v[4 * i + c] = 4 * (i * kT + t) + c < n ? as_float(a[c]) : fill;
+        for (int c = 0; c < 4; c++) v[4 * i + c] = as_float(a[c]);
     }
+    if (n == kT * kN) return;
+#pragma unroll
+    for (int i = 0; i < kN; i++)
+        if (4 * ((i >> 2) * kT + t) + (i & 3) >= n) v[i] = fill;
 }
 
 // The request that owns `row` (its offsets in order and within the rows), or -1; the same for every lane of the wave.
@@ -148,7 +165,7 @@ __device__ __forceinline__ int owner_of(const VerifyArgs& a, int row) {
 
 __global__ __launch_bounds__(kThreads, 8) void verify_stats_kernel(const VerifyArgs a) {
     constexpr int kEach = kHalf / 64;
-    __shared__ double powers[32];
+    __shared__ u32x2 powers[kPowers];
     const int row = (int)(blockIdx.z * gridDim.y + blockIdx.y), half = (int)blockIdx.x * (kThreads / 64) + wave_id();
     const int lane = threadIdx.x & 63, lo = half * kHalf;
     if (row >= a.rows) return;
@@ -166,10 +183,7 @@ __global__ __launch_bounds__(kThreads, 8) void verify_stats_kernel(const VerifyA
         const float temperature = a.temperature ? a.temperature[request] : 1.0f;
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            v[i] = clean(v[i]);
-            m = fmaxf(m, v[i]);
-        }
+        for (int i = 0; i < kEach; i++) m = fmaxf(m, v[i]);  // (passes over NaN, as add_exp's maximum does)
         out.max = m = wave_max(m);
         if (is_greedy(temperature)) {
             int at = 0x7fffffff;
@@ -178,10 +192,10 @@ __global__ __launch_bounds__(kThreads, 8) void verify_stats_kernel(const VerifyA
                 if (v[i] == m) at = lo + 4 * ((i >> 2) * 64 + lane) + (i & 3);
             out.at = wave_min(at);
         } else if (m > -INFINITY && m < INFINITY) {
-            const double inv = 1.0 / (double)temperature;
+            const double per = kPer / (double)temperature, floor = -700.0 * (double)temperature;
             double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-            for (int i = 0; i < kEach; i++) s[i & 3] += negative_exp<false>(((double)v[i] - (double)m) * inv, powers);
+            for (int i = 0; i < kEach; i++) s[i & 3] = add_exp(s[i & 3], (double)v[i] - (double)m, per, floor, powers);
             out.sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
         }
     }
@@ -195,17 +209,17 @@ __device__ __forceinline__ Pair load_pair(const VerifyArgs& a, int row, int piec
     return *reinterpret_cast<const Pair*>(a.stats + ((int64_t)row * a.pieces + piece) * 2);
 }
 // A piece's sum relative to `most`.
-__device__ __forceinline__ double sum_of(const Pair& p, float most, double inv, const double* powers) {
+__device__ __forceinline__ double sum_of(const Pair& p, float most, double inv, const u32x2* powers) {
     double sum = 0.0;
 #pragma unroll
     for (int h = 0; h < 2; h++)
-        if (p.half[h].sum > 0.0) sum += p.half[h].sum * negative_exp<true>(((double)p.half[h].max - (double)most) * inv, powers);
+        if (p.half[h].sum > 0.0) sum += p.half[h].sum * negative_exp(((double)p.half[h].max - (double)most) * inv, powers);
     return sum;
 }
 
 // A row's pieces joined by one wave: the largest logit, its first token, and the sum of exponentials relative to it. first: the
 // lane's piece; mine: its sum relative to the row's largest.
-__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const double* powers, const Pair& first,
+__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& a, int row, double inv, const u32x2* powers, const Pair& first,
                                                double& mine) {
     const int lane = threadIdx.x & 63;
     float m = fmaxf(first.half[0].max, first.half[1].max);
@@ -243,7 +257,8 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 template <bool kProbs>
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyArgs a) {
     constexpr int kEach = kPiece / kDrawThreads;
-    __shared__ double powers[32], shared[kDrawWaves], totals[kSpan > kEach / 4 ? kSpan : kEach / 4][kDrawWaves];
+    __shared__ u32x2 powers[kPowers];
+    __shared__ double shared[kDrawWaves], totals[kSpan > kEach / 4 ? kSpan : kEach / 4][kDrawWaves];
     __shared__ int first, found, last;
     __shared__ VerifyStat drawn;
     __shared__ double pieces[64], chance;  // of the row to draw from: the first pieces' sums, and p of its draft
@@ -290,7 +305,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
         bool ok = false;
         p = 0.0;
         if (x >= 0 && x < a.vocab && has_distribution(s)) {
-            p = greedy ? (x == s.at ? 1.0 : 0.0) : negative_exp<true>(((double)logit - (double)s.max) * inv, powers) / s.sum;
+            p = greedy ? (x == s.at ? 1.0 : 0.0) : negative_exp(((double)logit - (double)s.max) * inv, powers) / s.sum;
             ok = (double)u * (double)q < p;
         }
         if (!ok) {
@@ -326,7 +341,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
     const float* probs = kProbs && rest ? a.draft_probs + (int64_t)d * a.vocab : nullptr;
     const int x = !kProbs && rest ? a.draft_tokens[d] : -1;
     auto weight = [&](float logit, float q) {
-        const double p = negative_exp<true>(((double)clean(logit) - (double)s.max) * inv, powers) * scale;
+        const double p = negative_exp(((double)clean(logit) - (double)s.max) * inv, powers) * scale;
         return kProbs && rest ? fmax(p - (double)fmaxf(q, 0.0f), 0.0) : p;
     };
     double* parts = a.parts + (int64_t)r * a.pieces;
