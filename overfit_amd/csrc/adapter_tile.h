@@ -350,7 +350,7 @@ __device__ __forceinline__ void adapter_add(const AdapterArgs& e, const AdapterJ
 // flight at once, however many slots the rows have. kLowPass: ranks staged at a time.
 template <int T, int W, int kLowPass>
 struct AdapterOuts {
-    static constexpr int kOuts = 256 * T, kPer = kOuts > 64 * W ? kOuts / (64 * W) : 1;
+    static constexpr int kPer = (256 * T + 64 * W - 1) / (64 * W);  // (past the rows: no row has a key there)
     static constexpr int kLds = 16 * T * (kLowPass + 4);  // floats of `staged`
     AdapterTiles<T, 1> rows;
     AdapterStage<16 * T, kLowPass, 64 * W> stage;

@@ -1,7 +1,7 @@
 """Verification of drafted tokens (ovfq_verify_drafts[_dev]) against the rule written out request by request in 64 bits.
 
-Both sides keep probabilities and running sums in fp64, so counts and tokens are equal unless a given random number falls
-within about 1e-14 of a border: none of the inputs here is made to.
+Both sides keep probabilities and running sums in fp64 (the library's exponentials are within 2.5e-12 of their values), so counts
+and tokens are equal unless a given random number falls within about 1e-11 of a border: none of the inputs here is made to.
 """
 import ctypes
 import sys
@@ -262,6 +262,52 @@ def test_rows_behind_the_last_request_stay():
     ov.verify_drafts(dev(logits), 700, dev(off[:3]), few, uu, dev(last), None, None, acc, tok)
     assert np.array_equal(acc.cpu().numpy(), want[0])
     assert np.array_equal(tok.cpu().numpy()[:7], want[1]) and (tok[7:] == 99).all()
+
+
+# on both sides of a wave's 2048 logits and of the 64 pieces of 4096 tokens that a wave holds
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("counts,vocab", [((2, 1), 2047), ((2, 1), 2048), ((1, 3), 2049), ((2,), 4097), ((1, 2), 262144), ((2, 1), 262145),
+                                          ((1,), 400003)])
+def test_pieces(counts, vocab, probs):
+    case("pieces", counts, vocab, probs)
+    rng = np.random.default_rng(vocab)
+    for seed in range(3):
+        logits, off, tokens, u, last, q = make(rng, counts, vocab, probs)
+        u = F(1) - (F(1) - u) * F(0.3) * F(seed)  # some accepted, some refused; then none accepted
+        run(logits, off, tokens, np.minimum(u, np.nextafter(F(1), F(0))), last, q, rng.uniform(0.3, 2.0, len(counts)).astype(F))
+
+
+@pytest.mark.parametrize("lead", [8, 14, 20, 36])
+@pytest.mark.parametrize("vocab", [100, 9001])
+def test_a_refused_draft_that_had_nearly_everything(vocab, lead):
+    # what is left of its piece is smaller than the rounding of the piece's sum: it is summed without the draft
+    case("nearly everything", vocab, lead)
+    rng = np.random.default_rng(lead + vocab)
+    logits = rng.standard_normal((6, vocab)).astype(F)
+    at = rng.integers(0, vocab, 3)
+    for r in range(3):
+        logits[2 * r, at[r]] = F(lead)
+    off = np.array([0, 2, 4, 6], np.int32)
+    u = np.full(3, 1.0, F)  # refuses any draft
+    for last in (0.0, 0.35, 0.8, 0.99999):
+        run(logits, off, at.astype(np.int32), u, np.full(3, last, F))
+
+
+def test_logits_far_apart():
+    # beyond the smallest number's exponential: no weight, as in the 64-bit rule
+    case("far apart")
+    vocab = 5000
+    logits = np.full((4, vocab), -760.0, F)
+    logits[:, 4000] = 1.0
+    logits[1, 4100] = 0.5
+    logits[2, :] = np.float32(-3e38)
+    logits[2, 7] = np.float32(3e38)
+    logits[3, 4500] = -705.0
+    off = np.arange(5, dtype=np.int32)
+    none = np.zeros(0, np.int32)
+    for last in (0.0, 0.5, 0.999999):
+        run(logits, off, none, np.zeros(0, F), np.full(4, last, F))
+        run(logits, off, none, np.zeros(0, F), np.full(4, last, F), temperature=np.array([1.0, 0.01, 1e30, 5.0], F))
 
 
 def test_captured_call():
