@@ -6,8 +6,8 @@
 //
 // Bound: HBM for many rows (each input element is read once and each output written once; a row stays in registers between its
 // two norms), launch and two dependent reductions for one. A group of kT threads owns a row: 16 to 64 lanes for rows of up to
-// 1024 elements (several rows a workgroup, sums by lane exchanges alone), a workgroup of up to 1024 threads for rows of up to
-// 16384, and past that a workgroup that reads the row once per step.
+// 512 elements (several rows a workgroup, sums by lane exchanges alone), two to sixteen waves for rows of up to 16384, and past
+// that a workgroup that reads the row once per step.
 #include "ovfq_device.h"
 #include "ovfq_launch.h"
 
@@ -40,11 +40,27 @@ __device__ __forceinline__ float group_sum(float v, float* red, int& turn) {
     return v;
 }
 
-// The norm of one row of k elements held as kNV four-element pieces a thread; elements past the row are zero and stay out of
-// the sums.
+// A side's weights and biases for the thread's pieces.
 template <int kT, int kNV>
-__device__ __forceinline__ void norm_row(f32x4 (&v)[kNV], const f32x4 (&w)[kNV], const f32x4 (&b)[kNV], const NormSide& n,
-                                         int k, int t, float* red, int& turn) {
+struct Side {
+    f32x4 w[kNV], b[kNV];
+    __device__ __forceinline__ void load(const NormSide& n, int k, int t) {
+        const __amdgpu_buffer_rsrc_t wr = make_rsrc(n.weight, n.weight ? (uint32_t)k * 4 : 0u);
+        const __amdgpu_buffer_rsrc_t br = make_rsrc(n.bias, n.bias ? (uint32_t)k * 4 : 0u);
+#pragma unroll
+        for (int i = 0; i < kNV; i++) w[i] = ldf4(wr, 16u * (uint32_t)(t + i * kT));
+        if (n.bias) {
+#pragma unroll
+            for (int i = 0; i < kNV; i++) b[i] = ldf4(br, 16u * (uint32_t)(t + i * kT));
+        }
+    }
+};
+
+// The norm of one row of k elements held as kNV four-element pieces a thread; elements past the row are zero and stay out of
+// the sums. kLate: the side is loaded here, not before.
+template <int kT, int kNV, bool kLate>
+__device__ __forceinline__ void norm_row(f32x4 (&v)[kNV], Side<kT, kNV>& side, const NormSide& n, int k, int t, float* red,
+                                         int& turn) {
     const float inv_k = 1.0f / (float)k;
     if (n.layer) {
         float s = 0.0f;
@@ -65,25 +81,29 @@ __device__ __forceinline__ void norm_row(f32x4 (&v)[kNV], const f32x4 (&w)[kNV],
         for (int c = 0; c < 4; c++) s = fmaf(v[i][c], v[i][c], s);
     const float var = group_sum<kT>(s, red, turn) * inv_k;
     const float r = 1.0f / sqrtf(var + n.eps);
+    if (!kLate) {
 #pragma unroll
-    for (int i = 0; i < kNV; i++)
+        for (int i = 0; i < kNV; i++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            v[i][c] *= r;
-            if (n.weight) v[i][c] *= w[i][c];
-            if (n.bias) v[i][c] += b[i][c];
-        }
-}
-
-template <int kT, int kNV>
-__device__ __forceinline__ void load_side(const NormSide& n, int k, int t, f32x4 (&w)[kNV], f32x4 (&b)[kNV]) {
+            for (int c = 0; c < 4; c++) {
+                v[i][c] *= r;
+                if (n.weight) v[i][c] *= side.w[i][c];
+                if (n.bias) v[i][c] += side.b[i][c];
+            }
+        return;
+    }
+    // piece by piece
     const __amdgpu_buffer_rsrc_t wr = make_rsrc(n.weight, n.weight ? (uint32_t)k * 4 : 0u);
     const __amdgpu_buffer_rsrc_t br = make_rsrc(n.bias, n.bias ? (uint32_t)k * 4 : 0u);
 #pragma unroll
-    for (int i = 0; i < kNV; i++) w[i] = ldf4(wr, 16u * (uint32_t)(t + i * kT));
+    for (int i = 0; i < kNV; i++) v[i] *= r;
+    if (n.weight) {
+#pragma unroll
+        for (int i = 0; i < kNV; i++) v[i] *= ldf4(wr, 16u * (uint32_t)(t + i * kT));
+    }
     if (n.bias) {
 #pragma unroll
-        for (int i = 0; i < kNV; i++) b[i] = ldf4(br, 16u * (uint32_t)(t + i * kT));
+        for (int i = 0; i < kNV; i++) v[i] += ldf4(br, 16u * (uint32_t)(t + i * kT));
     }
 }
 
@@ -102,10 +122,11 @@ __device__ __forceinline__ void store_row(float* p, const f32x4 (&v)[kNV], int k
     }
 }
 
-// Rows of up to 4 * kT * kNV elements. Everything that the row needs is loaded before its first sum.
-template <int kT, int kNV>
-__global__ __launch_bounds__(kT < 256 ? 256 : kT) void residual_norm_kernel(const NormArgs a) {
-    constexpr int kRows = kT < 256 ? 256 / kT : 1;  // rows a workgroup
+// Rows of up to 4 * kT * kNV elements. Everything that the row needs is loaded before its first sum; kLate: the weights and the
+// gate only where they are used, so that twice the waves fit the registers.
+template <int kT, int kNV, bool kLate>
+__global__ __launch_bounds__(kT <= 64 ? 256 : kT, !kLate ? 1 : kNV == 4 && kT < 1024 ? 6 : 8) void residual_norm_kernel(const NormArgs a) {
+    constexpr int kRows = kT <= 64 ? 256 / kT : 1;  // rows a workgroup
     __shared__ float red[kT > 64 ? 2 * (kT / 64) : 1];
     const int t = kRows > 1 ? (int)threadIdx.x % kT : (int)threadIdx.x;
     const int64_t row0 = (int64_t)blockIdx.x * kRows;
@@ -117,37 +138,47 @@ __global__ __launch_bounds__(kT < 256 ? 256 : kT) void residual_norm_kernel(cons
     const int64_t left = a.rows - row0 < kRows ? a.rows - row0 : kRows;
     const uint32_t bytes = (uint32_t)left * (uint32_t)k * 4;
     const uint32_t base = (uint32_t)sub * (uint32_t)k * 4;
-    f32x4 v[kNV], h[kNV], g[kNV], pw[kNV], pb[kNV], qw[kNV], qb[kNV];
+    f32x4 v[kNV], h[kNV], g[kNV];
+    Side<kT, kNV> post, pre;
     auto load_plane = [&](const float* p, f32x4(&d)[kNV]) {
         const __amdgpu_buffer_rsrc_t r = make_rsrc(p + row0 * k, bytes);
 #pragma unroll
         for (int i = 0; i < kNV; i++) d[i] = ldf4(r, base + 16u * (uint32_t)(t + i * kT));
     };
-    load_plane(a.y, v);
-    if (a.h) load_plane(a.h, h);
-    if (a.has_post) load_side<kT, kNV>(a.post, k, t, pw, pb);
-    float g_row = a.scale;
-    if (a.gate_mode == kGateFull) {
-        load_plane(a.gate, g);
-    } else if (a.gate_mode == kGateChannel) {
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.gate, (uint32_t)k * 4);
+    auto load_gate = [&] {
+        if (a.gate_mode == kGateFull) {
+            load_plane(a.gate, g);
+        } else if (a.gate_mode == kGateChannel) {
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(a.gate, (uint32_t)k * 4);
 #pragma unroll
-        for (int i = 0; i < kNV; i++) g[i] = ldf4(r, 16u * (uint32_t)(t + i * kT));
-    } else if (a.gate_mode == kGateRow) {
+            for (int i = 0; i < kNV; i++) g[i] = ldf4(r, 16u * (uint32_t)(t + i * kT));
+        }
+    };
+    load_plane(a.y, v);
+    constexpr bool kLateH = kLate && kT == 1024 && kNV == 4;  // (does not fit the registers of two workgroups a CU)
+    if (a.h && !kLateH) load_plane(a.h, h);
+    float g_row = a.scale;
+    if (a.gate_mode == kGateRow) {
         const __amdgpu_buffer_rsrc_t r = make_rsrc(a.gate + row0, (uint32_t)left * 4);
         g_row *= as_float(ld1(r, (uint32_t)sub * 4));
     }
-    if (a.has_pre) load_side<kT, kNV>(a.pre, k, t, qw, qb);
+    if (!kLate) {
+        if (a.has_post) post.load(a.post, k, t);
+        load_gate();
+        if (a.has_pre) pre.load(a.pre, k, t);
+    }
 #pragma unroll
     for (int i = 0; i < kNV; i++)
 #pragma unroll
         for (int c = 0; c < 4; c++)
             if (4 * (t + i * kT) + c >= k) v[i][c] = 0.0f;
-    if (a.has_post) norm_row<kT, kNV>(v, pw, pb, a.post, k, t, red, turn);
+    if (a.has_post) norm_row<kT, kNV, kLate>(v, post, a.post, k, t, red, turn);
+    if (kLate) load_gate();
     if (a.gate_mode == kGateFull || a.gate_mode == kGateChannel) {
 #pragma unroll
         for (int i = 0; i < kNV; i++) v[i] *= g[i];
     }
+    if (a.h && kLateH) load_plane(a.h, h);
 #pragma unroll
     for (int i = 0; i < kNV; i++)
 #pragma unroll
@@ -158,7 +189,7 @@ __global__ __launch_bounds__(kT < 256 ? 256 : kT) void residual_norm_kernel(cons
     const bool live = row < a.rows;
     if (a.h_out && live) store_row<kT, kNV>(a.h_out + row * k, v, k, t);
     if (!a.has_pre) return;
-    norm_row<kT, kNV>(v, qw, qb, a.pre, k, t, red, turn);
+    norm_row<kT, kNV, kLate>(v, pre, a.pre, k, t, red, turn);
     if (live) store_row<kT, kNV>(a.x_out + row * k, v, k, t);
 }
 
@@ -217,27 +248,33 @@ __global__ __launch_bounds__(1024) void residual_norm_long_kernel(const NormArgs
     }
 }
 
-template <int kT, int kNV>
+template <int kT, int kNV, bool kLate>
 hipError_t launch(const NormArgs& a, hipStream_t st) {
-    constexpr int kRows = kT < 256 ? 256 / kT : 1;
-    hipLaunchKernelGGL((residual_norm_kernel<kT, kNV>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
-                       dim3(kT < 256 ? 256 : kT), 0, st, a);
+    constexpr int kRows = kT <= 64 ? 256 / kT : 1;
+    hipLaunchKernelGGL((residual_norm_kernel<kT, kNV, kLate>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
+                       dim3(kT <= 64 ? 256 : kT), 0, st, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
+// Two pieces a thread and all loads first up to 2048 elements (the 161 registers of four pieces so leave three waves a SIMD); past
+// that the weights late (us, two norms, residual, channel gate, all first with four pieces / late with four / late with two:
+// 4096 wide 1 row 3.9 / 3.8 / 3.4, 512 rows 7.5 / 6.9 / 6.8, 1024 rows 14.7 / 12.7 / 12.9, 2048 rows 29.0 / 28.6 / 29.5; 2049 wide
+// 3000 rows 25.0 / 21.9 / 23.3; 8192 wide 1 row 4.5 / 4.3 / 4.2, 1024 rows 34.6 / 30.8 / 29.0; 1024 wide 64 rows 3.8 / 3.7 / 3.2, 8192
+// rows 27.9 / 28.2 / 27.3; 16384 wide 1 row 13.8 / 6.6, 512 rows 53.5 / 32.6; two pieces, first / late: 2048 wide 1 row 3.1 / 3.2, 4096 rows
+// 27.4 / 28.1; 512 wide 16384 rows 26.4 / 27.0). At 26 to 29 us these planes of 134 MB move at 4.6 to 5.1 TB/s, a large copy's rate.
 hipError_t launch_residual_norm(const NormArgs& a, hipStream_t st) {
     const int k = a.k;
-    if (k <= 64) return launch<16, 1>(a, st);
-    if (k <= 128) return launch<32, 1>(a, st);
-    if (k <= 256) return launch<64, 1>(a, st);
-    if (k <= 512) return launch<64, 2>(a, st);
-    if (k <= 1024) return launch<64, 4>(a, st);
-    if (k <= 2048) return launch<256, 2>(a, st);
-    if (k <= 4096) return launch<256, 4>(a, st);
-    if (k <= 8192) return launch<512, 4>(a, st);
-    if (k <= 16384) return launch<1024, 4>(a, st);
+    if (k <= 64) return launch<16, 1, false>(a, st);
+    if (k <= 128) return launch<32, 1, false>(a, st);
+    if (k <= 256) return launch<64, 1, false>(a, st);
+    if (k <= 512) return launch<64, 2, false>(a, st);
+    if (k <= 1024) return launch<128, 2, true>(a, st);
+    if (k <= 2048) return launch<256, 2, false>(a, st);
+    if (k <= 4096) return a.rows > 1024 ? launch<256, 4, true>(a, st) : launch<512, 2, true>(a, st);
+    if (k <= 8192) return launch<1024, 2, true>(a, st);
+    if (k <= 16384) return launch<1024, 4, true>(a, st);
     hipLaunchKernelGGL(residual_norm_long_kernel, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
     return hipGetLastError();
 }
