@@ -324,12 +324,12 @@ struct AdapterTiles {
 };
 
 // add() for out[T][4] and one output tile, kBy row tiles at a time (the registers that T at once would take).
-template <int T, int kBy, int kPass, int kThreads>
+template <int T, int kBy, int kPass, int kThreads, int kAhead = 1>
 __device__ __forceinline__ void adapter_add(const AdapterArgs& e, const AdapterJob& j, int m0, int n0, float (&out)[T][4], float* lds) {
     static_assert(T % kBy == 0, "whole groups of tiles");
 #pragma unroll
     for (int t0 = 0; t0 < T; t0 += kBy) {
-        AdapterTiles<kBy, 1, kPass> tiles;
+        AdapterTiles<kBy, 1, kPass, kAhead> tiles;
         tiles.load(e, j, m0 + 16 * t0);
         float v[kBy][1][4];
 #pragma unroll

@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_kernel(const std::conditio
                 for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
             bias_o = 0.0f;
             static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act), "staged products");
-            adapter_add<kSub, 2, 32, 256>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
+            adapter_add<kSub, 2, 32, 256, 2>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
         }
     }
     if (o >= n_out) return;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(512) void kquant_mfma_pair_kernel(const MArgs a, co
                 for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
             bias_o = 0.0f;
             static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act), "staged products");
-            adapter_add<kSub, 2, 32, 512>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
+            adapter_add<kSub, 2, 32, 512, 2>(ad, aj, n0, o0, out, reinterpret_cast<float*>(&act[0][0]));
         }
     }
     if (par != 0 || o >= n_out) return;
@@ -856,7 +856,7 @@ __global__ __launch_bounds__(512) void kquant_mfma_pairwide_kernel(const MArgs a
                 for (int i = 0; i < 4; i++) out[s][i] = bias_o + out[s][i];
             bias_o = 0.0f;
             static_assert(AdapterTiles<2, 1, 32>::kLds * 4 <= (int)sizeof(act00), "staged products");
-            adapter_add<2 * kSubH, 2, 32, 512>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act00));
+            adapter_add<2 * kSubH, 2, 32, 512, 2>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act00));
         }
     }
     if (par != 0 || o >= n_out) return;
@@ -1056,7 +1056,7 @@ __global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a,
             // (gate/up at 512 rows, 512 x 4096 -> 2 x 14336 of Q4_K and ranks to 16: 184 us for the call, the projection alone 157,
             // four tiles of 32 ranks 186, two 189; with a launch of their own behind the projection the adapters cost 54).
             static_assert(AdapterTiles<8, 1, 16>::kLds * 4 <= (int)sizeof(act0), "staged products");
-            adapter_add<2 * kSubH, 8, 16, 256>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act0));
+            adapter_add<2 * kSubH, 8, 16, 256, 2>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act0));
         }
     }
     if (o >= n_out) return;
