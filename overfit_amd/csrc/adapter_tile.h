@@ -1,9 +1,11 @@
 // adapter_tile.h — B times the rows' low-rank products, for the epilogues of the projection kernels and for the launch that
 // adds adapters to finished outputs (adapters.hip). Products and sums are fp32 whatever the adapters are kept in.
 //
-// Rows share a multiplication only where they share the slot: a tile's slots are taken in turn, each multiplied over fp32 MFMA
-// (16x16x4) with all rows of the tile, and its results go to its own rows only, by selection and not by a zero factor, so that an
-// infinity in one request's adapter stays out of the others' rows.
+// Rows share a multiplication only where they share the slot. Tiles of few slots (a prompt's): the slots in turn, each multiplied
+// over fp32 MFMA (16x16x4) with the tile's rows, and its results go to its own rows only, by selection and not by a zero factor, so
+// that an infinity in one request's adapter stays out of the others' rows. Tiles of many (a decode step's): row by row, each
+// output's lane with the row of B that its slot names, so that the loads are in flight together, where the walk over the slots
+// waits for each group of them.
 #pragma once
 
 #include "ovfq_device.h"
@@ -169,11 +171,57 @@ __device__ __forceinline__ float adapter_dot(const AdapterArgs& e, const Adapter
     return sum;
 }
 
+// The same for half as many ranks of fp32 adapters, in eight registers: 16 ranks of the 16-bit types, 8 of fp32.
+struct AdapterOct {
+    u32x4 w[2];
+
+    __device__ __forceinline__ static int ranks(const AdapterArgs& e) { return e.type == kAdapterF32 ? 8 : 16; }
+    __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, AdapterRow row, int n, int r0) {
+        const int end = row.pad() - r0, steps = adapter_tiles16(row.pad());
+        const char* b = adapter_b(e, j, row.slot());
+        auto at = [&](int q) {
+            return b + (size_t)adapter_b_at(n, 4 * q < end ? r0 + 4 * q : r0, steps) * adapter_elem(e.type);
+        };
+        if (e.type == kAdapterF32) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) w[q] = *reinterpret_cast<const u32x4*>(at(q));
+        } else {
+            u32x2 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) v[q] = *reinterpret_cast<const u32x2*>(at(q));
+#pragma unroll
+            for (int q = 0; q < 2; q++) w[q] = u32x4{v[2 * q].x, v[2 * q].y, v[2 * q + 1].x, v[2 * q + 1].y};
+        }
+    }
+    __device__ __forceinline__ float add(const AdapterArgs& e, AdapterRow row, const float* low, int r0, float sum) const {
+        const int end = row.pad() - r0;
+        auto quad = [&](int q, u32x4 v) {
+            const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(low + 4 * q);
+            const adapter_f32x4 f = adapter_widen4(e.type, v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum = 4 * q < end ? fmaf(l[i], f[i], sum) : sum;
+        };
+        if (e.type == kAdapterF32) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) quad(q, w[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                quad(2 * q, u32x4{w[q].x, w[q].y, 0u, 0u});
+                quad(2 * q + 1, u32x4{w[q].z, w[q].w, 0u, 0u});
+            }
+        }
+        return sum;
+    }
+};
+
 // The adapters' part of a wave's outputs in the MFMA result layout: T tiles of 16 rows from m0 on and kN tiles of 16 outputs
 // from n0 on, lane (g, l16) holding rows 4 g .. 4 g + 3 of output l16 of each. All waves of the workgroup share the rows and call
-// load() and add() together. kPass: ranks staged at a time. kAhead: slots whose B values are loaded together.
-template <int T, int kN, int kPass = 32, int kAhead = 1>
+// load() and add() together. kPass: ranks staged at a time. kAhead: slots whose B values are loaded together. kTiles: row tiles
+// that go row by row at a time; 0: none do (that takes more registers than the tiled kernels have).
+template <int T, int kN, int kPass = 32, int kAhead = 1, int kTiles = 0>
 struct AdapterTiles {
+    static constexpr int kFew = 4;  // changes of the slot from row to row of a tile, up to which its slots are taken in turn
     uint32_t key[T];  // of row m0 + 16 t + l16
     float scale[T];
 
@@ -221,6 +269,48 @@ struct AdapterTiles {
             }
     }
 
+    // sum += B low of the ranks from r0 on for the tiles in `by_row`.
+    __device__ __forceinline__ void row_by_row(const AdapterArgs& e, const AdapterJob& j, int n0, int r0, int most, const float* lds,
+                                               const bool (&by_row)[T], adapter_f32x4 (&sum)[T][kN]) const {
+        const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+        const int step = AdapterOct::ranks(e), ranks = most - r0 < kPass ? most - r0 : kPass;
+#pragma unroll
+        for (int t0 = 0; t0 < T; t0 += kTiles) {
+            bool any = false;
+#pragma unroll
+            for (int t = t0; t < T && t < t0 + kTiles; t++) any = any || by_row[t];
+            if (!any) continue;
+#pragma unroll
+            for (int c = 0; c < kN; c++) {
+                const int n = n0 + 16 * c + l16;
+                AdapterRow row[kTiles][4];
+#pragma unroll
+                for (int t = 0; t < kTiles && t0 + t < T; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        row[t][i] = AdapterRow{(uint32_t)__shfl((int)key[t0 + t], 4 * g + i, 64), 0.0f};
+                        if (!by_row[t0 + t] || n >= j.out) row[t][i].key = 0;
+                    }
+#pragma unroll 1
+                for (int h = 0; h < ranks; h += step) {
+                    AdapterOct b[kTiles][4];
+#pragma unroll
+                    for (int t = 0; t < kTiles && t0 + t < T; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (row[t][i].pad() > r0 + h) b[t][i].load(e, j, row[t][i], n, r0 + h);
+#pragma unroll
+                    for (int t = 0; t < kTiles && t0 + t < T; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (row[t][i].pad() > r0 + h)
+                                sum[t0 + t][c][i] = b[t][i].add(e, row[t][i], lds + (16 * (t0 + t) + 4 * g + i) * kRow + h, r0 + h,
+                                                                sum[t0 + t][c][i]);
+                }
+            }
+        }
+    }
+
     // out[t][c][i] += scale * (B low) for the rows that have an adapter. The products of all rows with a slot's B go on from the
     // sums, and the slot's own rows keep them.
     template <int kThreads>
@@ -231,12 +321,18 @@ struct AdapterTiles {
         Stage staged;
         staged.load(e, j, m0, 0);
         uint32_t left[T], any = 0;
+        bool by_row[T];
         int most = 0;  // the largest padded rank
 #pragma unroll
         for (int t = 0; t < T; t++) {
             left[t] = (uint32_t)__ballot((key[t] & 0xffffu) != 0) & 0xffffu;
             any |= left[t];
             most = max(most, (int)(key[t] & 0xffffu));
+            by_row[t] = false;
+            if constexpr (!kTiles) continue;
+            const uint32_t above = (uint32_t)__builtin_amdgcn_update_dpp((int)key[t], (int)key[t], 0x111, 0xf, 0xf, false);  // row_shr:1
+            by_row[t] = __builtin_popcount((uint32_t)__ballot(key[t] != above) & 0xffffu) > kFew;
+            if (by_row[t]) left[t] = 0;
         }
         if (!any) return;
         uint32_t k[kAhead], rows[kAhead][T];
@@ -302,10 +398,11 @@ struct AdapterTiles {
                 }
                 next(r0);
             }
+            if constexpr (kTiles > 0) row_by_row(e, j, n0, r0, most, lds, by_row, sum);
             r0 += kPass;
             if (r0 >= most) break;
 #pragma unroll
-            for (int t = 0; t < T; t++) left[t] = (uint32_t)__ballot((int)(key[t] & 0xffffu) > r0) & 0xffffu;
+            for (int t = 0; t < T; t++) left[t] = by_row[t] ? 0u : (uint32_t)__ballot((int)(key[t] & 0xffffu) > r0) & 0xffffu;
             next(r0);
             adapter_barrier();
             Stage::fill(e, j, m0, r0, lds);

@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
     const int m0 = (int)blockIdx.x * 16, n0 = ((int)blockIdx.y * 4 + wave_id()) * 16 * kN;
     if (!j.slots || (int)blockIdx.y * 64 * kN >= j.out) return;
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    AdapterTiles<1, kN, 32, 2> tiles;
+    AdapterTiles<1, kN, 32, 2, 1> tiles;
     tiles.load(a, j, m0);
     const uint32_t any = (uint32_t)__ballot((tiles.key[0] & 0xffffu) != 0) & 0xffffu;
     float y[1][kN][4];

@@ -602,7 +602,7 @@ __global__ __launch_bounds__(256, 2) void kquant_mfma_panel_kernel(const PanelAr
     stage(0, act0, bs0, sc0);
     asm volatile("" ::: "memory");
     fetch(1, 1);
-    [[maybe_unused]] AdapterTiles<T, 1, 32, 4> low;
+    [[maybe_unused]] AdapterTiles<T, 1, 32, 4, T == 1 ? 1 : 2> low;
     [[maybe_unused]] AdapterJob aj;
     if constexpr (kAd) {
         aj = adapter_job(ad, job);

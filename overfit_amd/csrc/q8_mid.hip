@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void q8_0_panel_kernel(const Q8Args a, cons
     stage(1, act1, sc1);
     asm volatile("" ::: "memory");
     fetch(1);
-    [[maybe_unused]] AdapterTiles<T, 1, 32, 4> low;
+    [[maybe_unused]] AdapterTiles<T, 1, 32, 4, T == 1 ? 1 : 2> low;
     if constexpr (kAd) low.load(ad, ad.job[0], n0);
     int gi = 0;
     for (; gi + 2 < ng; gi += 3) {
