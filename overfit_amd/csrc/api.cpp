@@ -11,6 +11,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1412,7 +1413,8 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
         return fail(OVFQ_ERR_SIZE, "an adapter of rank %d for %d x %d is too large", max_rank, output_size, input_size);
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
-    ovfq_adapters* s = new ovfq_adapters();
+    ovfq_adapters* s = new (std::nothrow) ovfq_adapters();
+    if (!s) return fail(OVFQ_ERR_HIP, "no host memory for an adapter set");
     s->ctx = ctx;
     s->type = type;
     s->in = input_size;

@@ -1054,7 +1054,8 @@ __global__ __launch_bounds__(256, 4) void kquant_mfma_wide_kernel(const MArgs a,
             bias_o = 0.0f;
             // All eight row tiles at once, so that their loads are one latency, and 16 ranks at a time, which fits the registers
             // (gate/up at 512 rows, 512 x 4096 -> 2 x 14336 of Q4_K and ranks to 16: 184 us for the call, the projection alone 157,
-            // four tiles of 32 ranks 186, two 189; with a launch of their own behind the projection the adapters cost 54).
+            // four tiles of 32 ranks 186, two 189; with a launch of their own behind the projection the adapters cost 54), the
+            // B values of two slots together (184 -> 180).
             static_assert(AdapterTiles<8, 1, 16>::kLds * 4 <= (int)sizeof(act0), "staged products");
             adapter_add<2 * kSubH, 8, 16, 256, 2>(ad, aj, n0, o0, out, reinterpret_cast<float*>(act0));
         }
