@@ -59,6 +59,12 @@ __device__ __forceinline__ AdapterRow adapter_row(const AdapterArgs& e, const Ad
     return AdapterRow{v.x, as_float(scale)};
 }
 
+// Whether a tile goes row by row: its slot changes more than kAdapterFew times from row to row. key: of the tile's row l16.
+__device__ __forceinline__ bool adapter_many(uint32_t key) {
+    const uint32_t above = (uint32_t)__builtin_amdgcn_update_dpp((int)key, (int)key, 0x111, 0xf, 0xf, false);  // row_shr:1
+    return __builtin_popcount((uint32_t)__ballot(key != above) & 0xffffu) > kAdapterFew;
+}
+
 // The low-rank products of kRows (a multiple of 16) activation rows from m0 on, ranks r0 .. r0 + kRanks, their shares added: into
 // LDS rows of kRanks + 4 floats, by the kThreads threads of the workgroup. Rows past the launch's hold zeros. In two steps, so
 // that other loads can go out between: every load of the first is in flight at once (four shares at a time).
@@ -218,10 +224,10 @@ struct AdapterOct {
 // The adapters' part of a wave's outputs in the MFMA result layout: T tiles of 16 rows from m0 on and kN tiles of 16 outputs
 // from n0 on, lane (g, l16) holding rows 4 g .. 4 g + 3 of output l16 of each. All waves of the workgroup share the rows and call
 // load() and add() together. kPass: ranks staged at a time. kAhead: slots whose B values are loaded together. kTiles: row tiles
-// that go row by row at a time; 0: none do (that takes more registers than the tiled kernels have).
+// that go row by row at a time; 0: none do (that takes more registers than the tiled kernels have), and those that would are left
+// to the launch behind where there is one (by_row).
 template <int T, int kN, int kPass = 32, int kAhead = 1, int kTiles = 0>
 struct AdapterTiles {
-    static constexpr int kFew = 4;  // changes of the slot from row to row of a tile, up to which its slots are taken in turn
     uint32_t key[T];  // of row m0 + 16 t + l16
     float scale[T];
 
@@ -234,6 +240,7 @@ struct AdapterTiles {
             const AdapterRow r = adapter_row(e, j, m0 + 16 * t + (int)(threadIdx.x & 15));
             key[t] = r.key;
             scale[t] = r.scale;
+            if (!kTiles && e.by_row && adapter_many(key[t])) key[t] = 0;  // the launch behind has this tile
         }
     }
 
@@ -329,9 +336,7 @@ struct AdapterTiles {
             any |= left[t];
             most = max(most, (int)(key[t] & 0xffffu));
             by_row[t] = false;
-            if constexpr (!kTiles) continue;
-            const uint32_t above = (uint32_t)__builtin_amdgcn_update_dpp((int)key[t], (int)key[t], 0x111, 0xf, 0xf, false);  // row_shr:1
-            by_row[t] = __builtin_popcount((uint32_t)__ballot(key[t] != above) & 0xffffu) > kFew;
+            if constexpr (kTiles > 0) by_row[t] = adapter_many(key[t]);
             if (by_row[t]) left[t] = 0;
         }
         if (!any) return;

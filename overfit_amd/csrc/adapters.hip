@@ -241,31 +241,82 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 3) void adapter_shrink_kernel(co
             tl[t].row[m] = AdapterRow{info[t].rank > 0 ? (uint32_t)slot << 16 | (uint32_t)rank_pad(info[t].rank) : 0u, info[t].scale};
 }
 
-// Outputs that a projection kernel without adapters has written: grid (row tiles, output tiles, jobs), a wave per 16 rows x 64
-// outputs.
+// Outputs that a projection kernel without adapters has written, or the tiles of many slots that one has left: 16 rows x 256 outputs
+// a workgroup, an output a thread, four rows at a time with 16 ranks of their slots' B. A row's slot is the same for the whole
+// wave, so that B takes scalar resources and one offset a row; the low-rank products are LDS broadcasts. Bound by B, which every row
+// reads from L2: grid (8 * row tiles, groups of 8 output tiles, jobs), the row tiles of an output tile on one XCD (gate/up of 14336,
+// 256 rows over 32 slots of rank 16: 36.6 us, 55 with the tiles over MFMA layouts and per-lane addresses).
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
-    constexpr int kN = 4;
+    constexpr int kRow = 256 + 4;
     const AdapterJob j = adapter_job(a, (int)blockIdx.z);
-    __shared__ float low[AdapterTiles<1, kN>::kLds];
-    const int m0 = (int)blockIdx.x * 16, n0 = ((int)blockIdx.y * 4 + wave_id()) * 16 * kN;
-    if (!j.slots || (int)blockIdx.y * 64 * kN >= j.out) return;
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    AdapterTiles<1, kN, 32, 2, 1> tiles;
-    tiles.load(a, j, m0);
-    const uint32_t any = (uint32_t)__ballot((tiles.key[0] & 0xffffu) != 0) & 0xffffu;
-    float y[1][kN][4];
-    float* yp = j.y + (int64_t)(m0 + 4 * g) * j.out + n0 + l16;
+    __shared__ __align__(16) float low[16 * kRow];
+    const int m0 = ((int)blockIdx.x >> 3) * 16, o_tile = (int)blockIdx.y * 8 + ((int)blockIdx.x & 7);
+    if (!j.slots || o_tile * 256 >= j.out) return;
+    const AdapterRow row = adapter_row(a, j, m0 + (int)(threadIdx.x & 15));
+    if (a.by_row && !adapter_many(row.key)) return;  // the whole workgroup
+    if (!((uint32_t)__ballot(row.pad() != 0) & 0xffffu)) return;
+    // the products, their shares added
+    const int quads = a.low_stride / 4, left = min(16, a.rows - m0);
+    for (int m = (int)threadIdx.x / 16; m < left; m += 16)
+        for (int q = (int)threadIdx.x % 16; q < quads; q += 16) {
+            f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int s0 = 0; s0 < a.shares; s0 += 4) {
+                f32x4 v[4];
 #pragma unroll
-    for (int c = 0; c < kN; c++)
+                for (int s = 0; s < 4; s++) {
+                    const int64_t share = s0 + s < a.shares ? s0 + s : 0;
+                    v[s] = *reinterpret_cast<const f32x4*>(j.low + (share * a.rows + m0 + m) * a.low_stride + 4 * q);
+                }
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    if (s0 + s < a.shares) sum += v[s];
+            }
+            *reinterpret_cast<f32x4*>(low + m * kRow + 4 * q) = sum;
+        }
+    __syncthreads();
+    const int n = o_tile * 256 + (int)threadIdx.x;
+    const int elem = adapter_elem(a.type);
+#pragma unroll 1
+    for (int i0 = 0; i0 < left; i0 += 4) {
+        int pad[4], most = 0;
+        float scale[4], y[4], sum[4];
+        __amdgpu_buffer_rsrc_t br[4];
+        uint32_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)row.key, i0 + i);
+            pad[i] = (int)(key & 0xffffu);  // 0 past the rows
+            most = max(most, pad[i]);
+            scale[i] = as_float((uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint32_t, row.scale), i0 + i));
+            const int steps = adapter_tiles16(pad[i]);
+            br[i] = make_rsrc(adapter_b(a, j, pad[i] ? (int)(key >> 16) : 0), (uint32_t)(adapter_tiles16(j.out) * steps * 256 * elem));
+            at[i] = adapter_b_at(n, 0, steps) * (uint32_t)elem;
+            if (pad[i] && n < j.out) y[i] = j.y[(int64_t)(m0 + i0 + i) * j.out + n];
+            sum[i] = 0.0f;
+        }
+#pragma unroll 1
+        for (int r0 = 0; r0 < most; r0 += 16) {
+            u32x4 b[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)  // (past the slot's ranks: zeros or other outputs' values, unused)
+                    b[i][q] = adapter_load4(a.type, br[i], at[i] + (uint32_t)((r0 * 16 + q * 64) * elem));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if (r0 + 4 * q >= pad[i]) continue;
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(low + (i0 + i) * kRow + r0 + 4 * q);
+                    const adapter_f32x4 w = adapter_widen4(a.type, b[i][q]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sum[i] = fmaf(l[c], w[c], sum[i]);
+                }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (any >> (4 * g + i) & 1 && n0 + 16 * c + l16 < j.out) y[0][c][i] = yp[(int64_t)i * j.out + 16 * c];
-    tiles.add<256>(a, j, m0, n0, y, low);
-#pragma unroll
-    for (int c = 0; c < kN; c++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (any >> (4 * g + i) & 1 && n0 + 16 * c + l16 < j.out) yp[(int64_t)i * j.out + 16 * c] = y[0][c][i];
+            if (pad[i] && n < j.out) j.y[(int64_t)(m0 + i0 + i) * j.out + n] = fmaf(sum[i], scale[i], y[i]);
+    }
 }
 
 __global__ __launch_bounds__(256) void adapter_slot_kernel(AdapterSlot* info, int first, int count, int rank, float scale) {
@@ -331,10 +382,14 @@ void plan_adapters(AdapterArgs& a, int max_rank) {
     if (a.shares > most) a.shares = most;
     if (a.shares > kMostShares) a.shares = kMostShares;
     a.each = (a.in / 32 + kShrinkWaves * a.shares - 1) / (kShrinkWaves * a.shares);
-    // a workgroup for each of a tile's slots at a few rows, which may all differ; two at many, for the tiles where one request
-    // ends and the next begins
+    // A workgroup for each of a tile's slots at a few rows, which may all differ. At many, two, for the tiles where one request ends
+    // and the next begins; four with one rank tile and sets of more slots than the projections take in turn (us, two / four / eight:
+    // gate/up of 14336 at 256 rows, every row its own of 32 slots 27.4 / 16.3 / 17.2, three requests 7.7 / 7.7 / 12.1; down 14336 ->
+    // 4096 at 300 rows 67.4 / 41.0 / 27.5, 14.1 / 16.1 / 20.9; with two rank tiles, q/k/v of 4096 at 400 rows 33.0 / 33.4 / 29.8, 9.9 / 16.1 /
+    // 18.9: workgroups without a slot wait for a place all the same).
     a.way_shift = 0;
-    while (a.way_shift < (a.rows <= 64 ? 4 : 1) && 1 << a.way_shift < slots && 1 << a.way_shift < a.rows) a.way_shift++;
+    const int ways = a.rows <= 64 ? 4 : a.rank_tiles == 1 && slots > kAdapterFew ? 2 : 1;
+    while (a.way_shift < ways && 1 << a.way_shift < slots && 1 << a.way_shift < a.rows) a.way_shift++;
     a.shrink_x = tiles << a.way_shift;
 }
 
@@ -347,7 +402,7 @@ hipError_t launch_adapters_shrink(const AdapterArgs& a, const ActQuantJob& quant
 hipError_t launch_adapters_expand(const AdapterArgs& a, hipStream_t st) {
     int out = 0;
     for (int i = 0; i < a.jobs; i++) out = a.job[i].slots && a.job[i].out > out ? a.job[i].out : out;
-    hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)((a.rows + 15) / 16), (unsigned)((out + 255) / 256), (unsigned)a.jobs),
+    hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)((a.rows + 15) / 16 * 8), (unsigned)((out + 2047) / 2048), (unsigned)a.jobs),
                        dim3(256), 0, st, a);
     return hipGetLastError();
 }

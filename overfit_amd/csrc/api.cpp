@@ -472,7 +472,7 @@ bool quantize_in_launch(const ovfq_ctx* c, int type, int in, int rows, int count
 // where the launch adds them to the outputs itself.
 int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, const float* const* biases,
                       float* const* ys, int rows, ovfq::ActQ act, const float* x = nullptr,
-                      const ovfq::AdapterArgs* ad = nullptr, bool* ad_done = nullptr) {
+                      ovfq::AdapterArgs* ad = nullptr, bool* ad_done = nullptr) {
     ovfq::ProjJob jobs[ovfq::kMaxJobs];
     for (int i = 0; i < count; i++) {
         jobs[i].w = static_cast<const uint8_t*>(ws[i]->blocks);
@@ -488,7 +488,7 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     if (x && rows > 1 && !use_gemv_rows(c, type, in, rows, count, pair_out))
         return fail(OVFQ_ERR_SIZE, "in-launch quantisation of %d rows needs the multi-row decode kernel", rows);
     // the adapters, for a kernel that adds them where `fits` says so
-    auto in_epilogue = [&](bool (*fits)(int, int, const ovfq::AdapterArgs&)) -> const ovfq::AdapterArgs* {
+    auto in_epilogue = [&](bool (*fits)(int, int, const ovfq::AdapterArgs&)) -> ovfq::AdapterArgs* {
         if (!ad || !fits(in, rows, *ad)) return nullptr;
         *ad_done = true;
         return ad;
@@ -552,8 +552,16 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     } else if (use_gemv_rows(c, type, in, rows, count, pair_out)) {
         HIP_TRY(ovfq::launch_gemv_rows_kquant(type, jobs, count, in, rows, x, act, c->stream, in_epilogue(ovfq::gemv_rows_adapters)));
     } else if (use_tiled_mfma(c, type, jobs, count, in, rows)) {
+        if (ad) {
+            // Sets of many slots: the row tiles where they meet (a decode step's) are left to a launch behind, which takes them row
+            // by row (us: down 14336 -> 4096 at 300 rows, every row its own of 32 slots 254 -> 154, gate/up of 14336 at 256 rows 171 ->
+            // 132; three requests on 32 slots 118 -> 126 and 99 -> 100, that launch with nothing to do).
+            int slots = 0;
+            for (int i = 0; i < count; i++) slots = ad->job[i].slots > slots ? ad->job[i].slots : slots;
+            ad->by_row = slots > ovfq::kAdapterFew;
+            *ad_done = !ad->by_row;
+        }
         HIP_TRY(ovfq::launch_project_mfma(type, jobs, count, in, rows, act, c->stream, ad));
-        if (ad) *ad_done = true;
     } else if (small_mfma_enabled(rows) && ovfq::mfma_small_supported(type, in)) {
         // Few rows: 16-row MFMA tiles with super-block-parallel waves; a gate/up-shaped pair shares one launch.
         const bool pair = count == 2 && jobs[0].n_rows == jobs[1].n_rows;
@@ -1181,7 +1189,7 @@ static int project_impl(ovfq_ctx* ctx, int count, const ovfq_weight* const* ws, 
     const bool tiled = use_mid(ctx, in, rows, ws, count) != ovfq::MidKernel::kNone ||
                        use_q8_mid(ctx, in, rows, ws, count);
     bool ad_done = false;
-    const ovfq::AdapterArgs* ap = any_set ? &aa : nullptr;
+    ovfq::AdapterArgs* ap = any_set ? &aa : nullptr;
     if (any_set) {
         aa.x = xd;
         aa.row_slots = slots_d;
