@@ -240,7 +240,7 @@ struct AdapterTiles {
             const AdapterRow r = adapter_row(e, j, m0 + 16 * t + (int)(threadIdx.x & 15));
             key[t] = r.key;
             scale[t] = r.scale;
-            if (!kTiles && e.by_row && adapter_many(key[t])) key[t] = 0;  // the launch behind has this tile
+            if (e.by_row && adapter_many(key[t])) key[t] = 0;  // the launch behind has this tile
         }
     }
 

@@ -241,24 +241,26 @@ __global__ __launch_bounds__(64 * kShrinkWaves, 3) void adapter_shrink_kernel(co
             tl[t].row[m] = AdapterRow{info[t].rank > 0 ? (uint32_t)slot << 16 | (uint32_t)rank_pad(info[t].rank) : 0u, info[t].scale};
 }
 
-// Outputs that a projection kernel without adapters has written, or the tiles of many slots that one has left: 16 rows x 256 outputs
-// a workgroup, an output a thread, four rows at a time with 16 ranks of their slots' B. A row's slot is the same for the whole
-// wave, so that B takes scalar resources and one offset a row; the low-rank products are LDS broadcasts. Bound by B, which every row
-// reads from L2: grid (8 * row tiles, groups of 8 output tiles, jobs), the row tiles of an output tile on one XCD (gate/up of 14336,
-// 256 rows over 32 slots of rank 16: 36.6 us, 55 with the tiles over MFMA layouts and per-lane addresses).
+// Outputs that a projection kernel without adapters has written, or the tiles of many slots that one has left: 4 rows x 256 outputs a
+// workgroup, an output a thread, with 16 ranks of the rows' B at a time. A row's slot is the same for the whole wave, so that B
+// takes scalar resources and one offset a row; the low-rank products are LDS broadcasts. Bound by B, which every row reads from L2:
+// grid (8 * groups of rows, groups of 8 output tiles, jobs), the rows of an output tile on one XCD (gate/up of 14336, 256 rows over
+// 32 slots of rank 16: 40 us, 55 with the tiles over MFMA layouts and per-lane addresses).
+constexpr int kExpandRows = 4;
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
     constexpr int kRow = 256 + 4;
     const AdapterJob j = adapter_job(a, (int)blockIdx.z);
-    __shared__ __align__(16) float low[16 * kRow];
-    const int m0 = ((int)blockIdx.x >> 3) * 16, o_tile = (int)blockIdx.y * 8 + ((int)blockIdx.x & 7);
+    __shared__ __align__(16) float low[kExpandRows * kRow];
+    const int m0 = ((int)blockIdx.x >> 3) * kExpandRows, o_tile = (int)blockIdx.y * 8 + ((int)blockIdx.x & 7);
     if (!j.slots || o_tile * 256 >= j.out) return;
-    const AdapterRow row = adapter_row(a, j, m0 + (int)(threadIdx.x & 15));
+    const int l0 = m0 & 15;
+    const AdapterRow row = adapter_row(a, j, m0 - l0 + (int)(threadIdx.x & 15));  // of the rows' tile of 16
     if (a.by_row && !adapter_many(row.key)) return;  // the whole workgroup
-    if (!((uint32_t)__ballot(row.pad() != 0) & 0xffffu)) return;
+    if (!((uint32_t)__ballot(row.pad() != 0) >> l0 & ((1u << kExpandRows) - 1))) return;
     // the products, their shares added
-    const int quads = a.low_stride / 4, left = min(16, a.rows - m0);
-    for (int m = (int)threadIdx.x / 16; m < left; m += 16)
-        for (int q = (int)threadIdx.x % 16; q < quads; q += 16) {
+    const int quads = a.low_stride / 4;
+    if (const int m = wave_id(); m0 + m < a.rows)
+        for (int q = (int)threadIdx.x & 63; q < quads; q += 64) {
             f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
             for (int s0 = 0; s0 < a.shares; s0 += 4) {
                 f32x4 v[4];
@@ -273,50 +275,53 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
             }
             *reinterpret_cast<f32x4*>(low + m * kRow + 4 * q) = sum;
         }
-    __syncthreads();
     const int n = o_tile * 256 + (int)threadIdx.x;
     const int elem = adapter_elem(a.type);
-#pragma unroll 1
-    for (int i0 = 0; i0 < left; i0 += 4) {
-        int pad[4], most = 0;
-        float scale[4], y[4], sum[4];
-        __amdgpu_buffer_rsrc_t br[4];
-        uint32_t at[4];
+    int pad[kExpandRows], most = 0;
+    float scale[kExpandRows], y[kExpandRows], sum[kExpandRows];
+    __amdgpu_buffer_rsrc_t br[kExpandRows];
+    uint32_t at[kExpandRows];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)row.key, i0 + i);
-            pad[i] = (int)(key & 0xffffu);  // 0 past the rows
-            most = max(most, pad[i]);
-            scale[i] = as_float((uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint32_t, row.scale), i0 + i));
-            const int steps = adapter_tiles16(pad[i]);
-            br[i] = make_rsrc(adapter_b(a, j, pad[i] ? (int)(key >> 16) : 0), (uint32_t)(adapter_tiles16(j.out) * steps * 256 * elem));
-            at[i] = adapter_b_at(n, 0, steps) * (uint32_t)elem;
-            if (pad[i] && n < j.out) y[i] = j.y[(int64_t)(m0 + i0 + i) * j.out + n];
-            sum[i] = 0.0f;
-        }
-#pragma unroll 1
-        for (int r0 = 0; r0 < most; r0 += 16) {
-            u32x4 b[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++)  // (past the slot's ranks: zeros or other outputs' values, unused)
-                    b[i][q] = adapter_load4(a.type, br[i], at[i] + (uint32_t)((r0 * 16 + q * 64) * elem));
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (r0 + 4 * q >= pad[i]) continue;
-                    const f32x4 l = *reinterpret_cast<const f32x4*>(low + (i0 + i) * kRow + r0 + 4 * q);
-                    const adapter_f32x4 w = adapter_widen4(a.type, b[i][q]);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) sum[i] = fmaf(l[c], w[c], sum[i]);
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (pad[i] && n < j.out) j.y[(int64_t)(m0 + i0 + i) * j.out + n] = fmaf(sum[i], scale[i], y[i]);
+    for (int i = 0; i < kExpandRows; i++) {
+        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)row.key, l0 + i);
+        pad[i] = (int)(key & 0xffffu);  // 0 past the rows
+        most = max(most, pad[i]);
+        scale[i] = as_float((uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint32_t, row.scale), l0 + i));
+        const int steps = adapter_tiles16(pad[i]);
+        br[i] = make_rsrc(adapter_b(a, j, pad[i] ? (int)(key >> 16) : 0), (uint32_t)(adapter_tiles16(j.out) * steps * 256 * elem));
+        at[i] = adapter_b_at(n, 0, steps) * (uint32_t)elem;
+        if (pad[i] && n < j.out) y[i] = j.y[(int64_t)(m0 + i) * j.out + n];
+        sum[i] = 0.0f;
     }
+    u32x4 b[kExpandRows][4];
+    const auto load = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < kExpandRows; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)  // (past the slot's ranks: zeros or other outputs' values, unused)
+                b[i][q] = adapter_load4(a.type, br[i], at[i] + (uint32_t)((r0 * 16 + q * 64) * elem));
+    };
+    load(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int r0 = 0;;) {
+#pragma unroll
+        for (int i = 0; i < kExpandRows; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (r0 + 4 * q >= pad[i]) continue;
+                const f32x4 l = *reinterpret_cast<const f32x4*>(low + i * kRow + r0 + 4 * q);
+                const adapter_f32x4 w = adapter_widen4(a.type, b[i][q]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) sum[i] = fmaf(l[c], w[c], sum[i]);
+            }
+        r0 += 16;
+        if (r0 >= most) break;
+        load(r0);
+    }
+#pragma unroll
+    for (int i = 0; i < kExpandRows; i++)
+        if (pad[i] && n < j.out) j.y[(int64_t)(m0 + i) * j.out + n] = fmaf(sum[i], scale[i], y[i]);
 }
 
 __global__ __launch_bounds__(256) void adapter_slot_kernel(AdapterSlot* info, int first, int count, int rank, float scale) {
@@ -402,7 +407,8 @@ hipError_t launch_adapters_shrink(const AdapterArgs& a, const ActQuantJob& quant
 hipError_t launch_adapters_expand(const AdapterArgs& a, hipStream_t st) {
     int out = 0;
     for (int i = 0; i < a.jobs; i++) out = a.job[i].slots && a.job[i].out > out ? a.job[i].out : out;
-    hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)((a.rows + 15) / 16 * 8), (unsigned)((out + 2047) / 2048), (unsigned)a.jobs),
+    hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)((a.rows + kExpandRows - 1) / kExpandRows * 8), (unsigned)((out + 2047) / 2048),
+                                                      (unsigned)a.jobs),
                        dim3(256), 0, st, a);
     return hipGetLastError();
 }

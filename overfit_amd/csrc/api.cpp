@@ -493,9 +493,24 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
         *ad_done = true;
         return ad;
     };
+    // Sets of many slots: the row tiles where they meet (a decode step's) are left to a launch behind, which takes them row by row.
+    // Behind the tiled kernels, which have no registers for that (us, rank 16, every row its own of 32 slots: down 14336 -> 4096 at
+    // 300 rows 254 -> 147, gate/up of 14336 at 256 rows 171 -> 134; three requests on 32 slots 118 -> 126 and 99 -> 103, that launch
+    // with nothing to do), and the panel kernels past rank 16 and 32 rows (Q8_0 896 -> 11786 + 2 x 2946, 187 rows of 98 requests, rank
+    // 75: 193 -> 148); not the split kernels (4096 -> 4096 at 64 rows, rank 64 32 -> 36).
+    auto leave_by_row = [&](bool when) {
+        if (!ad) return;
+        int slots = 0;
+        for (int i = 0; i < count; i++) slots = ad->job[i].slots > slots ? ad->job[i].slots : slots;
+        ad->by_row = when && slots > ovfq::kAdapterFew;
+        *ad_done = !ad->by_row;
+    };
     // Every kernel below reads either the fp32 input (decode kernels that quantise it) or the quantised activation.
     if (!x && (!act.q || !act.s)) return fail(OVFQ_ERR_NULL, "projection launch without a quantised activation");
     if (act.tiled && type == OVFQ_TYPE_Q8_0) {
+        bool panel = false;
+        for (int i = 0; i < count; i++) panel = panel || ovfq::q8_0_mid_panel(jobs[i].n_rows, rows);
+        leave_by_row(panel && ad && rows > 32 && ad->low_stride > 16);
         for (int i = 0; i < count; i++) {
             const int8_t* wq = reinterpret_cast<const int8_t*>(jobs[i].w);
             ovfq::AdapterArgs one{};  // this weight's adapters
@@ -507,13 +522,13 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
             HIP_TRY(ovfq::launch_q8_0_mid(&wq, &jobs[i].ws, 1, false, in, jobs[i].n_rows, rows, jobs[i].bias, act.q, act.s,
                                           jobs[i].y, c->stream, ad && ad->job[i].slots ? &one : nullptr));
         }
-        if (ad) *ad_done = true;
     } else if (act.tiled) {
-        if (use_mid(c, in, rows, ws, count) == ovfq::MidKernel::kPanel)
+        const bool panel = use_mid(c, in, rows, ws, count) == ovfq::MidKernel::kPanel;
+        leave_by_row(panel && ad && rows > 32 && ad->low_stride > 16);
+        if (panel)
             HIP_TRY(ovfq::launch_project_panel(type, jobs, count, in, rows, act, c->stream, ad));
         else
             HIP_TRY(ovfq::launch_project_split(type, jobs, count, in, rows, act, c->stream, ad));
-        if (ad) *ad_done = true;
     } else if (type == OVFQ_TYPE_Q8_0) {
         // Batches that q8_mid.hip does not take (a caller's quantised activation, the fixed-scratch entry point, more than
         // 512 rows, what q8_mid_choice leaves, OVFQ_SPLIT=0). The int8-MFMA kernel from 8 rows; for inputs up to 8192 from 6
@@ -552,15 +567,7 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     } else if (use_gemv_rows(c, type, in, rows, count, pair_out)) {
         HIP_TRY(ovfq::launch_gemv_rows_kquant(type, jobs, count, in, rows, x, act, c->stream, in_epilogue(ovfq::gemv_rows_adapters)));
     } else if (use_tiled_mfma(c, type, jobs, count, in, rows)) {
-        if (ad) {
-            // Sets of many slots: the row tiles where they meet (a decode step's) are left to a launch behind, which takes them row
-            // by row (us: down 14336 -> 4096 at 300 rows, every row its own of 32 slots 254 -> 154, gate/up of 14336 at 256 rows 171 ->
-            // 132; three requests on 32 slots 118 -> 126 and 99 -> 100, that launch with nothing to do).
-            int slots = 0;
-            for (int i = 0; i < count; i++) slots = ad->job[i].slots > slots ? ad->job[i].slots : slots;
-            ad->by_row = slots > ovfq::kAdapterFew;
-            *ad_done = !ad->by_row;
-        }
+        leave_by_row(true);
         HIP_TRY(ovfq::launch_project_mfma(type, jobs, count, in, rows, act, c->stream, ad));
     } else if (small_mfma_enabled(rows) && ovfq::mfma_small_supported(type, in)) {
         // Few rows: 16-row MFMA tiles with super-block-parallel waves; a gate/up-shaped pair shares one launch.

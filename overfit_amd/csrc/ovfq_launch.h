@@ -223,6 +223,7 @@ inline size_t q8_tiled_records(int rows, int planes, int plane_in) {
     return (size_t)((rows + 15) / 16) * (size_t)planes * (size_t)((plane_in / 32 + 3) / 4);
 }
 bool q8_0_mid_supported(int planes, int plane_in, int rows);
+bool q8_0_mid_panel(int n_out, int rows);  // whether its panel kernel takes a weight, not the split kernel
 hipError_t launch_quantize_q8_0_tiled(const float* x, int rows, int planes, int plane_in, int8_t* q, float* s,
                                       hipStream_t st);
 hipError_t launch_q8_0_mid(const int8_t* const* wq, const float* const* ws, int planes, bool heads, int plane_in, int n_out,

@@ -528,6 +528,14 @@ static hipError_t launch_panel(Q8Args& a, const AD& ad, hipStream_t st) {
     return launch_panel_t<kHeads, 4>(a, T, grid, ad, st);
 }
 
+// Workgroups of the split kernel, as the busiest XCD has them (293x1088 at 370 rows, 228 workgroups, 36 on three XCDs: 14.5,
+// panel 9.8).
+static long split_workgroups(int n_out, int rows) {
+    const int subs = (rows + 15) / 16, T = subs == 1 ? 1 : 2;
+    return (long)(((n_out + 15) / 16 + 7) / 8) * ((subs + T - 1) / T) * 8;
+}
+bool q8_0_mid_panel(int n_out, int rows) { return split_workgroups(n_out, rows) > (rows > 16 ? 256 : 512); }
+
 template <bool kHeads, class AD>
 static hipError_t launch_mid(Q8Args& a, const AD& ad, hipStream_t st) {
     const int wnb = a.in / 32, ng = (kHeads ? a.planes : 1) * ((wnb + 3) / 4);
@@ -539,8 +547,7 @@ static hipError_t launch_mid(Q8Args& a, const AD& ad, hipStream_t st) {
     a.o_tiles = (a.n_out + 15) / 16;
     const int T = a.subs == 1 ? 1 : 2;
     a.n_tiles = (a.subs + T - 1) / T;
-    const long wgs = (long)((a.o_tiles + 7) / 8) * a.n_tiles * 8;  // as the busiest XCD has them (293x1088 at 370 rows, 228
-                                                                   // workgroups, 36 on three XCDs: 14.5, panel 9.8)
+    const long wgs = split_workgroups(a.n_out, a.rows);
     if (wgs > 256 && (T == 2 || wgs > 512)) return launch_panel<kHeads>(a, ad, st);
     const dim3 grid((a.o_tiles + 7) / 8 * 8 * a.n_tiles);
     if (wgs > 256 || ng <= 4) {
