@@ -149,35 +149,47 @@ __device__ __forceinline__ uint32_t adapter_b_at(int n, int r, int steps) {
     return ((uint32_t)((n >> 4) * steps + (r >> 4)) * 64u + (uint32_t)((r & 12) << 2) + (uint32_t)(n & 15)) * 4u;
 }
 
-// sum + sum_r low[r] B[slot][n][r] over the kRanks ranks from r0 on of one row and output, r0 below the row's; low: the row's
-// staged products. All of B's values are loaded before the first is used. n < j.out.
+// One row's and output's values of B for the kRanks ranks from r0 on, and sum + sum_r low[r] B[slot][n][r] over them, r0 below the
+// row's ranks; low: the row's staged products. All values are loaded before the first is used. n < j.out.
+template <int kRanks>
+struct AdapterDot {
+    u32x4 w[kRanks / 4];
+
+    __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, AdapterRow row, int n, int r0) {
+        const int end = row.pad() - r0, steps = adapter_tiles16(row.pad());
+        const char* b = adapter_b(e, j, row.slot());
+#pragma unroll
+        for (int q = 0; q < kRanks / 4; q++) {
+            const char* at = b + (size_t)adapter_b_at(n, 4 * q < end ? r0 + 4 * q : r0, steps) * adapter_elem(e.type);
+            if (e.type == kAdapterF32) {
+                w[q] = *reinterpret_cast<const u32x4*>(at);
+            } else {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(at);
+                w[q] = u32x4{v.x, v.y, 0u, 0u};
+            }
+        }
+    }
+    __device__ __forceinline__ float add(const AdapterArgs& e, AdapterRow row, const float* low, int r0, float sum) const {
+        const int end = row.pad() - r0;
+#pragma unroll
+        for (int q = 0; q < kRanks / 4; q++) {
+            const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(low + 4 * q);
+            const adapter_f32x4 f = adapter_widen4(e.type, w[q]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum = 4 * q < end ? fmaf(l[i], f[i], sum) : sum;
+        }
+        return sum;
+    }
+};
 template <int kRanks>
 __device__ __forceinline__ float adapter_dot(const AdapterArgs& e, const AdapterJob& j, AdapterRow row, int n, const float* low,
                                              int r0, float sum) {
-    const int end = row.pad() - r0, steps = adapter_tiles16(row.pad());
-    const char* b = adapter_b(e, j, row.slot());
-    u32x4 w[kRanks / 4];
-#pragma unroll
-    for (int q = 0; q < kRanks / 4; q++) {
-        const char* at = b + (size_t)adapter_b_at(n, 4 * q < end ? r0 + 4 * q : r0, steps) * adapter_elem(e.type);
-        if (e.type == kAdapterF32) {
-            w[q] = *reinterpret_cast<const u32x4*>(at);
-        } else {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(at);
-            w[q] = u32x4{v.x, v.y, 0u, 0u};
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < kRanks / 4; q++) {
-        const adapter_f32x4 l = *reinterpret_cast<const adapter_f32x4*>(low + 4 * q);
-        const adapter_f32x4 f = adapter_widen4(e.type, w[q]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) sum = 4 * q < end ? fmaf(l[i], f[i], sum) : sum;
-    }
-    return sum;
+    AdapterDot<kRanks> b;
+    b.load(e, j, row, n, r0);
+    return b.add(e, row, low, r0, sum);
 }
 
-// The same for half as many ranks of fp32 adapters, in eight registers: 16 ranks of the 16-bit types, 8 of fp32.
+// The same in eight registers: 16 ranks of the 16-bit types, 8 of fp32.
 struct AdapterOct {
     u32x4 w[2];
 
@@ -454,12 +466,33 @@ template <int T, int W, int kLowPass>
 struct AdapterOuts {
     static constexpr int kPer = (256 * T + 64 * W - 1) / (64 * W);  // (past the rows: no row has a key there)
     static constexpr int kLds = 16 * T * (kLowPass + 4);  // floats of `staged`
+    static constexpr int kAtOnce = kPer == 1 ? kLowPass : 32;  // ranks of B in registers at once
     AdapterTiles<T, 1> rows;
     AdapterStage<16 * T, kLowPass, 64 * W> stage;
 
     __device__ __forceinline__ void load(const AdapterArgs& e, const AdapterJob& j, int m0) {
         rows.load(e, j, m0);
         stage.load(e, j, m0, 0);
+    }
+
+    // kRanks of every output of the thread from r0 on, all outputs' values of B loaded together; first: the products are staged too.
+    template <int kRanks>
+    __device__ __forceinline__ void together(const AdapterArgs& e, const AdapterJob& j, const AdapterRow (&row)[kPer], int o0, int r0,
+                                             bool first, float* staged, float (&sum)[kPer], int m0) {
+        AdapterDot<kRanks> b[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (row[i].pad() > r0) b[i].load(e, j, row[i], o0 + ((((int)threadIdx.x + 64 * W * i) >> 4) & 15), r0);
+        if (first) {
+            stage.store(e, j, m0, r0, staged);
+            adapter_barrier();
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int idx = (int)threadIdx.x + 64 * W * i;
+            const float* low = staged + ((idx >> 8) * 16 + (idx & 15)) * (kLowPass + 4) + r0 % kLowPass;
+            if (row[i].pad() > r0) sum[i] = b[i].add(e, row[i], low, r0, sum[i]);
+        }
     }
 
     // Leaves the thread's parts in out[idx] and returns which of its outputs have one. All waves; `staged` is free again after.
@@ -486,6 +519,18 @@ struct AdapterOuts {
             if (r0) {
                 adapter_barrier();
                 stage.load(e, j, m0, r0);
+            }
+            if constexpr (T <= 2) {
+                // B's first values are under way while the products are staged (down 14336 -> 4096, 7 rows of rank 64: the kernel
+                // 21.9 -> 21.1 us; with three and four row tiles the registers spill, 64 rows of 4096 -> 4096 19.8 -> 21.9)
+                const int left = most - r0;  // the same for every wave
+                if (left <= 16)
+                    together<16>(e, j, row, o0, r0, true, staged, sum, m0);
+                else if (left <= 32 || kAtOnce == 32)
+                    for (int h = 0; h < kLowPass && h < left; h += 32) together<32>(e, j, row, o0, r0 + h, !h, staged, sum, m0);
+                else
+                    together<kAtOnce>(e, j, row, o0, r0, true, staged, sum, m0);
+                continue;
             }
             stage.store(e, j, m0, r0, staged);
             adapter_barrier();
