@@ -348,7 +348,7 @@ struct AdapterTiles {
             any |= left[t];
             most = max(most, (int)(key[t] & 0xffffu));
             by_row[t] = false;
-            if constexpr (kTiles > 0) by_row[t] = adapter_many(key[t]);
+            if constexpr (kTiles > 0) by_row[t] = j.slots > kAdapterFew && adapter_many(key[t]);
             if (by_row[t]) left[t] = 0;
         }
         if (!any) return;
