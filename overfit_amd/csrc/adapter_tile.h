@@ -59,10 +59,10 @@ __device__ __forceinline__ AdapterRow adapter_row(const AdapterArgs& e, const Ad
     return AdapterRow{v.x, as_float(scale)};
 }
 
-// Whether a tile goes row by row: its slot changes more than kAdapterFew times from row to row. key: of the tile's row l16.
-__device__ __forceinline__ bool adapter_many(uint32_t key) {
+// Whether a tile goes row by row: its slot changes more than `few` times from row to row. key: of the tile's row l16.
+__device__ __forceinline__ bool adapter_many(uint32_t key, int few) {
     const uint32_t above = (uint32_t)__builtin_amdgcn_update_dpp((int)key, (int)key, 0x111, 0xf, 0xf, false);  // row_shr:1
-    return __builtin_popcount((uint32_t)__ballot(key != above) & 0xffffu) > kAdapterFew;
+    return __builtin_popcount((uint32_t)__ballot(key != above) & 0xffffu) > few;
 }
 
 // The low-rank products of kRows (a multiple of 16) activation rows from m0 on, ranks r0 .. r0 + kRanks, their shares added: into
@@ -252,7 +252,7 @@ struct AdapterTiles {
             const AdapterRow r = adapter_row(e, j, m0 + 16 * t + (int)(threadIdx.x & 15));
             key[t] = r.key;
             scale[t] = r.scale;
-            if (e.by_row && adapter_many(key[t])) key[t] = 0;  // the launch behind has this tile
+            if (e.by_row && adapter_many(key[t], e.by_row)) key[t] = 0;  // the launch behind has this tile
         }
     }
 
@@ -348,7 +348,7 @@ struct AdapterTiles {
             any |= left[t];
             most = max(most, (int)(key[t] & 0xffffu));
             by_row[t] = false;
-            if constexpr (kTiles > 0) by_row[t] = j.slots > kAdapterFew && adapter_many(key[t]);
+            if constexpr (kTiles > 0) by_row[t] = j.slots > kAdapterFew && adapter_many(key[t], kAdapterFew);
             if (by_row[t]) left[t] = 0;
         }
         if (!any) return;

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
     if (!j.slots || o_tile * 256 >= j.out) return;
     const int l0 = m0 & 15;
     const AdapterRow row = adapter_row(a, j, m0 - l0 + (int)(threadIdx.x & 15));  // of the rows' tile of 16
-    if (a.by_row && !adapter_many(row.key)) return;  // the whole workgroup
+    if (a.by_row && !adapter_many(row.key, a.by_row)) return;  // the whole workgroup
     if (!((uint32_t)__ballot(row.pad() != 0) >> l0 & ((1u << kExpandRows) - 1))) return;
     // the products, their shares added
     const int quads = a.low_stride / 4;

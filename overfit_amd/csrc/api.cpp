@@ -497,12 +497,13 @@ int launch_projection(ovfq_ctx* c, const ovfq_weight* const* ws, int count, cons
     // Behind the tiled kernels, which have no registers for that (us, rank 16, every row its own of 32 slots: down 14336 -> 4096 at
     // 300 rows 254 -> 147, gate/up of 14336 at 256 rows 171 -> 134; three requests on 32 slots 118 -> 126 and 99 -> 103, that launch
     // with nothing to do), and the panel kernels past rank 16 and 32 rows (Q8_0 896 -> 11786 + 2 x 2946, 187 rows of 98 requests, rank
-    // 75: 193 -> 148); not the split kernels (4096 -> 4096 at 64 rows, rank 64 32 -> 36).
+    // 75: 193 -> 113, 148 where the tiles of three and four changes stayed); not the split kernels (4096 -> 4096 at 64 rows, rank 64
+    // 32 -> 36). A prompt's tiles have two changes at most.
     auto leave_by_row = [&](bool when) {
         if (!ad) return;
         int slots = 0;
         for (int i = 0; i < count; i++) slots = ad->job[i].slots > slots ? ad->job[i].slots : slots;
-        ad->by_row = when && slots > ovfq::kAdapterFew;
+        ad->by_row = when && slots > ovfq::kAdapterFew ? 2 : 0;
         *ad_done = !ad->by_row;
     };
     // Every kernel below reads either the fp32 input (decode kernels that quantise it) or the quantised activation.

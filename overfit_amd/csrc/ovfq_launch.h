@@ -284,7 +284,7 @@ struct AdapterArgs {
     int each;        // chunks of 32 inputs a wave
     int way_shift;   // log2 of the workgroups that divide the distinct slots of a row tile
     int shrink_x;    // row tiles << way_shift
-    int by_row;      // the tiles of many slots are left to launch_adapters_expand, which then takes no others
+    int by_row;      // not 0: tiles of more changes of the slot are left to launch_adapters_expand, which then takes no others
 };
 constexpr int kAdapterFew = 4;  // changes of the slot from row to row of a tile, up to which its slots are taken in turn
 __host__ __device__ constexpr int rank_pad(int rank) { return (rank + 3) & ~3; }
