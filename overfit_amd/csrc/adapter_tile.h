@@ -1,5 +1,6 @@
-// adapter_tile.h — B times the rows' low-rank products, for the epilogues of the projection kernels and for the launch that
-// adds adapters to finished outputs (adapters.hip). Products and sums are fp32 whatever the adapters are kept in.
+// adapter_tile.h — B times the rows' low-rank products in the epilogues of the projection kernels (AdapterTiles: MFMA result layout;
+// AdapterOuts: a thread's outputs, the split kernels; AdapterLanes: the decode kernels), and what the launch that adds adapters to
+// finished outputs shares with them (adapters.hip). Products and sums are fp32 whatever the adapters are kept in.
 //
 // Rows share a multiplication only where they share the slot. Tiles of few slots (a prompt's): the slots in turn, each multiplied
 // over fp32 MFMA (16x16x4) with the tile's rows, and its results go to its own rows only, by selection and not by a zero factor, so
