@@ -156,3 +156,36 @@ def test_two_graphs_share_the_scratch(kind, rows):
                     check(o.cpu().numpy(), b, x, h, slots, f"turn {turn}")
     finally:
         ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("slots", [3, 9])
+@pytest.mark.parametrize("kind,n,rows,force", [("q4k", 12400, 50, None), ("q4k", 200, 150, "tiled"), ("q4k", 14336, 140, "tiled"),
+                                               ("q6k", 6200, 140, "tiled"), ("q8", 3000, 200, None), ("q8", 300, 20, None)])
+def test_a_bad_adapter_stays_with_its_rows(kind, n, rows, force, slots):
+    # infinities and NaN in one request's adapter reach no other request's outputs, in runs of rows and one beside the other
+    case("bad", kind, n, rows, force, slots)
+    rng = np.random.default_rng(rows)
+    gen = torch.Generator().manual_seed(rows)
+    k = 512
+    w = make_weight(rng, kind, k, n)
+    s = ov.AdapterSet(k, n, slots, 40, BF16)
+    good = make_adapter(gen, k, n, 40, BF16)
+    bad = [t.clone() for t in make_adapter(gen, k, n, 20, BF16)]
+    bad[0][3, 5] = float("nan")
+    bad[1][:, 2] = float("inf")
+    s.load(0, *bad, 1.0)
+    s.load(2, *good, 0.5)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    sl = np.where(np.arange(rows) < rows // 2, np.arange(rows) % 2 * 2, np.arange(rows) // 20 % 2 * 2).astype(np.int32)
+    xd, sd = torch.from_numpy(x).to(DEV), torch.from_numpy(sl).to(DEV)
+    ctx = ov.default_context()
+    if force:
+        ctx.set_batched_kernel(force)
+    try:
+        base = ov.project(w, xd, rows=rows).cpu().numpy().reshape(rows, n)
+        got = ov.project_adapters([w], [s], xd, sd, rows)[0].cpu().numpy().reshape(rows, n)
+    finally:
+        ctx.set_batched_kernel("auto")
+    mine = sl == 2
+    check(got[mine], base[mine], x[mine], {2: (*good, 0.5)}, sl[mine], "the good rows")
+    assert not np.isfinite(got[~mine]).any()
