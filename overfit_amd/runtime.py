@@ -223,7 +223,8 @@ class BoundMulti:
 
 
 class BoundCall:
-    """A prepared call of a library function: its converted arguments, and what they point into."""
+    """A prepared call of a library function: its converted arguments, and the buffers that they point into (not the caller's
+    lists and norms, which may get others meanwhile)."""
 
     __slots__ = ("_ctx", "_fn", "_args", "_keep")
 

@@ -159,7 +159,7 @@ def _adapters_call(weights, adapters, x, row_slots, rows, biases, outs):
             arr(*[None if s is None else s.handle.value for s in adapters]), xb.ptr, rows, sb.ptr,
             arr(*[_ptr(b) for b in bb]), arr(*[o.ptr for o in ob]))
     fn = ctx.lib.ovfq_project_adapters_dev if dev else ctx.lib.ovfq_project_adapters
-    return BoundCall(ctx, fn, args, (list(weights), list(adapters), x, row_slots, biases, outs)), outs
+    return BoundCall(ctx, fn, args, (list(weights), list(adapters), [xb, sb, *ob, *bb])), outs
 
 
 def project_adapters(weights, adapters, x, row_slots, rows=1, biases=None, outs=None):
@@ -227,8 +227,7 @@ def _norm_call(y, rows, residual, post, gate, gate_axis, scale, pre, h_out, x_ou
     fn = ctx.lib.ovfq_residual_norm_dev if dev else ctx.lib.ovfq_residual_norm
     args = (ctx.handle, yb.ptr, _ptr(rb), rows, k, None if norms[0] is None else ctypes.byref(norms[0]), _ptr(gb),
             GATE_AXES[gate_axis], float(scale), None if norms[1] is None else ctypes.byref(norms[1]), _ptr(hb), _ptr(xb))
-    keep = (y, residual, gate, post, pre, norms, h_out, x_out)
-    return BoundCall(ctx, fn, args, keep), h_out, x_out
+    return BoundCall(ctx, fn, args, (side, norms)), h_out, x_out
 
 
 def residual_norm(y, rows, residual=None, post=None, gate=None, gate_axis=None, scale=1.0, pre=None, h_out=None,
@@ -274,8 +273,7 @@ def _verify_call(logits, vocab, row_offsets, draft_tokens, accept_uniforms, fina
     fn = ctx.lib.ovfq_verify_drafts_dev if dev else ctx.lib.ovfq_verify_drafts
     args = (ctx.handle, lb.ptr, rows, vocab, requests, rb.ptr, _ptr(none(tb)), _ptr(none(qb)), _ptr(pb), _ptr(none(ub)),
             fb.ptr, ab.ptr, ob.ptr)
-    keep = (logits, row_offsets, draft_tokens, accept_uniforms, final_uniforms, draft_probs, temperature, accepted, tokens)
-    return BoundCall(ctx, fn, args, keep), accepted, tokens
+    return BoundCall(ctx, fn, args, side), accepted, tokens
 
 
 def verify_drafts(logits, vocab, row_offsets, draft_tokens, accept_uniforms, final_uniforms, draft_probs=None,
