@@ -157,17 +157,21 @@ class Context:
         return BoundMulti(self, weights, x, ys, biases, rows)
 
     def bind_adapters_dev(self, weights, adapters, x, row_slots, ys, biases=None, rows=1):
-        """`step.project_adapters` on device tensors with its arguments converted once (see bind_multi_dev)."""
+        """`step.project_adapters` on device tensors with its arguments converted once (see bind_multi_dev); every output is
+        given."""
         from .step import _adapters_call
 
+        if ys is None:
+            raise ValueError("a prepared call needs its outputs")
         return _device_call(_adapters_call(weights, adapters, x, row_slots, rows, biases, ys)[0])
 
     def bind_residual_norm_dev(self, y, rows, residual=None, post=None, gate=None, gate_axis=None, scale=1.0, pre=None,
                                h_out=None, x_out=None):
-        """`step.residual_norm` on device tensors with its arguments converted once; h_out or x_out is given."""
+        """`step.residual_norm` on device tensors with its arguments converted once; x_out is given beside a pre norm, h_out
+        without one."""
         from .step import _norm_call
 
-        if h_out is None and x_out is None:
+        if (h_out if pre is None else x_out) is None:
             raise ValueError("a prepared call needs its outputs")
         return _device_call(_norm_call(y, rows, residual, post, gate, gate_axis, scale, pre, h_out, x_out, self, False)[0])
 

@@ -92,3 +92,15 @@ def test_views_of_tensors_that_are_let_go():
     del logits, off, final, tokens, uniforms, accepted, out
     held(named.clear, refs)
     del call
+
+
+def test_a_prepared_call_needs_every_output():
+    # an output that the call would make for itself reaches nobody
+    ctx = context()
+    y = plane(64)
+    with pytest.raises(ValueError):
+        ctx.bind_residual_norm_dev(y, 4, residual=plane(64), pre=ov.Norm(), h_out=plane(64))
+    with pytest.raises(ValueError):
+        ctx.bind_adapters_dev([FakeWeight(ctx)], [None], plane(64), plane(2, torch.int32), None, rows=2)
+    ctx.bind_residual_norm_dev(y, 4, residual=plane(64), h_out=plane(64))
+    ctx.bind_residual_norm_dev(y, 4, residual=plane(64), pre=ov.Norm(), x_out=plane(64))
