@@ -163,7 +163,7 @@ class Context:
 
         if ys is None:
             raise ValueError("a prepared call needs its outputs")
-        return _device_call(_adapters_call(weights, adapters, x, row_slots, rows, biases, ys)[0])
+        return _device_call(_adapters_call(weights, adapters, x, row_slots, rows, biases, ys, self)[0])
 
     def bind_residual_norm_dev(self, y, rows, residual=None, post=None, gate=None, gate_axis=None, scale=1.0, pre=None,
                                h_out=None, x_out=None):

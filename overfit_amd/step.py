@@ -137,7 +137,7 @@ def _ptr(b):
     return None if b is None else b.ptr
 
 
-def _adapters_call(weights, adapters, x, row_slots, rows, biases, outs):
+def _adapters_call(weights, adapters, x, row_slots, rows, biases, outs, ctx=None):
     n = len(weights)
     if not 1 <= n <= 4:
         raise OverfitArgumentOutOfRangeError(f"{n} weights: 1 to 4 are taken")
@@ -153,6 +153,8 @@ def _adapters_call(weights, adapters, x, row_slots, rows, biases, outs):
     bb = [as_buf(b, np.float32, "bias", allow_none=True) for b in (biases or [None] * n)]
     bb = [None if b is None or b.size == 0 else _sized(b, w.OutputSize, "bias") for b, w in zip(bb, weights)]
     dev = same_side(xb, sb, *ob, *bb)
+    if ctx is not None and ctx is not weights[0].context:
+        raise OverfitArgumentError("the weights belong to another context")
     ctx = _context(weights[0].context, [xb, sb, *ob, *bb])
     arr = ctypes.c_void_p * n
     args = (ctx.handle, n, arr(*[w.handle.value for w in weights]),

@@ -104,3 +104,12 @@ def test_a_prepared_call_needs_every_output():
         ctx.bind_adapters_dev([FakeWeight(ctx)], [None], plane(64), plane(2, torch.int32), None, rows=2)
     ctx.bind_residual_norm_dev(y, 4, residual=plane(64), h_out=plane(64))
     ctx.bind_residual_norm_dev(y, 4, residual=plane(64), pre=ov.Norm(), x_out=plane(64))
+
+
+def test_adapters_on_another_context_than_their_weights():
+    # not silently on the weights' context and its stream
+    ctx, other = context(), context()
+    args = ([FakeWeight(ctx)], [None], plane(64), plane(2, torch.int32), [plane(16)])
+    with pytest.raises(ov.OverfitArgumentError):
+        other.bind_adapters_dev(*args, rows=2)
+    ctx.bind_adapters_dev(*args, rows=2)
