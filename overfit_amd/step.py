@@ -103,6 +103,8 @@ class AdapterSet:
         pb, db, _kb = _as_elements(b, self.type_id, "b", rank * self.output_size)
         if da != db:
             raise OverfitArgumentError("host and device buffers cannot be mixed in one call")
+        if da and {a.device.index, b.device.index} != {self._ctx.device}:
+            raise OverfitArgumentError("a, b and the set must be on one device")
         fn = self._ctx.lib.ovfq_adapters_load_dev if da else self._ctx.lib.ovfq_adapters_load
         raise_for_status(fn(self.handle, slot, pa, pb, rank, float(scale)), self._ctx.lib)
 
