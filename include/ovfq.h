@@ -275,7 +275,8 @@ OVFQ_API int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const
  * in `type` (OVFQ_TYPE_F32, _F16 or _BF16; the tensors of a GGUF adapter file, lora_a and lora_b, lie in memory like this).
  * All memory is allocated here: slots * max_rank * (input_size + output_size) values, max_rank and output_size rounded up to
  * multiples of 16. A set belongs to its context like a weight. input_size % 32 == 0, at most OVFQ_MAX_ADAPTER_INPUT, and
- * a slot's A and B each below 2^28 values. */
+ * a slot's A and B each below 2^28 values. Not while the context's stream is captured (OVFQ_ERR_STATE). A set that is destroyed
+ * then leaves its memory with the superseded scratch, until ovfq_ctx_release_retired or ovfq_ctx_destroy. */
 #define OVFQ_MAX_ADAPTER_SLOTS 4096
 #define OVFQ_MAX_ADAPTER_RANK 256
 #define OVFQ_MAX_ADAPTER_INPUT (1 << 20)

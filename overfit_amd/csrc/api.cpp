@@ -1408,6 +1408,22 @@ int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const ovfq_wei
 
 // ---------------------------------------------------------------------------------------- low-rank adapters
 
+// No work of an adapter set's making or loading goes into a captured graph: it copies from the caller's memory and waits.
+static int check_not_capturing(ovfq_ctx* ctx, const char* what) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(OVFQ_ERR_STATE, "%s while the context's stream is captured", what);
+    return OVFQ_OK;
+}
+
+// Allocations, frees and waits of this thread while some other stream is captured, which they have no part in: unless the thread's
+// capture mode is relaxed the runtime refuses them and ends that capture.
+struct RelaxedCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
 int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_size, int slots, int max_rank,
                          ovfq_adapters** out) {
     if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
@@ -1429,6 +1445,9 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
         return fail(OVFQ_ERR_SIZE, "an adapter of rank %d for %d x %d is too large", max_rank, output_size, input_size);
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
+    int rc = check_not_capturing(ctx, "an adapter set cannot be created");
+    if (rc) return rc;
+    const RelaxedCapture relaxed;
     ovfq_adapters* s = new (std::nothrow) ovfq_adapters();
     if (!s) return fail(OVFQ_ERR_HIP, "no host memory for an adapter set");
     s->ctx = ctx;
@@ -1467,22 +1486,28 @@ int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_siz
 int ovfq_adapters_destroy(ovfq_adapters* s) {
     if (!s) return fail(OVFQ_ERR_NULL, "adapter set is NULL");
     {
-        std::lock_guard<std::mutex> lk(s->ctx->mu);
-        (void)hipSetDevice(s->ctx->device);
-        (void)hipStreamSynchronize(s->ctx->stream);
-        (void)hipFree(s->a);  // the allocation's first piece
-        s->ctx->live_adapters--;
+        ovfq_ctx* c = s->ctx;
+        std::lock_guard<std::mutex> lk(c->mu);
+        (void)hipSetDevice(c->device);
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+            // The stream cannot be waited for, and what is captured may read the set: its memory goes the way of superseded scratch.
+            (void)hipGetLastError();
+            try {
+                c->retired.push_back(s->a);
+            } catch (const std::bad_alloc&) {
+                return fail(OVFQ_ERR_HIP, "no host memory to put the adapter set aside");
+            }
+            c->retired_bytes += s->nbytes;
+        } else {
+            const RelaxedCapture relaxed;
+            (void)hipStreamSynchronize(c->stream);
+            (void)hipFree(s->a);  // the allocation's first piece
+        }
+        c->live_adapters--;
     }
     delete s;
     return ok();
-}
-
-// No work of an adapter's load goes into a captured graph: it copies from the caller's memory and waits.
-static int check_not_capturing(ovfq_ctx* ctx, const char* what) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
-    if (st != hipStreamCaptureStatusNone) return fail(OVFQ_ERR_STATE, "%s while the context's stream is captured", what);
-    return OVFQ_OK;
 }
 
 static int adapters_load_impl(ovfq_adapters* s, int slot, const void* a, const void* b, int rank, float scale, bool host) {
@@ -1497,6 +1522,7 @@ static int adapters_load_impl(ovfq_adapters* s, int slot, const void* a, const v
     HIP_TRY(hipSetDevice(ctx->device));
     int rc = check_not_capturing(ctx, "an adapter cannot be loaded");
     if (rc) return rc;
+    const RelaxedCapture relaxed;
     const size_t a_bytes = (size_t)rank * s->in * s->elem(), b_bytes = (size_t)rank * s->out * s->elem();
     const char *a_dev = static_cast<const char*>(a), *b_dev = static_cast<const char*>(b);
     char* staged = nullptr;
