@@ -21,7 +21,8 @@
  *    its head-parallel workers, RT/CachedMultiHeadAttention.cs:280, :876-907).
  *  - Lifetime: a weight belongs to the context it was created on, and that context must outlive it
  *    (ovfq_ctx_destroy returns OVFQ_ERR_STATE, destroying nothing, while any of its weights is alive; the
- *    reference's counterpart of that state error is InvalidOperationException).
+ *    reference's counterpart of that state error is InvalidOperationException). No weight is created while the context's
+ *    stream is captured (OVFQ_ERR_STATE); one destroyed then leaves its memory with the superseded scratch below.
  *  - Sizes: every activation and output plane (rows x its width) stays below 2^31 elements, the length limit
  *    of the reference's Span<T> scratch and outputs; larger calls return OVFQ_ERR_SIZE.
  *  - Scratch and HIP graphs: the context grows its device scratch on demand (activation quantisation, FFN and

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -79,6 +80,7 @@ struct ovfq_ctx {
 struct SharedPlane {
     void* p = nullptr;
     int refs = 0;
+    size_t bytes = 0;
 };
 
 struct ovfq_weight {
@@ -241,6 +243,46 @@ int check_weight_shape(int type, int in, int out) {
     return OVFQ_OK;
 }
 
+// Making a weight or an adapter set, or loading an adapter, goes into no captured graph: it copies from the caller's memory and waits.
+int check_not_capturing(ovfq_ctx* ctx, const char* what) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(OVFQ_ERR_STATE, "%s while the context's stream is captured", what);
+    return OVFQ_OK;
+}
+
+// Allocations, frees and waits of this thread while some other stream is captured, which they have no part in: unless the thread's
+// capture mode is relaxed the runtime refuses them and ends that capture.
+struct RelaxedCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Frees device memory of `bytes` in all that queued work may read. While the context's stream is captured it cannot be waited for, and
+// what is captured may read the memory: it goes the way of superseded scratch then.
+int free_device(ovfq_ctx* c, std::initializer_list<void*> pieces, size_t bytes) {
+    (void)hipSetDevice(c->device);
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+        (void)hipGetLastError();
+        try {
+            c->retired.reserve(c->retired.size() + pieces.size());
+        } catch (const std::bad_alloc&) {
+            return fail(OVFQ_ERR_HIP, "no host memory to put device memory aside");
+        }
+        for (void* p : pieces)
+            if (p) c->retired.push_back(p);
+        c->retired_bytes += bytes;
+        return OVFQ_OK;
+    }
+    const RelaxedCapture relaxed;
+    (void)hipStreamSynchronize(c->stream);
+    for (void* p : pieces)
+        if (p) (void)hipFree(p);
+    return OVFQ_OK;
+}
+
 int weight_create(ovfq_ctx* ctx, int type, const void* blocks, size_t nbytes, const float* q8_scales, int in,
                   int out, ovfq_weight** res, hipMemcpyKind kind) {
     if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
@@ -254,6 +296,8 @@ int weight_create(ovfq_ctx* ctx, int type, const void* blocks, size_t nbytes, co
     if (type == OVFQ_TYPE_Q8_0 && !q8_scales) return fail(OVFQ_ERR_NULL, "Q8_0 weight needs a scale plane");
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
+    if ((rc = check_not_capturing(ctx, "a weight cannot be created"))) return rc;
+    const RelaxedCapture relaxed;
     ovfq_weight* w = new ovfq_weight();
     w->ctx = ctx;
     w->type = type;
@@ -807,6 +851,8 @@ static int weight_create_gguf(ovfq_ctx* ctx, int type, const void* src, size_t n
         return fail(OVFQ_ERR_SIZE, "device gguf_bytes must be 2-byte aligned");
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
+    if ((rc = check_not_capturing(ctx, "a weight cannot be created"))) return rc;
+    const RelaxedCapture relaxed;
     ovfq_weight* w = new ovfq_weight();
     w->ctx = ctx;
     w->type = OVFQ_TYPE_Q8_0;
@@ -878,6 +924,8 @@ static int experts_gguf_impl(ovfq_ctx* ctx, int type, const void* src, size_t nb
     const hipMemcpyKind kind = host ? hipMemcpyHostToDevice : hipMemcpyDeviceToDevice;
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
+    if ((rc = check_not_capturing(ctx, "expert weights cannot be created"))) return rc;
+    const RelaxedCapture relaxed;
     char* base = nullptr;
     void* staged = nullptr;
     hipError_t e = hipMalloc((void**)&base, E * (q_stride + s_stride));
@@ -907,6 +955,7 @@ static int experts_gguf_impl(ovfq_ctx* ctx, int type, const void* src, size_t nb
     SharedPlane* sp = new SharedPlane();
     sp->p = base;
     sp->refs = n_experts;
+    sp->bytes = E * (q_stride + s_stride);
     for (size_t x = 0; x < E; x++) {
         ovfq_weight* w = new ovfq_weight();
         w->ctx = ctx;
@@ -936,20 +985,19 @@ int ovfq_weight_create_experts_gguf_dev(ovfq_ctx* ctx, int type, const void* ggu
 int ovfq_weight_destroy(ovfq_weight* w) {
     if (!w) return fail(OVFQ_ERR_NULL, "weight is NULL");
     {
-        std::lock_guard<std::mutex> lk(w->ctx->mu);
-        (void)hipSetDevice(w->ctx->device);
-        (void)hipStreamSynchronize(w->ctx->stream);
-        if (w->shared) {
-            if (--w->shared->refs == 0) {
-                (void)hipFree(w->shared->p);
-                delete w->shared;
-            }
-        } else {
-            if (w->blocks) (void)hipFree(w->blocks);
-            if (w->scales) (void)hipFree(w->scales);
-        }
-        if (w->mfma) (void)hipFree(w->mfma);
-        w->ctx->live_weights--;
+        ovfq_ctx* c = w->ctx;
+        std::lock_guard<std::mutex> lk(c->mu);
+        const size_t mfma_bytes = w->mfma ? ovfq::mfma_prepared_bytes(w->in, w->out) : 0;
+        int rc = OVFQ_OK;
+        if (!w->shared)
+            rc = free_device(c, {w->blocks, w->scales, w->mfma}, w->nbytes + mfma_bytes);
+        else if (w->shared->refs > 1)  // its slice goes with the last one
+            rc = w->mfma ? free_device(c, {w->mfma}, mfma_bytes) : OVFQ_OK;
+        else
+            rc = free_device(c, {w->shared->p, w->mfma}, w->shared->bytes + mfma_bytes);
+        if (rc) return rc;
+        if (w->shared && --w->shared->refs == 0) delete w->shared;
+        c->live_weights--;
     }
     delete w;
     return ok();
@@ -967,6 +1015,8 @@ int ovfq_weight_prepare_mfma(ovfq_ctx* ctx, ovfq_weight* w) {
     std::lock_guard<std::mutex> lk(ctx->mu);
     if (w->mfma) return ok();
     HIP_TRY(hipSetDevice(ctx->device));
+    if ((rc = check_not_capturing(ctx, "an MFMA-ready copy cannot be made"))) return rc;
+    const RelaxedCapture relaxed;
     void* pre = nullptr;
     hipError_t e = hipMalloc(&pre, ovfq::mfma_prepared_bytes(w->in, w->out));
     if (e == hipSuccess)
@@ -1408,22 +1458,6 @@ int ovfq_project_multi_prequantized_dev(ovfq_ctx* ctx, int count, const ovfq_wei
 
 // ---------------------------------------------------------------------------------------- low-rank adapters
 
-// No work of an adapter set's making or loading goes into a captured graph: it copies from the caller's memory and waits.
-static int check_not_capturing(ovfq_ctx* ctx, const char* what) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
-    if (st != hipStreamCaptureStatusNone) return fail(OVFQ_ERR_STATE, "%s while the context's stream is captured", what);
-    return OVFQ_OK;
-}
-
-// Allocations, frees and waits of this thread while some other stream is captured, which they have no part in: unless the thread's
-// capture mode is relaxed the runtime refuses them and ends that capture.
-struct RelaxedCapture {
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
-    ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
-};
-
 int ovfq_adapters_create(ovfq_ctx* ctx, int type, int input_size, int output_size, int slots, int max_rank,
                          ovfq_adapters** out) {
     if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
@@ -1488,22 +1522,8 @@ int ovfq_adapters_destroy(ovfq_adapters* s) {
     {
         ovfq_ctx* c = s->ctx;
         std::lock_guard<std::mutex> lk(c->mu);
-        (void)hipSetDevice(c->device);
-        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
-            // The stream cannot be waited for, and what is captured may read the set: its memory goes the way of superseded scratch.
-            (void)hipGetLastError();
-            try {
-                c->retired.push_back(s->a);
-            } catch (const std::bad_alloc&) {
-                return fail(OVFQ_ERR_HIP, "no host memory to put the adapter set aside");
-            }
-            c->retired_bytes += s->nbytes;
-        } else {
-            const RelaxedCapture relaxed;
-            (void)hipStreamSynchronize(c->stream);
-            (void)hipFree(s->a);  // the allocation's first piece
-        }
+        const int rc = free_device(c, {s->a}, s->nbytes);  // the allocation's first piece
+        if (rc) return rc;
         c->live_adapters--;
     }
     delete s;
