@@ -314,6 +314,7 @@ OVFQ_API int ovfq_project_adapters_dev(ovfq_ctx* ctx, int count, const ovfq_weig
 
 /* ------------------------------------------------------------------------- norms around the residual sum */
 
+#define OVFQ_MAX_NORM_ROWS ((1 << 28) - 16)
 #define OVFQ_NORM_RMS 0   /* v / sqrt(mean(v^2) + eps) * weight (+ bias)                              */
 #define OVFQ_NORM_LAYER 1 /* (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias        */
 typedef struct ovfq_norm {
@@ -334,6 +335,7 @@ typedef struct ovfq_norm {
  *   h_out = residual + scale * gate * t   (residual NULL: without it; gate by gate_mode)
  *   x_out = pre(h_out)     the norm before the next block (NULL: no x_out)
  * h_out may be NULL when only x_out is wanted (residual, post and gate NULL: a plain norm). Per-head norms are rows of head_dim.
+ * At most OVFQ_MAX_NORM_ROWS rows.
  * h_out may be the residual plane or the y plane itself, x_out the y plane or, with h_out NULL, the residual plane; planes
  * must not overlap otherwise. Sums are fp32. Host pointers, synchronous. */
 OVFQ_API int ovfq_residual_norm(ovfq_ctx* ctx, const float* y, const float* residual, int rows, int k,

@@ -1631,6 +1631,8 @@ static int norm_impl(ovfq_ctx* ctx, const float* y, const float* residual, int r
     if (k <= 0) return fail(OVFQ_ERR_RANGE, "k (%d) must be positive", k);
     int rc;
     if ((rc = check_plane(rows, k, "activation"))) return rc;
+    // 16 threads a row of up to 64 elements, 256 a workgroup, fewer than 2^32 a launch (wider rows have fewer by their plane)
+    if (rows > OVFQ_MAX_NORM_ROWS) return fail(OVFQ_ERR_RANGE, "rows (%d) above %d", rows, OVFQ_MAX_NORM_ROWS);
     if ((rc = check_norm(post, "post", host)) || (rc = check_norm(pre, "pre", host))) return rc;
     if (gate_mode < OVFQ_GATE_NONE || gate_mode > OVFQ_GATE_FULL) return fail(OVFQ_ERR_RANGE, "unknown gate_mode %d", gate_mode);
     if ((gate != nullptr) != (gate_mode != OVFQ_GATE_NONE))
