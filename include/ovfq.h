@@ -299,11 +299,12 @@ OVFQ_API int ovfq_adapters_info(const ovfq_adapters* set, int* type, int* input_
 
 /* ovfq_project_multi with each row's adapter added: for weight i and row m with s = row_slots[m],
  *   ys[i][m] = (biases[i] +) W_i q(x[m]) + scale_s B_s (A_s x[m])
- * where (A_s, B_s, scale_s) is slot s of sets[i]; x is not quantised in the second term, and its products and sums are fp32. A
- * row whose slot is negative, past the set or empty gets the projection alone (bit-identical to ovfq_project_multi), and
- * so does every row of a weight whose sets[i] is NULL. row_slots [rows] is read on the device at each call, so one captured
- * graph serves any assignment. Sets of one call share a type; each has its weight's sizes. At most 4 weights. Host
- * pointers, synchronous. */
+ * where (A_s, B_s, scale_s) is slot s of sets[i]; x is not quantised in the second term, and its products and sums are fp32 (in
+ * A_s x over bf16 parts, for an fp32 A without the products of 2^-24 of the whole and less; an infinity in x or A_s gives NaN
+ * there). What is not finite stays in the rows that have it. A row whose slot is negative, past the set or empty gets the
+ * projection alone (bit-identical to ovfq_project_multi), and so does every row of a weight whose sets[i] is NULL. row_slots
+ * [rows] is read on the device at each call, so one captured graph serves any assignment. Sets of one call share a type; each has
+ * its weight's sizes. At most 4 weights. Host pointers, synchronous. */
 OVFQ_API int ovfq_project_adapters(ovfq_ctx* ctx, int count, const ovfq_weight* const* weights,
                                    const ovfq_adapters* const* sets, const float* x, int rows, const int* row_slots,
                                    const float* const* biases, float* const* ys);
@@ -354,13 +355,15 @@ OVFQ_API int ovfq_residual_norm_dev(ovfq_ctx* ctx, const float* y, const float* 
  * last token and after each of its n_r = (its rows) - 1 drafted tokens, so there are drafts = rows - requests of those, draft
  * i of request r at index row_offsets[r] - r + i of draft_tokens, accept_uniforms and draft_probs [drafts][vocab] (the
  * distributions that they were drawn from; NULL: drafted with certainty). With p = softmax(logits / temperature[r]) in
- * fp64 (temperature NULL: 1; not in (0, inf): all of p on the first of the largest logits):
+ * fp64, its exponentials within 2.5e-12 of their values (temperature NULL: 1; not in (0, inf): all of p on the first of the largest
+ * logits):
  *   draft x is accepted while accept_uniform * q(x) < p(x);
  *   the first one refused is replaced by a draw from max(p - q, 0) (from p, where that is all zero), or, with none refused,
  *   one more token is drawn from the last row's p: the lowest token whose running sum passes final_uniforms[r] times the total.
  * accepted[r] is the number of drafts kept; tokens [rows] holds, from row_offsets[r] on, those and the drawn token, then -1.
- * Logits of -inf or NaN have no probability; a row without a finite largest logit refuses its draft, and draws -1. A draft
- * outside the vocabulary is refused. Negative or NaN draft probabilities count as 0. */
+ * A target that samples from fewer tokens (top-k, top-p, min-p) has the others' logits set to -inf before. Logits of -inf or NaN
+ * have no probability; a row without a finite largest logit refuses its draft, and draws -1. A draft outside the vocabulary is
+ * refused. Negative or NaN draft probabilities count as 0. */
 OVFQ_API int ovfq_verify_drafts(ovfq_ctx* ctx, const float* logits, int rows, int vocab, int requests,
                                 const int* row_offsets, const int* draft_tokens, const float* draft_probs,
                                 const float* temperature, const float* accept_uniforms, const float* final_uniforms,

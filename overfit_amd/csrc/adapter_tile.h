@@ -562,7 +562,9 @@ struct AdapterOuts {
 
 // The adapters' part of a decode kernel's outputs: output oi of a wave's item (weight row n, activation row m) has the L lanes
 // from L oi on, each with every L-th quad of the ranks. The rows' adapters are loaded at the start, a lane's first P quads of B
-// beside the item's weights; the launch's low-rank products wait in LDS, [job][row][low_stride].
+// beside the item's weights; the launch's low-rank products wait in LDS, [job][row][low_stride]. In launches of several weights the
+// choice of key and scale by the job keeps the whole of it in private memory (176 bytes a lane): q/k/v of 4096 Q4_K, one row, rank 16
+// 19.5 us, 4.4 without adapters; the output projection alone, whose kernel has none there, 9.8 and 3.9.
 template <int L, int P, int kThreads>
 struct AdapterLanes {
     uint32_t key[kMaxJobs];  // of the lane's activation row

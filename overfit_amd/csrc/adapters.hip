@@ -55,7 +55,7 @@ __device__ __forceinline__ Raw8<kType> load_raw8(__amdgpu_buffer_rsrc_t r, uint3
 
 // acc += x w over 32 inputs, the small products first. bf16 adapters are their own part (three MFMAs), fp16 ones (11 bits)
 // two parts (six, every product exact), fp32 ones three: of their nine products the three that are 2^-24 of the whole or less are
-// left out.
+// left out. (An infinity's parts are itself and NaN, so its products are NaN.)
 template <int kType>
 __device__ __forceinline__ f32x4 multiply(const Parts& x, const Raw8<kType>& w, f32x4 acc) {
     if constexpr (kType == kAdapterBF16) {
