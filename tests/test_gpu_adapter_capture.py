@@ -17,12 +17,13 @@ K, N, ROWS = 512, 72, 6
 
 
 class Work:
-    """A context on a stream of its own, a weight, and a set with one adapter."""
+    """A context, usually on a stream of its own, a weight, and a set with one adapter."""
 
-    def __init__(self):
+    def __init__(self, own_stream=True):
         rng, self.gen = np.random.default_rng(1), torch.Generator().manual_seed(1)
         self.ctx, self.stream = ov.Context(0), torch.cuda.Stream()
-        self.ctx.set_stream(self.stream.cuda_stream)
+        if own_stream:  # else torch's default one
+            self.ctx.set_stream(self.stream.cuda_stream)
         self.w = make_weight(rng, "q4k", K, N, self.ctx)
         self.x = normal(rng, (ROWS, K))
         self.xd = torch.from_numpy(self.x).to(DEV)
@@ -85,8 +86,9 @@ def test_on_the_captured_stream():
     t.close()
 
 
-def test_while_another_stream_is_captured():
-    t = Work()
+@pytest.mark.parametrize("own_stream", [True, False])
+def test_while_another_stream_is_captured(own_stream):
+    t = Work(own_stream)
     gone, v, other = t.set(), torch.ones(1000, device=DEV), torch.cuda.Stream()
     torch.cuda.synchronize()
     retired = t.ctx.scratch_bytes()[1]

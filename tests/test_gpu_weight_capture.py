@@ -16,12 +16,13 @@ K, N, ROWS = 512, 72, 6
 
 
 class Work:
-    """A context on a stream of its own and the ways to a weight on it."""
+    """A context, usually on a stream of its own and the ways to a weight on it."""
 
-    def __init__(self):
+    def __init__(self, own_stream=True):
         self.rng = np.random.default_rng(2)
         self.ctx, self.stream = ov.Context(0), torch.cuda.Stream()
-        self.ctx.set_stream(self.stream.cuda_stream)
+        if own_stream:  # else torch's default one
+            self.ctx.set_stream(self.stream.cuda_stream)
         nb = N * K // 256
         self.q4k, self.q6k = random_q4k_blocks(self.rng, nb).reshape(-1), random_q6k_blocks(self.rng, nb).reshape(-1)
         self.quants = self.rng.integers(-127, 128, size=N * K, dtype=np.int8)
@@ -80,8 +81,9 @@ def test_on_the_captured_stream():
     t.ctx.close()
 
 
-def test_while_another_stream_is_captured():
-    t = Work()
+@pytest.mark.parametrize("own_stream", [True, False])
+def test_while_another_stream_is_captured(own_stream):
+    t = Work(own_stream)
     gone, v, other = [way() for way in t.ways()], torch.ones(1000, device=DEV), torch.cuda.Stream()
     want = t.projected(gone[0])
     retired = t.ctx.scratch_bytes()[1]
