@@ -359,7 +359,8 @@ OVFQ_API int ovfq_residual_norm_dev(ovfq_ctx* ctx, const float* y, const float* 
  * logits):
  *   draft x is accepted while accept_uniform * q(x) < p(x);
  *   the first one refused is replaced by a draw from max(p - q, 0) (from p, where that is all zero), or, with none refused,
- *   one more token is drawn from the last row's p: the lowest token whose running sum passes final_uniforms[r] times the total.
+ *   one more token is drawn from the last row's p: the lowest token whose running sum passes final_uniforms[r] times the total (a
+ *   number in [0, 1); not below 1: the last token with a weight).
  * accepted[r] is the number of drafts kept; tokens [rows] holds, from row_offsets[r] on, those and the drawn token, then -1.
  * A target that samples from fewer tokens (top-k, top-p, min-p) has the others' logits set to -inf before. Logits of -inf or NaN
  * have no probability; a row without a finite largest logit refuses its draft, and draws -1. A draft outside the vocabulary is

@@ -427,7 +427,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(const VerifyA
         alone = -1.0;
         total = add_up();
     }
-    const double target = (double)final_u * total;
+    // (a number of 1 or more: no running sum passes the total, also not one that rounding puts above it)
+    const double target = final_u < 1.0f ? (double)final_u * total : INFINITY;
     // the piece in which the running sum passes (every wave the same)
     double before = 0.0, some_before = 0.0;
     int hit = -1, some = 0;

@@ -67,3 +67,25 @@ def test_units_are_weights(temperature):
     t = np.array([temperature], F)
     for last in (0.0, 0.5):
         run(row, off, none, np.zeros(0, F), np.array([last], F), temperature=t)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("vocab", [2, 25, 460, 9000])
+def test_a_number_of_one_gives_the_last_token_with_a_weight(vocab, probs):
+    # no running sum passes the whole total, also not one that was rounded up
+    print("[case]", vocab, probs, flush=True, file=sys.stderr)
+    rng = np.random.default_rng(vocab)
+    requests = 300 if vocab < 5000 else 60
+    logits = (rng.standard_normal((2 * requests, vocab)) * rng.choice([1.0, 20.0, 150.0], (2 * requests, 1))).astype(F)
+    logits[rng.random(logits.shape) < 0.2] = -np.inf
+    logits[:, 0] = 1.0
+    off = (2 * np.arange(requests + 1)).astype(np.int32)
+    drafts = rng.integers(0, vocab, requests).astype(np.int32)
+    q = None
+    if probs:
+        q = rng.random((requests, vocab)).astype(F) ** 8
+        q /= q.sum(1, keepdims=True)
+    u = rng.random(requests).astype(F)
+    last = rng.choice(np.array([1.0, 1.5, np.inf, np.nan], F), requests)
+    _, out = run(logits, off, drafts, u, last, q)
+    assert (out.reshape(requests, 2).max(1) >= 0).all()
