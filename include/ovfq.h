@@ -60,9 +60,10 @@ extern "C" {
 #define OVFQ_TYPE_Q5_0 6
 #define OVFQ_TYPE_Q5_K 13
 
-/* Plain element types (ggml's ids), for what is kept unquantized: low-rank adapters. */
+/* Plain element types (ggml's ids), for what is kept unquantized: low-rank adapters, keys and values. OVFQ_TYPE_I8: caches only. */
 #define OVFQ_TYPE_F32 0
 #define OVFQ_TYPE_F16 1
+#define OVFQ_TYPE_I8 24
 #define OVFQ_TYPE_BF16 30
 
 /* Block geometry. */
@@ -75,6 +76,7 @@ extern "C" {
 typedef struct ovfq_ctx ovfq_ctx;
 typedef struct ovfq_weight ovfq_weight;
 typedef struct ovfq_adapters ovfq_adapters;
+typedef struct ovfq_kv ovfq_kv;
 
 /* ------------------------------------------------------------------------------------------------ context */
 
@@ -377,6 +379,95 @@ OVFQ_API int ovfq_verify_drafts_dev(ovfq_ctx* ctx, const float* logits, int rows
                                     const int* row_offsets, const int* draft_tokens, const float* draft_probs,
                                     const float* temperature, const float* accept_uniforms,
                                     const float* final_uniforms, int* accepted, int* tokens);
+
+/* --------------------------------------------------------------------------- paged keys and values, attention */
+
+/* A cache of keys and values for many requests (the reference keeps one request's, RT/KeyValueCache.cs, in fp32 or 8 bits):
+ * `pages` pages of `page_size` tokens (32, 64, 128 or 256) of `kv_heads` heads of `head_dim` channels (a multiple of 8, at most 256), kept
+ * in `type`: OVFQ_TYPE_F16, OVFQ_TYPE_BF16, or OVFQ_TYPE_I8, int8 quants with one fp32 scale for each token and head, absmax / 127,
+ * rounded as Q8_0 activations are. Which page holds what is the caller's: a request's table lists its pages in order, and requests may
+ * share pages that no call writes. All memory is allocated here, in the kernels' own order, and zeroed; head_dim is rounded up to
+ * 64, 96 (not I8), 128 or 256 in it. `sums` != 0: each full page's sum of keys is kept too (ovfq_attend_selected needs it). A cache
+ * belongs to its context like a weight; not while the context's stream is captured (OVFQ_ERR_STATE), and destroyed then it
+ * leaves its memory as an adapter set does. pages * page_size stays below 2^31. */
+#define OVFQ_MAX_KV_HEADS 1024
+#define OVFQ_MAX_HEAD_DIM 256
+OVFQ_API int ovfq_kv_create(ovfq_ctx* ctx, int type, int kv_heads, int head_dim, int page_size, int pages, int sums,
+                            ovfq_kv** out);
+OVFQ_API int ovfq_kv_destroy(ovfq_kv* kv);
+/* Any out pointer may be NULL. padded_dim: head_dim rounded up; device_blocks, device_sums: addresses of the memory (sums NULL without
+ * them), whose order overfit_amd/csrc/kv_cache.h describes. */
+OVFQ_API int ovfq_kv_info(const ovfq_kv* kv, int* type, int* kv_heads, int* head_dim, int* page_size, int* pages,
+                          int* padded_dim, size_t* byte_count, const void** device_blocks, const float** device_sums);
+
+/* The requests of one call. Request r's new tokens are rows row_offsets[r] .. row_offsets[r + 1] - 1 of the call's planes; lengths[r]
+ * counts all of its tokens, the new ones among them, so that row row_offsets[r] + i is its token lengths[r] - (its rows) + i, in page
+ * tables[r][token / page_size]. A request may have no rows. max_rows bounds every request's rows (0: not known; it sizes launches). */
+typedef struct ovfq_kv_batch {
+    int requests;
+    int table_width;        /* entries of a request's table                                       */
+    int max_rows;
+    const int* row_offsets; /* [requests + 1]                                                     */
+    const int* lengths;     /* [requests]                                                         */
+    const int* tables;      /* [requests][table_width]; entries past a request's tokens: anything */
+} ovfq_kv_batch;
+
+/* Rotary positions: pair j of a head, j < rotary_dim / 2, is turned by the angle position * inv_freq[j]; channels from rotary_dim on are
+ * left. Each cosine and sine is multiplied by `scale`. With several axes (time, height, width) pair j takes the position of axis
+ * pair_axes[j]; an axis that there is no position of counts as position 0. */
+#define OVFQ_ROPE_PAIRS 0  /* pair j is channels 2 j and 2 j + 1              */
+#define OVFQ_ROPE_HALVES 1 /* pair j is channels j and j + rotary_dim / 2     */
+#define OVFQ_MAX_ROPE_AXES 4
+typedef struct ovfq_rope {
+    int rotary_dim;       /* even, at most head_dim  */
+    int style;
+    int axes;             /* of positions, 1 .. OVFQ_MAX_ROPE_AXES */
+    float scale;
+    const float* inv_freq; /* [rotary_dim / 2]                     */
+    const int* pair_axes;  /* [rotary_dim / 2]; NULL: all axis 0   */
+} ovfq_rope;
+
+/* New tokens into the cache: k and v [rows][kv_heads * head_dim], k turned by its position and both rounded to the cache's type; q
+ * [rows][heads * head_dim] turned by the same angles into q_out (which may be q). q may be NULL (keys and values only), or k and v
+ * (queries only). rope NULL: nothing is turned (q then has no place here). positions [axes][rows]; NULL: each token's place in its request,
+ * on every axis. Angles are fp64, cosines and sines fp32, the rotation single fp32 operations. Tables of different requests must not share
+ * pages that the call writes. Where the cache keeps sums, a page's is taken when its last token is appended. Not more rows than 65536, nor
+ * rows * kv_heads than OVFQ_MAX_ATTEND_ROWS. Host pointers (also in the structures), synchronous. */
+#define OVFQ_MAX_ATTEND_ROWS (1 << 22)
+OVFQ_API int ovfq_kv_append(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
+                            const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out);
+/* As ovfq_kv_append; the pointers are device pointers, the structures themselves lie in host memory and are read during the call.
+ * The host form refuses offsets that do not start at 0, fall or do not end at rows, more rows than max_rows, lengths below a request's rows
+ * or past its table, pages outside the cache, and pages that two requests of the call would write. Here a request whose offsets fall or
+ * leave the rows has no rows; rows of no request are left as they were; a token before the first, past the table or in a page outside the
+ * cache is not stored (its query is turned all the same). Offsets of different requests must not overlap. */
+OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
+                                const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out);
+
+/* Attention of each request's new tokens, already appended, over its pages (the reference's per-head loops, RT/CachedAttentionKernel.cs and
+ * RT/BatchedAttentionKernel.cs): for row m, token p of its request, and query head h, whose keys are head h / (heads / kv_heads)'s,
+ *   out[m][h] = sum over tokens j, p - window < j <= p (window 0: 0 <= j <= p), of softmax(scale q[m][h] . k_j) v_j
+ * heads is a multiple of kv_heads. q and the probabilities enter the products with all but the last two of fp32's bits at least, sums are
+ * fp32. Tokens in pages outside the cache count as hidden; a row that sees no token gives 0. What is not finite stays in the rows
+ * that see it. The host form refuses what ovfq_kv_append does, but for shared pages; in the other a request of more than max_rows rows
+ * is left out (its rows of `out` stay as they were), and offsets count as there. Host pointers, synchronous. */
+OVFQ_API int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
+                         float scale, int window, float* out);
+/* As ovfq_attend, with device pointers (enqueued on the context's stream). */
+OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
+                             float scale, int window, float* out);
+
+/* The same over a few pages for each row and key head: the page of the row's own token, and of the full pages before it the top_pages - 1
+ * whose mean key fits its query heads best (the largest q[m][h] . mean over the key head's h, in fp64; of equal fits the lower page, one
+ * that is no number last). pages [rows][kv_heads][top_pages], if not NULL, receives their places in the request's table in rising order,
+ * then -1. The cache keeps sums. Tables of up to OVFQ_MAX_SELECT_WIDTH pages; heads / kv_heads * head_dim at most 16384. */
+#define OVFQ_MAX_SELECT_WIDTH 65536
+#define OVFQ_MAX_TOP_PAGES 4096
+OVFQ_API int ovfq_attend_selected(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
+                                  int heads, float scale, int top_pages, float* out, int* pages);
+/* As ovfq_attend_selected, with device pointers (enqueued on the context's stream). */
+OVFQ_API int ovfq_attend_selected_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
+                                      int heads, float scale, int top_pages, float* out, int* pages);
 
 /* ---------------------------------------------------------------------------- per-head attention output */
 

@@ -27,8 +27,13 @@ TYPE_Q5_K = 13
 TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_BF16 = 30
+TYPE_I8 = 24
 MAX_ADAPTER_SLOTS = 4096
 MAX_ADAPTER_RANK = 256
+MAX_KV_HEADS = 1024
+MAX_HEAD_DIM = 256
+MAX_ROPE_AXES = 4
+MAX_TOP_PAGES = 4096
 
 vp = ctypes.c_void_p
 ci = ctypes.c_int
@@ -45,6 +50,22 @@ class NormStruct(ctypes.Structure):
 
 
 NP = ctypes.POINTER(NormStruct)
+
+
+class KvBatchStruct(ctypes.Structure):
+    """ovfq_kv_batch."""
+
+    _fields_ = [("requests", ci), ("table_width", ci), ("max_rows", ci), ("row_offsets", vp), ("lengths", vp), ("tables", vp)]
+
+
+class RopeStruct(ctypes.Structure):
+    """ovfq_rope."""
+
+    _fields_ = [("rotary_dim", ci), ("style", ci), ("axes", ci), ("scale", cf), ("inv_freq", vp), ("pair_axes", vp)]
+
+
+BP = ctypes.POINTER(KvBatchStruct)
+RP = ctypes.POINTER(RopeStruct)
 
 # name -> (restype, argtypes). Every symbol include/ovfq.h declares.
 SIGNATURES = {
@@ -108,6 +129,15 @@ SIGNATURES = {
     "ovfq_residual_norm_dev": (ci, [vp, vp, vp, ci, ci, NP, vp, ci, cf, NP, vp, vp]),
     "ovfq_verify_drafts": (ci, [vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp]),
     "ovfq_verify_drafts_dev": (ci, [vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "ovfq_kv_create": (ci, [vp] + [ci] * 6 + [PP]),
+    "ovfq_kv_destroy": (ci, [vp]),
+    "ovfq_kv_info": (ci, [vp] + [ctypes.POINTER(ci)] * 6 + [ctypes.POINTER(sz), PP, PP]),
+    "ovfq_kv_append": (ci, [vp, vp, BP, vp, vp, ci, RP, vp, vp, ci, vp]),
+    "ovfq_kv_append_dev": (ci, [vp, vp, BP, vp, vp, ci, RP, vp, vp, ci, vp]),
+    "ovfq_attend": (ci, [vp, vp, BP, vp, ci, ci, cf, ci, vp]),
+    "ovfq_attend_dev": (ci, [vp, vp, BP, vp, ci, ci, cf, ci, vp]),
+    "ovfq_attend_selected": (ci, [vp, vp, BP, vp, ci, ci, cf, ci, vp, vp]),
+    "ovfq_attend_selected_dev": (ci, [vp, vp, BP, vp, ci, ci, cf, ci, vp, vp]),
     "ovfq_quantize_weight_q4k_dev": (ci, [vp, vp, ci, ci, vp]),
     "ovfq_quantize_weight_q6k_dev": (ci, [vp, vp, ci, ci, vp]),
     "ovfq_quantize_weight_q8_0_dev": (ci, [vp, vp, ci, ci, vp, vp]),

@@ -73,6 +73,7 @@ struct ovfq_ctx {
     // Live weights created on this context (ovfq_ctx_destroy refuses while any remain).
     int live_weights = 0;
     int live_adapters = 0;  // the same for adapter sets
+    int live_caches = 0;    // and for caches of keys and values
 };
 
 // One device allocation holding every expert sliced from a 3-D GGUF expert tensor; the last expert weight
@@ -111,6 +112,13 @@ struct ovfq_adapters {
     size_t elem() const { return (size_t)ovfq::adapter_elem(type); }
     size_t a_slot() const { return (size_t)ovfq::adapter_a_slot(in, max_rank) * elem(); }
     size_t b_slot() const { return (size_t)ovfq::adapter_b_slot(out, max_rank) * elem(); }
+};
+
+// A paged cache of keys and values (ovfq_kv_create): its blocks, and the pages' sums behind them, in one allocation.
+struct ovfq_kv {
+    ovfq_ctx* ctx = nullptr;
+    ovfq::KvPool pool{};
+    size_t nbytes = 0;
 };
 
 namespace {
@@ -719,6 +727,8 @@ int ovfq_ctx_destroy(ovfq_ctx* c) {
             return fail(OVFQ_ERR_STATE, "context still owns %d weight(s): destroy them first", c->live_weights);
         if (c->live_adapters > 0)
             return fail(OVFQ_ERR_STATE, "context still owns %d adapter set(s): destroy them first", c->live_adapters);
+        if (c->live_caches > 0)
+            return fail(OVFQ_ERR_STATE, "context still owns %d cache(s) of keys and values: destroy them first", c->live_caches);
         (void)hipSetDevice(c->device);
         (void)hipStreamSynchronize(c->stream);
         DevBuf* bufs[] = {&c->act_q,   &c->act_s,   &c->act_b,      &c->x_stage,
@@ -1792,6 +1802,354 @@ int ovfq_verify_drafts_dev(ovfq_ctx* ctx, const float* logits, int rows, int voc
                            const float* accept_uniforms, const float* final_uniforms, int* accepted, int* tokens) {
     return verify_impl(ctx, logits, rows, vocab, requests, row_offsets, draft_tokens, draft_probs, temperature,
                        accept_uniforms, final_uniforms, accepted, tokens, false);
+}
+
+// ---------------------------------------------------------------------------------------- paged keys and values
+
+int ovfq_kv_create(ovfq_ctx* ctx, int type, int kv_heads, int head_dim, int page_size, int pages, int sums, ovfq_kv** out) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    if (!out) return fail(OVFQ_ERR_NULL, "out is NULL");
+    if (type != OVFQ_TYPE_F16 && type != OVFQ_TYPE_BF16 && type != OVFQ_TYPE_I8)
+        return fail(OVFQ_ERR_TYPE, "unsupported cache type %d", type);
+    if (kv_heads <= 0 || kv_heads > OVFQ_MAX_KV_HEADS)
+        return fail(OVFQ_ERR_RANGE, "kv_heads (%d) must be in [1, %d]", kv_heads, OVFQ_MAX_KV_HEADS);
+    if (head_dim <= 0 || head_dim > OVFQ_MAX_HEAD_DIM)
+        return fail(OVFQ_ERR_RANGE, "head_dim (%d) must be in [8, %d]", head_dim, OVFQ_MAX_HEAD_DIM);
+    if (head_dim % 8) return fail(OVFQ_ERR_SIZE, "head_dim (%d) must be a multiple of 8", head_dim);
+    if (page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+        return fail(OVFQ_ERR_RANGE, "page_size (%d) must be 32, 64, 128 or 256", page_size);
+    if (pages <= 0) return fail(OVFQ_ERR_RANGE, "pages (%d) must be positive", pages);
+    if ((int64_t)pages * page_size >= (int64_t)1 << 31)
+        return fail(OVFQ_ERR_SIZE, "%d pages of %d tokens exceed 2^31 - 1", pages, page_size);
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    int rc = check_not_capturing(ctx, "a cache cannot be created");
+    if (rc) return rc;
+    const RelaxedCapture relaxed;
+    ovfq_kv* kv = new (std::nothrow) ovfq_kv();
+    if (!kv) return fail(OVFQ_ERR_HIP, "no host memory for a cache");
+    kv->ctx = ctx;
+    ovfq::KvPool& p = kv->pool;
+    p.type = type;
+    p.kv_heads = kv_heads;
+    p.dim = head_dim;
+    p.dp = ovfq::kv_padded_dim(type, head_dim);
+    p.page = page_size;
+    p.pages = pages;
+    auto carve = [&](Carver& c) {
+        p.mem = c.take<char>((size_t)pages * kv_heads * (page_size / ovfq::kKvBlock) * ovfq::kv_block_bytes(type, p.dp));
+        p.sums = sums ? c.take<float>((size_t)pages * kv_heads * head_dim * sizeof(float)) : nullptr;
+    };
+    Carver sizing{nullptr};
+    carve(sizing);
+    kv->nbytes = sizing.used;
+    void* mem = nullptr;
+    hipError_t e = hipMalloc(&mem, kv->nbytes);
+    if (e == hipSuccess) {
+        Carver c{static_cast<char*>(mem)};
+        carve(c);
+        e = ovfq::launch_kv_clear(mem, kv->nbytes, ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    }
+    if (e != hipSuccess) {
+        if (mem) (void)hipFree(mem);
+        (void)hipGetLastError();
+        const size_t n = kv->nbytes;
+        delete kv;
+        return fail(OVFQ_ERR_HIP, "cache of %zu B: %s", n, hipGetErrorString(e));
+    }
+    ctx->live_caches++;
+    *out = kv;
+    return ok();
+}
+
+int ovfq_kv_destroy(ovfq_kv* kv) {
+    if (!kv) return fail(OVFQ_ERR_NULL, "cache is NULL");
+    {
+        ovfq_ctx* c = kv->ctx;
+        std::lock_guard<std::mutex> lk(c->mu);
+        const int rc = free_device(c, {kv->pool.mem}, kv->nbytes);
+        if (rc) return rc;
+        c->live_caches--;
+    }
+    delete kv;
+    return ok();
+}
+
+int ovfq_kv_info(const ovfq_kv* kv, int* type, int* kv_heads, int* head_dim, int* page_size, int* pages, int* padded_dim,
+                 size_t* byte_count, const void** device_blocks, const float** device_sums) {
+    if (!kv) return fail(OVFQ_ERR_NULL, "cache is NULL");
+    const ovfq::KvPool& p = kv->pool;
+    if (type) *type = p.type;
+    if (kv_heads) *kv_heads = p.kv_heads;
+    if (head_dim) *head_dim = p.dim;
+    if (page_size) *page_size = p.page;
+    if (pages) *pages = p.pages;
+    if (padded_dim) *padded_dim = p.dp;
+    if (byte_count) *byte_count = kv->nbytes;
+    if (device_blocks) *device_blocks = p.mem;
+    if (device_sums) *device_sums = p.sums;
+    return ok();
+}
+
+// What the calls on a cache have in common; host: what the batch says is checked too, for the pages that a call stores to (writes) or
+// sees (window 0: all).
+static int check_kv_call(const ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* b, int rows, bool host, bool writes, int window) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    if (!kv) return fail(OVFQ_ERR_NULL, "cache is NULL");
+    if (kv->ctx != ctx) return fail(OVFQ_ERR_SIZE, "cache belongs to another context");
+    if (!b) return fail(OVFQ_ERR_NULL, "batch is NULL");
+    if (!b->row_offsets || !b->lengths || !b->tables) return fail(OVFQ_ERR_NULL, "row_offsets / lengths / tables is NULL");
+    int rc;
+    if ((rc = check_rows(rows))) return rc;
+    if (b->requests <= 0 || b->requests > 65536) return fail(OVFQ_ERR_RANGE, "requests (%d) must be in [1, 65536]", b->requests);
+    if (b->table_width <= 0) return fail(OVFQ_ERR_RANGE, "table_width (%d) must be positive", b->table_width);
+    if (b->max_rows < 0) return fail(OVFQ_ERR_RANGE, "max_rows (%d) must not be negative", b->max_rows);
+    if ((rc = check_plane(b->requests, b->table_width, "tables"))) return rc;
+    const ovfq::KvPool& p = kv->pool;
+    if ((int64_t)rows * p.kv_heads > OVFQ_MAX_ATTEND_ROWS)
+        return fail(OVFQ_ERR_SIZE, "rows (%d) * kv_heads (%d) above %d", rows, p.kv_heads, OVFQ_MAX_ATTEND_ROWS);
+    if ((rc = check_plane(rows, (int64_t)p.kv_heads * p.dim, "keys"))) return rc;
+    if (!host) {
+        if (rc_align(b->row_offsets) || rc_align(b->lengths) || rc_align(b->tables))
+            return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+        return OVFQ_OK;
+    }
+    bool good = b->row_offsets[0] == 0 && b->row_offsets[b->requests] == rows;
+    for (int r = 0; r < b->requests; r++) good = good && b->row_offsets[r] <= b->row_offsets[r + 1];
+    if (!good) return fail(OVFQ_ERR_SIZE, "row_offsets must start at 0, not fall and end at rows (%d)", rows);
+    std::vector<bool> written;
+    try {
+        if (writes) written.resize((size_t)p.pages);
+    } catch (const std::bad_alloc&) {
+        return fail(OVFQ_ERR_HIP, "no host memory to check the tables");
+    }
+    for (int r = 0; r < b->requests; r++) {
+        const int n = b->row_offsets[r + 1] - b->row_offsets[r], len = b->lengths[r];
+        if (!n) continue;
+        if (b->max_rows && n > b->max_rows) return fail(OVFQ_ERR_SIZE, "request %d has %d rows, max_rows is %d", r, n, b->max_rows);
+        if (len < n) return fail(OVFQ_ERR_SIZE, "request %d has %d tokens in all and %d new ones", r, len, n);
+        if ((int64_t)len > (int64_t)b->table_width * p.page)
+            return fail(OVFQ_ERR_SIZE, "request %d has %d tokens, its table takes %lld", r, len, (long long)b->table_width * p.page);
+        const int *table = b->tables + (size_t)r * b->table_width, last = (len - 1) / p.page, first_new = (len - n) / p.page;
+        const int first = writes ? first_new : window > 0 && len - n >= window ? (len - n - window + 1) / p.page : 0;
+        for (int i = first; i <= last; i++) {
+            if (table[i] < 0 || table[i] >= p.pages)
+                return fail(OVFQ_ERR_RANGE, "request %d: page %d out of range [0, %d)", r, table[i], p.pages);
+            if (!writes) continue;
+            if (written[table[i]]) return fail(OVFQ_ERR_SIZE, "page %d would be written twice", table[i]);
+            written[table[i]] = true;
+        }
+    }
+    return OVFQ_OK;
+}
+
+static int check_heads(const ovfq_kv* kv, int rows, int heads) {
+    if (heads <= 0) return fail(OVFQ_ERR_RANGE, "heads (%d) must be positive", heads);
+    if (heads % kv->pool.kv_heads) return fail(OVFQ_ERR_SIZE, "heads (%d) must be a multiple of kv_heads (%d)", heads, kv->pool.kv_heads);
+    return check_plane(rows, (int64_t)heads * kv->pool.dim, "queries");
+}
+
+static ovfq::KvBatch kv_batch(const ovfq_kv_batch* b, int rows, const void* const* in) {
+    ovfq::KvBatch k{};
+    k.row_offsets = (const int*)in[0];
+    k.lengths = (const int*)in[1];
+    k.tables = (const int*)in[2];
+    k.requests = b->requests;
+    k.width = b->table_width;
+    k.rows = rows;
+    k.most = b->max_rows && b->max_rows < rows ? b->max_rows : rows;
+    return k;
+}
+
+static int kv_append_impl(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
+                          const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out, bool host) {
+    int rc = check_kv_call(ctx, kv, batch, rows, host, k != nullptr, 1);
+    if (rc) return rc;
+    const ovfq::KvPool& p = kv->pool;
+    if ((k == nullptr) != (v == nullptr)) return fail(OVFQ_ERR_NULL, "k and v go together");
+    if (!k && !q) return fail(OVFQ_ERR_NULL, "k, v and q are NULL");
+    if ((q == nullptr) != (q_out == nullptr)) return fail(OVFQ_ERR_NULL, "q and q_out go together");
+    if (q && !rope) return fail(OVFQ_ERR_NULL, "q without a rope");
+    if (q && (rc = check_heads(kv, rows, heads))) return rc;
+    if (positions && !rope) return fail(OVFQ_ERR_NULL, "positions without a rope");
+    if (rope) {
+        if (rope->rotary_dim <= 0 || rope->rotary_dim > p.dim)
+            return fail(OVFQ_ERR_RANGE, "rotary_dim (%d) must be in [2, %d]", rope->rotary_dim, p.dim);
+        if (rope->rotary_dim % 2) return fail(OVFQ_ERR_SIZE, "rotary_dim (%d) must be even", rope->rotary_dim);
+        if (rope->style != OVFQ_ROPE_PAIRS && rope->style != OVFQ_ROPE_HALVES)
+            return fail(OVFQ_ERR_RANGE, "rope style %d is neither OVFQ_ROPE_PAIRS nor OVFQ_ROPE_HALVES", rope->style);
+        if (rope->axes < 1 || rope->axes > OVFQ_MAX_ROPE_AXES)
+            return fail(OVFQ_ERR_RANGE, "axes (%d) must be in [1, %d]", rope->axes, OVFQ_MAX_ROPE_AXES);
+        if (!std::isfinite(rope->scale)) return fail(OVFQ_ERR_RANGE, "the rope's scale must be finite");
+        if (!rope->inv_freq) return fail(OVFQ_ERR_NULL, "inv_freq is NULL");
+        if (host && rope->pair_axes) {
+            for (int j = 0; j < rope->rotary_dim / 2; j++)
+                if (rope->pair_axes[j] < 0 || rope->pair_axes[j] >= rope->axes)
+                    return fail(OVFQ_ERR_RANGE, "pair %d: axis %d out of range [0, %d)", j, rope->pair_axes[j], rope->axes);
+        }
+        if (!host && (rc_align(rope->inv_freq) || rc_align(rope->pair_axes)))
+            return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    }
+    if (!host && (rc_align(k) || rc_align(v) || rc_align(q) || rc_align(q_out) || rc_align(positions)))
+        return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    const size_t R = (size_t)rows, Q = (size_t)batch->requests, half = rope ? (size_t)rope->rotary_dim / 2 : 0;
+    const size_t key_bytes = R * p.kv_heads * p.dim * 4, query_bytes = R * (size_t)heads * p.dim * 4;
+    const void* in[9] = {batch->row_offsets, batch->lengths, batch->tables, k, v, q, positions, rope ? rope->inv_freq : nullptr,
+                         rope ? rope->pair_axes : nullptr};
+    const size_t bytes[9] = {(Q + 1) * 4, Q * 4, Q * batch->table_width * 4, key_bytes, key_bytes, query_bytes,
+                             rope ? R * rope->axes * 4 : 0, half * 4, half * 4};
+    float* turned = q_out;
+    HostIO io(ctx);
+    if (host) {
+        void* dev[9];
+        auto carve = [&](Carver& c) {
+            for (int i = 0; i < 9; i++) dev[i] = in[i] ? c.take<char>(bytes[i]) : nullptr;
+            if (q) turned = c.take<float>(query_bytes);
+        };
+        Carver sizing{nullptr};
+        carve(sizing);
+        if ((rc = ensure(ctx, ctx->step, sizing.used))) return rc;
+        Carver c{static_cast<char*>(ctx->step.p)};
+        carve(c);
+        for (int i = 0; i < 9; i++) {
+            if (in[i] && (rc = io.up(dev[i], in[i], bytes[i]))) return rc;
+            in[i] = dev[i];
+        }
+    }
+    ovfq::KvAppendArgs a{};
+    a.pool = p;
+    a.batch = kv_batch(batch, rows, in);
+    a.k = (const float*)in[3];
+    a.v = (const float*)in[4];
+    a.q = (const float*)in[5];
+    a.q_out = turned;
+    a.heads = heads;
+    if (rope) {
+        a.rope.positions = (const int*)in[6];
+        a.rope.freq = (const float*)in[7];
+        a.rope.axes = (const int*)in[8];
+        a.rope.rotary = rope->rotary_dim;
+        a.rope.n_axes = rope->axes;
+        a.rope.halves = rope->style == OVFQ_ROPE_HALVES;
+        a.rope.scale = rope->scale;
+    }
+    HIP_TRY(ovfq::launch_kv_append(a, ctx->stream));
+    if (host && ((q && (rc = io.down(q_out, turned, query_bytes))) || (rc = io.finish()))) return rc;
+    return ok();
+}
+
+int ovfq_kv_append(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
+                   const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out) {
+    return kv_append_impl(ctx, kv, batch, k, v, rows, rope, positions, q, heads, q_out, true);
+}
+
+int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
+                       const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out) {
+    return kv_append_impl(ctx, kv, batch, k, v, rows, rope, positions, q, heads, q_out, false);
+}
+
+// top: pages a row and key head, 0 for all of them.
+static int attend_impl(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads, float scale,
+                       int window, int top, float* out, int* pages, bool host) {
+    int rc = check_kv_call(ctx, kv, batch, rows, host, false, window);
+    if (rc) return rc;
+    if (!q) return fail(OVFQ_ERR_NULL, "q is NULL");
+    if (!out) return fail(OVFQ_ERR_NULL, "out is NULL");
+    if ((rc = check_heads(kv, rows, heads))) return rc;
+    if (!std::isfinite(scale)) return fail(OVFQ_ERR_RANGE, "scale must be finite");
+    if (window < 0) return fail(OVFQ_ERR_RANGE, "window (%d) must not be negative", window);
+    const ovfq::KvPool& p = kv->pool;
+    if (top) {
+        if (!p.sums) return fail(OVFQ_ERR_STATE, "the cache keeps no sums of its pages");
+        if (batch->table_width > OVFQ_MAX_SELECT_WIDTH)
+            return fail(OVFQ_ERR_SIZE, "table_width (%d) above %d", batch->table_width, OVFQ_MAX_SELECT_WIDTH);
+        if (heads / p.kv_heads * p.dim > 16384)
+            return fail(OVFQ_ERR_SIZE, "heads / kv_heads (%d) * head_dim (%d) above 16384", heads / p.kv_heads, p.dim);
+        if ((rc = check_plane((int64_t)rows * p.kv_heads, top, "pages")) ||
+            (rc = check_plane((int64_t)rows * p.kv_heads, batch->table_width, "fits")))
+            return rc;
+    }
+    if (!host && (rc_align(q) || rc_align(out) || rc_align(pages)))
+        return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
+    const size_t R = (size_t)rows, Q = (size_t)batch->requests, plane = R * heads * p.dim * 4, list = R * p.kv_heads * top * 4;
+    const void* in[4] = {batch->row_offsets, batch->lengths, batch->tables, q};
+    const size_t bytes[4] = {(Q + 1) * 4, Q * 4, Q * batch->table_width * 4, plane};
+    ovfq::AttendArgs a{};
+    a.pool = p;
+    a.batch = kv_batch(batch, rows, in);
+    a.heads = heads;
+    a.window = window;
+    a.scale = scale;
+    a.top = top;
+    const size_t parts = top ? ovfq::attend_selected_scratch(a) : ovfq::attend_scratch(a);
+    void* dev[4];
+    float* o = out;
+    int* chosen = pages;
+    auto carve = [&](Carver& c) {
+        a.parts = parts ? c.take<float>(parts) : nullptr;
+        if (top) {
+            a.where = c.take<int>(R * 4);
+            a.fits = c.take<double>(R * p.kv_heads * batch->table_width * sizeof(double));
+            if (host || !pages) chosen = c.take<int>(list);
+        }
+        if (!host) return;
+        for (int i = 0; i < 4; i++) dev[i] = c.take<char>(bytes[i]);
+        o = c.take<float>(plane);
+    };
+    Carver sizing{nullptr};
+    carve(sizing);
+    if ((rc = ensure(ctx, ctx->step, sizing.used))) return rc;
+    Carver c{static_cast<char*>(ctx->step.p)};
+    carve(c);
+    HostIO io(ctx);
+    if (host) {
+        for (int i = 0; i < 4; i++) {
+            if ((rc = io.up(dev[i], in[i], bytes[i]))) return rc;
+            in[i] = dev[i];
+        }
+    }
+    a.batch = kv_batch(batch, rows, in);
+    a.q = (const float*)in[3];
+    a.out = o;
+    a.chosen = chosen;
+    HIP_TRY(top ? ovfq::launch_attend_selected(a, ctx->stream) : ovfq::launch_attend(a, ctx->stream));
+    if (host && ((rc = io.down(out, o, plane)) || (pages && (rc = io.down(pages, chosen, list))) || (rc = io.finish()))) return rc;
+    return ok();
+}
+
+int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads, float scale,
+                int window, float* out) {
+    return attend_impl(ctx, kv, batch, q, rows, heads, scale, window, 0, out, nullptr, true);
+}
+
+int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads, float scale,
+                    int window, float* out) {
+    return attend_impl(ctx, kv, batch, q, rows, heads, scale, window, 0, out, nullptr, false);
+}
+
+static int check_top(int top_pages) {
+    if (top_pages < 1 || top_pages > OVFQ_MAX_TOP_PAGES)
+        return fail(OVFQ_ERR_RANGE, "top_pages (%d) must be in [1, %d]", top_pages, OVFQ_MAX_TOP_PAGES);
+    return OVFQ_OK;
+}
+
+int ovfq_attend_selected(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
+                         float scale, int top_pages, float* out, int* pages) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    const int rc = check_top(top_pages);
+    return rc ? rc : attend_impl(ctx, kv, batch, q, rows, heads, scale, 0, top_pages, out, pages, true);
+}
+
+int ovfq_attend_selected_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
+                             float scale, int top_pages, float* out, int* pages) {
+    if (!ctx) return fail(OVFQ_ERR_NULL, "ctx is NULL");
+    const int rc = check_top(top_pages);
+    return rc ? rc : attend_impl(ctx, kv, batch, q, rows, heads, scale, 0, top_pages, out, pages, false);
 }
 
 // ---------------------------------------------------------------------------------------- per-head Q8_0 Wo

@@ -1,0 +1,344 @@
+// attend_few.hip — attention of few columns (up to 32 (row, query head) pairs of a request and key head: decode steps, drafted tokens)
+// over a paged cache, of any columns over selected pages, and the joining of partial outputs. Arithmetic: attend.h.
+//
+// Bound: HBM, each key and value is read once for its request. Four waves take a piece's blocks in turn, straight into registers in
+// operand order (no LDS, no transposition): a block's keys are loaded while the block before it goes through its softmax and second
+// product, its values during its own first one. Pieces are cut so that all key heads together give a few workgroups for each CU
+// whatever the lengths; their partial outputs are joined by a second launch. Waves join theirs in LDS, in a fixed order.
+#include <type_traits>
+
+#include "attend.h"
+
+namespace ovfq {
+
+namespace {
+
+// Where a wave's columns come from and which tokens it walks.
+template <int kType, int kDp, int kCols, bool kSelected>
+__global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void attend_few_kernel(AttendArgs a, Cut cut) {
+    using Att = Attention<kType, kDp, kCols>;
+    using M = KvMath<kType>;
+    __shared__ f32x4 joined[2][kCols * Att::kTiles][64];
+    __shared__ float refs[4][kCols * 16];
+    __shared__ float sums[4][kCols * 16];
+    const KvPool& pool = a.pool;
+    const KvBatch& b = a.batch;
+    const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15;
+    const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads), item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
+    TileWork w;
+    int whole = 0;  // selected: the row's pages, and how many
+    const int* pages = nullptr;
+    const int shift = 31 - __builtin_clz(pool.page / kKvBlock);
+    if constexpr (kSelected) {
+        // item: row, tile of query heads, piece
+        const int tiles = (cut.group + 15) >> 4, per = tiles * cut.target;
+        const int row = item / per;
+        const int r = a.where[row];
+        if (r < 0) return;
+        const KvRows m = kv_rows(b, r);
+        w.r = r;
+        w.first_row = row;
+        w.rows = 1;
+        w.place = kv_length(b, r) - m.n + (row - m.first);
+        w.tile = (item - row * per) / cut.target;
+        w.piece = (item - row * per) % cut.target;
+        w.col0 = 16 * w.tile;
+        w.slot = item;
+        pages = a.chosen + ((size_t)row * pool.kv_heads + head) * a.top;
+        for (int i = 0; i < a.top; i += 64) whole += __popcll(__ballot(i + lane < a.top && pages[min(i + lane, a.top - 1)] >= 0));
+        const int blocks = whole << shift, each = cut.least_blocks;
+        w.pieces = cut_pieces(blocks, each);
+        if (w.piece >= w.pieces) return;
+        w.block0 = w.piece * each;
+        w.block1 = min(blocks, w.block0 + each);
+    } else {
+        if (!cut_item(cut, pool, b, item, w)) return;
+    }
+    Att att;
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = w.col0 + 16 * t + col, i = c / cut.group;
+        const bool used = i < w.rows;
+        const int qh = head * cut.group + (c - i * cut.group);
+        const float* x = used ? a.q + ((size_t)(w.first_row + i) * a.heads + qh) * pool.dim : nullptr;
+        const int last = w.place + i;
+        att.column(t, x, pool.dim, a.scale * kLog2e, a.window ? max(last - a.window + 1, 0) : 0, last);
+    }
+    const int first_last = w.place + w.col0 / cut.group;  // the tile's rows see up to first_last .. last_last
+    const int last_last = w.place + min(w.rows - 1, (w.col0 + 16 * kCols - 1) / cut.group);
+    const int last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+
+    constexpr int kLoads = kv_plane_bytes(kType, kDp) / 1024;
+    u32x4 keys[kLoads], values[kLoads];
+    f32x4 ks[2], vs[2];
+    const int* table = b.tables + (size_t)w.r * b.width;
+    BlockWalk walk;
+    int held = 0;  // selected: lanes' page numbers
+    auto block_of = [&](int i) { return w.block0 + wave + 4 * i; };
+    const int mine = w.block1 > w.block0 + wave ? (w.block1 - w.block0 - wave + 3) >> 2 : 0;
+    int phys = -1;
+    auto selected_fetch = [&](int i) {
+        const int at = (block_of(i) + 4 * lane) >> shift;
+        const int p = at < whole ? pages[at] : -1;
+        held = p;
+        const int t = p >= 0 && p < b.width ? table[p] : -1;
+        phys = t >= 0 && t < pool.pages ? t : -1;
+    };
+    // the page of the wave's i-th block and its first token
+    auto locate = [&](int i, int& page, int& first) {
+        const int block = block_of(i);
+        if constexpr (kSelected) {
+            if (i && (i & 63) == 0) selected_fetch(i);
+            page = __builtin_amdgcn_readlane(phys, i & 63);
+            first = __builtin_amdgcn_readlane(held, i & 63) * pool.page + (block & ((1 << shift) - 1)) * kKvBlock;
+        } else {
+            page = walk.page(i);
+            first = block * kKvBlock;
+        }
+    };
+    // (a page that is not there: its tokens count as hidden)
+    auto source = [&](int i, int page) {
+        return (const char*)kv_block(pool, max(page, 0), head, block_of(i) & ((1 << shift) - 1)) + lane * 16;
+    };
+    auto load_keys = [&](const char* p) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) keys[i] = *(const u32x4*)(p + i * 1024);
+        if constexpr (kType == kKvI8) {
+            const char* s = p - lane * 16 + 2 * kv_plane_bytes(kType, kDp) + (lane >> 4) * 16;
+            ks[0] = *(const f32x4*)s;
+            ks[1] = *(const f32x4*)(s + 64);
+        }
+    };
+    auto load_values = [&](const char* p) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) values[i] = *(const u32x4*)(p + kv_plane_bytes(kType, kDp) + i * 1024);
+        if constexpr (kType == kKvI8) {
+            const char* s = p - lane * 16 + 2 * kv_plane_bytes(kType, kDp) + 128 + (lane >> 4) * 16;
+            vs[0] = *(const f32x4*)s;
+            vs[1] = *(const f32x4*)(s + 64);
+        }
+    };
+    if (mine) {
+        if constexpr (kSelected)
+            selected_fetch(0);
+        else
+            walk.start(pool, table, b.width, block_of(0), 4);
+        int page, first;
+        locate(0, page, first);
+        const char* now = source(0, page);
+        load_keys(now);
+        load_values(now);
+        for (int i = 0; i < mine; i++) {
+            int next_page = -1, next_first = 0;
+            const char* next = now;
+            if (i + 1 < mine) {
+                locate(i + 1, next_page, next_first);
+                next = source(i + 1, next_page);
+            }
+            f32x4 s[kCols][2];
+            att.scores(s, [&](int tile, int chunk) { return key_operand<kType, kDp>(tile, chunk, [&](int at) { return keys[at >> 10]; }); });
+            f32x4 ks_now[2] = {ks[0], ks[1]}, vs_now[2] = {vs[0], vs[1]};
+            if (i + 1 < mine) load_keys(next);
+            const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
+            if (page >= 0) {
+                u32x4 p[kCols][M::kParts];
+                att.probabilities(s, p, masked, first, ks_now, vs_now);
+                att.products(p, masked, first, [&](int tile) {
+                    return value_operand<kType, kDp>(tile, [&](int at) { return values[(at - kv_plane_bytes(kType, kDp)) >> 10]; });
+                });
+            }
+            if (i + 1 < mine) load_values(next);
+            page = next_page;
+            first = next_first;
+            now = next;
+        }
+    }
+    att.close();
+    // join the waves: 2 and 3 into 0 and 1, then 1 into 0
+    if (lane < 16) {
+#pragma unroll
+        for (int t = 0; t < kCols; t++) {
+            refs[wave][16 * t + lane] = att.ref[t];
+            sums[wave][16 * t + lane] = att.l[t];
+        }
+    }
+    __syncthreads();
+    float top[kCols], l[kCols];
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = 16 * t + col;
+        top[t] = fmaxf(fmaxf(refs[0][c], refs[1][c]), fmaxf(refs[2][c], refs[3][c]));
+        const float m = top[t] == -kInf ? 0.0f : top[t];
+        l[t] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; v++) l[t] += sums[v][c] * __builtin_amdgcn_exp2f(refs[v][c] - m);
+        const float f = __builtin_amdgcn_exp2f(att.ref[t] - m);
+#pragma unroll
+        for (int d = 0; d < Att::kTiles; d++) att.o[t][d] *= f;
+    }
+    for (int from = 2; from >= 1; from >>= 1) {
+        if (wave >= from && wave < 2 * from) {
+#pragma unroll
+            for (int t = 0; t < kCols; t++)
+#pragma unroll
+                for (int d = 0; d < Att::kTiles; d++) joined[wave - from][t * Att::kTiles + d][lane] = att.o[t][d];
+        }
+        __syncthreads();
+        if (wave < from) {
+#pragma unroll
+            for (int t = 0; t < kCols; t++)
+#pragma unroll
+                for (int d = 0; d < Att::kTiles; d++) att.o[t][d] += joined[wave][t * Att::kTiles + d][lane];
+        }
+        __syncthreads();
+    }
+    if (wave) return;
+    if (w.pieces > 1) {
+        float* part = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(16 * kCols, kDp);
+#pragma unroll
+        for (int t = 0; t < kCols; t++) {
+            if (lane < 16) {
+                part[32 * t + lane] = top[t];
+                part[32 * t + 16 + lane] = l[t];
+            }
+#pragma unroll
+            for (int d = 0; d < Att::kTiles; d++)
+                *(f32x4*)(part + 32 * kCols + ((t * Att::kTiles + d) * 64 + lane) * 4) = att.o[t][d];
+        }
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = w.col0 + 16 * t + col, i = c / cut.group;
+        if (i >= w.rows) continue;
+        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        float* y = a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim;
+#pragma unroll
+        for (int d = 0; d < Att::kTiles; d++) {
+            const int at = 16 * d + 4 * (lane >> 4);
+            if (at < pool.dim) *(f32x4u*)(y + at) = att.o[t][d] * inv;
+        }
+    }
+}
+
+}  // namespace
+
+// Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l. A workgroup per tile's 16 columns, key head and four
+// 16-channel tiles (blockIdx.y); four waves share the pieces, in a fixed order.
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, bool selected) {
+    __shared__ float tops[16][16], ls[16][16];
+    __shared__ f32x4 part_o[4][64];
+    const KvPool& pool = a.pool;
+    const KvBatch& b = a.batch;
+    const int subs = cut.cols >> 4, lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15;
+    const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads);
+    int item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
+    const int sub = item % subs;
+    item /= subs;
+    TileWork w;
+    if (selected) {
+        const int tiles = (cut.group + 15) >> 4, row = item / tiles;
+        const int r = a.where[row];
+        if (r < 0) return;
+        const int* pages = a.chosen + ((size_t)row * pool.kv_heads + head) * a.top;
+        int whole = 0;
+        for (int i = 0; i < a.top; i += 64) whole += __popcll(__ballot(i + lane < a.top && pages[min(i + lane, a.top - 1)] >= 0));
+        w.first_row = row;
+        w.rows = 1;
+        w.col0 = 16 * (item - row * tiles);
+        w.slot = item * cut.target;
+        w.pieces = cut_pieces(whole * (pool.page / kKvBlock), cut.least_blocks);
+    } else {
+        int r = 0, tiles_before = 0;
+        const int piece = cut_piece(cut, pool, b);
+        int tile = item;
+        if (!kv_find(b.requests, tile, r, tiles_before, [&](int q) { return cut_tiles(cut, kv_rows(b, q).n); })) return;
+        // the pieces of the requests before it
+        int before = 0;
+        for (int q = lane; q < r; q += 64) {
+            const int n = kv_rows(b, q).n, tiles = cut_tiles(cut, n);
+            before += tiles ? tiles * cut_pieces(cut_request_blocks(cut, pool, b, q, n), piece) : 0;
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
+        if (!cut_tile(cut, pool, b, piece, r, tile, 0, before, w)) return;
+    }
+    if (w.pieces <= 1) return;
+    const int c = w.col0 + 16 * sub + col, i = c / cut.group;
+    const bool used = i < w.rows;
+    if (!__ballot(used)) return;
+    const size_t stride = (size_t)part_floats(cut.cols, dp) * pool.kv_heads;
+    const float* base = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(cut.cols, dp);
+    const float* ml = base + 32 * sub + col;
+    // the column's top and sum: 16 threads a column
+    const int share = wave * 4 + (lane >> 4);
+    float top = -kInf;
+    for (int j = share; j < w.pieces; j += 16) top = fmaxf(top, ml[j * stride]);
+    tops[share][col] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; k++) top = fmaxf(top, tops[k][col]);
+    const float m = top == -kInf ? 0.0f : top;
+    float l = 0.0f;
+    for (int j = share; j < w.pieces; j += 16) l += ml[j * stride + 16] * __builtin_amdgcn_exp2f(ml[j * stride] - m);
+    ls[share][col] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) l += ls[k][col];
+    const int tiles = dp >> 4, d = blockIdx.y;
+    f32x4 o = {0, 0, 0, 0};
+    const float* mine = base + 32 * subs + ((sub * tiles + d) * 64 + lane) * 4;
+#pragma unroll 4
+    for (int j = wave; j < w.pieces; j += 4) {
+        const float f = __builtin_amdgcn_exp2f(ml[j * stride] - m);
+        const f32x4 v = used ? *(const f32x4*)(mine + j * stride) : f32x4{0, 0, 0, 0};
+        o += v * f;
+    }
+    part_o[wave][lane] = o;
+    __syncthreads();
+    if (wave || !used) return;
+    o = part_o[0][lane] + part_o[1][lane] + part_o[2][lane] + part_o[3][lane];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int at = 16 * d + 4 * (lane >> 4);
+    if (at < pool.dim)
+        *(f32x4u*)(a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim + at) = o * inv;
+}
+
+hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items, hipStream_t st) {
+    const unsigned grid = items * (unsigned)a.pool.kv_heads;
+    auto go = [&](auto type, auto dp) {
+        constexpr int kType = decltype(type)::value, kDp = decltype(dp)::value;
+        if constexpr (kType != kKvI8 || kDp != 96) {
+            if (a.where)
+                attend_few_kernel<kType, kDp, 1, true><<<grid, 256, 0, st>>>(a, cut);
+            else if (cut.cols == 16)
+                attend_few_kernel<kType, kDp, 1, false><<<grid, 256, 0, st>>>(a, cut);
+            else if constexpr (kDp <= 128)
+                attend_few_kernel<kType, kDp, 2, false><<<grid, 256, 0, st>>>(a, cut);
+        }
+    };
+    using std::integral_constant;
+    auto sized = [&](auto type) {
+        switch (a.pool.dp) {
+            case 64: go(type, integral_constant<int, 64>{}); break;
+            case 96: go(type, integral_constant<int, 96>{}); break;
+            case 128: go(type, integral_constant<int, 128>{}); break;
+            default: go(type, integral_constant<int, 256>{});
+        }
+    };
+    switch (a.pool.type) {
+        case kKvF16: sized(integral_constant<int, kKvF16>{}); break;
+        case kKvBf16: sized(integral_constant<int, kKvBf16>{}); break;
+        default: sized(integral_constant<int, kKvI8>{});
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_attend_join(const AttendArgs& a, const Cut& cut, unsigned tiles, hipStream_t st) {
+    const dim3 grid(tiles * (unsigned)(cut.cols >> 4) * (unsigned)a.pool.kv_heads, (unsigned)(a.pool.dp >> 4));
+    attend_join_kernel<<<grid, 256, 0, st>>>(a, cut, a.pool.dp, a.where != nullptr);
+    return hipGetLastError();
+}
+
+}  // namespace ovfq

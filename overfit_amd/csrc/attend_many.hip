@@ -1,0 +1,250 @@
+// attend_many.hip — attention of many columns (prompts, chunks of them) over a paged cache. Arithmetic: attend.h.
+//
+// Bound: MFMA, 4 D flops per (column, token) times the parts that q and p are split in (two fp16, three bf16), beside the softmax's
+// vector work. Four waves of 16 kTiles16 columns each share a tile; a block's keys and values go to LDS once for all of them, by DMA in
+// the operand order that they have in memory (reads of it are 1 KiB in a row, free of conflicts), one block ahead. Workgroups of one
+// key head come to one XCD where the head count allows, so its blocks are read from HBM once.
+#include <type_traits>
+
+#include "attend.h"
+
+namespace ovfq {
+
+namespace {
+
+template <int kType, int kDp, int kCols>
+__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut cut) {
+    using Att = Attention<kType, kDp, kCols>;
+    using M = KvMath<kType>;
+    constexpr int kBytes = kv_bytes(kType, kDp), kPlane = kv_plane_bytes(kType, kDp);
+    __shared__ __attribute__((aligned(16))) char ring[2][kBytes];
+    const KvPool& pool = a.pool;
+    const KvBatch& b = a.batch;
+    const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15;
+    const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads), item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
+    TileWork w;
+    if (!cut_item(cut, pool, b, item, w)) return;
+    Att att;
+    const int wave_col = w.col0 + 16 * kCols * wave;
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = wave_col + 16 * t + col, i = c / cut.group;
+        const bool used = i < w.rows;
+        const int qh = head * cut.group + (c - i * cut.group);
+        const float* x = used ? a.q + ((size_t)(w.first_row + i) * a.heads + qh) * pool.dim : nullptr;
+        const int last = w.place + i;
+        att.column(t, x, pool.dim, a.scale * kLog2e, a.window ? max(last - a.window + 1, 0) : 0, last);
+    }
+    // what the wave's rows see
+    const int i0 = wave_col / cut.group, i1 = min(w.rows - 1, (wave_col + 16 * kCols - 1) / cut.group);
+    const bool live = i0 < w.rows;
+    const int first_last = w.place + i0, last_last = w.place + i1;
+    const int first_low = a.window ? max(first_last - a.window + 1, 0) : 0, last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+
+    BlockWalk walk;
+    const int blocks = max(w.block1 - w.block0, 0);
+    const int in_page = pool.page / kKvBlock - 1;
+    if (blocks) walk.start(pool, b.tables + (size_t)w.r * b.width, b.width, w.block0, 1);
+    auto stage = [&](int i, int page) {
+        const char* src = kv_block(pool, page, head, (w.block0 + i) & in_page);
+        char* dst = ring[i & 1];
+        constexpr int kPieces = 2 * kPlane / 1024;
+#pragma unroll
+        for (int k = 0; k < kPieces; k += 4)
+            if (kPieces % 4 == 0 || k + wave < kPieces)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (k + wave) * 1024 + lane * 16),
+                                                 (__attribute__((address_space(3))) void*)(dst + (k + wave) * 1024), 16, 0, 0);
+        if constexpr (kType == kKvI8) {
+            if (wave == 0)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + 2 * kPlane + lane * 4),
+                                                 (__attribute__((address_space(3))) void*)(dst + 2 * kPlane), 4, 0, 0);
+        }
+    };
+    int page = blocks ? walk.page(0) : -1;
+    if (page >= 0) stage(0, page);
+    for (int i = 0; i < blocks; i++) {
+        const int next = i + 1 < blocks ? walk.page(i + 1) : -1;
+        // this wave's share of block i has landed; behind the barrier all of it, and every wave is past the block before
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (next >= 0) stage(i + 1, next);
+        const int first = (w.block0 + i) * kKvBlock;
+        if (page >= 0 && live && first <= last_last && first + kKvBlock > first_low) {
+            const char* at = ring[i & 1] + lane * 16;
+            f32x4 ks[2] = {}, vs[2] = {};
+            if constexpr (kType == kKvI8) {
+                const char* s = ring[i & 1] + 2 * kPlane + (lane >> 4) * 16;
+                ks[0] = *(const f32x4*)s;
+                ks[1] = *(const f32x4*)(s + 64);
+                vs[0] = *(const f32x4*)(s + 128);
+                vs[1] = *(const f32x4*)(s + 192);
+            }
+            auto load = [&](int off) { return *(const u32x4*)(at + off); };
+            f32x4 s[kCols][2];
+            att.scores(s, [&](int tile, int chunk) { return key_operand<kType, kDp>(tile, chunk, load); });
+            const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
+            u32x4 p[kCols][M::kParts];
+            att.probabilities(s, p, masked, first, ks, vs);
+            att.products(p, masked, first, [&](int tile) { return value_operand<kType, kDp>(tile, load); });
+        }
+        page = next;
+    }
+    att.close();
+    if (w.pieces > 1) {
+        float* part = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(64 * kCols, kDp);
+#pragma unroll
+        for (int t = 0; t < kCols; t++) {
+            const int sub = wave * kCols + t;
+            if (lane < 16) {
+                part[32 * sub + lane] = att.ref[t];
+                part[32 * sub + 16 + lane] = att.l[t];
+            }
+#pragma unroll
+            for (int d = 0; d < Att::kTiles; d++)
+                *(f32x4*)(part + 32 * 4 * kCols + ((sub * Att::kTiles + d) * 64 + lane) * 4) = att.o[t][d];
+        }
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = wave_col + 16 * t + col, i = c / cut.group;
+        if (i >= w.rows) continue;
+        const float inv = att.l[t] == 0.0f ? 0.0f : 1.0f / att.l[t];
+        float* y = a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim;
+#pragma unroll
+        for (int d = 0; d < Att::kTiles; d++) {
+            const int at = 16 * d + 4 * (lane >> 4);
+            if (at < pool.dim) *(f32x4u*)(y + at) = att.o[t][d] * inv;
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items, hipStream_t st);
+hipError_t launch_attend_join(const AttendArgs& a, const Cut& cut, unsigned tiles, hipStream_t st);
+
+namespace {
+
+// Columns that the few-column kernel takes of a request, and those of a tile of the other one.
+int few_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 32 : 16; }
+int many_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 128 : 64; }
+
+struct Plan {
+    Cut cut;
+    bool run;
+    unsigned items, tiles;  // most of a key head
+};
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// The few-column launch: pieces for kFewItems workgroups over the key heads, none of fewer than eight blocks.
+constexpr int kFewItems = 1024, kManyItems = 512;
+
+Plan plan_few(const AttendArgs& a) {
+    const int group = a.heads / a.pool.kv_heads, few = few_columns(a);
+    const int most = a.batch.most;  // rows of a request
+    Plan p{};
+    p.run = group <= few && (a.batch.requests > 1 || most * (int64_t)group <= few);
+    const int cols = most * (int64_t)group <= 16 ? 16 : few;
+    p.cut = Cut{cols, 1, (int)(most * (int64_t)group < few ? most * group : few), ceil_div(kFewItems, a.pool.kv_heads), 8, true, a.window, group, 0};
+    const int tiles = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
+    p.tiles = (unsigned)tiles;
+    p.items = (unsigned)(tiles + p.cut.target + 1);
+    p.cut.slots = (int)p.items;
+    return p;
+}
+
+Plan plan_many(const AttendArgs& a) {
+    const int group = a.heads / a.pool.kv_heads, few = few_columns(a), cols = many_columns(a);
+    Plan p{};
+    p.run = group > few || a.batch.most * (int64_t)group > few;
+    const int least = group > few ? 1 : few + 1;
+    p.cut = Cut{cols, least, (int)(a.batch.most * (int64_t)group), ceil_div(kManyItems, a.pool.kv_heads), 16, false, a.window, group, 0};
+    const int requests = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
+    p.tiles = (unsigned)(a.batch.rows * (int64_t)group / cols + requests);
+    p.cut.split = a.batch.rows * (int64_t)group / cols * a.pool.kv_heads < kManyItems;
+    p.items = p.tiles + (p.cut.split ? p.cut.target + 1 : 0);
+    p.cut.slots = (int)p.items;
+    return p;
+}
+
+size_t part_bytes(const AttendArgs& a, const Plan& p) {
+    if (!p.run || !p.cut.split) return 0;
+    return ((size_t)p.items * a.pool.kv_heads * part_floats(p.cut.cols, a.pool.dp) * 4 + 255) & ~size_t(255);
+}
+
+}  // namespace
+
+size_t attend_scratch(const AttendArgs& a) { return part_bytes(a, plan_few(a)) + part_bytes(a, plan_many(a)); }
+
+hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
+    const Plan few = plan_few(a), many = plan_many(a);
+    hipError_t e = hipSuccess;
+    if (few.run) {
+        e = launch_attend_few(a, few.cut, few.items, st);
+        if (e == hipSuccess && few.cut.split) e = launch_attend_join(a, few.cut, few.tiles, st);
+    }
+    if (e != hipSuccess || !many.run) return e;
+    AttendArgs m = a;
+    m.parts = (float*)((char*)a.parts + part_bytes(a, few));
+    const unsigned grid = many.items * (unsigned)a.pool.kv_heads;
+    auto go = [&](auto type, auto dp) {
+        constexpr int kType = decltype(type)::value, kDp = decltype(dp)::value;
+        if constexpr (kType != kKvI8 || kDp != 96) attend_many_kernel<kType, kDp, kDp <= 128 ? 2 : 1><<<grid, 256, 0, st>>>(m, many.cut);
+    };
+    using std::integral_constant;
+    auto sized = [&](auto type) {
+        switch (a.pool.dp) {
+            case 64: go(type, integral_constant<int, 64>{}); break;
+            case 96: go(type, integral_constant<int, 96>{}); break;
+            case 128: go(type, integral_constant<int, 128>{}); break;
+            default: go(type, integral_constant<int, 256>{});
+        }
+    };
+    switch (a.pool.type) {
+        case kKvF16: sized(integral_constant<int, kKvF16>{}); break;
+        case kKvBf16: sized(integral_constant<int, kKvBf16>{}); break;
+        default: sized(integral_constant<int, kKvI8>{});
+    }
+    e = hipGetLastError();
+    if (e == hipSuccess && many.cut.split) e = launch_attend_join(m, many.cut, many.tiles, st);
+    return e;
+}
+
+// ------------------------------------------------------------------------------------------------- selected pages
+
+namespace {
+
+// A row's pages in pieces of so many blocks that all rows and key heads give about kFewItems workgroups (at least 16 blocks each).
+Plan plan_selected(const AttendArgs& a) {
+    const int group = a.heads / a.pool.kv_heads, tiles = (group + 15) / 16;
+    const int64_t blocks = (int64_t)a.top * (a.pool.page / kKvBlock), all = (int64_t)a.batch.rows * a.pool.kv_heads * tiles;
+    int64_t pieces = (kFewItems + all - 1) / all;
+    if (pieces > blocks / 16) pieces = blocks / 16;
+    if (pieces < 1) pieces = 1;
+    const int each = ceil_div(blocks, pieces);
+    Plan p{};
+    p.run = true;
+    p.cut = Cut{16, 1, 16, ceil_div(blocks, each), each, false, 0, group, 0};
+    p.cut.split = p.cut.target > 1;
+    p.tiles = (unsigned)(a.batch.rows * tiles);
+    p.items = p.tiles * (unsigned)p.cut.target;
+    return p;
+}
+
+}  // namespace
+
+hipError_t launch_select_pages(const AttendArgs& a, hipStream_t st);
+
+size_t attend_selected_scratch(const AttendArgs& a) { return part_bytes(a, plan_selected(a)); }
+
+hipError_t launch_attend_selected(const AttendArgs& a, hipStream_t st) {
+    const Plan p = plan_selected(a);
+    hipError_t e = launch_select_pages(a, st);
+    if (e == hipSuccess) e = launch_attend_few(a, p.cut, p.items, st);
+    if (e == hipSuccess && p.cut.split) e = launch_attend_join(a, p.cut, p.tiles, st);
+    return e;
+}
+
+}  // namespace ovfq

@@ -352,6 +352,65 @@ struct VerifyArgs {
 };
 hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st);
 
+// A paged cache of keys and values (kv_append.hip, attend.hip, attend_select.hip). Its unit is the block: kKvBlock consecutive tokens
+// of one key head, keys and values in MFMA operand order (kv_cache.h).
+constexpr int kKvBlock = 32;
+struct KvPool {
+    char* mem;     // [pages][kv_heads][page / kKvBlock] blocks
+    float* sums;   // [pages][kv_heads][dim]: each full page's sum of keys, or NULL
+    int type;      // 1 (fp16), 30 (bf16) or 24 (int8 with an fp32 scale for each token and head)
+    int kv_heads, dim, dp;  // dp: the channels that a block has room for
+    int page, pages;
+};
+int kv_padded_dim(int type, int dim);   // 64, 96 (not int8), 128 or 256
+size_t kv_block_bytes(int type, int dp);
+// The requests of one call: request r's new tokens are rows row_offsets[r] .. row_offsets[r + 1] - 1, the last of lengths[r] tokens,
+// whose page i is tables[r][i].
+struct KvBatch {
+    const int* row_offsets;  // [requests + 1]
+    const int* lengths;      // [requests]
+    const int* tables;       // [requests][width]
+    int requests, width, rows;
+    int most;  // no request has more rows than this
+};
+struct KvRope {
+    const float* freq;       // [rotary / 2]
+    const int* axes;         // [rotary / 2] or NULL
+    const int* positions;    // [n_axes][rows] or NULL
+    int rotary, n_axes;
+    bool halves;
+    float scale;
+};
+struct KvAppendArgs {
+    KvPool pool;
+    KvBatch batch;
+    KvRope rope;
+    const float *k, *v, *q;  // k NULL: queries only; q NULL: none
+    float* q_out;
+    int heads;
+};
+hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st);
+hipError_t launch_kv_clear(void* p, size_t bytes, hipStream_t st);  // zeroes whole 16-byte pieces
+
+struct AttendArgs {
+    KvPool pool;
+    KvBatch batch;
+    const float* q;  // [rows][heads][dim]
+    float* out;
+    int heads, window;  // window 0: none
+    float scale;
+    float* parts;  // scratch (attend_scratch): partial outputs of launches that split the keys
+    // selected pages only (launch_attend_selected)
+    int top;
+    int* chosen;  // [rows][kv_heads][top], the request's page numbers in rising order, then -1
+    int* where;   // scratch [rows]: the row's request, or -1
+    double* fits;  // scratch [rows][kv_heads][width]
+};
+size_t attend_scratch(const AttendArgs& a);
+hipError_t launch_attend(const AttendArgs& a, hipStream_t st);
+size_t attend_selected_scratch(const AttendArgs& a);  // for parts
+hipError_t launch_attend_selected(const AttendArgs& a, hipStream_t st);
+
 // GGUF Q8_0 (34-byte blocks) -> int8 quant plane + f32 scale plane.
 hipError_t launch_q8_0_deinterleave(const void* gguf, int64_t n_blocks, int8_t* q, float* s, hipStream_t st);
 // GGUF Q5_0 (22-byte blocks of 32) or Q5_K (176-byte super-blocks) -> resident Q8_0 planes: decoded and requantised
