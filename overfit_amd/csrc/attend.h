@@ -15,7 +15,10 @@
 // column.
 //
 // Masks: a hidden token's score is -inf whatever its key holds. A hidden token's value meets a probability of zero, which would still
-// make NaN of what is not finite, so blocks with a mask look at their values and, if some are not finite, add their tokens one by one.
+// make NaN of what is not finite, so blocks with a mask look at their values first: what is not finite is noted for the columns that see
+// it (their outputs become NaN in the end) and taken out of the operand. (Adding such tokens one by one in a path of its own doubled the
+// accumulators' registers: the prompt kernel's 256 were not enough, and a spilled register's reload waits for the next block's DMA as
+// well. 4100 rows of three prompts 243 us that way.)
 #pragma once
 
 #include "kv_cache.h"
@@ -29,6 +32,8 @@ typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
@@ -81,14 +86,27 @@ __device__ __forceinline__ u32x4 widened(uint32_t lo, uint32_t hi) {
     return r;
 }
 
-// Whether one of the eight values of an fp16 or bf16 operand is not finite.
+// Bits 15 and 31 of each word: which of an fp16 or bf16 operand's eight values are not finite.
 template <int kType>
-__device__ __forceinline__ uint32_t not_finite(u32x4 v) {
+__device__ __forceinline__ u32x4 not_finite(u32x4 v) {
     constexpr uint32_t kExp = kType == kKvBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kType == kKvBf16 ? 0x00800080u : 0x04000400u;
-    uint32_t any = 0;
+    u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) any |= (v[i] & kExp) + kOne;
-    return any & 0x80008000u;
+    for (int i = 0; i < 4; i++) r[i] = ((v[i] & kExp) + kOne) & 0x80008000u;
+    return r;
+}
+template <int kType>
+__device__ __forceinline__ bool any_not_finite(u32x4 v) {
+    const u32x4 b = not_finite<kType>(v);
+    return (b.x | b.y | b.z | b.w) != 0;
+}
+// The operand with zeros in their places.
+template <int kType>
+__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
+    const u32x4 b = not_finite<kType>(v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] &= ~((b[i] >> 15) * 0xffffu);
+    return v;
 }
 
 // kCols 16-column tiles of queries against a request's blocks, one wave.
@@ -102,6 +120,7 @@ struct Attention {
     f32x4 o[kCols][kTiles];
     float ref[kCols], l[kCols];  // l: of this lane's tokens
     float ev[kCols];             // int8: the power of two that value scales are divided by, 0 at first
+    uint32_t bad[kCols][2];      // bit 4 d + i: the column sees a value that is not finite in o[][d][i]'s channel (of masked blocks)
 
     // Column `col` of the tile has query row x (NULL: none) and sees the tokens [first, last].
     __device__ __forceinline__ void column(int t, const float* x, int dim, float scale, int first, int last) {
@@ -142,6 +161,7 @@ struct Attention {
         ref[t] = -kInf;
         l[t] = 0.0f;
         ev[t] = 0.0f;
+        bad[t][0] = bad[t][1] = 0;
 #pragma unroll
         for (int d = 0; d < kTiles; d++) o[t][d] = f32x4{0, 0, 0, 0};
     }
@@ -171,26 +191,40 @@ struct Attention {
         float top[kCols], vtop[kCols];
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    s[t][h][i] *= qs[t];
+                    if constexpr (kType == kKvI8) s[t][h][i] *= ks[h][i];
+                }
+        }
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < kCols; t++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = mine + 16 * h + i;
+                        s[t][h][i] = (int)(j <= lim[t]) & (int)(j >= low[t]) ? s[t][h][i] : -kInf;
+                    }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kCols; t++) {
             top[t] = -kInf;
             vtop[t] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float x = s[t][h][i] * qs[t];
-                    if constexpr (kType == kKvI8) x *= ks[h][i];
-                    bool seen = true;
-                    if (masked) {
-                        const int j = mine + 16 * h + i;
-                        seen = j <= lim[t] && j >= low[t];
-                        x = seen ? x : -kInf;
-                    }
-                    s[t][h][i] = x;
-                    top[t] = fmaxf(top[t], x);
-                    if constexpr (kType == kKvI8) vtop[t] = fmaxf(vtop[t], seen ? vs[h][i] : 0.0f);
+                    top[t] = fmaxf(top[t], s[t][h][i]);
+                    // (a hidden token's scale counts for nothing)
+                    if constexpr (kType == kKvI8) vtop[t] = fmaxf(vtop[t], masked && s[t][h][i] == -kInf ? 0.0f : vs[h][i]);
                 }
-            move = move || top[t] > ref[t] + kTop + kRoom;
-            if constexpr (kType == kKvI8) move = move || vtop[t] > ev[t];
+            move = move | (top[t] > ref[t] + kTop + kRoom);
+            if constexpr (kType == kKvI8) move = move | (vtop[t] > ev[t]);
         }
         if (__ballot(move)) {
 #pragma unroll
@@ -230,12 +264,8 @@ struct Attention {
                     l[t] += v;
                     x[4 * h + i] = v;
                     if constexpr (kType == kKvI8) {
-                        float w = v * (vs[h][i] * down);
-                        if (masked) {
-                            const int j = mine + 16 * h + i;
-                            w = j <= lim[t] && j >= low[t] ? w : 0.0f;
-                        }
-                        x[4 * h + i] = w;
+                        const float w = v * (vs[h][i] * down);
+                        x[4 * h + i] = masked && s[t][h][i] == -kInf ? 0.0f : w;
                     }
                 }
             M::split(x, p[t]);
@@ -244,18 +274,7 @@ struct Attention {
 
     // o += p times the block's values; value(tile): the operand of 16 channels.
     template <class Value>
-    __device__ __forceinline__ void products(const u32x4 (&p)[kCols][M::kParts], bool masked, int first, Value value) {
-        if constexpr (kType != kKvI8) {
-            if (masked) {
-                uint32_t bad = 0;
-#pragma unroll
-                for (int d = 0; d < kTiles; d++) bad |= not_finite<kType>(value(d));
-                if (__ballot(bad != 0)) {
-                    one_by_one(p, first, value);
-                    return;
-                }
-            }
-        }
+    __device__ __forceinline__ void products(const u32x4 (&p)[kCols][M::kParts], Value value) {
 #pragma unroll
         for (int d = 0; d < kTiles; d += 2) {
             const u32x4 a = value(d), b = value(d + 1);
@@ -269,32 +288,35 @@ struct Attention {
         }
     }
 
-    // The same, each token's product by itself and left out where the column does not see it.
-    template <class Value>
-    __device__ __forceinline__ void one_by_one(const u32x4 (&p)[kCols][M::kParts], int first, Value value) {
-        const int g = (threadIdx.x >> 4) & 3;
-        for (int j = 0; j < kKvBlock; j++) {
-            const int slot = ((j >> 4) << 2) + (j & 3);
-            const uint32_t half = g == ((j >> 2) & 3) ? 0xffffu << (16 * (slot & 1)) : 0u;
+    // Notes which columns see values that are not finite: ones in their places times ones for the tokens seen.
+    template <int kUnrollNotes, class Value>
+    __device__ __forceinline__ void note_bad(int first, Value value) {
+        constexpr uint32_t kOne = kType == kKvBf16 ? 0x3f80u : 0x3c00u;
+        const int mine = first + ((threadIdx.x >> 4) & 3) * 4;
 #pragma unroll
-            for (int d = 0; d < kTiles; d++) {
-                u32x4 a = value(d);
+        for (int t = 0; t < kCols; t++) {
+            u32x4 seen = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; i++) a[i] &= i == (slot >> 1) ? half : 0u;
-#pragma unroll
-                for (int t = 0; t < kCols; t++) {
-                    f32x4 s = {0, 0, 0, 0};
-#pragma unroll
-                    for (int k = 0; k < M::kParts; k++) s = M::mfma(a, p[t][k], s);
-                    const bool seen = first + j <= lim[t] && first + j >= low[t];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[t][d][i] += seen ? s[i] : 0.0f;
-                }
+            for (int i = 0; i < 8; i++) {
+                const int j = mine + (i >> 2) * 16 + (i & 3);
+                seen[i >> 1] |= j <= lim[t] && j >= low[t] ? kOne << (16 * (i & 1)) : 0u;
             }
+            uint64_t found = 0;
+#pragma unroll kUnrollNotes
+            for (int d = 0; d < kTiles; d++) {
+                u32x4 a = not_finite<kType>(value(d));
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = (a[i] >> 15) * kOne;
+                const f32x4 n = M::mfma(a, seen, f32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int i = 0; i < 4; i++) found |= (uint64_t)(n[i] > 0.0f) << (4 * d + i);
+            }
+            bad[t][0] |= (uint32_t)found;
+            bad[t][1] |= (uint32_t)(found >> 32);
         }
     }
 
-    // After the last block: l over the column's lanes, int8's power of two back into o.
+    // After the last block: l over the column's lanes, int8's power of two back into o, NaN where bad values were noted.
     __device__ __forceinline__ void close() {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
@@ -303,6 +325,11 @@ struct Attention {
             if constexpr (kType == kKvI8) {
 #pragma unroll
                 for (int d = 0; d < kTiles; d++) o[t][d] *= ev[t];
+            } else if (__ballot((bad[t][0] | bad[t][1]) != 0)) {
+#pragma unroll
+                for (int d = 0; d < kTiles; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t][d][i] = bad[t][d >> 3] >> ((4 * d + i) & 31) & 1 ? __builtin_nanf("") : o[t][d][i];
             }
         }
     }
@@ -372,22 +399,24 @@ __device__ __forceinline__ int cut_piece(const Cut& c, const KvPool& pool, const
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
-    return max((int)fminf(ceilf(all / (float)c.target), 1.0e9f), c.least_blocks);
+    return uniform(max((int)fminf(ceilf(all / (float)c.target), 1.0e9f), c.least_blocks));
 }
 __device__ __forceinline__ int cut_pieces(int blocks, int piece) { return blocks > piece ? (blocks + piece - 1) / piece : 1; }
 
 // A request's tile and its piece, or false where it has no such piece.
 __device__ __forceinline__ bool cut_tile(const Cut& c, const KvPool& pool, const KvBatch& b, int piece, int r, int tile, int j,
                                          int before, TileWork& w) {
-    const KvRows m = kv_rows(b, r);
+    KvRows m = kv_rows(b, r);
+    m.first = uniform(m.first);
+    m.n = uniform(m.n);
     w.r = r;
     w.tile = tile;
     w.piece = j;
     w.first_row = m.first;
     w.rows = m.n;
-    w.place = kv_length(b, r) - m.n;
+    w.place = uniform(kv_length(b, r)) - m.n;
     w.col0 = tile * c.cols;
-    w.pieces_of_request = cut_pieces(cut_request_blocks(c, pool, b, r, m.n), piece);
+    w.pieces_of_request = uniform(cut_pieces(cut_request_blocks(c, pool, b, r, m.n), piece));
     w.slot = before + tile * w.pieces_of_request + j;
     const int2 s = cut_blocks(c, pool, b, w.place, w.col0 / c.group, min(m.n - 1, (w.col0 + c.cols - 1) / c.group));
     w.pieces = cut_pieces(s.y - s.x, piece);
@@ -404,7 +433,7 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
         return tiles ? tiles * cut_pieces(cut_request_blocks(c, pool, b, q, n), piece) : 0;
     });
     if (!any) return false;
-    const int n = kv_rows(b, r).n, each = cut_pieces(cut_request_blocks(c, pool, b, r, n), piece);
+    const int n = uniform(kv_rows(b, r).n), each = uniform(cut_pieces(cut_request_blocks(c, pool, b, r, n), piece));
     return cut_tile(c, pool, b, piece, r, cut_tiles(c, n) - 1 - item / each, item % each, before, w);
 }
 

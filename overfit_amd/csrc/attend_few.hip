@@ -143,9 +143,22 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
             if (page >= 0) {
                 u32x4 p[kCols][M::kParts];
                 att.probabilities(s, p, masked, first, ks_now, vs_now);
-                att.products(p, masked, first, [&](int tile) {
+                auto value = [&](int tile) {
                     return value_operand<kType, kDp>(tile, [&](int at) { return values[(at - kv_plane_bytes(kType, kDp)) >> 10]; });
-                });
+                };
+                if constexpr (kType != kKvI8) {
+                    if (masked) {
+                        bool any = false;
+#pragma unroll
+                        for (int k = 0; k < kLoads; k++) any = any | any_not_finite<kType>(values[k]);
+                        if (__ballot(any)) {
+                            att.template note_bad<Att::kTiles>(first, value);
+#pragma unroll
+                            for (int k = 0; k < kLoads; k++) values[k] = finite_part<kType>(values[k]);
+                        }
+                    }
+                }
+                att.products(p, value);
             }
             if (i + 1 < mine) load_values(next);
             page = next_page;

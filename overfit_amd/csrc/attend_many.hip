@@ -40,6 +40,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     const bool live = i0 < w.rows;
     const int first_last = w.place + i0, last_last = w.place + i1;
     const int first_low = a.window ? max(first_last - a.window + 1, 0) : 0, last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+    // and the least that a column of the tile sees
+    const int tile_last = w.place + w.col0 / cut.group;
+    const int tile_low = a.window ? max(w.place + min(w.rows - 1, (w.col0 + 64 * kCols - 1) / cut.group) - a.window + 1, 0) : 0;
 
     BlockWalk walk;
     const int blocks = max(w.block1 - w.block0, 0);
@@ -69,6 +72,19 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
         __syncthreads();
         if (next >= 0) stage(i + 1, next);
         const int first = (w.block0 + i) * kKvBlock;
+        if constexpr (kType != kKvI8) {
+            if (page >= 0 && (first + kKvBlock - 1 > tile_last || first < tile_low)) {  // masked for one of the tile's columns
+                char* values = ring[i & 1] + kPlane;
+                bool any = false;
+                for (int k = threadIdx.x * 16; k < kPlane; k += 4096) any = any | any_not_finite<kType>(*(const u32x4*)(values + k));
+                if (__syncthreads_or(any)) {
+                    att.template note_bad<1>(first, [&](int tile) { return *(const u32x4*)(values + tile * 1024 + lane * 16); });
+                    __syncthreads();
+                    for (int k = threadIdx.x * 16; k < kPlane; k += 4096) *(u32x4*)(values + k) = finite_part<kType>(*(const u32x4*)(values + k));
+                    __syncthreads();
+                }
+            }
+        }
         if (page >= 0 && live && first <= last_last && first + kKvBlock > first_low) {
             const char* at = ring[i & 1] + lane * 16;
             f32x4 ks[2] = {}, vs[2] = {};
@@ -85,7 +101,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
             const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
             u32x4 p[kCols][M::kParts];
             att.probabilities(s, p, masked, first, ks, vs);
-            att.products(p, masked, first, [&](int tile) { return value_operand<kType, kDp>(tile, load); });
+            att.products(p, [&](int tile) { return value_operand<kType, kDp>(tile, load); });
         }
         page = next;
     }

@@ -65,7 +65,7 @@ __device__ __forceinline__ bool kv_find(int requests, int& item, int& r, int& be
         const int all = __builtin_amdgcn_readlane(upto, 63);
         if (item < before + all) {
             const int l = __ffsll((unsigned long long)__ballot(before + upto > item)) - 1;
-            r = base + l;
+            r = __builtin_amdgcn_readfirstlane(base + l);
             before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
             item -= before;
             return true;
