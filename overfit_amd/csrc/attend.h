@@ -356,85 +356,167 @@ __device__ __forceinline__ u32x4 value_operand(int tile, Load load) {
     }
 }
 
-// How a launch cuts its work: tiles of `cols` columns, each tile's blocks in pieces of so many that all tiles of one key head give
-// about `target` pieces (whole tiles where !split). Which requests: those of `least` to `most` columns.
+// How a launch cuts its work. A request of `least` to `most` columns has tiles of `cols` columns (2^cols_log2), and a tile's blocks are
+// cut into pieces so that a key head has about `target` of them, none of fewer blocks than least_blocks. Where the tiles alone are that
+// many, pieces are half as long again, and where no tile is longer than that, the tiles go by the place of their last column, the
+// last ones (with the longest spans) first: 4100 rows of three prompts TODO us in the order of the requests.
 struct Cut {
-    int cols, least, most, target, least_blocks;
-    bool split;
+    int cols_log2, least, most, target, least_blocks;
     int window, group;
-    int slots;  // of a key head's partial outputs (offsets that overlap could ask for more: those pieces are left out)
+    int slots, tiles;  // of a key head's partial outputs and plans (offsets that overlap could ask for more: that is left out)
 };
-struct TileWork {
-    int r, tile, piece, slot;  // slot: the piece's place among the head's partial outputs
-    int first_row, rows;       // the request's
-    int place;                 // of its first new token
-    int col0;                  // the tile's first column
-    int block0, block1;        // the piece's blocks
-    int pieces;                // of the tile
-    int pieces_of_request;     // slots that each of its tiles has
+// What the join needs to know of a tile, written by the tile's first piece.
+struct TilePlan {
+    int first_row, rows, col0;
+    int pieces, slot;  // slot: the first piece's place among the head's partial outputs
+};
+struct TileWork : TilePlan {
+    int r, tile, piece;
+    int tile_index;      // among all requests' tiles
+    int place;           // of the request's first new token
+    int block0, block1;  // the piece's blocks
 };
 
-__device__ __forceinline__ int cut_tiles(const Cut& c, int n) {
-    const int cols = n * c.group;
-    return n && cols >= c.least && cols <= c.most ? (cols + c.cols - 1) / c.cols : 0;
-}
-// Blocks that the rows i0 .. i1 of a request see: [x, y).
+// A lane's request.
+struct CutRequest {
+    int first, n, place, tiles, blocks;  // blocks: of its longest tile, at most
+    float sum;                           // of its tiles' blocks, about
+};
+__device__ __forceinline__ int cut_pieces(int blocks, int piece) { return blocks > piece ? (blocks + piece - 1) / piece : 1; }
+// Blocks that the tokens place + i0 .. place + i1 see: [x, y).
 __device__ __forceinline__ int2 cut_blocks(const Cut& c, const KvPool& pool, const KvBatch& b, int place, int i0, int i1) {
     const int64_t last = min((int64_t)place + i1, (int64_t)b.width * pool.page - 1);
     const int64_t first = c.window ? max((int64_t)place + i0 - c.window + 1, (int64_t)0) : 0;
     const int x = (int)(first / kKvBlock);
     return make_int2(x, last < first ? x : (int)(last / kKvBlock) + 1);
 }
-__device__ __forceinline__ int cut_request_blocks(const Cut& c, const KvPool& pool, const KvBatch& b, int r, int n) {
-    const int2 s = cut_blocks(c, pool, b, kv_length(b, r) - n, 0, n - 1);
-    return s.y - s.x;
+__device__ __forceinline__ CutRequest cut_load(const Cut& c, const KvPool& pool, const KvBatch& b, int r) {
+    CutRequest q{0, 0, 0, 0, 0, 0.0f};
+    if (r >= b.requests) return q;
+    const KvRows m = kv_rows(b, r);
+    const int len = kv_length(b, r), cols = m.n * c.group;
+    if (!m.n || cols < c.least || cols > c.most) return q;
+    q.first = m.first;
+    q.n = m.n;
+    q.place = len - m.n;
+    q.tiles = ((cols - 1) >> c.cols_log2) + 1;
+    const int2 s = cut_blocks(c, pool, b, q.place, 0, m.n - 1);
+    const int all = s.y - s.x, rows = min((1 << c.cols_log2) / c.group + 2, m.n);  // a tile's rows, at most
+    q.blocks = c.window ? min(all, (int)(((int64_t)c.window + rows) / kKvBlock) + 2) : all;
+    const int2 f = cut_blocks(c, pool, b, q.place, 0, min(rows, m.n) - 1);
+    q.sum = (float)q.tiles * (c.window ? (float)q.blocks : 0.5f * (float)(q.blocks + f.y - f.x));
+    return q;
 }
-// Blocks a piece.
-__device__ __forceinline__ int cut_piece(const Cut& c, const KvPool& pool, const KvBatch& b) {
-    if (!c.split) return 0x7fffffff;
-    float all = 0.0f;
-    for (int r = threadIdx.x & 63; r < b.requests; r += 64) {
-        const int n = kv_rows(b, r).n, tiles = cut_tiles(c, n);
-        if (tiles) all += (float)tiles * (float)cut_request_blocks(c, pool, b, r, n);
+
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    return uniform(v);
+}
+
+// Item `item` of a key head; false past the last one. Every wave finds it for itself: lanes hold 64 requests at a time.
+__device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, int item, TileWork& w) {
+    const int lane = threadIdx.x & 63;
+    CutRequest q = cut_load(c, pool, b, lane);
+    float sum = q.sum;
+    int tiles = q.tiles, longest = q.blocks;
+    for (int base = 64; base < b.requests; base += 64) {
+        const CutRequest o = cut_load(c, pool, b, base + lane);
+        sum += o.sum;
+        tiles += o.tiles;
+        longest = max(longest, o.blocks);
     }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
-    return uniform(max((int)fminf(ceilf(all / (float)c.target), 1.0e9f), c.least_blocks));
-}
-__device__ __forceinline__ int cut_pieces(int blocks, int piece) { return blocks > piece ? (blocks + piece - 1) / piece : 1; }
-
-// A request's tile and its piece, or false where it has no such piece.
-__device__ __forceinline__ bool cut_tile(const Cut& c, const KvPool& pool, const KvBatch& b, int piece, int r, int tile, int j,
-                                         int before, TileWork& w) {
-    KvRows m = kv_rows(b, r);
-    m.first = uniform(m.first);
-    m.n = uniform(m.n);
-    w.r = r;
-    w.tile = tile;
-    w.piece = j;
-    w.first_row = m.first;
-    w.rows = m.n;
-    w.place = uniform(kv_length(b, r)) - m.n;
-    w.col0 = tile * c.cols;
-    w.pieces_of_request = uniform(cut_pieces(cut_request_blocks(c, pool, b, r, m.n), piece));
-    w.slot = before + tile * w.pieces_of_request + j;
-    const int2 s = cut_blocks(c, pool, b, w.place, w.col0 / c.group, min(m.n - 1, (w.col0 + c.cols - 1) / c.group));
-    w.pieces = cut_pieces(s.y - s.x, piece);
-    w.block0 = s.x + j * min(piece, s.y - s.x);
+    for (int off = 32; off >= 1; off >>= 1) {
+        sum += __shfl_xor(sum, off, 64);
+        tiles += __shfl_xor(tiles, off, 64);
+        longest = max(longest, __shfl_xor(longest, off, 64));
+    }
+    tiles = uniform(tiles);
+    const float each = sum / (float)c.target * (tiles >= c.target ? 1.5f : 1.0f);
+    const int piece = uniform(max((int)fminf(ceilf(each), 1.0e9f), c.least_blocks));
+    int l = 0, before = 0, tiles_before = 0;
+    w.piece = 0;
+    w.r = 0;
+    if (b.requests <= 64 && uniform(longest) <= piece) {
+        if (item >= tiles) return false;
+        // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
+        const int base = (int)min(max(((int64_t)q.place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
+        int lo = -1, hi = q.tiles ? base + q.tiles : 0;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) hi = max(hi, __shfl_xor(hi, off, 64));
+        hi = uniform(hi);  // none past hi; more than `item` past lo
+        int past = 0;
+        while (hi - lo > 1) {
+            const int x = lo + (hi - lo) / 2;
+            const int n = wave_sum(min(max(base + q.tiles - 1 - x, 0), q.tiles));
+            if (n <= item) {
+                hi = x;
+                past = n;
+            } else {
+                lo = x;
+            }
+        }
+        const int at = hi - base;  // the tile that ends there
+        uint64_t votes = __ballot(at >= 0 && at < q.tiles);
+        for (int i = past; i < item; i++) votes &= votes - 1;
+        l = __ffsll((unsigned long long)votes) - 1;
+        w.r = l;
+        w.tile = __builtin_amdgcn_readlane(at, l);
+        w.slot = 0;
+        w.tile_index = item;
+    } else {
+        for (int base = 0;; base += 64) {
+            if (base >= b.requests) return false;
+            if (base) q = cut_load(c, pool, b, base + lane);
+            const int mine = q.tiles * cut_pieces(q.blocks, piece);
+            int upto = mine, tiles_upto = q.tiles;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int v = __shfl_up(upto, off, 64), t = __shfl_up(tiles_upto, off, 64);
+                if (lane >= off) {
+                    upto += v;
+                    tiles_upto += t;
+                }
+            }
+            const int all = __builtin_amdgcn_readlane(upto, 63);
+            if (item >= before + all) {
+                before += all;
+                tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
+                continue;
+            }
+            l = __ffsll((unsigned long long)__ballot(before + upto > item)) - 1;
+            w.r = base + l;
+            before += __builtin_amdgcn_readlane(upto - mine, l);
+            tiles_before += __builtin_amdgcn_readlane(tiles_upto - q.tiles, l);
+            break;
+        }
+        const int pieces = cut_pieces(__builtin_amdgcn_readlane(q.blocks, l), piece);
+        const int nth = uniform((item - before) / pieces);
+        w.piece = item - before - nth * pieces;
+        w.tile = __builtin_amdgcn_readlane(q.tiles, l) - 1 - nth;
+        w.slot = before + nth * pieces;
+        w.tile_index = tiles_before + nth;
+    }
+    w.first_row = __builtin_amdgcn_readlane(q.first, l);
+    w.rows = __builtin_amdgcn_readlane(q.n, l);
+    w.place = __builtin_amdgcn_readlane(q.place, l);
+    w.col0 = w.tile << c.cols_log2;
+    const int2 s = cut_blocks(c, pool, b, w.place, uniform(w.col0 / c.group), uniform(min(w.rows - 1, (w.col0 + (1 << c.cols_log2) - 1) / c.group)));
+    w.pieces = uniform(cut_pieces(s.y - s.x, piece));
+    w.block0 = s.x + w.piece * min(piece, s.y - s.x);
     w.block1 = s.y - w.block0 > piece ? w.block0 + piece : s.y;
-    return j < w.pieces && (w.pieces == 1 || w.slot - j + w.pieces <= c.slots);
+    if ((w.slot + w.pieces > c.slots && w.pieces > 1) || w.tile_index >= c.tiles) return false;
+    return w.piece < w.pieces;
 }
-// Item `item` of a key head: the pieces of its requests' tiles, the last tiles (with the longest spans) first.
-__device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, int item, TileWork& w) {
-    const int piece = cut_piece(c, pool, b);
-    int r = 0, before = 0;
-    const bool any = kv_find(b.requests, item, r, before, [&](int q) {
-        const int n = kv_rows(b, q).n, tiles = cut_tiles(c, n);
-        return tiles ? tiles * cut_pieces(cut_request_blocks(c, pool, b, q, n), piece) : 0;
-    });
-    if (!any) return false;
-    const int n = uniform(kv_rows(b, r).n), each = uniform(cut_pieces(cut_request_blocks(c, pool, b, r, n), piece));
-    return cut_tile(c, pool, b, piece, r, cut_tiles(c, n) - 1 - item / each, item % each, before, w);
+// All tiles of a launch's requests.
+__device__ __forceinline__ int cut_count(const Cut& c, const KvBatch& b) {
+    int tiles = 0;
+    for (int r = threadIdx.x & 63; r < b.requests; r += 64) {
+        const int cols = kv_rows(b, r).n * c.group;
+        if (cols && cols >= c.least && cols <= c.most) tiles += ((cols - 1) >> c.cols_log2) + 1;
+    }
+    return wave_sum(tiles);
 }
 
 // A walk over blocks first, first + step, ..: their pages in 64 lanes at a time.

@@ -43,7 +43,8 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
         w.tile = (item - row * per) / cut.target;
         w.piece = (item - row * per) % cut.target;
         w.col0 = 16 * w.tile;
-        w.slot = item;
+        w.slot = item - w.piece;
+        w.tile_index = item / cut.target;
         pages = a.chosen + ((size_t)row * pool.kv_heads + head) * a.top;
         for (int i = 0; i < a.top; i += 64) whole += __popcll(__ballot(i + lane < a.top && pages[min(i + lane, a.top - 1)] >= 0));
         const int blocks = whole << shift, each = cut.least_blocks;
@@ -54,6 +55,7 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
     } else {
         if (!cut_item(cut, pool, b, item, w)) return;
     }
+    if (a.plans && threadIdx.x == 0 && w.piece == 0 && head == 0) a.plans[w.tile_index] = w;
     Att att;
 #pragma unroll
     for (int t = 0; t < kCols; t++) {
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
     }
     if (wave) return;
     if (w.pieces > 1) {
-        float* part = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(16 * kCols, kDp);
+        float* part = a.parts + ((size_t)(w.slot + w.piece) * pool.kv_heads + head) * (size_t)part_floats(16 * kCols, kDp);
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             if (lane < 16) {
@@ -236,86 +238,78 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
 
 }  // namespace
 
-// Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l. A workgroup per tile's 16 columns, key head and four
-// 16-channel tiles (blockIdx.y); four waves share the pieces, in a fixed order.
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, bool selected) {
+// Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l, in a fixed order. A workgroup per 16 columns of a tile,
+// key head and 16 channels * `wide` (blockIdx.y): a thread has a column that is used and four channels, and what is left of the
+// workgroup's threads shares the pieces.
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, int wide) {
     __shared__ float tops[16][16], ls[16][16];
-    __shared__ f32x4 part_o[4][64];
+    __shared__ f32x4 part_o[256];
     const KvPool& pool = a.pool;
-    const KvBatch& b = a.batch;
-    const int subs = cut.cols >> 4, lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15;
+    const int subs = 1 << (cut.cols_log2 - 4), cols = 16 * subs, tid = threadIdx.x;
     const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads);
-    int item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
-    const int sub = item % subs;
-    item /= subs;
-    TileWork w;
-    if (selected) {
-        const int tiles = (cut.group + 15) >> 4, row = item / tiles;
-        const int r = a.where[row];
-        if (r < 0) return;
-        const int* pages = a.chosen + ((size_t)row * pool.kv_heads + head) * a.top;
-        int whole = 0;
-        for (int i = 0; i < a.top; i += 64) whole += __popcll(__ballot(i + lane < a.top && pages[min(i + lane, a.top - 1)] >= 0));
-        w.first_row = row;
-        w.rows = 1;
-        w.col0 = 16 * (item - row * tiles);
-        w.slot = item * cut.target;
-        w.pieces = cut_pieces(whole * (pool.page / kKvBlock), cut.least_blocks);
-    } else {
-        int r = 0, tiles_before = 0;
-        const int piece = cut_piece(cut, pool, b);
-        int tile = item;
-        if (!kv_find(b.requests, tile, r, tiles_before, [&](int q) { return cut_tiles(cut, kv_rows(b, q).n); })) return;
-        // the pieces of the requests before it
-        int before = 0;
-        for (int q = lane; q < r; q += 64) {
-            const int n = kv_rows(b, q).n, tiles = cut_tiles(cut, n);
-            before += tiles ? tiles * cut_pieces(cut_request_blocks(cut, pool, b, q, n), piece) : 0;
+    const int item = (int)(blockIdx.x / (unsigned)pool.kv_heads), index = item / subs, sub = item - index * subs;
+    if (index >= (a.where ? a.batch.rows * ((cut.group + 15) >> 4) : cut_count(cut, a.batch))) return;
+    if (a.where && a.where[index / ((cut.group + 15) >> 4)] < 0) return;
+    const TilePlan w = a.plans[index];
+    // (a plan that nothing wrote, for offsets that overlap, must not lead out of the planes)
+    if (w.pieces <= 1 || w.slot < 0 || w.slot > cut.slots - w.pieces || w.first_row < 0 || w.rows <= 0 ||
+        w.rows > a.batch.rows - w.first_row || w.col0 < 0 || w.col0 >= w.rows * cut.group)
+        return;
+    const int first = w.col0 + 16 * sub, used = min(16, w.rows * cut.group - first);
+    if (used <= 0) return;
+    const size_t stride = (size_t)part_floats(cols, dp) * pool.kv_heads;
+    const float* base = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(cols, dp);
+    const float* ml = base + 32 * sub;
+    {  // the columns' tops and sums: 16 threads a column
+        const int col = tid & 15, share = tid >> 4;
+        float top = -kInf;
+        for (int j = share; j < w.pieces; j += 16) top = fmaxf(top, ml[j * stride + col]);
+        tops[share][col] = top;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 16; k++) top = fmaxf(top, tops[k][col]);
+        const float m = top == -kInf ? 0.0f : top;
+        float l = 0.0f;
+        for (int j = share; j < w.pieces; j += 16) l += ml[j * stride + 16 + col] * __builtin_amdgcn_exp2f(ml[j * stride + col] - m);
+        ls[share][col] = l;
+        __syncthreads();
+        if (share == 0) {
+            tops[0][col] = m;
+            l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; k++) l += ls[k][col];
+            ls[0][col] = l;
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
-        if (!cut_tile(cut, pool, b, piece, r, tile, 0, before, w)) return;
+        __syncthreads();
     }
-    if (w.pieces <= 1) return;
-    const int c = w.col0 + 16 * sub + col, i = c / cut.group;
-    const bool used = i < w.rows;
-    if (!__ballot(used)) return;
-    const size_t stride = (size_t)part_floats(cut.cols, dp) * pool.kv_heads;
-    const float* base = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(cut.cols, dp);
-    const float* ml = base + 32 * sub + col;
-    // the column's top and sum: 16 threads a column
-    const int share = wave * 4 + (lane >> 4);
-    float top = -kInf;
-    for (int j = share; j < w.pieces; j += 16) top = fmaxf(top, ml[j * stride]);
-    tops[share][col] = top;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++) top = fmaxf(top, tops[k][col]);
-    const float m = top == -kInf ? 0.0f : top;
-    float l = 0.0f;
-    for (int j = share; j < w.pieces; j += 16) l += ml[j * stride + 16] * __builtin_amdgcn_exp2f(ml[j * stride] - m);
-    ls[share][col] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 16; k++) l += ls[k][col];
-    const int tiles = dp >> 4, d = blockIdx.y;
-    f32x4 o = {0, 0, 0, 0};
-    const float* mine = base + 32 * subs + ((sub * tiles + d) * 64 + lane) * 4;
+    const int tiles = dp >> 4, d0 = (int)blockIdx.y * wide, quads = min(wide, tiles - d0) * 4;
+    const int units = used * quads, shares = units >= 256 ? 1 : 256 / units;
+    for (int u0 = 0; u0 < units; u0 += 256) {
+        const int share = shares == 1 ? 0 : tid / units, u = shares == 1 ? u0 + tid : tid - share * units;
+        const bool live = u < units && share < shares;
+        const int col = live ? u % used : 0, quad = live ? u / used : 0, d = d0 + (quad >> 2), g = quad & 3;
+        f32x4 o = {0, 0, 0, 0};
+        if (live) {
+            const float m = tops[0][col];
+            const float* mine = base + 32 * subs + ((sub * tiles + d) * 64 + g * 16 + col) * 4;
 #pragma unroll 4
-    for (int j = wave; j < w.pieces; j += 4) {
-        const float f = __builtin_amdgcn_exp2f(ml[j * stride] - m);
-        const f32x4 v = used ? *(const f32x4*)(mine + j * stride) : f32x4{0, 0, 0, 0};
-        o += v * f;
+            for (int j = share; j < w.pieces; j += shares) {
+                const float f = __builtin_amdgcn_exp2f(ml[j * stride + col] - m);
+                o += *(const f32x4*)(mine + j * stride) * f;
+            }
+        }
+        if (shares > 1) {
+            part_o[tid] = o;
+            __syncthreads();
+            if (share == 0)
+                for (int k = 1; k < shares; k++) o += part_o[tid + k * units];
+        }
+        if (!live || share) continue;
+        const int c = first + col, i = c / cut.group, at = 16 * d + 4 * g;
+        const float l = ls[0][col], inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (at < pool.dim)
+            *(f32x4u*)(a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim + at) = o * inv;
     }
-    part_o[wave][lane] = o;
-    __syncthreads();
-    if (wave || !used) return;
-    o = part_o[0][lane] + part_o[1][lane] + part_o[2][lane] + part_o[3][lane];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int at = 16 * d + 4 * (lane >> 4);
-    if (at < pool.dim)
-        *(f32x4u*)(a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim + at) = o * inv;
 }
 
 hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items, hipStream_t st) {
@@ -325,7 +319,7 @@ hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items
         if constexpr (kType != kKvI8 || kDp != 96) {
             if (a.where)
                 attend_few_kernel<kType, kDp, 1, true><<<grid, 256, 0, st>>>(a, cut);
-            else if (cut.cols == 16)
+            else if (cut.cols_log2 == 4)
                 attend_few_kernel<kType, kDp, 1, false><<<grid, 256, 0, st>>>(a, cut);
             else if constexpr (kDp <= 128)
                 attend_few_kernel<kType, kDp, 2, false><<<grid, 256, 0, st>>>(a, cut);
@@ -349,8 +343,9 @@ hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items
 }
 
 hipError_t launch_attend_join(const AttendArgs& a, const Cut& cut, unsigned tiles, hipStream_t st) {
-    const dim3 grid(tiles * (unsigned)(cut.cols >> 4) * (unsigned)a.pool.kv_heads, (unsigned)(a.pool.dp >> 4));
-    attend_join_kernel<<<grid, 256, 0, st>>>(a, cut, a.pool.dp, a.where != nullptr);
+    const unsigned x = (tiles << (cut.cols_log2 - 4)) * (unsigned)a.pool.kv_heads, all = (unsigned)a.pool.dp >> 4;
+    const unsigned wide = x >= 512 ? all : x >= 128 ? 2 : 1;  // few tiles: their channels over several workgroups
+    attend_join_kernel<<<dim3(x, (all + wide - 1) / wide), 256, 0, st>>>(a, cut, a.pool.dp, (int)wide);
     return hipGetLastError();
 }
 

@@ -24,6 +24,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads), item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
     TileWork w;
     if (!cut_item(cut, pool, b, item, w)) return;
+    if (a.plans && threadIdx.x == 0 && w.piece == 0 && head == 0) a.plans[w.tile_index] = w;
     Att att;
     const int wave_col = w.col0 + 16 * kCols * wave;
 #pragma unroll
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     }
     att.close();
     if (w.pieces > 1) {
-        float* part = a.parts + ((size_t)w.slot * pool.kv_heads + head) * (size_t)part_floats(64 * kCols, kDp);
+        float* part = a.parts + ((size_t)(w.slot + w.piece) * pool.kv_heads + head) * (size_t)part_floats(64 * kCols, kDp);
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             const int sub = wave * kCols + t;
@@ -142,72 +143,68 @@ hipError_t launch_attend_join(const AttendArgs& a, const Cut& cut, unsigned tile
 
 namespace {
 
-// Columns that the few-column kernel takes of a request, and those of a tile of the other one.
+// Columns of a request that the few-column kernel takes.
 int few_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 32 : 16; }
-int many_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 128 : 64; }
-
-struct Plan {
-    Cut cut;
-    bool run;
-    unsigned items, tiles;  // most of a key head
-};
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// The few-column launch: pieces for kFewItems workgroups over the key heads, none of fewer than eight blocks.
 constexpr int kFewItems = 1024, kManyItems = 512;
 
-Plan plan_few(const AttendArgs& a) {
-    const int group = a.heads / a.pool.kv_heads, few = few_columns(a);
-    const int most = a.batch.most;  // rows of a request
-    Plan p{};
-    p.run = group <= few && (a.batch.requests > 1 || most * (int64_t)group <= few);
-    const int cols = most * (int64_t)group <= 16 ? 16 : few;
-    p.cut = Cut{cols, 1, (int)(most * (int64_t)group < few ? most * group : few), ceil_div(kFewItems, a.pool.kv_heads), 8, true, a.window, group, 0};
-    const int tiles = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
-    p.tiles = (unsigned)tiles;
-    p.items = (unsigned)(tiles + p.cut.target + 1);
-    p.cut.slots = (int)p.items;
-    return p;
-}
+struct Plan {
+    Cut cut;
+    bool few, split;
+    unsigned items, tiles;  // most of a key head
+};
 
-Plan plan_many(const AttendArgs& a) {
-    const int group = a.heads / a.pool.kv_heads, few = few_columns(a), cols = many_columns(a);
-    Plan p{};
-    p.run = group > few || a.batch.most * (int64_t)group > few;
-    const int least = group > few ? 1 : few + 1;
-    p.cut = Cut{cols, least, (int)(a.batch.most * (int64_t)group), ceil_div(kManyItems, a.pool.kv_heads), 16, false, a.window, group, 0};
+// One kernel a call: the few-column one where no request has more columns than it takes, else the other for all of them. (Its tiles
+// waste three waves of four on a decode step's columns, but read their keys as fast; a launch of each cost batches without such
+// requests 13 us for nothing.)
+Plan plan_attend(const AttendArgs& a) {
+    const int group = a.heads / a.pool.kv_heads;
+    const int64_t most = (int64_t)a.batch.most * group;
     const int requests = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
-    p.tiles = (unsigned)(a.batch.rows * (int64_t)group / cols + requests);
-    p.cut.split = a.batch.rows * (int64_t)group / cols * a.pool.kv_heads < kManyItems;
-    p.items = p.tiles + (p.cut.split ? p.cut.target + 1 : 0);
+    Plan p{};
+    p.few = most <= few_columns(a);
+    p.split = true;
+    const int log2 = p.few ? (most <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
+    p.cut = Cut{log2, 1, (int)most, ceil_div(p.few ? kFewItems : kManyItems, a.pool.kv_heads), p.few ? 8 : 16, a.window, group, 0, 0};
+    p.tiles = (unsigned)(p.few ? requests : (((int64_t)a.batch.rows * group) >> log2) + requests);
+    p.items = p.tiles + 2 * (unsigned)p.cut.target + 1;
     p.cut.slots = (int)p.items;
+    p.cut.tiles = (int)p.tiles;
     return p;
 }
 
+size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
 size_t part_bytes(const AttendArgs& a, const Plan& p) {
-    if (!p.run || !p.cut.split) return 0;
-    return ((size_t)p.items * a.pool.kv_heads * part_floats(p.cut.cols, a.pool.dp) * 4 + 255) & ~size_t(255);
+    return rounded((size_t)p.items * a.pool.kv_heads * part_floats(1 << p.cut.cols_log2, a.pool.dp) * 4);
+}
+size_t plan_bytes(const Plan& p) { return rounded((size_t)p.tiles * sizeof(TilePlan)); }
+AttendArgs with_scratch(const AttendArgs& a, const Plan& p) {
+    AttendArgs m = a;
+    if (p.split) m.plans = (TilePlan*)((char*)a.parts + part_bytes(a, p));
+    return m;
 }
 
 }  // namespace
 
-size_t attend_scratch(const AttendArgs& a) { return part_bytes(a, plan_few(a)) + part_bytes(a, plan_many(a)); }
+size_t attend_scratch(const AttendArgs& a) {
+    const Plan p = plan_attend(a);
+    return part_bytes(a, p) + plan_bytes(p);
+}
 
 hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
-    const Plan few = plan_few(a), many = plan_many(a);
+    const Plan p = plan_attend(a);
+    const AttendArgs m = with_scratch(a, p);
     hipError_t e = hipSuccess;
-    if (few.run) {
-        e = launch_attend_few(a, few.cut, few.items, st);
-        if (e == hipSuccess && few.cut.split) e = launch_attend_join(a, few.cut, few.tiles, st);
+    if (p.few) {
+        e = launch_attend_few(m, p.cut, p.items, st);
+        return e == hipSuccess ? launch_attend_join(m, p.cut, p.tiles, st) : e;
     }
-    if (e != hipSuccess || !many.run) return e;
-    AttendArgs m = a;
-    m.parts = (float*)((char*)a.parts + part_bytes(a, few));
-    const unsigned grid = many.items * (unsigned)a.pool.kv_heads;
+    const unsigned grid = p.items * (unsigned)a.pool.kv_heads;
     auto go = [&](auto type, auto dp) {
         constexpr int kType = decltype(type)::value, kDp = decltype(dp)::value;
-        if constexpr (kType != kKvI8 || kDp != 96) attend_many_kernel<kType, kDp, kDp <= 128 ? 2 : 1><<<grid, 256, 0, st>>>(m, many.cut);
+        if constexpr (kType != kKvI8 || kDp != 96) attend_many_kernel<kType, kDp, kDp <= 128 ? 2 : 1><<<grid, 256, 0, st>>>(m, p.cut);
     };
     using std::integral_constant;
     auto sized = [&](auto type) {
@@ -224,8 +221,7 @@ hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
         default: sized(integral_constant<int, kKvI8>{});
     }
     e = hipGetLastError();
-    if (e == hipSuccess && many.cut.split) e = launch_attend_join(m, many.cut, many.tiles, st);
-    return e;
+    return e == hipSuccess ? launch_attend_join(m, p.cut, p.tiles, st) : e;
 }
 
 // ------------------------------------------------------------------------------------------------- selected pages
@@ -241,11 +237,13 @@ Plan plan_selected(const AttendArgs& a) {
     if (pieces < 1) pieces = 1;
     const int each = ceil_div(blocks, pieces);
     Plan p{};
-    p.run = true;
-    p.cut = Cut{16, 1, 16, ceil_div(blocks, each), each, false, 0, group, 0};
-    p.cut.split = p.cut.target > 1;
+    p.few = true;
+    p.cut = Cut{4, 1, 16, ceil_div(blocks, each), each, 0, group, 0, 0};
+    p.split = p.cut.target > 1;
     p.tiles = (unsigned)(a.batch.rows * tiles);
     p.items = p.tiles * (unsigned)p.cut.target;
+    p.cut.slots = (int)p.items;
+    p.cut.tiles = (int)p.tiles;
     return p;
 }
 
@@ -253,13 +251,17 @@ Plan plan_selected(const AttendArgs& a) {
 
 hipError_t launch_select_pages(const AttendArgs& a, hipStream_t st);
 
-size_t attend_selected_scratch(const AttendArgs& a) { return part_bytes(a, plan_selected(a)); }
+size_t attend_selected_scratch(const AttendArgs& a) {
+    const Plan p = plan_selected(a);
+    return p.split ? part_bytes(a, p) + plan_bytes(p) : 0;
+}
 
 hipError_t launch_attend_selected(const AttendArgs& a, hipStream_t st) {
     const Plan p = plan_selected(a);
-    hipError_t e = launch_select_pages(a, st);
-    if (e == hipSuccess) e = launch_attend_few(a, p.cut, p.items, st);
-    if (e == hipSuccess && p.cut.split) e = launch_attend_join(a, p.cut, p.tiles, st);
+    const AttendArgs m = with_scratch(a, p);
+    hipError_t e = launch_select_pages(m, st);
+    if (e == hipSuccess) e = launch_attend_few(m, p.cut, p.items, st);
+    if (e == hipSuccess && p.split) e = launch_attend_join(m, p.cut, p.tiles, st);
     return e;
 }
 
