@@ -35,6 +35,16 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Over the four lanes of a column: l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float column_max(float v) {
+    auto f = [](int a, int b) { return (int)__builtin_bit_cast(uint32_t, fmaxf(as_float((uint32_t)a), as_float((uint32_t)b))); };
+    return as_float((uint32_t)join32(join16((int)__builtin_bit_cast(uint32_t, v), f), f));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    auto f = [](int a, int b) { return (int)__builtin_bit_cast(uint32_t, as_float((uint32_t)a) + as_float((uint32_t)b)); };
+    return as_float((uint32_t)join32(join16((int)__builtin_bit_cast(uint32_t, v), f), f));
+}
+
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTop = 10.0f, kRoom = 4.0f;  // log2 of p at a new reference, and how far it may grow before the next
@@ -55,20 +65,14 @@ struct KvMath {
             f32x2 v = {x[2 * i], x[2 * i + 1]};
 #pragma unroll
             for (int p = 0; p < kParts; p++) {
-                uint32_t w;
-                f32x2 back;
                 if constexpr (kType == kKvBf16) {
-                    w = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b16x2));
-                    back = f32x2{as_float(w << 16), as_float(w & 0xffff0000u)};
+                    const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b16x2));
+                    part[p][i] = w;
+                    if (p + 1 < kParts) v = f32x2{v.x - as_float(w << 16), v.y - as_float(w & 0xffff0000u)};
                 } else {
                     const h16x2 h = __builtin_convertvector(v, h16x2);
-                    w = __builtin_bit_cast(uint32_t, h);
-                    back = __builtin_convertvector(h, f32x2);
-                }
-                part[p][i] = w;
-                if (p + 1 < kParts) {
-                    v.x = v.x - back.x;
-                    v.y = v.y - back.y;
+                    part[p][i] = __builtin_bit_cast(uint32_t, h);
+                    if (p + 1 < kParts) v = f32x2{fmaf((float)h.x, -1.0f, v.x), fmaf((float)h.y, -1.0f, v.y)};  // (v_fma_mix)
                 }
             }
         }
@@ -141,8 +145,7 @@ struct Attention {
                 top = fmaxf(top, fabsf(v[c][i]));
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = column_max(top);
         const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23), 1), 253);
         const float down = as_float((uint32_t)(254 - e) << 23);
         qs[t] = as_float((uint32_t)e << 23);
@@ -183,21 +186,15 @@ struct Attention {
             }
     }
 
-    // Scores into probabilities, split for the second product. first: the block's first token; ks, vs: int8's scales of this lane's tokens.
-    __device__ __forceinline__ void probabilities(f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts], bool masked, int first,
-                                                  const f32x4 (&ks)[2], const f32x4 (&vs)[2]) {
+    // A block's scores before their powers: int8's key scales, masks, and the columns' references. first: the block's first token; ks,
+    // vs: int8's scales of this lane's tokens.
+    __device__ __forceinline__ void settle(f32x4 (&s)[kCols][2], bool masked, int first, const f32x4 (&ks)[2], const f32x4 (&vs)[2]) {
         const int mine = first + ((threadIdx.x >> 4) & 3) * 4;
-        bool move = false;
-        float top[kCols], vtop[kCols];
+        if constexpr (kType == kKvI8) {
 #pragma unroll
-        for (int t = 0; t < kCols; t++) {
+            for (int t = 0; t < kCols; t++)
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    s[t][h][i] *= qs[t];
-                    if constexpr (kType == kKvI8) s[t][h][i] *= ks[h][i];
-                }
+                for (int h = 0; h < 2; h++) s[t][h] *= ks[h];
         }
         if (masked) {
 #pragma unroll
@@ -211,26 +208,28 @@ struct Attention {
                     }
             }
         }
+        bool move = false;
+        float top[kCols], vtop[kCols];
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
-            top[t] = -kInf;
+            top[t] = s[t][0][0];
             vtop[t] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    top[t] = fmaxf(top[t], s[t][h][i]);
+                    if (h + i) top[t] = fmaxf(top[t], s[t][h][i]);
                     // (a hidden token's scale counts for nothing)
                     if constexpr (kType == kKvI8) vtop[t] = fmaxf(vtop[t], masked && s[t][h][i] == -kInf ? 0.0f : vs[h][i]);
                 }
+            top[t] *= qs[t];
             move = move | (top[t] > ref[t] + kTop + kRoom);
             if constexpr (kType == kKvI8) move = move | (vtop[t] > ev[t]);
         }
         if (__ballot(move)) {
 #pragma unroll
             for (int t = 0; t < kCols; t++) {
-                float m = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
+                const float m = column_max(top[t]);
                 float f = 1.0f;
                 if (m > ref[t] + kTop + kRoom) {
                     f = __builtin_amdgcn_exp2f(ref[t] - (m - kTop));
@@ -238,8 +237,7 @@ struct Attention {
                     l[t] *= f;
                 }
                 if constexpr (kType == kKvI8) {
-                    float v = fmaxf(vtop[t], __shfl_xor(vtop[t], 16, 64));
-                    v = fmaxf(v, __shfl_xor(v, 32, 64));
+                    const float v = column_max(vtop[t]);
                     if (v > ev[t]) {
                         const uint32_t e = min((__builtin_bit_cast(uint32_t, v) >> 23) + 1u, 253u);
                         f *= ev[t] * as_float((254u - e) << 23);
@@ -250,6 +248,11 @@ struct Attention {
                 for (int d = 0; d < kTiles; d++) o[t][d] *= f;
             }
         }
+    }
+
+    // Settled scores into probabilities, split for the second product.
+    __device__ __forceinline__ void probabilities(const f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts], bool masked,
+                                                  const f32x4 (&vs)[2]) {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             const float r = ref[t] == -kInf ? 0.0f : ref[t];
@@ -260,7 +263,7 @@ struct Attention {
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float v = __builtin_amdgcn_exp2f(s[t][h][i] - r);
+                    const float v = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], qs[t], -r));
                     l[t] += v;
                     x[4 * h + i] = v;
                     if constexpr (kType == kKvI8) {
@@ -320,8 +323,7 @@ struct Attention {
     __device__ __forceinline__ void close() {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
-            l[t] += __shfl_xor(l[t], 16, 64);
-            l[t] += __shfl_xor(l[t], 32, 64);
+            l[t] = column_sum(l[t]);
             if constexpr (kType == kKvI8) {
 #pragma unroll
                 for (int d = 0; d < kTiles; d++) o[t][d] *= ev[t];
@@ -408,12 +410,6 @@ __device__ __forceinline__ CutRequest cut_load(const Cut& c, const KvPool& pool,
     return q;
 }
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return uniform(v);
-}
-
 // Item `item` of a key head; false past the last one. Every wave finds it for itself: lanes hold 64 requests at a time.
 __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, int item, TileWork& w) {
     const int lane = threadIdx.x & 63;
@@ -426,26 +422,20 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
         tiles += o.tiles;
         longest = max(longest, o.blocks);
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        sum += __shfl_xor(sum, off, 64);
-        tiles += __shfl_xor(tiles, off, 64);
-        longest = max(longest, __shfl_xor(longest, off, 64));
-    }
-    tiles = uniform(tiles);
+    sum = wave_sum(sum);
+    tiles = wave_sum(tiles);
+    longest = wave_max(longest);
     const float each = sum / (float)c.target * (tiles >= c.target ? 1.5f : 1.0f);
     const int piece = uniform(max((int)fminf(ceilf(each), 1.0e9f), c.least_blocks));
     int l = 0, before = 0, tiles_before = 0;
     w.piece = 0;
     w.r = 0;
-    if (b.requests <= 64 && uniform(longest) <= piece) {
+    if (b.requests <= 64 && longest <= piece) {
         if (item >= tiles) return false;
         // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
         const int base = (int)min(max(((int64_t)q.place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
         int lo = -1, hi = q.tiles ? base + q.tiles : 0;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) hi = max(hi, __shfl_xor(hi, off, 64));
-        hi = uniform(hi);  // none past hi; more than `item` past lo
+        hi = wave_max(hi);  // none past hi; more than `item` past lo
         int past = 0;
         while (hi - lo > 1) {
             const int x = lo + (hi - lo) / 2;
@@ -470,15 +460,7 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
             if (base >= b.requests) return false;
             if (base) q = cut_load(c, pool, b, base + lane);
             const int mine = q.tiles * cut_pieces(q.blocks, piece);
-            int upto = mine, tiles_upto = q.tiles;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int v = __shfl_up(upto, off, 64), t = __shfl_up(tiles_upto, off, 64);
-                if (lane >= off) {
-                    upto += v;
-                    tiles_upto += t;
-                }
-            }
+            const int upto = wave_upto(mine), tiles_upto = wave_upto(q.tiles);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item >= before + all) {
                 before += all;

@@ -144,7 +144,8 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
             const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
             if (page >= 0) {
                 u32x4 p[kCols][M::kParts];
-                att.probabilities(s, p, masked, first, ks_now, vs_now);
+                att.settle(s, masked, first, ks_now, vs_now);
+                att.probabilities(s, p, masked, vs_now);
                 auto value = [&](int tile) {
                     return value_operand<kType, kDp>(tile, [&](int at) { return values[(at - kv_plane_bytes(kType, kDp)) >> 10]; });
                 };

@@ -48,6 +48,47 @@ __device__ __forceinline__ KvRows kv_rows(const KvBatch& b, int r) {
 
 __device__ __forceinline__ int kv_length(const KvBatch& b, int r) { return max(b.lengths[r], 0); }
 
+// Across a wave's lanes without LDS: the other 16 or 32 lanes' value comes from a swap of rows, neighbours' from DPP.
+template <class F>
+__device__ __forceinline__ int join16(int v, F f) {  // lanes l, l ^ 16
+    const auto p = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    return f((int)p[0], (int)p[1]);
+}
+template <class F>
+__device__ __forceinline__ int join32(int v, F f) {  // lanes l, l ^ 32
+    const auto p = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    return f((int)p[0], (int)p[1]);
+}
+template <class F>
+__device__ __forceinline__ int wave_join(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));  // row_half_mirror
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false));  // row_mirror
+    return __builtin_amdgcn_readfirstlane(join32(join16(v, f), f));
+}
+__device__ __forceinline__ int wave_sum(int v) {
+    return wave_join(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_max(int v) {
+    return wave_join(v, [](int a, int b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return as_float((uint32_t)wave_join((int)__builtin_bit_cast(uint32_t, v), [](int a, int b) {
+        return (int)__builtin_bit_cast(uint32_t, as_float((uint32_t)a) + as_float((uint32_t)b));
+    }));
+}
+// Inclusive running sum.
+__device__ __forceinline__ int wave_upto(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int row = (int)(threadIdx.x >> 4) & 3, a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31),
+              c = __builtin_amdgcn_readlane(v, 47);
+    return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
 // Walks the requests 64 at a time with `count(r)` items each (every lane of a wave calls it) until item number `item`; false past the
 // last one. r: its request; item: its number within it; before: the items of the requests before r.
 template <class Count>
@@ -56,12 +97,7 @@ __device__ __forceinline__ bool kv_find(int requests, int& item, int& r, int& be
     before = 0;
     for (int base = 0; base < requests; base += 64) {
         const int mine = base + lane < requests ? count(base + lane) : 0;
-        int upto = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int v = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += v;
-        }
+        const int upto = wave_upto(mine);
         const int all = __builtin_amdgcn_readlane(upto, 63);
         if (item < before + all) {
             const int l = __ffsll((unsigned long long)__ballot(before + upto > item)) - 1;
