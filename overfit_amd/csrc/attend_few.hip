@@ -1,9 +1,11 @@
 // attend_few.hip — attention of few columns (up to 32 (row, query head) pairs of a request and key head: decode steps, drafted tokens)
 // over a paged cache, of any columns over selected pages, and the joining of partial outputs. Arithmetic: attend.h.
 //
-// Bound: HBM, each key and value is read once for its request. Four waves take a piece's blocks in turn, straight into registers in
-// operand order (no LDS, no transposition): a block's keys are loaded while the block before it goes through its softmax and second
-// product, its values during its own first one. Pieces are cut so that all key heads together give a few workgroups for each CU
+// Bound: HBM, each key and value is read once for its request. Four waves take a piece's blocks in turn, each through a ring of its own
+// in LDS that the DMA fills in operand order (no transposition, no barriers): a block's keys are loaded while the block before it goes
+// through its softmax and second product, its values during its own first one. Keys and values loaded into registers instead, with as
+// many under way, are 1 to 2 % faster on one column tile (64 decode rows of 5 k tokens 237 / 239 us), but two tiles leave a wave a SIMD
+// then (60 drafted rows, 8-bit cache, 150 / 112). Pieces are cut so that all key heads together give a few workgroups for each CU
 // whatever the lengths; their partial outputs are joined by a second launch. Waves join theirs in LDS, in a fixed order.
 #include <type_traits>
 
@@ -13,12 +15,19 @@ namespace ovfq {
 
 namespace {
 
-// Where a wave's columns come from and which tokens it walks.
+// Blocks that a wave has under way: rings of half of a CU's LDS at most (all of it for heads past 128), so that two workgroups fit.
+constexpr int few_depth(int type, int dp) { return dp > 128 ? 1 : 18432 / kv_bytes(type, dp); }
+
 template <int kType, int kDp, int kCols, bool kSelected>
-__global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void attend_few_kernel(AttendArgs a, Cut cut) {
+__global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, Cut cut) {
     using Att = Attention<kType, kDp, kCols>;
     using M = KvMath<kType>;
-    __shared__ f32x4 joined[2][kCols * Att::kTiles][64];
+    constexpr int kPlane = kv_plane_bytes(kType, kDp), kBytes = kv_bytes(kType, kDp), kLoads = kPlane / 1024;
+    constexpr int kKeyLoads = kLoads + (kType == kKvI8 ? 1 : 0), kLoadsOfBlock = kKeyLoads + kLoads;
+    constexpr int kDepth = few_depth(kType, kDp);
+    __shared__ __attribute__((aligned(16))) char shared[4 * kDepth * kBytes];  // the waves' rings, then the join of their outputs
+    f32x4(*joined)[kCols * Att::kTiles][64] = (f32x4(*)[kCols * Att::kTiles][64])shared;
+    static_assert(2 * kCols * Att::kTiles * 64 * 16 <= 4 * kDepth * kBytes, "the join fits into the rings");
     __shared__ float refs[4][kCols * 16];
     __shared__ float sums[4][kCols * 16];
     const KvPool& pool = a.pool;
@@ -70,15 +79,11 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
     const int last_last = w.place + min(w.rows - 1, (w.col0 + 16 * kCols - 1) / cut.group);
     const int last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
 
-    constexpr int kLoads = kv_plane_bytes(kType, kDp) / 1024;
-    u32x4 keys[kLoads], values[kLoads];
-    f32x4 ks[2], vs[2];
     const int* table = b.tables + (size_t)w.r * b.width;
     BlockWalk walk;
-    int held = 0;  // selected: lanes' page numbers
+    int held = 0, phys = -1;  // selected: lanes' page numbers in the request's table, and in the cache
     auto block_of = [&](int i) { return w.block0 + wave + 4 * i; };
     const int mine = w.block1 > w.block0 + wave ? (w.block1 - w.block0 - wave + 3) >> 2 : 0;
-    int phys = -1;
     auto selected_fetch = [&](int i) {
         const int at = (block_of(i) + 4 * lane) >> shift;
         const int p = at < whole ? pages[at] : -1;
@@ -86,38 +91,35 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
         const int t = p >= 0 && p < b.width ? table[p] : -1;
         phys = t >= 0 && t < pool.pages ? t : -1;
     };
-    // the page of the wave's i-th block and its first token
-    auto locate = [&](int i, int& page, int& first) {
-        const int block = block_of(i);
+    // a block's page (-1: not there, its tokens count as hidden), first token and bytes, in rising order
+    struct At {
+        int page, first;
+        const char* bytes;
+    };
+    auto locate = [&](int i) {
+        At at;
+        const int block = block_of(i), within = block & ((1 << shift) - 1);
         if constexpr (kSelected) {
             if (i && (i & 63) == 0) selected_fetch(i);
-            page = __builtin_amdgcn_readlane(phys, i & 63);
-            first = __builtin_amdgcn_readlane(held, i & 63) * pool.page + (block & ((1 << shift) - 1)) * kKvBlock;
+            at.page = __builtin_amdgcn_readlane(phys, i & 63);
+            at.first = __builtin_amdgcn_readlane(held, i & 63) * pool.page + within * kKvBlock;
         } else {
-            page = walk.page(i);
-            first = block * kKvBlock;
+            at.page = walk.page(i);
+            at.first = block * kKvBlock;
         }
+        at.bytes = kv_block(pool, max(at.page, 0), head, within);
+        return at;
     };
-    // (a page that is not there: its tokens count as hidden)
-    auto source = [&](int i, int page) {
-        return (const char*)kv_block(pool, max(page, 0), head, block_of(i) & ((1 << shift) - 1)) + lane * 16;
-    };
-    auto load_keys = [&](const char* p) {
+    auto stage = [&](char* dst, const char* src, bool values) {
+        const int plane = values ? kPlane : 0;
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) keys[i] = *(const u32x4*)(p + i * 1024);
+        for (int k = 0; k < kLoads; k++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + plane + k * 1024 + lane * 16),
+                                             (__attribute__((address_space(3))) void*)(dst + plane + k * 1024), 16, 0, 0);
         if constexpr (kType == kKvI8) {
-            const char* s = p - lane * 16 + 2 * kv_plane_bytes(kType, kDp) + (lane >> 4) * 16;
-            ks[0] = *(const f32x4*)s;
-            ks[1] = *(const f32x4*)(s + 64);
-        }
-    };
-    auto load_values = [&](const char* p) {
-#pragma unroll
-        for (int i = 0; i < kLoads; i++) values[i] = *(const u32x4*)(p + kv_plane_bytes(kType, kDp) + i * 1024);
-        if constexpr (kType == kKvI8) {
-            const char* s = p - lane * 16 + 2 * kv_plane_bytes(kType, kDp) + 128 + (lane >> 4) * 16;
-            vs[0] = *(const f32x4*)s;
-            vs[1] = *(const f32x4*)(s + 64);
+            if (!values)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + 2 * kPlane + lane * 4),
+                                                 (__attribute__((address_space(3))) void*)(dst + 2 * kPlane), 4, 0, 0);
         }
     };
     if (mine) {
@@ -125,50 +127,72 @@ __global__ __launch_bounds__(256, (kCols == 1 && kDp <= 128) ? 2 : 1) void atten
             selected_fetch(0);
         else
             walk.start(pool, table, b.width, block_of(0), 4);
-        int page, first;
-        locate(0, page, first);
-        const char* now = source(0, page);
-        load_keys(now);
-        load_values(now);
+        char* ring = shared + wave * kDepth * kBytes;
+        At ahead[kDepth];  // blocks i .. i + kDepth - 1
+#pragma unroll
+        for (int j = 0; j < kDepth; j++) {
+            ahead[j] = j && j >= mine ? ahead[j ? j - 1 : 0] : locate(j);
+            stage(ring + j * kBytes, ahead[j].bytes, false);
+            stage(ring + j * kBytes, ahead[j].bytes, true);
+        }
+        int slot = 0;
         for (int i = 0; i < mine; i++) {
-            int next_page = -1, next_first = 0;
-            const char* next = now;
-            if (i + 1 < mine) {
-                locate(i + 1, next_page, next_first);
-                next = source(i + 1, next_page);
+            const At now = ahead[0];
+            // (past the last block its predecessor is loaded again: the counts of loads under way stay)
+            const At next = i + kDepth < mine ? locate(i + kDepth) : ahead[kDepth - 1];
+            char* place = ring + slot * kBytes;
+            const char* at = place + lane * 16;
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads + (kDepth - 1) * kLoadsOfBlock) : "memory");
+            f32x4 ks[2] = {}, vs[2] = {};
+            if constexpr (kType == kKvI8) {
+                const char* c = place + 2 * kPlane + (lane >> 4) * 16;
+                ks[0] = *(const f32x4*)c;
+                ks[1] = *(const f32x4*)(c + 64);
+                vs[0] = *(const f32x4*)(c + 128);
+                vs[1] = *(const f32x4*)(c + 192);
             }
             f32x4 s[kCols][2];
-            att.scores(s, [&](int tile, int chunk) { return key_operand<kType, kDp>(tile, chunk, [&](int at) { return keys[at >> 10]; }); });
-            f32x4 ks_now[2] = {ks[0], ks[1]}, vs_now[2] = {vs[0], vs[1]};
-            if (i + 1 < mine) load_keys(next);
-            const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
-            if (page >= 0) {
-                u32x4 p[kCols][M::kParts];
-                att.settle(s, masked, first, ks_now, vs_now);
-                att.probabilities(s, p, masked, vs_now);
+            att.scores(s, [&](int tile, int chunk) {
+                return key_operand<kType, kDp>(tile, chunk, [&](int off) { return *(const u32x4*)(at + off); });
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys are read: their place takes the next ones
+            stage(place, next.bytes, false);
+            const bool masked = now.first + kKvBlock - 1 > first_last || now.first < last_low;
+            u32x4 p[kCols][M::kParts];
+            if (now.page >= 0) {
+                att.settle(s, masked, now.first, ks, vs);
+                att.probabilities(s, p, masked, vs);
+            }
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kKeyLoads + (kDepth - 1) * kLoadsOfBlock) : "memory");
+            if (now.page >= 0) {
                 auto value = [&](int tile) {
-                    return value_operand<kType, kDp>(tile, [&](int at) { return values[(at - kv_plane_bytes(kType, kDp)) >> 10]; });
+                    return value_operand<kType, kDp>(tile, [&](int off) { return *(const u32x4*)(at + off); });
                 };
                 if constexpr (kType != kKvI8) {
                     if (masked) {
                         bool any = false;
-#pragma unroll
-                        for (int k = 0; k < kLoads; k++) any = any | any_not_finite<kType>(values[k]);
+                        for (int k = 0; k < kLoads; k++) any = any | any_not_finite<kType>(*(const u32x4*)(at + kPlane + k * 1024));
                         if (__ballot(any)) {
-                            att.template note_bad<Att::kTiles>(first, value);
-#pragma unroll
-                            for (int k = 0; k < kLoads; k++) values[k] = finite_part<kType>(values[k]);
+                            att.template note_bad<1>(now.first, value);
+                            for (int k = 0; k < kLoads; k++) {
+                                u32x4* v = (u32x4*)(place + kPlane + k * 1024 + lane * 16);
+                                *v = finite_part<kType>(*v);
+                            }
                         }
                     }
                 }
                 att.products(p, value);
             }
-            if (i + 1 < mine) load_values(next);
-            page = next_page;
-            first = next_first;
-            now = next;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            stage(place, next.bytes, true);
+            slot = slot + 1 < kDepth ? slot + 1 : 0;
+#pragma unroll
+            for (int j = 0; j + 1 < kDepth; j++) ahead[j] = ahead[j + 1];
+            ahead[kDepth - 1] = next;
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads land before their places serve the join
     }
+    __syncthreads();
     att.close();
     // join the waves: 2 and 3 into 0 and 1, then 1 into 0
     if (lane < 16) {
