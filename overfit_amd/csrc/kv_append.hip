@@ -195,23 +195,14 @@ __device__ __forceinline__ void store8(const KvPool& p, char* block, int t, int 
 template <int kType, bool kFast>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int parts) {
     __shared__ float cs[2 * kMaxPairs];
-    __shared__ int found;
     // 32 consecutive rows go to one XCD (workgroups are dealt round the eight in turn): they share the lines of the values' blocks.
     int row = blockIdx.x;
     if ((int)gridDim.x > a.batch.rows || a.batch.rows % 256 == 0) row = (row >> 8) * 256 + (row & 7) * 32 + ((row >> 3) & 31);
     if (row >= a.batch.rows) return;
     const int tid = threadIdx.x, part = blockIdx.y;
-    if (tid == 0) found = a.batch.requests;
-    __syncthreads();
-    for (int r = tid; r < a.batch.requests; r += 256) {
-        const KvRows m = kv_rows(a.batch, r);
-        if (m.n && row >= m.first && row < m.first + m.n) atomicMin(&found, r);
-    }
-    __syncthreads();
-    const int r = __builtin_amdgcn_readfirstlane(found);
-    if (r >= a.batch.requests) return;
-    const KvRows m = kv_rows(a.batch, r);
-    const int place = kv_length(a.batch, r) - m.n + (row - m.first);
+    const KvRowPlace at = kv_row_place(a.batch, row, a.batch.rows);
+    if (at.r < 0) return;
+    const int r = at.r, place = at.place;
     const KvRope& rope = a.rope;
     for (int j = tid; j < rope.rotary >> 1; j += 256) {
         int position = place;

@@ -111,4 +111,26 @@ __device__ __forceinline__ bool kv_find(int requests, int& item, int& r, int& be
     return false;
 }
 
+// The request that a row belongs to (the first whose rows have it, of at most `most` rows; r -1: none), every wave for itself.
+struct KvRowPlace {
+    int r, place;  // place: the row's token
+};
+__device__ __forceinline__ KvRowPlace kv_row_place(const KvBatch& b, int row, int most) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < b.requests; base += 64) {
+        KvRows m{0, 0};
+        int len = 0;
+        if (base + lane < b.requests) {
+            m = kv_rows(b, base + lane);
+            len = kv_length(b, base + lane);
+        }
+        const uint64_t votes = __ballot(m.n && m.n <= most && row >= m.first && row - m.first < m.n);
+        if (votes) {
+            const int l = __ffsll((unsigned long long)votes) - 1;
+            return KvRowPlace{__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readlane(len - m.n + (row - m.first), l)};
+        }
+    }
+    return KvRowPlace{-1, -1};
+}
+
 }  // namespace ovfq
