@@ -7,9 +7,10 @@
 // near one, and cos and sin come from polynomials of the remainder (10^-13 off); both are rounded to fp32 once. Products and sums of
 // the rotation are single fp32 operations; the rounding to the cache's type is the only other one, half a step of that type.
 //
-// Bound: HBM for many rows (each fp32 row is read once, written once), the launch and three dependent reads (offsets, length and page,
-// then the rows, which are under way meanwhile) for one. A workgroup a row, four for batches below the chip's workgroups, which share
-// the row's heads.
+// Bound: HBM for many rows (each fp32 row is read once, written once), the launch and three dependent reads (offsets and length, page,
+// rows) for one. Queries and keys have a workgroup a row, four for batches below the chip's workgroups, which share the row's heads;
+// values one for a share of a block of the cache. (us, 1 / 1297 / 4096 rows of 32 and 8 heads of 128: 4.1 / 13.3 / 42.7; a copy of the bytes 0.01 / 11.4
+// / 36.1.)
 #include "kv_cache.h"
 
 namespace ovfq {
@@ -150,56 +151,145 @@ __device__ __forceinline__ uint16_t rounded(float v) {
     return __builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
-// Eight channels of a token's keys or values into its block. int8: a token and head's scale is absmax / 127 over its channels, held
-// by 8, 16 or 32 neighbouring lanes (the channels past dim are zeros); what is not finite makes it so.
+// A token's scale in an int8 cache: absmax / 127 over its head's channels, which `lanes` neighbouring lanes hold (the channels past dim
+// are zeros). `top`: the largest bits of the lane's magnitudes, which are ordered like them, NaN above all.
+struct Scaled {
+    float scale, inv;
+};
+__device__ __forceinline__ Scaled token_scale(uint32_t top, int lanes) {
+    for (int off = lanes / 2; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+    const float scale = as_float(top) / 127.0f;
+    return Scaled{scale, scale > 0.0f ? 1.0f / scale : 0.0f};
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, fabsf(v)); }
+__device__ __forceinline__ uint32_t quant(float v, float inv) {
+    return (uint32_t)((int)fminf(fmaxf(rintf(v * inv), -127.0f), 127.0f) + 128) & 0xffu;
+}
+
+// Eight channels of a token's keys into its block.
 template <int kType>
-__device__ __forceinline__ void store8(const KvPool& p, char* block, int t, int d, const float (&o)[8], bool values, bool live) {
-    char* plane = block + (values ? kv_plane_bytes(kType, p.dp) : 0);
+__device__ __forceinline__ void store_key(const KvPool& p, char* block, int t, int d, const float (&o)[8], bool live) {
     if constexpr (kType == kKvI8) {
-        uint32_t top = 0;  // the bits of magnitudes are ordered like them, NaN above all
+        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) top = max(top, __builtin_bit_cast(uint32_t, fabsf(o[i])));
-        for (int off = p.dp / 16; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-        const float scale = __builtin_bit_cast(float, top) / 127.0f;
-        const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+        for (int i = 0; i < 8; i++) top = max(top, magnitude(o[i]));
+        const Scaled s = token_scale(top, p.dp / 8);
         if (!live) return;
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int q = (int)fminf(fmaxf(rintf(o[i] * inv), -127.0f), 127.0f) + 128;
-            w[i >> 2] |= (uint32_t)(q & 0xff) << (8 * (i & 3));
-        }
-        if (values) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) plane[kv_value_at(true, t, d + i)] = (char)(w[i >> 2] >> (8 * (i & 3)));
-        } else {
-            *(u32x2*)(plane + kv_key_at(true, p.dp, t, d)) = u32x2{w[0], w[1]};
-        }
-        if (d == 0) ((float*)(block + 2 * kv_plane_bytes(kType, p.dp)))[(values ? kKvBlock : 0) + t] = scale;
+        for (int i = 0; i < 8; i++) w[i >> 2] |= quant(o[i], s.inv) << (8 * (i & 3));
+        *(u32x2*)(block + kv_key_at(true, p.dp, t, d)) = u32x2{w[0], w[1]};
+        if (d == 0) ((float*)(block + 2 * kv_plane_bytes(kType, p.dp)))[t] = s.scale;
     } else {
         if (!live) return;
         uint16_t h[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) h[i] = rounded<kType>(o[i]);
-        if (values) {
+        *(u32x4*)(block + kv_key_at(false, p.dp, t, d)) =
+            u32x4{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16, (uint32_t)h[4] | (uint32_t)h[5] << 16,
+                  (uint32_t)h[6] | (uint32_t)h[7] << 16};
+    }
+}
+
+// The new tokens' values of one block of the cache (at most rows / 32 + 2 a request), a share of its heads: a thread has four channels
+// of the eight tokens that lie together in it, and writes them as one piece each. (Token by token, in the rows' workgroups, a store had
+// a lane's 2 bytes in every 16: 4096 rows 54.6 us, 1297 rows 17.6.)
+template <int kType>
+__device__ __forceinline__ void append_values(const KvAppendArgs& a, int item, int part) {
+    const KvPool& p = a.pool;
+    const KvBatch& b = a.batch;
+    int r = 0, before = 0;
+    const bool any = kv_find(b.requests, item, r, before, [&](int q) {
+        const int n = kv_rows(b, q).n, len = kv_length(b, q), from = max(len - n, 0);
+        return n && len > from ? ((len - 1) / kKvBlock) - from / kKvBlock + 1 : 0;
+    });
+    if (!any) return;
+    const KvRows m = kv_rows(b, r);
+    const int len = kv_length(b, r), start = len - m.n;  // the first row's token, before the first if negative
+    const int block = max(start, 0) / kKvBlock + item, entry = block / (p.page / kKvBlock);
+    if (entry >= b.width) return;
+    const int page = b.tables[(size_t)r * b.width + entry];
+    if (page < 0 || page >= p.pages) return;
+    const int quads = p.dp >> 2, u = part * 256 + (int)threadIdx.x, quad = u % quads, g = (u / quads) & 3, head = u / (4 * quads);
+    if (head >= p.kv_heads) return;
+    const int d = 4 * quad;
+    const bool live = d < p.dim;
+    float x[8][4];
+    uint32_t here = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) *(uint16_t*)(plane + kv_value_at(false, t, d + i)) = h[i];
-        } else {
-            *(u32x4*)(plane + kv_key_at(false, p.dp, t, d)) =
-                u32x4{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16, (uint32_t)h[4] | (uint32_t)h[5] << 16,
-                      (uint32_t)h[6] | (uint32_t)h[7] << 16};
+    for (int i = 0; i < 8; i++) {
+        const int token = block * kKvBlock + (i >> 2) * 16 + g * 4 + (i & 3), row = token - start;
+        f32x4u v = {0, 0, 0, 0};
+        if (token < len && row >= 0) {
+            here |= 1u << i;
+            if (live) v = *(const f32x4u*)(a.v + ((size_t)(m.first + row) * p.kv_heads + head) * p.dim + d);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) x[i][c] = v[c];
+    }
+    char* at = kv_block(p, page, head, block & (p.page / kKvBlock - 1));
+    char* plane = at + kv_plane_bytes(kType, p.dp);
+    if constexpr (kType == kKvI8) {
+        float inv[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < 4; c++) top = max(top, magnitude(x[i][c]));
+            const Scaled s = token_scale(top, quads);
+            inv[i] = s.inv;
+            if (quad == 0 && (here >> i & 1))
+                ((float*)(at + 2 * kv_plane_bytes(kType, p.dp)))[kKvBlock + (i >> 2) * 16 + g * 4 + (i & 3)] = s.scale;
+        }
+        if (!live) return;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            char* to = plane + kv_value_at(true, 4 * g, d + c);
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i >> 2] |= quant(x[i][c], inv[i]) << (8 * (i & 3));
+            if (here == 0xff) {
+                *(u32x2*)to = u32x2{w[0], w[1]};
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (here >> i & 1) to[i] = (char)(w[i >> 2] >> (8 * (i & 3)));
+            }
+        }
+    } else {
+        if (!live) return;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            char* to = plane + kv_value_at(false, 4 * g, d + c);
+            uint16_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[i] = rounded<kType>(x[i][c]);
+            if (here == 0xff) {
+                *(u32x4*)to = u32x4{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16,
+                                    (uint32_t)h[4] | (uint32_t)h[5] << 16, (uint32_t)h[6] | (uint32_t)h[7] << 16};
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (here >> i & 1) ((uint16_t*)to)[i] = h[i];
+            }
         }
     }
 }
 
 template <int kType, bool kFast>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int parts) {
+__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int parts, int value_blocks, int value_parts) {
     __shared__ float cs[2 * kMaxPairs];
-    // 32 consecutive rows go to one XCD (workgroups are dealt round the eight in turn): they share the lines of the values' blocks.
-    int row = blockIdx.x;
-    if ((int)gridDim.x > a.batch.rows || a.batch.rows % 256 == 0) row = (row >> 8) * 256 + (row & 7) * 32 + ((row >> 3) & 31);
+    int index = blockIdx.x;
+    if (index < value_blocks * value_parts) {
+        append_values<kType>(a, index / value_parts, index % value_parts);
+        return;
+    }
+    index -= value_blocks * value_parts;
+    // 32 consecutive rows go to one XCD (workgroups are dealt round the eight in turn): they share the lines of the keys' blocks.
+    const int part = parts == 1 ? 0 : index % parts;
+    const int row = parts == 1 ? (index >> 8) * 256 + (index & 7) * 32 + ((index >> 3) & 31) : index / parts;
     if (row >= a.batch.rows) return;
-    const int tid = threadIdx.x, part = blockIdx.y;
+    const int tid = threadIdx.x;
     const KvRowPlace at = kv_row_place(a.batch, row, a.batch.rows);
     if (at.r < 0) return;
     const int r = at.r, place = at.place;
@@ -230,29 +320,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int part
     if (entry >= a.batch.width) return;
     const int page = a.batch.tables[(size_t)r * a.batch.width + entry];
     if (page < 0 || page >= a.pool.pages) return;
-    // keys and values in turn, a head's channels in neighbouring lanes; whole head groups of lanes run together
-    const int units = a.pool.dp >> 3, all = 2 * a.pool.kv_heads * units;
-    for (int u = from; u < all; u += step) {
-        const bool values = u >= (all >> 1);
-        const int w = values ? u - (all >> 1) : u;
-        const int h = w / units, d = (w - h * units) * 8;
+    // a head's channels in neighbouring lanes; whole head groups of lanes run together
+    const int units = a.pool.dp >> 3;
+    for (int u = from; u < a.pool.kv_heads * units; u += step) {
+        const int h = u / units, d = (u - h * units) * 8;
         char* block = kv_block(a.pool, page, h, in_page / kKvBlock);
-        const float* x = (values ? a.v : a.k) + ((size_t)row * a.pool.kv_heads + h) * dim;
         float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         const bool live = d < dim;
-        if (live) {
-            if (values) {
-                const f32x4u p = *(const f32x4u*)(x + d), q = *(const f32x4u*)(x + d + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    o[i] = p[i];
-                    o[4 + i] = q[i];
-                }
-            } else {
-                rotated8<kFast>(x, d, rope, cs, o);
-            }
-        }
-        store8<kType>(a.pool, block, in_page % kKvBlock, d, o, values, live);
+        if (live) rotated8<kFast>(a.k + ((size_t)row * a.pool.kv_heads + h) * dim, d, rope, cs, o);
+        store_key<kType>(a.pool, block, in_page % kKvBlock, d, o, live);
     }
 }
 
@@ -329,10 +405,14 @@ hipError_t launch_kv_clear(void* p, size_t bytes, hipStream_t st) {
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st) {
     const int rot = a.rope.rotary, dim = a.pool.dim;
     const bool fast = rot % 16 == 0 && dim % 8 == 0;
-    const int rows = a.batch.rows, parts = rows < 256 ? 4 : 1;
-    const dim3 grid((unsigned)(rows < 256 ? rows : (rows + 255) / 256 * 256), (unsigned)parts);
+    const int rows = a.batch.rows, requests = a.batch.requests < rows ? a.batch.requests : rows, parts = rows < 256 ? 4 : 1;
+    // blocks that the new tokens lie in: of n tokens at most n, and at most (n + 62) / 32
+    const int64_t blocks = ((int64_t)rows + 62 * (int64_t)requests) / 32;
+    const int value_blocks = !a.k ? 0 : (int)(blocks < rows ? blocks : rows);
+    const int value_parts = (a.pool.kv_heads * a.pool.dp + 255) / 256;
+    const unsigned grid = (unsigned)(value_blocks * value_parts + (parts == 1 ? (rows + 255) / 256 * 256 : rows * parts));
     auto go = [&](auto type, auto quick) {
-        kv_append_kernel<decltype(type)::value, decltype(quick)::value><<<grid, 256, 0, st>>>(a, parts);
+        kv_append_kernel<decltype(type)::value, decltype(quick)::value><<<grid, 256, 0, st>>>(a, parts, value_blocks, value_parts);
     };
     using std::integral_constant;
     auto typed = [&](auto type) {
@@ -348,7 +428,7 @@ hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st) {
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.pool.sums || !a.k) return e;
-    const int64_t ends = (int64_t)rows / a.pool.page + (a.batch.requests < rows ? a.batch.requests : rows);
+    const int64_t ends = (int64_t)rows / a.pool.page + requests;
     const dim3 pages((unsigned)ends, (unsigned)a.pool.kv_heads);
     switch (a.pool.type) {
         case kKvF16: kv_sums_kernel<kKvF16><<<pages, 256, 0, st>>>(a.pool, a.batch); break;
