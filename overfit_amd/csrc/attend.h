@@ -359,11 +359,15 @@ __device__ __forceinline__ u32x4 value_operand(int tile, Load load) {
 }
 
 // How a launch cuts its work. A request of `least` to `most` columns has tiles of `cols` columns (2^cols_log2), and a tile's blocks are
-// cut into pieces so that a key head has about `target` of them, none of fewer blocks than least_blocks. Where the tiles alone are that
-// many, pieces are half as long again, and where no tile is longer than that, the tiles go by the place of their last column, the
-// last ones (with the longest spans) first: 4100 rows of three prompts TODO us in the order of the requests.
+// cut into pieces of the same size, none of fewer blocks than least_blocks. `target` is the number of workgroups that the chip holds at
+// a time, for each key head. Fewer tiles are cut into the smallest pieces that still are no more than that: a workgroup more is a round
+// more (64 decode rows of 1 k to 8 k tokens in 512 workgroups 221 us, 1072 pieces of one size and their remainders 238;
+// 60 drafted rows over 24 k in 8 bits 95 and 107).
+// More tiles than that stay whole, but for those longer than `slack` times what a workgroup has on average, and if there are none go by
+// the place of their last column, the last ones (with the longest spans) first.
 struct Cut {
     int cols_log2, least, most, target, least_blocks;
+    float slack;
     int window, group;
     int slots, tiles;  // of a key head's partial outputs and plans (offsets that overlap could ask for more: that is left out)
 };
@@ -384,7 +388,8 @@ struct CutRequest {
     int first, n, place, tiles, blocks;  // blocks: of its longest tile, at most
     float sum;                           // of its tiles' blocks, about
 };
-__device__ __forceinline__ int cut_pieces(int blocks, int piece) { return blocks > piece ? (blocks + piece - 1) / piece : 1; }
+// Pieces of a tile of so many blocks, `inv` being one over a piece's most, give or take a thousandth: their sizes follow from the number.
+__device__ __forceinline__ int cut_pieces(int blocks, float inv) { return max((int)ceilf(fmaf((float)blocks, inv, -1.0e-3f)), 1); }
 // Blocks that the tokens place + i0 .. place + i1 see: [x, y).
 __device__ __forceinline__ int2 cut_blocks(const Cut& c, const KvPool& pool, const KvBatch& b, int place, int i0, int i1) {
     const int64_t last = min((int64_t)place + i1, (int64_t)b.width * pool.page - 1);
@@ -425,12 +430,27 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     sum = wave_sum(sum);
     tiles = wave_sum(tiles);
     longest = wave_max(longest);
-    const float each = sum / (float)c.target * (tiles >= c.target ? 1.5f : 1.0f);
-    const int piece = uniform(max((int)fminf(ceilf(each), 1.0e9f), c.least_blocks));
-    int l = 0, before = 0, tiles_before = 0;
+    const float mean = sum / (float)c.target;
+    float piece = fmaxf(ceilf(mean * (tiles >= c.target ? c.slack : 1.0f)), (float)c.least_blocks);
+    if (tiles < c.target && b.requests <= 64 && (float)longest > piece) {
+        // halving what lies between the mean, which may give too many, and the longest tile
+        float over = piece;
+        if (wave_sum(q.tiles * cut_pieces(q.blocks, 1.0f / piece)) > c.target) {
+            piece = (float)longest;
+            for (int i = 0; i < 5 && piece - over > 1.0f; i++) {
+                const float half = floorf(0.5f * (piece + over));
+                if (wave_sum(q.tiles * cut_pieces(q.blocks, 1.0f / half)) > c.target)
+                    over = half;
+                else
+                    piece = half;
+            }
+        }
+    }
+    const float inv = as_float((uint32_t)uniform((int)__builtin_bit_cast(uint32_t, 1.0f / piece)));
+    int l = 0, before = 0, tiles_before = 0, slots_before = 0;
     w.piece = 0;
     w.r = 0;
-    if (b.requests <= 64 && longest <= piece) {
+    if (b.requests <= 64 && cut_pieces(longest, inv) == 1) {
         if (item >= tiles) return false;
         // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
         const int base = (int)min(max(((int64_t)q.place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
@@ -459,25 +479,28 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
         for (int base = 0;; base += 64) {
             if (base >= b.requests) return false;
             if (base) q = cut_load(c, pool, b, base + lane);
-            const int mine = q.tiles * cut_pieces(q.blocks, piece);
-            const int upto = wave_upto(mine), tiles_upto = wave_upto(q.tiles);
+            const int mine = q.tiles * cut_pieces(q.blocks, inv);
+            const int slots = mine > q.tiles ? mine : 0;  // whole tiles have none
+            const int upto = wave_upto(mine), tiles_upto = wave_upto(q.tiles), slots_upto = wave_upto(slots);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item >= before + all) {
                 before += all;
                 tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
+                slots_before += __builtin_amdgcn_readlane(slots_upto, 63);
                 continue;
             }
             l = __ffsll((unsigned long long)__ballot(before + upto > item)) - 1;
             w.r = base + l;
             before += __builtin_amdgcn_readlane(upto - mine, l);
             tiles_before += __builtin_amdgcn_readlane(tiles_upto - q.tiles, l);
+            slots_before += __builtin_amdgcn_readlane(slots_upto - slots, l);
             break;
         }
-        const int pieces = cut_pieces(__builtin_amdgcn_readlane(q.blocks, l), piece);
+        const int pieces = uniform(cut_pieces(__builtin_amdgcn_readlane(q.blocks, l), inv));
         const int nth = uniform((item - before) / pieces);
         w.piece = item - before - nth * pieces;
         w.tile = __builtin_amdgcn_readlane(q.tiles, l) - 1 - nth;
-        w.slot = before + nth * pieces;
+        w.slot = slots_before + nth * pieces;
         w.tile_index = tiles_before + nth;
     }
     w.first_row = __builtin_amdgcn_readlane(q.first, l);
@@ -485,9 +508,10 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     w.place = __builtin_amdgcn_readlane(q.place, l);
     w.col0 = w.tile << c.cols_log2;
     const int2 s = cut_blocks(c, pool, b, w.place, uniform(w.col0 / c.group), uniform(min(w.rows - 1, (w.col0 + (1 << c.cols_log2) - 1) / c.group)));
-    w.pieces = uniform(cut_pieces(s.y - s.x, piece));
-    w.block0 = s.x + w.piece * min(piece, s.y - s.x);
-    w.block1 = s.y - w.block0 > piece ? w.block0 + piece : s.y;
+    w.pieces = uniform(cut_pieces(s.y - s.x, inv));
+    const int size = w.pieces == 1 ? s.y - s.x : (uniform((s.y - s.x + w.pieces - 1) / w.pieces) + 3) & ~3;  // (whole turns of four waves)
+    w.block0 = min(s.x + w.piece * size, s.y);
+    w.block1 = min(w.block0 + size, s.y);
     if ((w.slot + w.pieces > c.slots && w.pieces > 1) || w.tile_index >= c.tiles) return false;
     return w.piece < w.pieces;
 }

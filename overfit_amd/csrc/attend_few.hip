@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
         pages = a.chosen + ((size_t)row * pool.kv_heads + head) * a.top;
         for (int i = 0; i < a.top; i += 64) whole += __popcll(__ballot(i + lane < a.top && pages[min(i + lane, a.top - 1)] >= 0));
         const int blocks = whole << shift, each = cut.least_blocks;
-        w.pieces = cut_pieces(blocks, each);
+        w.pieces = blocks > each ? (blocks + each - 1) / each : 1;
         if (w.piece >= w.pieces) return;
         w.block0 = w.piece * each;
         w.block1 = min(blocks, w.block0 + each);

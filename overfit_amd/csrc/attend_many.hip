@@ -149,7 +149,7 @@ int few_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 32 : 16; }
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-constexpr int kFewItems = 1024, kManyItems = 512;
+constexpr int kItems = 512;  // two workgroups a CU: registers and LDS
 
 struct Plan {
     Cut cut;
@@ -168,17 +168,19 @@ Plan plan_attend(const AttendArgs& a) {
     p.few = most <= few_columns(a);
     p.split = true;
     const int log2 = p.few ? (most <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
-    p.cut = Cut{log2, 1, (int)most, ceil_div(p.few ? kFewItems : kManyItems, a.pool.kv_heads), p.few ? 8 : 16, a.window, group, 0, 0};
+    p.cut = Cut{log2, 1, (int)most, ceil_div(kItems, a.pool.kv_heads), p.few ? 8 : 16, p.few ? 2.0f : 1.5f, a.window, group, 0, 0};
     p.tiles = (unsigned)(p.few ? requests : (((int64_t)a.batch.rows * group) >> log2) + requests);
-    p.items = p.tiles + 2 * (unsigned)p.cut.target + 1;
-    p.cut.slots = (int)p.items;
+    // Pieces are no longer than the mean by more than `slack`, and the sum of the tiles' lengths that it comes from is half of their number
+    // times the longest at least: so many pieces at most, and so many of tiles that are cut.
+    p.items = p.tiles + 2 * (unsigned)p.cut.target + 2;
+    p.cut.slots = 4 * p.cut.target + 2;
     p.cut.tiles = (int)p.tiles;
     return p;
 }
 
 size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
 size_t part_bytes(const AttendArgs& a, const Plan& p) {
-    return rounded((size_t)p.items * a.pool.kv_heads * part_floats(1 << p.cut.cols_log2, a.pool.dp) * 4);
+    return rounded((size_t)p.cut.slots * a.pool.kv_heads * part_floats(1 << p.cut.cols_log2, a.pool.dp) * 4);
 }
 size_t plan_bytes(const Plan& p) { return rounded((size_t)p.tiles * sizeof(TilePlan)); }
 AttendArgs with_scratch(const AttendArgs& a, const Plan& p) {
@@ -229,17 +231,17 @@ hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
 
 namespace {
 
-// A row's pages in pieces of so many blocks that all rows and key heads give about kFewItems workgroups (at least 16 blocks each).
+// A row's pages in pieces of so many blocks that all rows and key heads give about kItems workgroups (at least 8 blocks each).
 Plan plan_selected(const AttendArgs& a) {
     const int group = a.heads / a.pool.kv_heads, tiles = (group + 15) / 16;
     const int64_t blocks = (int64_t)a.top * (a.pool.page / kKvBlock), all = (int64_t)a.batch.rows * a.pool.kv_heads * tiles;
-    int64_t pieces = (kFewItems + all - 1) / all;
-    if (pieces > blocks / 16) pieces = blocks / 16;
+    int64_t pieces = kItems / all;
+    if (pieces > blocks / 8) pieces = blocks / 8;
     if (pieces < 1) pieces = 1;
     const int each = ceil_div(blocks, pieces);
     Plan p{};
     p.few = true;
-    p.cut = Cut{4, 1, 16, ceil_div(blocks, each), each, 0, group, 0, 0};
+    p.cut = Cut{4, 1, 16, ceil_div(blocks, each), each, 1.0f, 0, group, 0, 0};
     p.split = p.cut.target > 1;
     p.tiles = (unsigned)(a.batch.rows * tiles);
     p.items = p.tiles * (unsigned)p.cut.target;
