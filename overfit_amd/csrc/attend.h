@@ -369,7 +369,7 @@ struct Cut {
     int cols_log2, least, most, target, least_blocks;
     float slack;
     int window, group;
-    int slots, tiles;  // of a key head's partial outputs and plans (offsets that overlap could ask for more: that is left out)
+    int slots, tiles;  // most of a key head's partial outputs, and of its tiles
 };
 // What the join needs to know of a tile, written by the tile's first piece.
 struct TilePlan {
@@ -430,6 +430,7 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     sum = wave_sum(sum);
     tiles = wave_sum(tiles);
     longest = wave_max(longest);
+    if (tiles > c.tiles) return false;  // offsets that overlap: none of the call's tiles
     const float mean = sum / (float)c.target;
     float piece = fmaxf(ceilf(mean * (tiles >= c.target ? c.slack : 1.0f)), (float)c.least_blocks);
     if (tiles < c.target && b.requests <= 64 && (float)longest > piece) {
@@ -512,7 +513,7 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     const int size = w.pieces == 1 ? s.y - s.x : (uniform((s.y - s.x + w.pieces - 1) / w.pieces) + 3) & ~3;  // (whole turns of four waves)
     w.block0 = min(s.x + w.piece * size, s.y);
     w.block1 = min(w.block0 + size, s.y);
-    if ((w.slot + w.pieces > c.slots && w.pieces > 1) || w.tile_index >= c.tiles) return false;
+    if (w.slot + w.pieces > c.slots && w.pieces > 1) return false;
     return w.piece < w.pieces;
 }
 // All tiles of a launch's requests.

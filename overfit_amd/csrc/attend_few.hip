@@ -6,7 +6,9 @@
 // through its softmax and second product, its values during its own first one. Keys and values loaded into registers instead, with as
 // many under way, are 1 to 2 % faster on one column tile (64 decode rows of 5 k tokens 237 / 239 us), but two tiles leave a wave a SIMD
 // then (60 drafted rows, 8-bit cache, 150 / 112). Pieces are cut so that all key heads together give a few workgroups for each CU
-// whatever the lengths; their partial outputs are joined by a second launch. Waves join theirs in LDS, in a fixed order.
+// whatever the lengths; their partial outputs are joined by a second launch (by the tile's last
+// workgroup, over agent-scope stores and a counter, it took as long: one row 12.0 us and 12.6, 60 drafted rows 101 and 95). Waves join
+// theirs in LDS, in a fixed order.
 #include <type_traits>
 
 #include "attend.h"
