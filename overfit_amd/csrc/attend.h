@@ -421,6 +421,7 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     CutRequest q = cut_load(c, pool, b, lane);
     float sum = q.sum;
     int tiles = q.tiles, longest = q.blocks;
+#pragma unroll 4
     for (int base = 64; base < b.requests; base += 64) {
         const CutRequest o = cut_load(c, pool, b, base + lane);
         sum += o.sum;

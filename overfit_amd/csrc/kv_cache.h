@@ -111,13 +111,16 @@ __device__ __forceinline__ bool kv_find(int requests, int& item, int& r, int& be
     return false;
 }
 
-// The request that a row belongs to (the first whose rows have it, of at most `most` rows; r -1: none), every wave for itself.
+// The request of at most `most` rows that a row belongs to (r -1: none), every wave for itself.
 struct KvRowPlace {
     int r, place;  // place: the row's token
 };
 __device__ __forceinline__ KvRowPlace kv_row_place(const KvBatch& b, int row, int most) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < b.requests; base += 64) {
+    // from where the row is if every request has one, which is the case that has many of them
+    const int guess = b.requests > 64 ? min(row, b.requests - 1) & ~63 : 0;
+    for (int turn = 0; turn < b.requests + 64; turn += 64) {
+        const int base = turn == 0 ? guess : turn - 64;
         KvRows m{0, 0};
         int len = 0;
         if (base + lane < b.requests) {
@@ -129,6 +132,7 @@ __device__ __forceinline__ KvRowPlace kv_row_place(const KvBatch& b, int row, in
             const int l = __ffsll((unsigned long long)votes) - 1;
             return KvRowPlace{__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readlane(len - m.n + (row - m.first), l)};
         }
+        if (b.requests <= 64) break;
     }
     return KvRowPlace{-1, -1};
 }
