@@ -60,6 +60,8 @@ struct KvMath {
     }
     // Eight fp32 values as kParts operands that add up to them.
     static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&part)[kParts]) {
+        float minus = -1.0f;
+        asm("" : "+v"(minus));  // (a constant would make a conversion and a subtraction of the v_fma_mix below)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             f32x2 v = {x[2 * i], x[2 * i + 1]};
@@ -72,7 +74,7 @@ struct KvMath {
                 } else {
                     const h16x2 h = __builtin_convertvector(v, h16x2);
                     part[p][i] = __builtin_bit_cast(uint32_t, h);
-                    if (p + 1 < kParts) v = f32x2{fmaf((float)h.x, -1.0f, v.x), fmaf((float)h.y, -1.0f, v.y)};  // (v_fma_mix)
+                    if (p + 1 < kParts) v = f32x2{fmaf((float)h.x, minus, v.x), fmaf((float)h.y, minus, v.y)};
                 }
             }
         }
