@@ -157,19 +157,33 @@ struct Plan {
     unsigned items, tiles;  // most of a key head
 };
 
-// One kernel a call: the few-column one where no request has more columns than it takes, else the other for all of them. (Its tiles
-// waste three waves of four on a decode step's columns, but read their keys as fast; a launch of each cost batches without such
-// requests 13 us for nothing.)
-Plan plan_attend(const AttendArgs& a) {
-    const int group = a.heads / a.pool.kv_heads;
-    const int64_t most = (int64_t)a.batch.most * group;
-    const int requests = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
+// Which kernels a call takes: the few-column one where no request has more columns than it takes; else the other one, and the first
+// beside it for the requests that it takes if the rows behind the longest request's are that few for each (a decode step with a chunk of a
+// prompt in it: 512 rows over 8 k beside 31 single ones 341 us, all of them in the many-column kernel 457, where they waste three
+// waves of four). A launch for nothing costs 13 us with its join, so prompts alone have one.
+struct Kinds {
+    bool few, many;
+};
+Kinds kinds_of(const AttendArgs& a) {
+    const int64_t group = a.heads / a.pool.kv_heads, few = few_columns(a);
+    if (a.batch.most * group <= few) return Kinds{true, false};
+    return Kinds{a.batch.requests > 1 && group <= few && (a.batch.rows - a.batch.most) * group <= (a.batch.requests - 1) * few, true};
+}
+
+Plan plan_attend(const AttendArgs& a, bool few) {
+    const Kinds kinds = kinds_of(a);
+    const int group = a.heads / a.pool.kv_heads, requests = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
     Plan p{};
-    p.few = most <= few_columns(a);
+    p.few = few;
     p.split = true;
-    const int log2 = p.few ? (most <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
-    p.cut = Cut{log2, 1, (int)most, ceil_div(kItems, a.pool.kv_heads), p.few ? 8 : 16, p.few ? 2.0f : 1.5f, a.window, group, 0, 0};
-    p.tiles = (unsigned)(p.few ? requests : (((int64_t)a.batch.rows * group) >> log2) + requests);
+    int64_t most = (int64_t)a.batch.most * group;
+    if (few && most > few_columns(a)) most = few_columns(a);
+    // columns of a tile: 16 or 32, by the requests' most or, beside the other kernel, their mean
+    const int64_t usual = kinds.many ? (int64_t)(a.batch.rows - a.batch.most) * group / (requests > 1 ? requests - 1 : 1) : most;
+    const int log2 = few ? (usual <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
+    const int least = !few && kinds.few ? few_columns(a) + 1 : 1;
+    p.cut = Cut{log2, least, (int)most, ceil_div(kItems, a.pool.kv_heads), few ? 8 : 16, few ? 2.0f : 1.5f, a.window, group, 0, 0};
+    p.tiles = (unsigned)(few ? requests * ceil_div(most, 1 << log2) : (((int64_t)a.batch.rows * group) >> log2) + requests);
     // Pieces are no longer than the mean by more than `slack`, and the sum of the tiles' lengths that it comes from is half of their number
     // times the longest at least: so many pieces at most, and so many of tiles that are cut.
     p.items = p.tiles + 2 * (unsigned)p.cut.target + 2;
@@ -192,18 +206,25 @@ AttendArgs with_scratch(const AttendArgs& a, const Plan& p) {
 }  // namespace
 
 size_t attend_scratch(const AttendArgs& a) {
-    const Plan p = plan_attend(a);
-    return part_bytes(a, p) + plan_bytes(p);
+    const Kinds kinds = kinds_of(a);
+    const Plan few = plan_attend(a, true), many = plan_attend(a, false);
+    return (kinds.few ? part_bytes(a, few) + plan_bytes(few) : 0) + (kinds.many ? part_bytes(a, many) + plan_bytes(many) : 0);
 }
 
 hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
-    const Plan p = plan_attend(a);
-    const AttendArgs m = with_scratch(a, p);
+    const Kinds kinds = kinds_of(a);
+    AttendArgs m = a;
     hipError_t e = hipSuccess;
-    if (p.few) {
+    if (kinds.few) {
+        const Plan p = plan_attend(a, true);
+        m = with_scratch(a, p);
         e = launch_attend_few(m, p.cut, p.items, st);
-        return e == hipSuccess ? launch_attend_join(m, p.cut, p.tiles, st) : e;
+        if (e == hipSuccess) e = launch_attend_join(m, p.cut, p.tiles, st);
+        if (e != hipSuccess || !kinds.many) return e;
+        m.parts = (float*)((char*)a.parts + part_bytes(a, p) + plan_bytes(p));
     }
+    const Plan p = plan_attend(a, false);
+    m = with_scratch(m, p);
     const unsigned grid = p.items * (unsigned)a.pool.kv_heads;
     auto go = [&](auto type, auto dp) {
         constexpr int kType = decltype(type)::value, kDp = decltype(dp)::value;

@@ -54,6 +54,7 @@ def test_lengths(length):
     ((1,) * 70, tuple(range(70))),          # more requests than lanes
     ((2, 9, 1, 40, 17), (300, 0, 1000, 64, 5)),  # both kernels in one call
     ((5,) * 9, (0, 1, 30, 31, 32, 33, 400, 800, 64)),
+    ((1, 1, 8, 1, 1, 40), (500, 0, 700, 3, 90, 200)),  # a request of two 16-column tiles between single rows and many
 ])
 @pytest.mark.parametrize("hint", [True, False])
 def test_batches(counts, contexts, hint):
