@@ -430,8 +430,8 @@ typedef struct ovfq_rope {
 /* New tokens into the cache: k and v [rows][kv_heads * head_dim], k turned by its position and both rounded to the cache's type; q
  * [rows][heads * head_dim] turned by the same angles into q_out (which may be q). q may be NULL (keys and values only), or k and v
  * (queries only). rope NULL: nothing is turned (q then has no place here). positions [axes][rows]; NULL: each token's place in its request,
- * on every axis. Angles are fp64, cosines and sines fp32, the rotation single fp32 operations. Tables of different requests must not share
- * pages that the call writes. Where the cache keeps sums, a page's is taken when its last token is appended. Not more rows than 65536, nor
+ * on every axis. Angles are fp64, cosines and sines fp32, the rotation single fp32 operations. No page that the call writes may be listed
+ * twice. Where the cache keeps sums, a page's is taken when its last token is appended. Not more rows than 65536, nor
  * rows * kv_heads than OVFQ_MAX_ATTEND_ROWS. Host pointers (also in the structures), synchronous. */
 #define OVFQ_MAX_ATTEND_ROWS (1 << 22)
 OVFQ_API int ovfq_kv_append(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
@@ -440,7 +440,7 @@ OVFQ_API int ovfq_kv_append(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* bat
  * The host form refuses offsets that do not start at 0, fall or do not end at rows, more rows than max_rows, lengths below a request's rows
  * or past its table, pages outside the cache, and pages that two requests of the call would write. Here a request whose offsets fall or
  * leave the rows has no rows; rows of no request are left as they were; a token before the first, past the table or in a page outside the
- * cache is not stored (its query is turned all the same). Offsets of different requests must not overlap. */
+ * cache is not stored (its query is turned all the same). Offsets of different requests must not overlap, nor q_out k, v or (without being it) q. */
 OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
                                 const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out);
 
@@ -453,7 +453,7 @@ OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch*
  * is left out (its rows of `out` stay as they were), and offsets count as there. Host pointers, synchronous. */
 OVFQ_API int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
                          float scale, int window, float* out);
-/* As ovfq_attend, with device pointers (enqueued on the context's stream). */
+/* As ovfq_attend, with device pointers (enqueued on the context's stream); out must not overlap q. */
 OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
                              float scale, int window, float* out);
 
@@ -465,7 +465,7 @@ OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_bat
 #define OVFQ_MAX_TOP_PAGES 4096
 OVFQ_API int ovfq_attend_selected(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
                                   int heads, float scale, int top_pages, float* out, int* pages);
-/* As ovfq_attend_selected, with device pointers (enqueued on the context's stream). */
+/* As ovfq_attend_selected, with device pointers (enqueued on the context's stream); out must not overlap q. */
 OVFQ_API int ovfq_attend_selected_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
                                       int heads, float scale, int top_pages, float* out, int* pages);
 

@@ -156,6 +156,11 @@ def _rows_of(x, width, name):
     return x.size // width
 
 
+def _overlap(a, b):
+    """Whether two planes of fp32 values share memory."""
+    return a is not None and b is not None and a.ptr < b.ptr + 4 * b.size and b.ptr < a.ptr + 4 * a.size
+
+
 def _batch(row_offsets, lengths, tables, max_rows):
     """(ovfq_kv_batch, its buffers)."""
     ob = as_buf(row_offsets, np.int32, "row_offsets")
@@ -199,7 +204,7 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
         if rope is None:
             raise OverfitArgumentNullError("q without a rope")
         if not rows:
-            rows = int(q.shape[0])
+            rows = int(q.shape[0]) if len(q.shape) > 1 else 1
         if rows <= 0 or qb.size == 0 or qb.size % (rows * cache.head_dim):
             raise OverfitArgumentError(f"q has {qb.size} elements, not whole heads of {cache.head_dim} for each of {rows} rows")
         heads = qb.size // (rows * cache.head_dim)
@@ -211,8 +216,9 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
         raise OverfitArgumentNullError("q_out without q")
     yb = _sized(as_buf(q_out, np.float32, "q_out", allow_none=True), rows * heads * cache.head_dim, "q_out")
     side += [kb, vb, qb, yb]
-    if kb is not None and vb is not None and yb is not None and yb.ptr in (kb.ptr, vb.ptr):
-        raise OverfitArgumentError("q_out is k's or v's plane")
+    for name, b in (("k", kb), ("v", vb), ("q", qb)):
+        if _overlap(yb, b) and not (b is qb and yb.ptr == qb.ptr):
+            raise OverfitArgumentError(f"q_out overlaps {name}")
     rs = pb = None
     if rope is not None:
         if not isinstance(rope, Rope):
@@ -263,8 +269,8 @@ def _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max
     if out is None:
         out = _empty(qb, qb.size).reshape(tuple(q.shape))
     ob = _sized(as_buf(out, np.float32, "out"), qb.size, "out")
-    if ob.ptr == qb.ptr:
-        raise OverfitArgumentError("out is q's plane")
+    if _overlap(ob, qb):
+        raise OverfitArgumentError("out overlaps q")
     side += [qb, ob]
     args = (ctypes.byref(batch), qb.ptr, rows, heads, scale)
     if top is None:

@@ -1944,6 +1944,12 @@ static int check_kv_call(const ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_b
     return OVFQ_OK;
 }
 
+// Planes of floats that a kernel reads and writes at once must be apart.
+static bool overlap(const float* a, size_t a_bytes, const float* b, size_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 static int check_heads(const ovfq_kv* kv, int rows, int heads) {
     if (heads <= 0) return fail(OVFQ_ERR_RANGE, "heads (%d) must be positive", heads);
     if (heads % kv->pool.kv_heads) return fail(OVFQ_ERR_SIZE, "heads (%d) must be a multiple of kv_heads (%d)", heads, kv->pool.kv_heads);
@@ -1993,10 +1999,15 @@ static int kv_append_impl(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch
     }
     if (!host && (rc_align(k) || rc_align(v) || rc_align(q) || rc_align(q_out) || rc_align(positions)))
         return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
-    std::lock_guard<std::mutex> lk(ctx->mu);
-    HIP_TRY(hipSetDevice(ctx->device));
     const size_t R = (size_t)rows, Q = (size_t)batch->requests, half = rope ? (size_t)rope->rotary_dim / 2 : 0;
     const size_t key_bytes = R * p.kv_heads * p.dim * 4, query_bytes = R * (size_t)heads * p.dim * 4;
+    if (!host && q_out) {
+        if (overlap(q_out, query_bytes, k, key_bytes) || overlap(q_out, query_bytes, v, key_bytes) ||
+            (q_out != q && overlap(q_out, query_bytes, q, query_bytes)))
+            return fail(OVFQ_ERR_SIZE, "q_out overlaps k, v or, without being it, q");
+    }
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    HIP_TRY(hipSetDevice(ctx->device));
     const void* in[9] = {batch->row_offsets, batch->lengths, batch->tables, k, v, q, positions, rope ? rope->inv_freq : nullptr,
                          rope ? rope->pair_axes : nullptr};
     const size_t bytes[9] = {(Q + 1) * 4, Q * 4, Q * batch->table_width * 4, key_bytes, key_bytes, query_bytes,
@@ -2071,12 +2082,15 @@ static int attend_impl(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* ba
         if ((rc = check_plane((int64_t)rows * p.kv_heads, top, "pages")) ||
             (rc = check_plane((int64_t)rows * p.kv_heads, batch->table_width, "fits")))
             return rc;
+        if ((int64_t)rows * p.kv_heads * ((heads / p.kv_heads + 15) / 16) >= 1 << 24)
+            return fail(OVFQ_ERR_SIZE, "rows (%d) with %d heads above 2^24 - 1 groups of 16", rows, heads);
     }
+    const size_t R = (size_t)rows, Q = (size_t)batch->requests, plane = R * heads * p.dim * 4, list = R * p.kv_heads * top * 4;
     if (!host && (rc_align(q) || rc_align(out) || rc_align(pages)))
         return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
+    if (!host && overlap(out, plane, q, plane)) return fail(OVFQ_ERR_SIZE, "out overlaps q");
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
-    const size_t R = (size_t)rows, Q = (size_t)batch->requests, plane = R * heads * p.dim * 4, list = R * p.kv_heads * top * 4;
     const void* in[4] = {batch->row_offsets, batch->lengths, batch->tables, q};
     const size_t bytes[4] = {(Q + 1) * 4, Q * 4, Q * batch->table_width * 4, plane};
     ovfq::AttendArgs a{};

@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
 }  // namespace
 
 // Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l, in a fixed order. A workgroup per 16 columns of a tile,
-// key head and 16 channels * `wide` (blockIdx.y): a thread has a column that is used and four channels, and what is left of the
+// key head and 16 channels * `wide` (blockIdx.y; blockIdx.z: the tiles past what x takes): a thread has a column that is used and four channels, and what is left of the
 // workgroup's threads shares the pieces.
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, int wide) {
     __shared__ float tops[16][16], ls[16][16];
@@ -274,8 +274,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut,
     const KvPool& pool = a.pool;
     const int subs = 1 << (cut.cols_log2 - 4), cols = 16 * subs, tid = threadIdx.x;
     const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads);
-    const int item = (int)(blockIdx.x / (unsigned)pool.kv_heads), index = item / subs, sub = item - index * subs;
-    if (index >= (a.where ? a.batch.rows * ((cut.group + 15) >> 4) : cut_count(cut, a.batch))) return;
+    const int item = (int)((blockIdx.x + blockIdx.z * gridDim.x) / (unsigned)pool.kv_heads), index = item / subs, sub = item - index * subs;
+    const int count = a.where ? a.batch.rows * ((cut.group + 15) >> 4) : cut_count(cut, a.batch);
+    if (index >= count || count > cut.tiles) return;  // (more than the launch's: offsets that overlap, the call's tiles are left)
     if (a.where && a.where[index / ((cut.group + 15) >> 4)] < 0) return;
     const TilePlan w = a.plans[index];
     // (a plan that nothing wrote, for offsets that overlap, must not lead out of the planes)
@@ -370,9 +371,10 @@ hipError_t launch_attend_few(const AttendArgs& a, const Cut& cut, unsigned items
 }
 
 hipError_t launch_attend_join(const AttendArgs& a, const Cut& cut, unsigned tiles, hipStream_t st) {
-    const unsigned x = (tiles << (cut.cols_log2 - 4)) * (unsigned)a.pool.kv_heads, all = (unsigned)a.pool.dp >> 4;
+    const unsigned heads = (unsigned)a.pool.kv_heads, most = (1u << 20) / heads, subs = tiles << (cut.cols_log2 - 4);
+    const unsigned x = (subs < most ? subs : most) * heads, z = (subs + most - 1) / most, all = (unsigned)a.pool.dp >> 4;
     const unsigned wide = x >= 512 ? all : x >= 128 ? 2 : 1;  // few tiles: their channels over several workgroups
-    attend_join_kernel<<<dim3(x, (all + wide - 1) / wide), 256, 0, st>>>(a, cut, a.pool.dp, (int)wide);
+    attend_join_kernel<<<dim3(x, (all + wide - 1) / wide, z), 256, 0, st>>>(a, cut, a.pool.dp, (int)wide);
     return hipGetLastError();
 }
 

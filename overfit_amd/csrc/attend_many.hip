@@ -1,7 +1,7 @@
 // attend_many.hip — attention of many columns (prompts, chunks of them) over a paged cache. Arithmetic: attend.h.
 //
 // Bound: MFMA, 4 D flops per (column, token) times the parts that q and p are split in (two fp16, three bf16), beside the softmax's
-// vector work. Four waves of 16 kTiles16 columns each share a tile; a block's keys and values go to LDS once for all of them, by DMA in
+// vector work. Four waves of 16 kCols columns each share a tile; a block's keys and values go to LDS once for all of them, by DMA in
 // the operand order that they have in memory (reads of it are 1 KiB in a row, free of conflicts), one block ahead. Workgroups of one
 // key head come to one XCD where the head count allows, so its blocks are read from HBM once.
 #include <type_traits>
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
                 }
             }
         }
-        if (page >= 0 && live && first <= last_last && first + kKvBlock > first_low) {
+        if (page >= 0 && live && first <= last_last && first + (kKvBlock - 1) >= first_low) {
             const char* at = ring[i & 1] + lane * 16;
             f32x4 ks[2] = {}, vs[2] = {};
             if constexpr (kType == kKvI8) {

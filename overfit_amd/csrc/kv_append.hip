@@ -152,14 +152,16 @@ __device__ __forceinline__ uint16_t rounded(float v) {
 }
 
 // A token's scale in an int8 cache: absmax / 127 over its head's channels, which `lanes` neighbouring lanes hold (the channels past dim
-// are zeros). `top`: the largest bits of the lane's magnitudes, which are ordered like them, NaN above all.
+// are zeros). `top`: the largest bits of the lane's magnitudes, which are ordered like them, NaN above all. A scale too small for its
+// reciprocal (a head below 4e-37) is taken as zero.
 struct Scaled {
     float scale, inv;
 };
 __device__ __forceinline__ Scaled token_scale(uint32_t top, int lanes) {
     for (int off = lanes / 2; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-    const float scale = as_float(top) / 127.0f;
-    return Scaled{scale, scale > 0.0f ? 1.0f / scale : 0.0f};
+    const float scale = as_float(top) / 127.0f, inv = 1.0f / scale;
+    if (scale >= 0.0f && !(inv < __builtin_inff())) return Scaled{0.0f, 0.0f};
+    return Scaled{scale, inv};
 }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, fabsf(v)); }
 __device__ __forceinline__ uint32_t quant(float v, float inv) {

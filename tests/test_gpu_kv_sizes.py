@@ -1,0 +1,105 @@
+"""Paged caches at their largest batches and smallest values, and planes that overlap."""
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+ov = pytest.importorskip("overfit_amd")
+from overfit_amd import _lib  # noqa: E402
+from kvdata import DEV, Requests, attention, case, check  # noqa: E402
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def test_many_requests_of_many_heads():
+    """Tiles by the million: no launch's threads pass 32 bits."""
+    requests, kv_heads = 33000, 64
+    case("requests", requests, "kv_heads", kv_heads)
+    cache = ov.KvCache(kv_heads, 8, 32, 64)
+    v = torch.randn(64, kv_heads * 8, device=DEV)
+    ov.kv_append(cache, v, v, torch.arange(65, dtype=torch.int32, device=DEV), i32([1] * 64), torch.arange(64, dtype=torch.int32, device=DEV)[:, None].contiguous())
+    pages = torch.arange(requests, dtype=torch.int32, device=DEV) % 64
+    off, lengths = torch.arange(requests + 1, dtype=torch.int32, device=DEV), torch.ones(requests, dtype=torch.int32, device=DEV)
+    q = torch.randn(requests, kv_heads * 8, device=DEV)
+    for most in (0, 1):
+        got = ov.attend(cache, q, off, lengths, pages[:, None].contiguous(), max_rows=most)  # each sees the first token of its page alone
+        assert torch.allclose(got, v.half().float()[pages.long()], rtol=1e-6, atol=1e-7)
+
+
+@pytest.mark.parametrize("counts,contexts", [((1300,), (700,)), ((650, 1, 640), (0, 5000, 900))])
+def test_more_tiles_than_joins(counts, contexts):
+    """Pieces of more tiles than the workgroups that join them."""
+    case("joins", counts)
+    rng = np.random.default_rng(8)
+    req = Requests(ov, rng, "f16", 8, 64, 64, counts, contexts).fill()
+    q = rng.standard_normal((req.rows, 32 * 64)).astype(np.float32)
+    out = ov.attend(req.cache, req.t(q), *req.batch()).cpu().numpy()
+    heads = [0, 7]
+    part = Requests.__new__(Requests)
+    part.__dict__.update(req.__dict__, kv_heads=2, k=[k[:, heads] for k in req.k], v=[v[:, heads] for v in req.v])
+    pick = lambda x: x.reshape(req.rows, 8, 4 * 64)[:, heads].reshape(req.rows, -1)  # noqa: E731
+    check(pick(out), *attention(part, pick(q), 8))
+
+
+@pytest.mark.parametrize("size", [1e-44, 1e-40, 1e-37, 3e-37, 5e-37, 1e-30])
+def test_smallest_values(size):
+    """8-bit heads whose scale has no reciprocal are zeros; above, their quants are those of larger ones."""
+    rng = np.random.default_rng(9)
+    x = (rng.uniform(-1, 1, (40, 64)) * size).astype(np.float32)
+    x[:, 3], x[:, 5] = np.float32(size), 0
+    cache = ov.KvCache(1, 64, 64, 1, ov.TYPE_I8)
+    t = torch.from_numpy(x).to(DEV)
+    ov.kv_append(cache, t, t, i32([0, 40]), i32([40]), i32([[0]]))
+    keys = cache.key_view().reshape(64, 64)[:40].cpu().numpy().astype(np.float64) - 128
+    values = cache.value_view().reshape(64, 64)[:40].cpu().numpy().astype(np.float64) - 128
+    scales = cache.scale_view().reshape(2, 2, 32).permute(1, 0, 2).reshape(2, 64, 1)[:, :40].cpu().numpy().astype(np.float64)
+    # a quant is off by half a step and the scale's and its reciprocal's roundings over 127 steps; a head of zeros by its values
+    bound = np.where(scales > 0, scales * (0.5 + 127 * 3 * 2.0 ** -24), 127 / 2.0 ** 128 * 1.01)
+    for got, s, b in ((keys, scales[0], bound[0]), (values, scales[1], bound[1])):
+        assert np.all(np.abs(got * s - x) <= b)
+        assert np.all(got[:, 5] == 0)
+    assert np.all(scales > 0) == (size > 4e-37)
+
+
+def test_planes_that_overlap():
+    cache = ov.KvCache(2, 16, 32, 4, sums=True)
+    ctx, lib = cache.context, cache.context.lib
+    mem = torch.zeros(1000, device=DEV)
+    f = mem.data_ptr()
+    off, lengths, table = i32([0, 3]), i32([3]), i32([[0]])
+    batch = _lib.KvBatchStruct(1, 1, 0, off.data_ptr(), lengths.data_ptr(), table.data_ptr())
+    freq = torch.ones(8, device=DEV)
+    rope = _lib.RopeStruct(16, 0, 1, 1.0, freq.data_ptr(), None)
+    q_bytes, k_bytes = 3 * 4 * 16 * 4, 3 * 2 * 16 * 4
+
+    def append(k, v, q, out):
+        return lib.ovfq_kv_append_dev(ctx.handle, cache.handle, ctypes.byref(batch), k, v, 3, ctypes.byref(rope), None, q, 4, out)
+
+    k, v = f + q_bytes, f + q_bytes + k_bytes
+    assert append(k, v, f, f) == _lib.OVFQ_OK
+    assert append(k, v, f, f + 4) == _lib.OVFQ_ERR_SIZE
+    assert append(k, v, f + 2000, f + 8) == _lib.OVFQ_ERR_SIZE  # into k
+    assert append(f + 2000, k, f + 3000, f + 4) == _lib.OVFQ_ERR_SIZE  # into v
+    assert append(f + 2000, v, v + k_bytes, f + q_bytes - 4) == _lib.OVFQ_ERR_SIZE
+    for out, want in ((f, _lib.OVFQ_ERR_SIZE), (f + q_bytes - 4, _lib.OVFQ_ERR_SIZE), (f + q_bytes, _lib.OVFQ_OK)):
+        assert lib.ovfq_attend_dev(ctx.handle, cache.handle, ctypes.byref(batch), f, 3, 4, 1.0, 0, out) == want
+        assert lib.ovfq_attend_selected_dev(ctx.handle, cache.handle, ctypes.byref(batch), f, 3, 4, 1.0, 2, out, None) == want
+    torch.cuda.synchronize()
+    with pytest.raises(ov.OverfitArgumentError):
+        ov.attend(cache, mem[:192].view(3, 64), off, lengths, table, out=mem[4:196].view(3, 64))
+
+
+def test_one_row_without_its_axis():
+    """A single row's queries as a vector."""
+    cache = ov.KvCache(2, 16, 32, 1)
+    rope = ov.Rope(torch.ones(8, device=DEV))
+    q = torch.randn(64, device=DEV)
+    batch = (i32([0, 1]), i32([5]), i32([[0]]))
+    got = ov.kv_append(cache, None, None, *batch, q=q, rope=rope)
+    assert got.shape == q.shape and torch.equal(got, ov.kv_append(cache, None, None, *batch, q=q[None], rope=rope)[0])
+    assert ov.attend(cache, got, *batch).shape == q.shape

@@ -170,3 +170,20 @@ def test_entry_points_refuse_null():
         assert fn(None, None, ctypes.byref(b), None, 1, 1, 1.0, 0, None) == _lib.OVFQ_ERR_NULL
     for fn in (lib.ovfq_attend_selected, lib.ovfq_attend_selected_dev):
         assert fn(None, None, ctypes.byref(b), None, 1, 1, 1.0, 4, None, None) == _lib.OVFQ_ERR_NULL
+
+
+@pytest.mark.parametrize("at", [0, 1, 95])
+def test_outputs_that_overlap_inputs(at):
+    mem = np.zeros(400, F)
+    with pytest.raises(ov.OverfitArgumentError):
+        ov.attend(loose_cache(), mem[:96].reshape(3, 32), **BATCH, out=mem[at:at + 96].reshape(3, 32))
+    call = dict(BATCH, k=mem[:48], v=np.zeros(48, F), q=np.zeros((3, 16), F), rope=ov.Rope(np.ones(4, F)))
+    with pytest.raises(ov.OverfitArgumentError):
+        ov.kv_append(loose_cache(), **call, q_out=mem[at // 2:at // 2 + 48].reshape(3, 16))
+    call["k"], call["v"] = call["v"], call["k"]
+    with pytest.raises(ov.OverfitArgumentError):
+        ov.kv_append(loose_cache(), **call, q_out=mem[at // 2:at // 2 + 48].reshape(3, 16))
+    if at:
+        call.update(v=np.zeros(48, F), q=mem[:48].reshape(3, 16))
+        with pytest.raises(ov.OverfitArgumentError):
+            ov.kv_append(loose_cache(), **call, q_out=mem[at // 4 + 1:at // 4 + 49].reshape(3, 16))
