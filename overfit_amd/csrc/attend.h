@@ -372,6 +372,17 @@ struct Cut {
     float slack;
     int window, group;
     int slots, tiles;  // most of a key head's partial outputs, and of its tiles
+    int planned;       // the requests' items are counted by a launch of their own (AttendArgs::plan holds them)
+};
+// A launch's tiles that the join has to look at (none if all are whole), and where the items were counted before: one over a piece's
+// size, and the items, tiles and slots of each 64 requests.
+struct CutPlan {
+    int joins, tiles;
+    float inv;
+    int unused;
+};
+struct CutChunk {
+    int items, tiles, slots, unused;
 };
 // What the join needs to know of a tile, written by the tile's first piece.
 struct TilePlan {
@@ -417,44 +428,63 @@ __device__ __forceinline__ CutRequest cut_load(const Cut& c, const KvPool& pool,
     return q;
 }
 
-// Item `item` of a key head; false past the last one. Every wave finds it for itself: lanes hold 64 requests at a time.
-__device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, int item, TileWork& w) {
+// Blocks of a piece, from all requests' sum of blocks and number of tiles, before it is fitted to the number of workgroups.
+__device__ __forceinline__ float cut_piece(const Cut& c, float sum, int tiles) {
+    return fmaxf(ceilf(sum / (float)c.target * (tiles >= c.target ? c.slack : 1.0f)), (float)c.least_blocks);
+}
+// A request's items, its tiles taken as long as the longest of them, and its slots: whole tiles have none.
+__device__ __forceinline__ int2 cut_items(const CutRequest& q, float inv) {
+    const int items = q.tiles * cut_pieces(q.blocks, inv);
+    return make_int2(items, items > q.tiles ? items : 0);
+}
+
+// Item `item` of a key head; false past the last one. Every wave finds it for itself: lanes hold 64 requests at a time, or in a planned
+// launch 64 times 64 of them and then the item's.
+__device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, CutPlan* plan, int item, TileWork& w) {
     const int lane = threadIdx.x & 63;
-    CutRequest q = cut_load(c, pool, b, lane);
-    float sum = q.sum;
-    int tiles = q.tiles, longest = q.blocks;
-#pragma unroll 4
-    for (int base = 64; base < b.requests; base += 64) {
-        const CutRequest o = cut_load(c, pool, b, base + lane);
-        sum += o.sum;
-        tiles += o.tiles;
-        longest = max(longest, o.blocks);
-    }
-    sum = wave_sum(sum);
-    tiles = wave_sum(tiles);
-    longest = wave_max(longest);
-    if (tiles > c.tiles) return false;  // offsets that overlap: none of the call's tiles
-    const float mean = sum / (float)c.target;
-    float piece = fmaxf(ceilf(mean * (tiles >= c.target ? c.slack : 1.0f)), (float)c.least_blocks);
-    if (tiles < c.target && b.requests <= 64 && (float)longest > piece) {
-        // halving what lies between the mean, which may give too many, and the longest tile
-        float over = piece;
-        if (wave_sum(q.tiles * cut_pieces(q.blocks, 1.0f / piece)) > c.target) {
-            piece = (float)longest;
-            for (int i = 0; i < 5 && piece - over > 1.0f; i++) {
-                const float half = floorf(0.5f * (piece + over));
-                if (wave_sum(q.tiles * cut_pieces(q.blocks, 1.0f / half)) > c.target)
-                    over = half;
-                else
-                    piece = half;
+    CutRequest q;
+    float inv;
+    int tiles = 0, longest = 0;
+    if (c.planned) {
+        if (!uniform(plan->tiles)) return false;
+        inv = as_float((uint32_t)uniform((int)__builtin_bit_cast(uint32_t, plan->inv)));
+    } else {
+        q = cut_load(c, pool, b, lane);
+        float sum = q.sum;
+        tiles = q.tiles, longest = q.blocks;
+        for (int base = 64; base < b.requests; base += 64) {
+            const CutRequest o = cut_load(c, pool, b, base + lane);
+            sum += o.sum;
+            tiles += o.tiles;
+            longest = max(longest, o.blocks);
+        }
+        sum = wave_sum(sum);
+        tiles = wave_sum(tiles);
+        longest = wave_max(longest);
+        float piece = cut_piece(c, sum, tiles);
+        if (tiles < c.target && b.requests <= 64 && (float)longest > piece) {
+            // halving what lies between the mean, which may give too many, and the longest tile
+            float over = piece;
+            if (wave_sum(cut_items(q, 1.0f / piece).x) > c.target) {
+                piece = (float)longest;
+                for (int i = 0; i < 5 && piece - over > 1.0f; i++) {
+                    const float half = floorf(0.5f * (piece + over));
+                    if (wave_sum(cut_items(q, 1.0f / half).x) > c.target)
+                        over = half;
+                    else
+                        piece = half;
+                }
             }
         }
+        inv = as_float((uint32_t)uniform((int)__builtin_bit_cast(uint32_t, 1.0f / piece)));
+        const bool fit = tiles <= c.tiles;  // (if not, offsets overlap: none of the call's tiles)
+        if (blockIdx.x == 0 && threadIdx.x == 0) plan->joins = fit && cut_pieces(longest, inv) > 1 ? tiles : 0;
+        if (!fit) return false;
     }
-    const float inv = as_float((uint32_t)uniform((int)__builtin_bit_cast(uint32_t, 1.0f / piece)));
     int l = 0, before = 0, tiles_before = 0, slots_before = 0;
     w.piece = 0;
     w.r = 0;
-    if (b.requests <= 64 && cut_pieces(longest, inv) == 1) {
+    if (!c.planned && b.requests <= 64 && cut_pieces(longest, inv) == 1) {
         if (item >= tiles) return false;
         // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
         const int base = (int)min(max(((int64_t)q.place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
@@ -480,26 +510,44 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
         w.slot = 0;
         w.tile_index = item;
     } else {
-        for (int base = 0;; base += 64) {
-            if (base >= b.requests) return false;
-            if (base) q = cut_load(c, pool, b, base + lane);
-            const int mine = q.tiles * cut_pieces(q.blocks, inv);
-            const int slots = mine > q.tiles ? mine : 0;  // whole tiles have none
-            const int upto = wave_upto(mine), tiles_upto = wave_upto(q.tiles), slots_upto = wave_upto(slots);
+        // of 64 sums at a time (a lane's items, tiles and slots) the one that `item` falls into
+        auto found = [&](int items, int its_tiles, int slots) {
+            const int upto = wave_upto(items), tiles_upto = wave_upto(its_tiles), slots_upto = wave_upto(slots);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item >= before + all) {
                 before += all;
                 tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
                 slots_before += __builtin_amdgcn_readlane(slots_upto, 63);
-                continue;
+                return false;
             }
             l = __ffsll((unsigned long long)__ballot(before + upto > item)) - 1;
-            w.r = base + l;
-            before += __builtin_amdgcn_readlane(upto - mine, l);
-            tiles_before += __builtin_amdgcn_readlane(tiles_upto - q.tiles, l);
+            before += __builtin_amdgcn_readlane(upto - items, l);
+            tiles_before += __builtin_amdgcn_readlane(tiles_upto - its_tiles, l);
             slots_before += __builtin_amdgcn_readlane(slots_upto - slots, l);
-            break;
+            return true;
+        };
+        int first = 0;
+        if (c.planned) {
+            const CutChunk* chunks = (const CutChunk*)(plan + 1);
+            const int count = (b.requests + 63) >> 6;
+            for (int base = 0;; base += 64) {
+                if (base >= count) return false;
+                const CutChunk s = base + lane < count ? chunks[base + lane] : CutChunk{0, 0, 0, 0};
+                if (found(s.items, s.tiles, s.slots)) {
+                    first = 64 * (base + l);
+                    break;
+                }
+            }
+            q = cut_load(c, pool, b, first + lane);
         }
+        for (;; first += 64) {
+            if (first >= b.requests) return false;
+            if (first && !c.planned) q = cut_load(c, pool, b, first + lane);
+            const int2 mine = cut_items(q, inv);
+            if (found(mine.x, q.tiles, mine.y)) break;
+            if (c.planned) return false;
+        }
+        w.r = first + l;
         const int pieces = uniform(cut_pieces(__builtin_amdgcn_readlane(q.blocks, l), inv));
         const int nth = uniform((item - before) / pieces);
         w.piece = item - before - nth * pieces;
@@ -519,16 +567,6 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     if (w.slot + w.pieces > c.slots && w.pieces > 1) return false;
     return w.piece < w.pieces;
 }
-// All tiles of a launch's requests.
-__device__ __forceinline__ int cut_count(const Cut& c, const KvBatch& b) {
-    int tiles = 0;
-    for (int r = threadIdx.x & 63; r < b.requests; r += 64) {
-        const int cols = kv_rows(b, r).n * c.group;
-        if (cols && cols >= c.least && cols <= c.most) tiles += ((cols - 1) >> c.cols_log2) + 1;
-    }
-    return wave_sum(tiles);
-}
-
 // A walk over blocks first, first + step, ..: their pages in 64 lanes at a time.
 struct BlockWalk {
     const int* table;  // the request's

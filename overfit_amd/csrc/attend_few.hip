@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
         w.block0 = w.piece * each;
         w.block1 = min(blocks, w.block0 + each);
     } else {
-        if (!cut_item(cut, pool, b, item, w)) return;
+        if (!cut_item(cut, pool, b, a.plan, item, w)) return;
     }
     if (a.plans && threadIdx.x == 0 && w.piece == 0 && head == 0) a.plans[w.tile_index] = w;
     Att att;
@@ -266,8 +266,8 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
 }  // namespace
 
 // Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l, in a fixed order. A workgroup per 16 columns of a tile,
-// key head and 16 channels * `wide` (blockIdx.y; blockIdx.z: the tiles past what x takes): a thread has a column that is used and four channels, and what is left of the
-// workgroup's threads shares the pieces.
+// key head and 16 channels * `wide` (blockIdx.y; blockIdx.z: the tiles past what x takes): a thread has a column that is used and four
+// channels, and what is left of the workgroup's threads shares the pieces.
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, int wide) {
     __shared__ float tops[16][16], ls[16][16];
     __shared__ f32x4 part_o[256];
@@ -275,10 +275,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut,
     const int subs = 1 << (cut.cols_log2 - 4), cols = 16 * subs, tid = threadIdx.x;
     const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads);
     const int item = (int)((blockIdx.x + blockIdx.z * gridDim.x) / (unsigned)pool.kv_heads), index = item / subs, sub = item - index * subs;
-    const int count = a.where ? a.batch.rows * ((cut.group + 15) >> 4) : cut_count(cut, a.batch);
-    if (index >= count || count > cut.tiles) return;  // (more than the launch's: offsets that overlap, the call's tiles are left)
-    if (a.where && a.where[index / ((cut.group + 15) >> 4)] < 0) return;
-    const TilePlan w = a.plans[index];
+    const int head_tiles = (cut.group + 15) >> 4;
+    const TilePlan w = a.plans[min(index, cut.tiles - 1)];  // (under way beside the count)
+    if (index >= (a.where ? a.batch.rows * head_tiles : a.plan->joins)) return;
+    if (a.where && a.where[index / head_tiles] < 0) return;
     // (a plan that nothing wrote, for offsets that overlap, must not lead out of the planes)
     if (w.pieces <= 1 || w.slot < 0 || w.slot > cut.slots - w.pieces || w.first_row < 0 || w.rows <= 0 ||
         w.rows > a.batch.rows - w.first_row || w.col0 < 0 || w.col0 >= w.rows * cut.group)

@@ -195,20 +195,28 @@ __device__ __forceinline__ void store_key(const KvPool& p, char* block, int t, i
 
 // The new tokens' values of one block of the cache (at most rows / 32 + 2 a request), a share of its heads: a thread has four channels
 // of the eight tokens that lie together in it, and writes them as one piece each. (Token by token, in the rows' workgroups, a store had
-// a lane's 2 bytes in every 16: 4096 rows 54.6 us, 1297 rows 17.6.)
+// a lane's 2 bytes in every 16: 4096 rows 54.6 us, 1297 rows 17.6.) by_rows: item is a row, and has its block if no row before it has.
 template <int kType>
-__device__ __forceinline__ void append_values(const KvAppendArgs& a, int item, int part) {
+__device__ __forceinline__ void append_values(const KvAppendArgs& a, int item, int part, bool by_rows) {
     const KvPool& p = a.pool;
     const KvBatch& b = a.batch;
     int r = 0, before = 0;
-    const bool any = kv_find(b.requests, item, r, before, [&](int q) {
-        const int n = kv_rows(b, q).n, len = kv_length(b, q), from = max(len - n, 0);
-        return n && len > from ? ((len - 1) / kKvBlock) - from / kKvBlock + 1 : 0;
-    });
-    if (!any) return;
+    if (by_rows) {
+        const KvRowPlace at = kv_row_place(b, item, b.rows);
+        if (at.r < 0 || at.place < 0 || (at.place % kKvBlock && !at.first)) return;
+        r = at.r;
+        item = at.place / kKvBlock;
+    } else {
+        const bool any = kv_find(b.requests, item, r, before, [&](int q) {
+            const int n = kv_rows(b, q).n, len = kv_length(b, q), from = max(len - n, 0);
+            return n && len > from ? ((len - 1) / kKvBlock) - from / kKvBlock + 1 : 0;
+        });
+        if (!any) return;
+        item += max(kv_length(b, r) - kv_rows(b, r).n, 0) / kKvBlock;
+    }
     const KvRows m = kv_rows(b, r);
     const int len = kv_length(b, r), start = len - m.n;  // the first row's token, before the first if negative
-    const int block = max(start, 0) / kKvBlock + item, entry = block / (p.page / kKvBlock);
+    const int block = item, entry = block / (p.page / kKvBlock);
     if (entry >= b.width) return;
     const int page = b.tables[(size_t)r * b.width + entry];
     if (page < 0 || page >= p.pages) return;
@@ -279,11 +287,11 @@ __device__ __forceinline__ void append_values(const KvAppendArgs& a, int item, i
 }
 
 template <int kType, bool kFast>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int parts, int value_blocks, int value_parts) {
+__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int parts, int value_blocks, int value_parts, bool by_rows) {
     __shared__ float cs[2 * kMaxPairs];
     int index = blockIdx.x;
     if (index < value_blocks * value_parts) {
-        append_values<kType>(a, index / value_parts, index % value_parts);
+        append_values<kType>(a, index / value_parts, index % value_parts, by_rows);
         return;
     }
     index -= value_blocks * value_parts;
@@ -354,19 +362,26 @@ __device__ __forceinline__ void load8(const KvPool& p, const char* block, int t,
 }
 
 // The sum of the keys of each page that a call has filled: in fp64 in the order of the tokens, rounded to fp32 once. A workgroup per
-// page that ends among the new tokens (at most rows / page + 1 a request) and key head.
+// page that ends among the new tokens (at most rows / page + 1 a request; by_rows: a workgroup per row) and key head.
 template <int kType>
-__global__ __launch_bounds__(256) void kv_sums_kernel(KvPool p, KvBatch b) {
+__global__ __launch_bounds__(256) void kv_sums_kernel(KvPool p, KvBatch b, bool by_rows) {
     __shared__ double part[256 * 8];
     int item = blockIdx.x, r = 0, before = 0;
-    const bool any = kv_find(b.requests, item, r, before, [&](int q) {
-        const int n = kv_rows(b, q).n, len = kv_length(b, q);
-        const int from = len - n > 0 ? len - n : 0;
-        return n && len > from ? len / p.page - from / p.page : 0;
-    });
-    if (!any) return;
-    const int n = kv_rows(b, r).n, len = kv_length(b, r);
-    const int entry = (len - n > 0 ? len - n : 0) / p.page + item;
+    if (by_rows) {
+        const KvRowPlace at = kv_row_place(b, item, b.rows);
+        if (at.r < 0 || at.place < 0 || (at.place + 1) % p.page) return;
+        r = at.r;
+        item = at.place / p.page;
+    } else {
+        const bool any = kv_find(b.requests, item, r, before, [&](int q) {
+            const int n = kv_rows(b, q).n, len = kv_length(b, q);
+            const int from = len - n > 0 ? len - n : 0;
+            return n && len > from ? len / p.page - from / p.page : 0;
+        });
+        if (!any) return;
+        item += max(kv_length(b, r) - kv_rows(b, r).n, 0) / p.page;
+    }
+    const int entry = item;
     if (entry >= b.width) return;
     const int page = b.tables[(size_t)r * b.width + entry];
     if (page < 0 || page >= p.pages) return;
@@ -410,11 +425,14 @@ hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st) {
     const int rows = a.batch.rows, requests = a.batch.requests < rows ? a.batch.requests : rows, parts = rows < 256 ? 4 : 1;
     // blocks that the new tokens lie in: of n tokens at most n, and at most (n + 62) / 32
     const int64_t blocks = ((int64_t)rows + 62 * (int64_t)requests) / 32;
-    const int value_blocks = !a.k ? 0 : (int)(blocks < rows ? blocks : rows);
+    // One or two rows a request: a row is found by search, a block or a page by a walk over the requests (4096 requests of one row 80 us by
+    // rows and 180 by blocks, with sums 97 and 870; of four, 1024 requests 78 and 61, 201 and 132).
+    const bool by_rows = rows <= 2 * requests;
+    const int value_blocks = !a.k ? 0 : (int)(blocks < rows && !by_rows ? blocks : rows);
     const int value_parts = (a.pool.kv_heads * a.pool.dp + 255) / 256;
     const unsigned grid = (unsigned)(value_blocks * value_parts + (parts == 1 ? (rows + 255) / 256 * 256 : rows * parts));
     auto go = [&](auto type, auto quick) {
-        kv_append_kernel<decltype(type)::value, decltype(quick)::value><<<grid, 256, 0, st>>>(a, parts, value_blocks, value_parts);
+        kv_append_kernel<decltype(type)::value, decltype(quick)::value><<<grid, 256, 0, st>>>(a, parts, value_blocks, value_parts, by_rows);
     };
     using std::integral_constant;
     auto typed = [&](auto type) {
@@ -430,12 +448,12 @@ hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st) {
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.pool.sums || !a.k) return e;
-    const int64_t ends = (int64_t)rows / a.pool.page + requests;
+    const int64_t ends = by_rows ? rows : (int64_t)rows / a.pool.page + requests;
     const dim3 pages((unsigned)ends, (unsigned)a.pool.kv_heads);
     switch (a.pool.type) {
-        case kKvF16: kv_sums_kernel<kKvF16><<<pages, 256, 0, st>>>(a.pool, a.batch); break;
-        case kKvBf16: kv_sums_kernel<kKvBf16><<<pages, 256, 0, st>>>(a.pool, a.batch); break;
-        default: kv_sums_kernel<kKvI8><<<pages, 256, 0, st>>>(a.pool, a.batch);
+        case kKvF16: kv_sums_kernel<kKvF16><<<pages, 256, 0, st>>>(a.pool, a.batch, by_rows); break;
+        case kKvBf16: kv_sums_kernel<kKvBf16><<<pages, 256, 0, st>>>(a.pool, a.batch, by_rows); break;
+        default: kv_sums_kernel<kKvI8><<<pages, 256, 0, st>>>(a.pool, a.batch, by_rows);
     }
     return hipGetLastError();
 }

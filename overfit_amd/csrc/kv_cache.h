@@ -114,13 +114,12 @@ __device__ __forceinline__ bool kv_find(int requests, int& item, int& r, int& be
 // The request of at most `most` rows that a row belongs to (r -1: none), every wave for itself.
 struct KvRowPlace {
     int r, place;  // place: the row's token
+    bool first;    // the request's first row
 };
 __device__ __forceinline__ KvRowPlace kv_row_place(const KvBatch& b, int row, int most) {
     const int lane = threadIdx.x & 63;
-    // from where the row is if every request has one, which is the case that has many of them
-    const int guess = b.requests > 64 ? min(row, b.requests - 1) & ~63 : 0;
-    for (int turn = 0; turn < b.requests + 64; turn += 64) {
-        const int base = turn == 0 ? guess : turn - 64;
+    KvRowPlace at{-1, -1, false};
+    auto among = [&](int base) {  // 64 requests
         KvRows m{0, 0};
         int len = 0;
         if (base + lane < b.requests) {
@@ -128,13 +127,29 @@ __device__ __forceinline__ KvRowPlace kv_row_place(const KvBatch& b, int row, in
             len = kv_length(b, base + lane);
         }
         const uint64_t votes = __ballot(m.n && m.n <= most && row >= m.first && row - m.first < m.n);
-        if (votes) {
-            const int l = __ffsll((unsigned long long)votes) - 1;
-            return KvRowPlace{__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readlane(len - m.n + (row - m.first), l)};
-        }
-        if (b.requests <= 64) break;
+        if (!votes) return false;
+        const int l = __ffsll((unsigned long long)votes) - 1;
+        at = KvRowPlace{__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readlane(len - m.n + (row - m.first), l),
+                        __builtin_amdgcn_readlane(m.first, l) == row};
+        return true;
+    };
+    if (b.requests <= 64) {
+        among(0);
+        return at;
     }
-    return KvRowPlace{-1, -1};
+    // where the row is if every request has one row; where the offsets lie around it; where offsets fall, all of them
+    if (among(min(row, b.requests - 1) & ~63)) return at;
+    int from = 0;
+    for (int step = b.requests > 4096 ? 4096 : 64;; step = 64) {
+        const int i = from + lane * step;
+        const uint64_t votes = __ballot(i < b.requests && b.row_offsets[min(i, b.requests)] <= row);
+        if (votes) from += (63 - __builtin_clzll(votes)) * step;
+        if (step == 64) break;
+    }
+    if (among(from)) return at;
+    for (int base = 0; base < b.requests; base += 64)
+        if (among(base)) return at;
+    return at;
 }
 
 }  // namespace ovfq

@@ -393,6 +393,7 @@ hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st);
 hipError_t launch_kv_clear(void* p, size_t bytes, hipStream_t st);  // zeroes whole 16-byte pieces
 
 struct TilePlan;
+struct CutPlan;
 struct AttendArgs {
     KvPool pool;
     KvBatch batch;
@@ -401,7 +402,9 @@ struct AttendArgs {
     int heads, window;  // window 0: none
     float scale;
     float* parts;  // scratch (attend_scratch): partial outputs of launches that split the keys, then
-    TilePlan* plans;  // what the join needs to know of each tile (set by the launch)
+    // set by the launch, in scratch: what the join needs to know of each tile, and how the launch's items were cut
+    TilePlan* plans;
+    CutPlan* plan;
     // selected pages only (launch_attend_selected)
     int top;
     int* chosen;  // [rows][kv_heads][top], the request's page numbers in rising order, then -1

@@ -10,6 +10,7 @@ torch = pytest.importorskip("torch")
 ov = pytest.importorskip("overfit_amd")
 from overfit_amd import _lib  # noqa: E402
 from kvdata import DEV, Requests, attention, case, check  # noqa: E402
+from test_gpu_attend_selected import choose  # noqa: E402
 
 
 def i32(v):
@@ -103,3 +104,53 @@ def test_one_row_without_its_axis():
     got = ov.kv_append(cache, None, None, *batch, q=q, rope=rope)
     assert got.shape == q.shape and torch.equal(got, ov.kv_append(cache, None, None, *batch, q=q[None], rope=rope)[0])
     assert ov.attend(cache, got, *batch).shape == q.shape
+
+
+@pytest.mark.parametrize("requests,most", [(129, 2), (1000, 3), (5000, 2)])
+def test_requests_past_a_walk(requests, most):
+    """So many requests that a row is searched for and items are counted by a launch of its own."""
+    case("requests", requests, most)
+    rng = np.random.default_rng(requests)
+    counts = rng.integers(0, most + 1, requests)
+    contexts = rng.integers(0, 40 if requests < 2000 else 20, requests)
+    contexts[rng.integers(requests, size=3)] = [1500, 31, 0]
+    req = Requests(ov, rng, "f16", 1, 64, 32, counts.tolist(), contexts.tolist(), sums=True)
+    # what came before in one call, page by page as it would come, then the new tokens in one
+    first = np.concatenate([[0], np.cumsum(contexts)]).astype(np.int32)
+    flat = lambda x, new: req.t(np.concatenate([t[c:] if new else t[:c] for t, c in zip(x, contexts)]).reshape(-1, 64))  # noqa: E731
+    ov.kv_append(req.cache, flat(req.k, False), flat(req.v, False), req.t(first), req.t(contexts.astype(np.int32)), req.t(req.tables))
+    q = rng.standard_normal((req.rows, 128)).astype(np.float32)
+    rope = ov.Rope(torch.zeros(32, device=DEV))  # turned by nothing
+    same = ov.kv_append(req.cache, flat(req.k, True), flat(req.v, True), *req.batch(), q=req.t(q), rope=rope)
+    assert torch.equal(same.cpu(), torch.from_numpy(q))
+    want, err = attention(req, q, 2)
+    check(ov.attend(req.cache, same, *req.batch(), max_rows=most), want, err)
+    check(ov.attend(req.cache, same, *req.batch()), want, err)
+    pages = choose(req, q, 2, 2)
+    want, err = attention(req, q, 2, keep=lambda row, a, seen: np.isin(seen // 32, pages[row, a]))
+    check(ov.attend_selected(req.cache, same, *req.batch(), 2), want, err)
+
+
+def test_bad_offsets_among_many():
+    """An offset past the rows, at a place that the search looks at: its two requests have no rows, the others theirs."""
+    requests, rows = 300, 600
+    cache = ov.KvCache(1, 8, 32, requests)
+    off = torch.arange(0, rows + 1, 2, dtype=torch.int32, device=DEV)
+    off[128] = rows + 5
+    lengths, tables = torch.full((requests,), 2, dtype=torch.int32, device=DEV), torch.arange(requests, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    k, v, q = (torch.randn(rows, 8, device=DEV) for _ in range(3))
+    out = torch.full_like(q, 7.0)
+    ov.kv_append(cache, k, v, off, lengths, tables, q=q, q_out=out, rope=ov.Rope(torch.zeros(4, device=DEV)))
+    gone = slice(254, 258)
+    want = q.clone()
+    want[gone] = 7.0
+    assert torch.equal(out, want)
+    stored = cache.value_view().reshape(requests, 32, -1)[:, :2, :8].reshape(rows, 8).float()
+    kept = v.half().float()
+    kept[gone] = 0
+    assert torch.equal(stored, kept)
+    out.fill_(7.0)
+    ov.attend(cache, q, off, lengths, tables, out=out)
+    assert torch.equal(out[gone], torch.full((4, 8), 7.0, device=DEV))
+    assert torch.allclose(out[0::2][:127], kept[0::2][:127], rtol=1e-6, atol=1e-7)  # a request's first token sees itself alone
+    assert torch.allclose(out[0::2][129:], kept[0::2][129:], rtol=1e-6, atol=1e-7)
