@@ -35,10 +35,16 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }  // (of a vector's element it is the first's)
+
 // Over the four lanes of a column: l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float column_max(float v) {
     auto f = [](int a, int b) { return (int)__builtin_bit_cast(uint32_t, fmaxf(as_float((uint32_t)a), as_float((uint32_t)b))); };
     return as_float((uint32_t)join32(join16((int)__builtin_bit_cast(uint32_t, v), f), f));
+}
+__device__ __forceinline__ uint32_t column_max(uint32_t v) {
+    auto f = [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); };
+    return (uint32_t)join32(join16((int)v, f), f);
 }
 __device__ __forceinline__ float column_sum(float v) {
     auto f = [](int a, int b) { return (int)__builtin_bit_cast(uint32_t, as_float((uint32_t)a) + as_float((uint32_t)b)); };
@@ -198,35 +204,45 @@ struct Attention {
 #pragma unroll
                 for (int h = 0; h < 2; h++) s[t][h] *= ks[h];
         }
+        // int8: the largest scale of the values seen, as bits, which are ordered like it, what is not finite above all
+        uint32_t vtop[kCols] = {};
+        if constexpr (kType == kKvI8) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) v = max(v, bits_of(vs[h][i]));
+#pragma unroll
+            for (int t = 0; t < kCols; t++) vtop[t] = v;
+        }
         if (masked) {
 #pragma unroll
             for (int t = 0; t < kCols; t++) {
+                vtop[t] = 0;
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int j = mine + 16 * h + i;
-                        s[t][h][i] = (int)(j <= lim[t]) & (int)(j >= low[t]) ? s[t][h][i] : -kInf;
+                        const bool seen = (int)(j <= lim[t]) & (int)(j >= low[t]);
+                        s[t][h][i] = seen ? s[t][h][i] : -kInf;
+                        if constexpr (kType == kKvI8) vtop[t] = max(vtop[t], seen ? bits_of(vs[h][i]) : 0u);
                     }
             }
         }
         bool move = false;
-        float top[kCols], vtop[kCols];
+        float top[kCols];
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             top[t] = s[t][0][0];
-            vtop[t] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 4; i++)
                     if (h + i) top[t] = fmaxf(top[t], s[t][h][i]);
-                    // (a hidden token's scale counts for nothing)
-                    if constexpr (kType == kKvI8) vtop[t] = fmaxf(vtop[t], masked && s[t][h][i] == -kInf ? 0.0f : vs[h][i]);
-                }
             top[t] *= qs[t];
             move = move | (top[t] > ref[t] + kTop + kRoom);
-            if constexpr (kType == kKvI8) move = move | (vtop[t] > ev[t]);
+            if constexpr (kType == kKvI8) move = move | (vtop[t] > __builtin_bit_cast(uint32_t, ev[t]));
         }
         if (__ballot(move)) {
 #pragma unroll
@@ -239,11 +255,12 @@ struct Attention {
                     l[t] *= f;
                 }
                 if constexpr (kType == kKvI8) {
-                    const float v = column_max(vtop[t]);
-                    if (v > ev[t]) {
-                        const uint32_t e = min((__builtin_bit_cast(uint32_t, v) >> 23) + 1u, 253u);
+                    const uint32_t v = column_max(vtop[t]);
+                    if (v > __builtin_bit_cast(uint32_t, ev[t])) {
+                        const uint32_t e = min((v >> 23) + 1u, 253u);
                         f *= ev[t] * as_float((254u - e) << 23);
                         ev[t] = as_float(e << 23);
+                        if (v >= 0x7f800000u) l[t] = __builtin_nanf("");  // one that is not finite makes the row that sees it NaN
                     }
                 }
 #pragma unroll
@@ -253,7 +270,7 @@ struct Attention {
     }
 
     // Settled scores into probabilities, split for the second product.
-    __device__ __forceinline__ void probabilities(const f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts], bool masked,
+    __device__ __forceinline__ void probabilities(const f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts],
                                                   const f32x4 (&vs)[2]) {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
@@ -268,10 +285,8 @@ struct Attention {
                     const float v = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], qs[t], -r));
                     l[t] += v;
                     x[4 * h + i] = v;
-                    if constexpr (kType == kKvI8) {
-                        const float w = v * (vs[h][i] * down);
-                        x[4 * h + i] = masked && s[t][h][i] == -kInf ? 0.0f : w;
-                    }
+                    // (a seen token's scale is at most ev; a hidden one's may be anything, and its probability is 0)
+                    if constexpr (kType == kKvI8) x[4 * h + i] = v * __builtin_amdgcn_fmed3f(vs[h][i] * down, 0.0f, 1.0f);
                 }
             M::split(x, p[t]);
         }

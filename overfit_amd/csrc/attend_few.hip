@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
             u32x4 p[kCols][M::kParts];
             if (now.page >= 0) {
                 att.settle(s, masked, now.first, ks, vs);
-                att.probabilities(s, p, masked, vs);
+                att.probabilities(s, p, vs);
             }
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kKeyLoads + (kDepth - 1) * kLoadsOfBlock) : "memory");
             if (now.page >= 0) {

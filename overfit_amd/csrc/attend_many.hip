@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
             const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
             u32x4 p[kCols][M::kParts];
             att.settle(s, masked, first, ks, vs);
-            att.probabilities(s, p, masked, vs);
+            att.probabilities(s, p, vs);
             att.products(p, [&](int tile) { return value_operand<kType, kDp>(tile, load); });
         }
         page = next;
