@@ -134,25 +134,44 @@ struct Attention {
     float ev[kCols];             // int8: the power of two that value scales are divided by, 0 at first
     uint32_t bad[kCols][2];      // bit 4 d + i: the column sees a value that is not finite in o[][d][i]'s channel (of masked blocks)
 
-    // Column `col` of the tile has query row x (NULL: none) and sees the tokens [first, last].
-    __device__ __forceinline__ void column(int t, const float* x, int dim, float scale, int first, int last) {
+    // A query row's channels of this lane, zeros if the column is not used.
+    using Row = float[kChunks][8];
+    static __device__ __forceinline__ void fetch(Row& v, const float* x, bool used, int dim) {
         const int g = (threadIdx.x >> 4) & 3;
-        float v[kChunks][8];
-        float top = 0.0f;
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
-            const int d = c * 32 + g * 8;
+            const int d = c * 32 + g * 8, in = d < dim ? d : 0;
             f32x4u a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-            if (x && d < dim) {
-                a = *(const f32x4u*)(x + d);
-                b = *(const f32x4u*)(x + d + 4);
+            if (used) {
+                a = *(const f32x4u*)(x + in);
+                b = *(const f32x4u*)(x + in + 4);
             }
 #pragma unroll
+            for (int i = 0; i < 8; i++) v[c][i] = i < 4 ? a[i & 3] : b[i & 3];
+        }
+    }
+    // Column t of the wave, if `used`, sees the tokens [first, last].
+    __device__ __forceinline__ void column(int t, bool used, int first, int last) {
+        lim[t] = used ? last : -1;
+        low[t] = first;
+        ref[t] = -kInf;
+        l[t] = 0.0f;
+        ev[t] = 0.0f;
+        bad[t][0] = bad[t][1] = 0;
+#pragma unroll
+        for (int d = 0; d < kTiles; d++) o[t][d] = f32x4{0, 0, 0, 0};
+    }
+    // Its query row; zeros for a column that is not used.
+    __device__ __forceinline__ void query(int t, Row& v, bool used, int dim, float scale) {
+        const int g = (threadIdx.x >> 4) & 3;
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kChunks; c++)
+#pragma unroll
             for (int i = 0; i < 8; i++) {
-                v[c][i] = (i < 4 ? a[i & 3] : b[i & 3]) * scale;
+                v[c][i] = used && c * 32 + g * 8 < dim ? v[c][i] * scale : 0.0f;
                 top = fmaxf(top, fabsf(v[c][i]));
             }
-        }
         top = column_max(top);
         const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23), 1), 253);
         const float down = as_float((uint32_t)(254 - e) << 23);
@@ -167,14 +186,6 @@ struct Attention {
 #pragma unroll
             for (int p = 0; p < M::kParts; p++) q[t][p][c] = part[p];
         }
-        lim[t] = x ? last : -1;
-        low[t] = first;
-        ref[t] = -kInf;
-        l[t] = 0.0f;
-        ev[t] = 0.0f;
-        bad[t][0] = bad[t][1] = 0;
-#pragma unroll
-        for (int d = 0; d < kTiles; d++) o[t][d] = f32x4{0, 0, 0, 0};
     }
 
     // Scores of a block; key(tile, chunk): the operand of its 16 tokens and 32 channels.
@@ -598,8 +609,8 @@ struct BlockWalk {
     }
     __device__ __forceinline__ void fetch() {
         const int64_t entry = ((int64_t)first + (int64_t)(threadIdx.x & 63) * step) >> shift;
-        const int p = entry < entries ? table[entry] : -1;
-        held = p >= 0 && p < pages ? p : -1;
+        const int p = table[min(entry, (int64_t)entries - 1)];
+        held = entry < entries && p >= 0 && p < pages ? p : -1;
     }
     // Page of block first + i * step, i rising by one from call to call, or -1.
     __device__ __forceinline__ int page(int i) {

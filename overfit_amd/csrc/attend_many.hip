@@ -25,30 +25,11 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     TileWork w;
     if (!cut_item(cut, pool, b, a.plan, item, w)) return;
     if (a.plans && threadIdx.x == 0 && w.piece == 0 && head == 0) a.plans[w.tile_index] = w;
-    Att att;
     const int wave_col = w.col0 + 16 * kCols * wave;
-#pragma unroll
-    for (int t = 0; t < kCols; t++) {
-        const int c = wave_col + 16 * t + col, i = c / cut.group;
-        const bool used = i < w.rows;
-        const int qh = head * cut.group + (c - i * cut.group);
-        const float* x = used ? a.q + ((size_t)(w.first_row + i) * a.heads + qh) * pool.dim : nullptr;
-        const int last = w.place + i;
-        att.column(t, x, pool.dim, a.scale * kLog2e, a.window ? max(last - a.window + 1, 0) : 0, last);
-    }
-    // what the wave's rows see
-    const int i0 = wave_col / cut.group, i1 = min(w.rows - 1, (wave_col + 16 * kCols - 1) / cut.group);
-    const bool live = i0 < w.rows;
-    const int first_last = w.place + i0, last_last = w.place + i1;
-    const int first_low = a.window ? max(first_last - a.window + 1, 0) : 0, last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
-    // and the least that a column of the tile sees
-    const int tile_last = w.place + w.col0 / cut.group;
-    const int tile_low = a.window ? max(w.place + min(w.rows - 1, (w.col0 + 64 * kCols - 1) / cut.group) - a.window + 1, 0) : 0;
-
     BlockWalk walk;
     const int blocks = max(w.block1 - w.block0, 0);
     const int in_page = pool.page / kKvBlock - 1;
-    if (blocks) walk.start(pool, b.tables + (size_t)w.r * b.width, b.width, w.block0, 1);
+    walk.start(pool, b.tables + (size_t)w.r * b.width, b.width, w.block0, 1);
     auto stage = [&](int i, int page) {
         const char* src = kv_block(pool, page, head, (w.block0 + i) & in_page);
         char* dst = ring[i & 1];
@@ -64,8 +45,32 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
                                                  (__attribute__((address_space(3))) void*)(dst + 2 * kPlane), 4, 0, 0);
         }
     };
+    typename Att::Row rows[kCols];  // (of columns that are not used the first row: at a branch's end the compiler would wait for the loads)
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int c = wave_col + 16 * t + col, i = c / cut.group, qh = head * cut.group + (c - i * cut.group);
+        Att::fetch(rows[t], a.q + ((size_t)(w.first_row + (i < w.rows ? i : 0)) * a.heads + qh) * pool.dim, true, pool.dim);
+    }
+    asm volatile("" ::: "memory");  // (the table's, the queries' and the first block's loads are on their way together)
     int page = blocks ? walk.page(0) : -1;
-    if (page >= 0) stage(0, page);
+    stage(0, max(page, 0));
+    asm volatile("" ::: "memory");
+    Att att;
+#pragma unroll
+    for (int t = 0; t < kCols; t++) {
+        const int i = (wave_col + 16 * t + col) / cut.group, last = w.place + i;
+        att.column(t, i < w.rows, a.window ? max(last - a.window + 1, 0) : 0, last);
+        att.query(t, rows[t], i < w.rows, pool.dim, a.scale * kLog2e);
+    }
+    // what the wave's rows see
+    const int i0 = wave_col / cut.group, i1 = min(w.rows - 1, (wave_col + 16 * kCols - 1) / cut.group);
+    const bool live = i0 < w.rows;
+    const int first_last = w.place + i0, last_last = w.place + i1;
+    const int first_low = a.window ? max(first_last - a.window + 1, 0) : 0, last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+    // and the least that a column of the tile sees
+    const int tile_last = w.place + w.col0 / cut.group;
+    const int tile_low = a.window ? max(w.place + min(w.rows - 1, (w.col0 + 64 * kCols - 1) / cut.group) - a.window + 1, 0) : 0;
+
     for (int i = 0; i < blocks; i++) {
         const int next = i + 1 < blocks ? walk.page(i + 1) : -1;
         // this wave's share of block i has landed; behind the barrier all of it, and every wave is past the block before
@@ -107,6 +112,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
         }
         page = next;
     }
+    if (!blocks) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the first one's load, which nothing waited for)
     att.close();
     if (w.pieces > 1) {
         float* part = a.parts + ((size_t)(w.slot + w.piece) * pool.kv_heads + head) * (size_t)part_floats(64 * kCols, kDp);
@@ -226,7 +232,7 @@ Plan plan_attend(const AttendArgs& a, bool few) {
     const int64_t usual = kinds.many ? (int64_t)(a.batch.rows - a.batch.most) * group / (requests > 1 ? requests - 1 : 1) : most;
     const int log2 = few ? (usual <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
     const int least = !few && kinds.few ? few_columns(a) + 1 : 1;
-    p.cut = Cut{log2, least, (int)most, ceil_div(kItems, a.pool.kv_heads), few ? 8 : 16, few ? 2.0f : 1.5f, a.window, group, 0, 0, 0};
+    p.cut = Cut{log2, least, (int)most, ceil_div(kItems, a.pool.kv_heads), 8, few ? 2.0f : 1.5f, a.window, group, 0, 0, 0};
     p.tiles = (unsigned)(few ? requests * ceil_div(most, 1 << log2) : (((int64_t)a.batch.rows * group) >> log2) + requests);
     // Pieces are no longer than the mean by more than `slack`, and the sum of the tiles' lengths that it comes from is half of their number
     // times the longest at least: so many pieces at most, and so many of tiles that are cut.
