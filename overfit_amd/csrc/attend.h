@@ -464,6 +464,121 @@ __device__ __forceinline__ int2 cut_items(const CutRequest& q, float inv) {
     return make_int2(items, items > q.tiles ? items : 0);
 }
 
+// Of lanes with `tiles` tiles from `place` on, the tile number `item` by the place of its last column, the last one first: its lane, and
+// its number there. There are more than `item` of them.
+__device__ __forceinline__ int cut_latest(const Cut& c, int place, int tiles, int item, int& tile) {
+    // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
+    const int base = (int)min(max(((int64_t)place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
+    int lo = -1, hi = tiles ? base + tiles : 0;
+    hi = wave_max(hi);  // none past hi; more than `item` past lo
+    int past = 0;
+    while (hi - lo > 1) {
+        const int x = lo + (hi - lo) / 2;
+        const int n = wave_sum(min(max(base + tiles - 1 - x, 0), tiles));
+        if (n <= item) {
+            hi = x;
+            past = n;
+        } else {
+            lo = x;
+        }
+    }
+    const int at = hi - base;  // the tile that ends there
+    uint64_t votes = __ballot(at >= 0 && at < tiles);
+    for (int i = past; i < item; i++) votes &= votes - 1;
+    const int l = __ffsll((unsigned long long)votes) - 1;
+    tile = __builtin_amdgcn_readlane(at, l);
+    return l;
+}
+
+// The same for up to 64 requests of many tiles each, whose spans differ: every tile has as many pieces as its own span gives, tiles of
+// the most pieces come first, whole ones last, the longest of them first. (Counting each tile as the longest of its request, 2048 prompt
+// rows of 32 query heads over 8 took 119 us, so 95: the items of no work between the others kept workgroups out for 50.)
+__device__ __forceinline__ bool cut_tiles(const Cut& c, const KvPool& pool, const KvBatch& b, CutPlan* plan, int item, TileWork& w) {
+    const CutRequest q = cut_load(c, pool, b, threadIdx.x & 63);
+    const int tiles = wave_sum(q.tiles), longest = wave_max(q.blocks);
+    // the request's blocks of tile u, and its first tile of more than x blocks
+    auto span = [&](int u) {
+        const int last = q.place + min(q.n - 1, (((u + 1) << c.cols_log2) - 1) / c.group);
+        return last < 0 ? 0 : min(last / kKvBlock + 1, q.blocks);
+    };
+    auto above = [&](int x) {
+        if (x >= q.blocks) return q.tiles;
+        const int row = x * kKvBlock - q.place;
+        return row <= 0 ? 0 : min((row * c.group) >> c.cols_log2, q.tiles - 1);
+    };
+    int piece = uniform((int)cut_piece(c, wave_sum(q.sum), tiles));
+    if (tiles < c.target && longest > piece) {
+        // halving what lies between the mean, which may give too many, and the longest tile
+        const int most = wave_max(q.tiles);
+        auto items = [&](int size) {
+            const int layers = uniform((longest + size - 1) / size);
+            int n = 0;
+            if (most < layers) {
+                for (int u = 0; u < most; u++) n += u < q.tiles ? max((span(u) + size - 1) / size, 1) : 0;
+            } else {
+                n = q.tiles;
+                for (int k = 1; k < layers; k++) n += q.tiles - above(k * size);
+            }
+            return wave_sum(n);
+        };
+        int over = piece;
+        if (items(piece) > c.target) {
+            piece = longest;
+            for (int i = 0; i < 5 && piece - over > 1; i++) {
+                const int half = (piece + over) >> 1;
+                if (items(half) > c.target)
+                    over = half;
+                else
+                    piece = half;
+            }
+        }
+    }
+    const bool fit = tiles <= c.tiles;  // (if not, offsets overlap: none of the call's tiles)
+    if (blockIdx.x == 0) {
+        const int joins = wave_sum(q.tiles - above(piece));
+        if (threadIdx.x == 0) plan->joins = fit ? joins : 0;
+    }
+    if (!fit) return false;
+    int left = q.tiles, l = -1;
+    w.slot = w.tile_index = w.piece = 0;
+    w.pieces = 1;
+    while (longest > piece) {
+        const int mine = left ? (span(left - 1) + piece - 1) / piece : 0, most = wave_max(mine);
+        if (most < 2) break;
+        const int low = mine == most ? above((most - 1) * piece) : left, n = left - low, upto = wave_upto(n);
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (item < all * most) {
+            const int nth = uniform(item / most);
+            l = __ffsll((unsigned long long)__ballot(upto > nth)) - 1;
+            w.pieces = most;
+            w.piece = item - nth * most;
+            w.tile = __builtin_amdgcn_readlane(left, l) - 1 - (nth - __builtin_amdgcn_readlane(upto - n, l));
+            w.slot += nth * most;
+            w.tile_index += nth;
+            break;
+        }
+        item -= all * most;
+        w.slot += all * most;
+        w.tile_index += all;
+        left = low;
+    }
+    if (l < 0) {
+        if (item >= wave_sum(left)) return false;
+        l = cut_latest(c, q.place, left, item, w.tile);
+        w.tile_index += item;
+    }
+    w.r = l;
+    w.first_row = __builtin_amdgcn_readlane(q.first, l);
+    w.rows = __builtin_amdgcn_readlane(q.n, l);
+    w.place = __builtin_amdgcn_readlane(q.place, l);
+    w.col0 = w.tile << c.cols_log2;
+    const int2 s = cut_blocks(c, pool, b, w.place, uniform(w.col0 / c.group), uniform(min(w.rows - 1, (w.col0 + (1 << c.cols_log2) - 1) / c.group)));
+    const int size = uniform((s.y - s.x + w.pieces - 1) / w.pieces);
+    w.block0 = min(s.x + w.piece * size, s.y);
+    w.block1 = min(w.block0 + size, s.y);
+    return w.pieces == 1 || w.slot + w.pieces <= c.slots;
+}
+
 // Item `item` of a key head; false past the last one. Every wave finds it for itself: lanes hold 64 requests at a time, or in a planned
 // launch 64 times 64 of them and then the item's.
 __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const KvBatch& b, CutPlan* plan, int item, TileWork& w) {
@@ -512,27 +627,8 @@ __device__ __forceinline__ bool cut_item(const Cut& c, const KvPool& pool, const
     w.r = 0;
     if (!c.planned && b.requests <= 64 && cut_pieces(longest, inv) == 1) {
         if (item >= tiles) return false;
-        // x: the largest number that no more than `item` tiles end past (base + tile: a tile's end, in tiles)
-        const int base = (int)min(max(((int64_t)q.place * c.group) >> c.cols_log2, (int64_t)0), (int64_t)1 << 30);
-        int lo = -1, hi = q.tiles ? base + q.tiles : 0;
-        hi = wave_max(hi);  // none past hi; more than `item` past lo
-        int past = 0;
-        while (hi - lo > 1) {
-            const int x = lo + (hi - lo) / 2;
-            const int n = wave_sum(min(max(base + q.tiles - 1 - x, 0), q.tiles));
-            if (n <= item) {
-                hi = x;
-                past = n;
-            } else {
-                lo = x;
-            }
-        }
-        const int at = hi - base;  // the tile that ends there
-        uint64_t votes = __ballot(at >= 0 && at < q.tiles);
-        for (int i = past; i < item; i++) votes &= votes - 1;
-        l = __ffsll((unsigned long long)votes) - 1;
+        l = cut_latest(c, q.place, q.tiles, item, w.tile);
         w.r = l;
-        w.tile = __builtin_amdgcn_readlane(at, l);
         w.slot = 0;
         w.tile_index = item;
     } else {

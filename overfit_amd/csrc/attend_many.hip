@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15;
     const int head = (int)(blockIdx.x % (unsigned)pool.kv_heads), item = (int)(blockIdx.x / (unsigned)pool.kv_heads);
     TileWork w;
-    if (!cut_item(cut, pool, b, a.plan, item, w)) return;
+    if (!(b.requests <= 64 ? cut_tiles(cut, pool, b, a.plan, item, w) : cut_item(cut, pool, b, a.plan, item, w))) return;
     if (a.plans && threadIdx.x == 0 && w.piece == 0 && head == 0) a.plans[w.tile_index] = w;
     const int wave_col = w.col0 + 16 * kCols * wave;
     BlockWalk walk;

@@ -154,3 +154,23 @@ def test_bad_offsets_among_many():
     assert torch.equal(out[gone], torch.full((4, 8), 7.0, device=DEV))
     assert torch.allclose(out[0::2][:127], kept[0::2][:127], rtol=1e-6, atol=1e-7)  # a request's first token sees itself alone
     assert torch.allclose(out[0::2][129:], kept[0::2][129:], rtol=1e-6, atol=1e-7)
+
+
+@pytest.mark.parametrize("kv_heads,counts,contexts,window", [
+    (8, (1500,), (0,), 0),               # tiles of one piece, two and three
+    (16, (700, 300, 90), (0, 2000, 5), 0),
+    (16, (700, 300, 90), (0, 2000, 5), 300),
+    (64, (40,) * 20, tuple(range(0, 4000, 200)), 0),
+    (2, (33, 70), (9000, 0), 0),         # more pieces than tiles
+])
+def test_pieces_by_each_tiles_span(kv_heads, counts, contexts, window):
+    case("spans", kv_heads, counts, window)
+    rng = np.random.default_rng(31)
+    req = Requests(ov, rng, "f16", kv_heads, 64, 64, counts, contexts).fill()
+    q = rng.standard_normal((req.rows, 2 * kv_heads * 64)).astype(np.float32)
+    out = ov.attend(req.cache, req.t(q), *req.batch(), window=window).cpu().numpy()
+    heads = [0, kv_heads - 1]
+    part = Requests.__new__(Requests)
+    part.__dict__.update(req.__dict__, kv_heads=2, k=[k[:, heads] for k in req.k], v=[v[:, heads] for v in req.v])
+    pick = lambda x: x.reshape(req.rows, kv_heads, 2 * 64)[:, heads].reshape(req.rows, -1)  # noqa: E731
+    check(pick(out), *attention(part, pick(q), 4, window=window))
