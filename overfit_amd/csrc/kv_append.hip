@@ -9,7 +9,7 @@
 //
 // Bound: HBM for many rows (each fp32 row is read once, written once), the launch and three dependent reads (offsets and length, page,
 // rows) for one. Queries and keys have a workgroup a row, four for batches below the chip's workgroups, which share the row's heads;
-// values one for a share of a block of the cache. (us, 1 / 1297 / 4096 rows of 32 and 8 heads of 128: 4.1 / 13.3 / 42.7; a copy of the bytes 0.01 / 11.4
+// values one for a share of a block of the cache. (us, 1 / 1297 / 4096 rows of 32 and 8 heads of 128: 4.1 / 13.6 / 42.5; a copy of the bytes 0.01 / 11.4
 // / 36.1.)
 #include "kv_cache.h"
 
