@@ -35,7 +35,7 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }  // (of a vector's element it is the first's)
+__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }  // (straight from a vector it reads element 0)
 
 // Over the four lanes of a column: l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float column_max(float v) {
@@ -545,7 +545,7 @@ __device__ __forceinline__ bool cut_tiles(const Cut& c, const KvPool& pool, cons
     while (longest > piece) {
         const int mine = left ? (span(left - 1) + piece - 1) / piece : 0, most = wave_max(mine);
         if (most < 2) break;
-        const int low = mine == most ? above((most - 1) * piece) : left, n = left - low, upto = wave_upto(n);
+        const int low = mine == most ? min(above((most - 1) * piece), left - 1) : left, n = left - low, upto = wave_upto(n);
         const int all = __builtin_amdgcn_readlane(upto, 63);
         if (item < all * most) {
             const int nth = uniform(item / most);

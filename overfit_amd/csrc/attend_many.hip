@@ -197,8 +197,8 @@ int few_columns(const AttendArgs& a) { return a.pool.dp <= 128 ? 32 : 16; }
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 constexpr int kItems = 512;  // two workgroups a CU: registers and LDS
-// More requests than that have their items counted by a launch of its own, whose 3 us are less than every workgroup's walk over them (single
-// rows of 256 tokens: 65 requests 28.5 us with it and 25.9 without, 130 40.2 / 41.6, 300 73.9 / 93.1, 4096 835 / 4883).
+// More requests than that have their items counted by a launch of its own, whose 3 us are less than every workgroup's walk over them
+// (single rows of 256 tokens: 65 requests 28.5 us with it and 25.9 without, 130 40.2 / 41.6, 300 73.9 / 93.1, 4096 835 / 4883).
 constexpr int kPlanned = 128;
 
 struct Plan {

@@ -174,3 +174,52 @@ def test_pieces_by_each_tiles_span(kv_heads, counts, contexts, window):
     part.__dict__.update(req.__dict__, kv_heads=2, k=[k[:, heads] for k in req.k], v=[v[:, heads] for v in req.v])
     pick = lambda x: x.reshape(req.rows, kv_heads, 2 * 64)[:, heads].reshape(req.rows, -1)  # noqa: E731
     check(pick(out), *attention(part, pick(q), 4, window=window))
+
+
+def test_a_graph_of_many_requests():
+    """Both kernels, their items counted on the device: a captured call follows lengths, offsets and tables as they are when it is replayed."""
+    rng = np.random.default_rng(41)
+    counts = [1] * 199 + [60]
+    req = Requests(ov, rng, "bf16", 2, 64, 32, counts, rng.integers(0, 300, 200).tolist(), sums=True).fill()
+    off, lengths, tables = req.batch()
+    q = req.t(rng.standard_normal((req.rows, 4 * 64)).astype(np.float32))
+    out, few = torch.zeros_like(q), torch.zeros_like(q)
+    calls = [req.cache.context.bind_attend_dev(req.cache, q, off, lengths, tables, out, max_rows=60),
+             req.cache.context.bind_attend_selected_dev(req.cache, q, off, lengths, tables, 3, few, max_rows=60)]
+
+    def run():
+        for c in calls:
+            c()
+    ctx, side = req.cache.context, torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(side.cuda_stream)
+    try:
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+        replays(req, rng, off, lengths, tables, q, out, few, run, graph)
+    finally:
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+
+
+def replays(req, rng, off, lengths, tables, q, out, few, run, graph):
+    order = np.array([60] + [1] * 199)
+    batches = [(req.off, req.lengths, req.tables),
+               (np.concatenate([[0], np.cumsum(order)]), np.roll(req.lengths, 1), np.roll(req.tables, 1, 0)),
+               (req.off, [n - (n > 80) for n in req.lengths], req.tables)]
+    for o, n, t in batches * 2:
+        for to, x in ((off, o), (lengths, n), (tables, t)):
+            to.copy_(torch.from_numpy(np.ascontiguousarray(np.array(x, np.int32))))
+        q.normal_()
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        want = out.clone(), few.clone()
+        out.zero_(), few.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(few, want[1])
+        assert out.abs().sum(1).min() > 0
