@@ -447,8 +447,9 @@ OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch*
 /* Attention of each request's new tokens, already appended, over its pages (the reference's per-head loops, RT/CachedAttentionKernel.cs and
  * RT/BatchedAttentionKernel.cs): for row m, token p of its request, and query head h, whose keys are head h / (heads / kv_heads)'s,
  *   out[m][h] = sum over tokens j, p - window < j <= p (window 0: 0 <= j <= p), of softmax(scale q[m][h] . k_j) v_j
- * heads is a multiple of kv_heads. q and the probabilities enter the products with all but the last two of fp32's bits at least, sums are
- * fp32. Tokens in pages outside the cache count as hidden; a row that sees no token gives 0. What is not finite stays in the rows
+ * heads is a multiple of kv_heads. A channel of q enters the products to 2^-23 of its row's largest one, a probability to 2^-22 of itself
+ * or 2^-34 of the row's largest (OVFQ_TYPE_I8: of the largest after each is multiplied by its value's scale); sums are fp32. Keys are
+ * below 2^118 and scores fit fp32; values may have any size, in OVFQ_TYPE_BF16 caches beyond 2^116 in up to 4096 tokens of like weight. Tokens in pages outside the cache count as hidden; a row that sees no token gives 0. What is not finite stays in the rows
  * that see it. The host form refuses what ovfq_kv_append does, but for shared pages; in the other a request of more than max_rows rows
  * is left out (its rows of `out` stay as they were), and offsets count as there. Host pointers, synchronous. */
 OVFQ_API int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,

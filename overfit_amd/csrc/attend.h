@@ -7,12 +7,18 @@
 // Products are MFMA 16x16x32 with the cache's operands as the first factor, so that a lane's results belong to one column (lane % 16)
 // and to the tokens whose values the same lane group loads for the second product: probabilities never change lanes.
 //
-// Rounding. q and p are fp32 and enter the products in parts that carry all of fp32's bits but the last two at most: two fp16 parts
-// beside fp16 and int8 operands (22 bits), three bf16 parts beside bf16 ones (24). q is scaled by a power of two to below 2 for that;
-// p is 2^10 at the largest score that its column has met when it last moved its reference, which it does when a score passes that by
-// 2^4, so fp16 has 2^24 below the largest p and no overflow above. Sums and references are fp32. int8 operands are widened to fp16,
-// which is exact; a token's key scale multiplies its scores, its value scale its probabilities, against a power of two kept for the
-// column.
+// Rounding. q and p are fp32 and enter the products in parts: two fp16 ones beside fp16 and int8 operands (22 bits, for numbers down to
+// 2^-14; what lies below is held to 2^-25 whatever its size), three bf16 ones beside bf16 operands (24 bits). q is scaled by a power of
+// two, its row's largest channel to between 1 and 2, so a channel is off by 2^-23 of that one at most. p is 2^kTop at the largest score
+// that its column has met when it last moved its reference, which it does when a score passes that by 2^kRoom: beside fp16 values
+// 2^10, so that fp16 has 2^24 below the largest p and no overflow above; beside bf16 values 2^-16, so that sums over 2^12 of the largest
+// values still fit fp32. Sums and references are fp32; outputs are divided by their sum before they are joined, and are never larger than
+// the values.
+// int8 operands are widened to fp16, which is exact. A token's key scale multiplies its scores, its value scale its p (2^2 at the
+// reference, so that the product fits fp32); what enters the second product is p scale / e, with a power of two e kept for the column
+// that puts the largest p scale so far between 2^10 and 2^15. Both move with the column's reference, so a large scale of little weight
+// takes nothing from the others. (Against the largest scale seen, whatever its weight, a token of 2^36 times the others' scales and no
+// weight made zeros of the rows that saw it.)
 //
 // Masks: a hidden token's score is -inf whatever its key holds. A hidden token's value meets a probability of zero, which would still
 // make NaN of what is not finite, so blocks with a mask look at their values first: what is not finite is noted for the columns that see
@@ -53,11 +59,12 @@ __device__ __forceinline__ float column_sum(float v) {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTop = 10.0f, kRoom = 4.0f;  // log2 of p at a new reference, and how far it may grow before the next
+constexpr float kRoom = 4.0f;  // log2 of how far p may grow past a new reference before the next
 
 template <int kType>
 struct KvMath {
     static constexpr int kParts = kType == kKvBf16 ? 3 : 2;
+    static constexpr float kTop = kType == kKvF16 ? 10.0f : kType == kKvBf16 ? -16.0f : 2.0f;  // log2 of p at a new reference
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         if constexpr (kType == kKvBf16)
             return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
@@ -131,7 +138,8 @@ struct Attention {
     int lim[kCols], low[kCols];  // the column's last token, and its first
     f32x4 o[kCols][kTiles];
     float ref[kCols], l[kCols];  // l: of this lane's tokens
-    float ev[kCols];             // int8: the power of two that value scales are divided by, 0 at first
+    float ev[kCols];             // int8: the power of two that p times the values' scales are divided by, so o as well
+    float fall[kCols];           // int8: what a new reference has made of earlier probabilities, 1 without one
     uint32_t bad[kCols][2];      // bit 4 d + i: the column sees a value that is not finite in o[][d][i]'s channel (of masked blocks)
 
     // A query row's channels of this lane, zeros if the column is not used.
@@ -156,7 +164,7 @@ struct Attention {
         low[t] = first;
         ref[t] = -kInf;
         l[t] = 0.0f;
-        ev[t] = 0.0f;
+        ev[t] = as_float(1u << 23);
         bad[t][0] = bad[t][1] = 0;
 #pragma unroll
         for (int d = 0; d < kTiles; d++) o[t][d] = f32x4{0, 0, 0, 0};
@@ -205,41 +213,28 @@ struct Attention {
             }
     }
 
-    // A block's scores before their powers: int8's key scales, masks, and the columns' references. first: the block's first token; ks,
-    // vs: int8's scales of this lane's tokens.
-    __device__ __forceinline__ void settle(f32x4 (&s)[kCols][2], bool masked, int first, const f32x4 (&ks)[2], const f32x4 (&vs)[2]) {
+    // Whether column t sees token j.
+    __device__ __forceinline__ bool sees(int t, int j) const { return (int)(j <= lim[t]) & (int)(j >= low[t]); }
+
+    // A block's scores before their powers: int8's key scales, masks, and the columns' references. first: the block's first token; ks:
+    // int8's scales of this lane's keys.
+    __device__ __forceinline__ void settle(f32x4 (&s)[kCols][2], bool masked, int first, const f32x4 (&ks)[2]) {
         const int mine = first + ((threadIdx.x >> 4) & 3) * 4;
         if constexpr (kType == kKvI8) {
 #pragma unroll
-            for (int t = 0; t < kCols; t++)
+            for (int t = 0; t < kCols; t++) {
+                fall[t] = 1.0f;
 #pragma unroll
                 for (int h = 0; h < 2; h++) s[t][h] *= ks[h];
-        }
-        // int8: the largest scale of the values seen, as bits, which are ordered like it, what is not finite above all
-        uint32_t vtop[kCols] = {};
-        if constexpr (kType == kKvI8) {
-            uint32_t v = 0;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) v = max(v, bits_of(vs[h][i]));
-#pragma unroll
-            for (int t = 0; t < kCols; t++) vtop[t] = v;
+            }
         }
         if (masked) {
 #pragma unroll
-            for (int t = 0; t < kCols; t++) {
-                vtop[t] = 0;
+            for (int t = 0; t < kCols; t++)
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int j = mine + 16 * h + i;
-                        const bool seen = (int)(j <= lim[t]) & (int)(j >= low[t]);
-                        s[t][h][i] = seen ? s[t][h][i] : -kInf;
-                        if constexpr (kType == kKvI8) vtop[t] = max(vtop[t], seen ? bits_of(vs[h][i]) : 0u);
-                    }
-            }
+                    for (int i = 0; i < 4; i++) s[t][h][i] = sees(t, mine + 16 * h + i) ? s[t][h][i] : -kInf;
         }
         bool move = false;
         float top[kCols];
@@ -252,53 +247,67 @@ struct Attention {
                 for (int i = 0; i < 4; i++)
                     if (h + i) top[t] = fmaxf(top[t], s[t][h][i]);
             top[t] *= qs[t];
-            move = move | (top[t] > ref[t] + kTop + kRoom);
-            if constexpr (kType == kKvI8) move = move | (vtop[t] > __builtin_bit_cast(uint32_t, ev[t]));
+            move = move | (top[t] > ref[t] + M::kTop + kRoom);
         }
         if (__ballot(move)) {
 #pragma unroll
             for (int t = 0; t < kCols; t++) {
                 const float m = column_max(top[t]);
                 float f = 1.0f;
-                if (m > ref[t] + kTop + kRoom) {
-                    f = __builtin_amdgcn_exp2f(ref[t] - (m - kTop));
-                    ref[t] = m - kTop;
+                if (m > ref[t] + M::kTop + kRoom) {
+                    f = __builtin_amdgcn_exp2f(ref[t] - (m - M::kTop));
+                    ref[t] = m - M::kTop;
                     l[t] *= f;
                 }
                 if constexpr (kType == kKvI8) {
-                    const uint32_t v = column_max(vtop[t]);
-                    if (v > __builtin_bit_cast(uint32_t, ev[t])) {
-                        const uint32_t e = min((v >> 23) + 1u, 253u);
-                        f *= ev[t] * as_float((254u - e) << 23);
-                        ev[t] = as_float(e << 23);
-                        if (v >= 0x7f800000u) l[t] = __builtin_nanf("");  // one that is not finite makes the row that sees it NaN
-                    }
-                }
+                    fall[t] = f;
+                } else {
 #pragma unroll
-                for (int d = 0; d < kTiles; d++) o[t][d] *= f;
+                    for (int d = 0; d < kTiles; d++) o[t][d] *= f;
+                }
             }
         }
     }
 
-    // Settled scores into probabilities, split for the second product.
-    __device__ __forceinline__ void probabilities(const f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts],
+    // Settled scores into probabilities (int8: times their values' scales vs), split for the second product.
+    __device__ __forceinline__ void probabilities(const f32x4 (&s)[kCols][2], u32x4 (&p)[kCols][M::kParts], bool masked, int first,
                                                   const f32x4 (&vs)[2]) {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             const float r = ref[t] == -kInf ? 0.0f : ref[t];
             float x[8];
-            float down = 0.0f;
-            if constexpr (kType == kKvI8) down = ev[t] > 0.0f ? as_float((254u << 23) - __builtin_bit_cast(uint32_t, ev[t])) : 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float v = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], qs[t], -r));
                     l[t] += v;
-                    x[4 * h + i] = v;
-                    // (a seen token's scale is at most ev; a hidden one's may be anything, and its probability is 0)
-                    if constexpr (kType == kKvI8) x[4 * h + i] = v * __builtin_amdgcn_fmed3f(vs[h][i] * down, 0.0f, 1.0f);
+                    x[4 * h + i] = kType == kKvI8 ? v * vs[h][i] : v;
                 }
+            if constexpr (kType == kKvI8) {
+                if (masked) {  // (a hidden token's scale may be anything, and its probability is 0)
+                    const int mine = first + ((threadIdx.x >> 4) & 3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = sees(t, mine + (i >> 2) * 16 + (i & 3)) ? x[i] : 0.0f;
+                }
+                float top = x[0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
+                if (__ballot(top > ev[t] * 16384.0f || fall[t] != 1.0f)) {
+                    top = column_max(top);
+                    if (top > ev[t] * 16384.0f || fall[t] != 1.0f) {
+                        const float was = ev[t] * fall[t];  // what o's unit is worth now
+                        const int e = min(max(max((int)(bits_of(was) >> 23), (int)(bits_of(top) >> 23) - 10), 1), 253);
+                        const float f = was * as_float((uint32_t)(254 - e) << 23);
+                        ev[t] = as_float((uint32_t)e << 23);
+#pragma unroll
+                        for (int d = 0; d < kTiles; d++) o[t][d] *= f;
+                    }
+                }
+                const float down = as_float((254u << 23) - bits_of(ev[t]));
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] *= down;
+            }
             M::split(x, p[t]);
         }
     }
@@ -347,23 +356,30 @@ struct Attention {
         }
     }
 
-    // After the last block: l over the column's lanes, int8's power of two back into o, NaN where bad values were noted.
+    // After the last block: l over the column's lanes, NaN where bad values were noted.
     __device__ __forceinline__ void close() {
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             l[t] = column_sum(l[t]);
-            if constexpr (kType == kKvI8) {
+            if constexpr (kType != kKvI8) {
+                if (__ballot((bad[t][0] | bad[t][1]) != 0)) {
 #pragma unroll
-                for (int d = 0; d < kTiles; d++) o[t][d] *= ev[t];
-            } else if (__ballot((bad[t][0] | bad[t][1]) != 0)) {
+                    for (int d = 0; d < kTiles; d++)
 #pragma unroll
-                for (int d = 0; d < kTiles; d++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[t][d][i] = bad[t][d >> 3] >> ((4 * d + i) & 31) & 1 ? __builtin_nanf("") : o[t][d][i];
+                        for (int i = 0; i < 4; i++) o[t][d][i] = bad[t][d >> 3] >> ((4 * d + i) & 31) & 1 ? __builtin_nanf("") : o[t][d][i];
+                }
             }
         }
     }
+    // Column t's four channels 16 d + 4 (lane / 16) .. + 3, times f, which is no more than one over the column's sum.
+    __device__ __forceinline__ f32x4 output(int t, int d, float f) const {
+        f32x4 y = o[t][d] * f;
+        if constexpr (kType == kKvI8) y *= ev[t];
+        return y;
+    }
 };
+// One over a sum of probabilities; a row that sees nothing has 0 and gives zeros.
+__device__ __forceinline__ float one_over(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
 // Key operands of a block's bytes, read through `load(byte)` (16 of them, this lane's), and value operands.
 template <int kType, int kDp, class Load>
@@ -718,7 +734,8 @@ struct BlockWalk {
     }
 };
 
-// Partial outputs of a piece: for each 16-column tile `ml` [16] references and [16] sums, and o as the lanes hold it.
+// Partial outputs of a piece: for each 16-column tile `ml` [16] references and [16] sums, and the outputs of the piece alone, divided by
+// its sums, as the lanes hold them.
 __host__ __device__ constexpr int part_floats(int cols, int dp) { return cols * (dp + 2); }
 
 }  // namespace ovfq

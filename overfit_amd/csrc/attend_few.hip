@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
             const bool masked = now.first + kKvBlock - 1 > first_last || now.first < last_low;
             u32x4 p[kCols][M::kParts];
             if (now.page >= 0) {
-                att.settle(s, masked, now.first, ks, vs);
-                att.probabilities(s, p, vs);
+                att.settle(s, masked, now.first, ks);
+                att.probabilities(s, p, masked, now.first, vs);
             }
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kKeyLoads + (kDepth - 1) * kLoadsOfBlock) : "memory");
             if (now.page >= 0) {
@@ -214,9 +214,9 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
         l[t] = 0.0f;
 #pragma unroll
         for (int v = 0; v < 4; v++) l[t] += sums[v][c] * __builtin_amdgcn_exp2f(refs[v][c] - m);
-        const float f = __builtin_amdgcn_exp2f(att.ref[t] - m);
+        const float f = __builtin_amdgcn_exp2f(att.ref[t] - m) * one_over(l[t]);
 #pragma unroll
-        for (int d = 0; d < Att::kTiles; d++) att.o[t][d] *= f;
+        for (int d = 0; d < Att::kTiles; d++) att.o[t][d] = att.output(t, d, f);
     }
     for (int from = 2; from >= 1; from >>= 1) {
         if (wave >= from && wave < 2 * from) {
@@ -253,19 +253,18 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
     for (int t = 0; t < kCols; t++) {
         const int c = w.col0 + 16 * t + col, i = c / cut.group;
         if (i >= w.rows) continue;
-        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
         float* y = a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim;
 #pragma unroll
         for (int d = 0; d < Att::kTiles; d++) {
             const int at = 16 * d + 4 * (lane >> 4);
-            if (at < pool.dim) *(f32x4u*)(y + at) = att.o[t][d] * inv;
+            if (at < pool.dim) *(f32x4u*)(y + at) = att.o[t][d];
         }
     }
 }
 
 }  // namespace
 
-// Joins the pieces of each tile: out = sum 2^(ref - top) o / sum 2^(ref - top) l, in a fixed order. A workgroup per 16 columns of a tile,
+// Joins the pieces of each tile: out = sum w o / sum w with w = 2^(ref - top) l, in a fixed order. A workgroup per 16 columns of a tile,
 // key head and 16 channels * `wide` (blockIdx.y; blockIdx.z: the tiles past what x takes): a thread has a column that is used and four
 // channels, and what is left of the workgroup's threads shares the pieces.
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut, int dp, int wide) {
@@ -306,7 +305,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut,
             l = 0.0f;
 #pragma unroll
             for (int k = 0; k < 16; k++) l += ls[k][col];
-            ls[0][col] = l;
+            ls[0][col] = one_over(l);
         }
         __syncthreads();
     }
@@ -318,11 +317,11 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut,
         const int col = live ? u % used : 0, quad = live ? u / used : 0, d = d0 + (quad >> 2), g = quad & 3;
         f32x4 o = {0, 0, 0, 0};
         if (live) {
-            const float m = tops[0][col];
+            const float m = tops[0][col], inv = ls[0][col];
             const float* mine = base + 32 * subs + ((sub * tiles + d) * 64 + g * 16 + col) * 4;
 #pragma unroll 4
             for (int j = share; j < w.pieces; j += shares) {
-                const float f = __builtin_amdgcn_exp2f(ml[j * stride + col] - m);
+                const float f = ml[j * stride + 16 + col] * __builtin_amdgcn_exp2f(ml[j * stride + col] - m) * inv;
                 o += *(const f32x4*)(mine + j * stride) * f;
             }
         }
@@ -334,9 +333,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, Cut cut,
         }
         if (!live || share) continue;
         const int c = first + col, i = c / cut.group, at = 16 * d + 4 * g;
-        const float l = ls[0][col], inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (at < pool.dim)
-            *(f32x4u*)(a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim + at) = o * inv;
+            *(f32x4u*)(a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim + at) = o;
     }
 }
 

@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
             att.scores(s, [&](int tile, int chunk) { return key_operand<kType, kDp>(tile, chunk, load); });
             const bool masked = first + kKvBlock - 1 > first_last || first < last_low;
             u32x4 p[kCols][M::kParts];
-            att.settle(s, masked, first, ks, vs);
-            att.probabilities(s, p, vs);
+            att.settle(s, masked, first, ks);
+            att.probabilities(s, p, masked, first, vs);
             att.products(p, [&](int tile) { return value_operand<kType, kDp>(tile, load); });
         }
         page = next;
@@ -119,13 +119,14 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
 #pragma unroll
         for (int t = 0; t < kCols; t++) {
             const int sub = wave * kCols + t;
+            const float inv = one_over(att.l[t]);
             if (lane < 16) {
                 part[32 * sub + lane] = att.ref[t];
                 part[32 * sub + 16 + lane] = att.l[t];
             }
 #pragma unroll
             for (int d = 0; d < Att::kTiles; d++)
-                *(f32x4*)(part + 32 * 4 * kCols + ((sub * Att::kTiles + d) * 64 + lane) * 4) = att.o[t][d];
+                *(f32x4*)(part + 32 * 4 * kCols + ((sub * Att::kTiles + d) * 64 + lane) * 4) = att.output(t, d, inv);
         }
         return;
     }
@@ -133,12 +134,12 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
     for (int t = 0; t < kCols; t++) {
         const int c = wave_col + 16 * t + col, i = c / cut.group;
         if (i >= w.rows) continue;
-        const float inv = att.l[t] == 0.0f ? 0.0f : 1.0f / att.l[t];
+        const float inv = one_over(att.l[t]);
         float* y = a.out + ((size_t)(w.first_row + i) * a.heads + head * cut.group + (c - i * cut.group)) * pool.dim;
 #pragma unroll
         for (int d = 0; d < Att::kTiles; d++) {
             const int at = 16 * d + 4 * (lane >> 4);
-            if (at < pool.dim) *(f32x4u*)(y + at) = att.o[t][d] * inv;
+            if (at < pool.dim) *(f32x4u*)(y + at) = att.output(t, d, inv);
         }
     }
 }
