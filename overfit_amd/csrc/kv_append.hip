@@ -3,8 +3,9 @@
 //   (a, b) -> (a c - b s, b c + a s) for pair j of a head, c and s = scale * cos and sin of position[axis_j] * freq_j
 // The pairs are neighbours (2 j, 2 j + 1) or halves (j, j + rotary / 2); channels past `rotary` stay.
 //
-// Angles are taken in turns in fp64, with the product's rounding error carried along, so a position of 2^31 has the same 2^-50 as a
-// near one, and cos and sin come from polynomials of the remainder (10^-13 off); both are rounded to fp32 once. Products and sums of
+// Angles are taken in turns in fp64, with the rounding errors of both products (position * freq has up to 55 bits) carried along, so a
+// position of 2^31 has the same 2^-50 as a near one, and cos and sin come from polynomials of the remainder (10^-13 off); both are
+// rounded to fp32 once. Products and sums of
 // the rotation are single fp32 operations; the rounding to the cache's type is the only other one, half a step of that type.
 //
 // Bound: HBM for many rows (each fp32 row is read once, written once), the launch and three dependent reads (offsets and length, page,
@@ -33,10 +34,10 @@ struct Turn {
     float c, s;
 };
 __device__ Turn turn_of(int position, float freq, float scale) {
-    const double a = (double)position * (double)freq;
+    const double a = (double)position * (double)freq, low = fma((double)position, (double)freq, -a);
     const double kInv = 0.15915494309189535, kInvLow = -9.839338337591243e-18;  // 1 / (2 pi) in two parts
     const double t = a * kInv;
-    const double rest = fma(a, kInv, -t) + a * kInvLow;
+    const double rest = fma(a, kInv, -t) + fma(a, kInvLow, low * kInv);
     double f = (t - rint(t)) + rest;  // in turns, [-1/2, 1/2]
     const double quarter = rint(f * 4.0);
     const double x = (f - quarter * 0.25) * 6.283185307179586;  // [-pi / 4, pi / 4]
