@@ -461,7 +461,9 @@ OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_bat
 /* The same over a few pages for each row and key head: the page of the row's own token, and of the full pages before it the top_pages - 1
  * whose mean key fits its query heads best (the largest q[m][h] . mean over the key head's h, in fp64; of equal fits the lower page, one
  * that is no number last). pages [rows][kv_heads][top_pages], if not NULL, receives their places in the request's table in rising order,
- * then -1. The cache keeps sums. Tables of up to OVFQ_MAX_SELECT_WIDTH pages; heads / kv_heads * head_dim at most 16384. */
+ * then -1. The cache keeps sums. Tables of up to OVFQ_MAX_SELECT_WIDTH pages; heads / kv_heads * head_dim at most 16384. The context's
+ * scratch holds the fits of as many rows as 128 MiB take, 8 * kv_heads * table_width bytes each (one row at least), and the pages if they
+ * are not asked for. */
 #define OVFQ_MAX_SELECT_WIDTH 65536
 #define OVFQ_MAX_TOP_PAGES 4096
 OVFQ_API int ovfq_attend_selected(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,

@@ -2101,6 +2101,7 @@ static int attend_impl(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* ba
     a.scale = scale;
     a.top = top;
     const size_t parts = top ? ovfq::attend_selected_scratch(a) : ovfq::attend_scratch(a);
+    a.fit_rows = top ? ovfq::attend_fit_rows(a) : 0;
     void* dev[4];
     float* o = out;
     int* chosen = pages;
@@ -2108,7 +2109,7 @@ static int attend_impl(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* ba
         a.parts = parts ? c.take<float>(parts) : nullptr;
         if (top) {
             a.where = c.take<int>(R * 4);
-            a.fits = c.take<double>(R * p.kv_heads * batch->table_width * sizeof(double));
+            a.fits = a.fit_rows ? c.take<double>((size_t)a.fit_rows * p.kv_heads * batch->table_width * sizeof(double)) : nullptr;
             if (host || !pages) chosen = c.take<int>(list);
         }
         if (!host) return;

@@ -26,12 +26,12 @@ __device__ __forceinline__ uint64_t ordered(double v) {
     return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-// A workgroup has `each` pages (a multiple of 64) of a row and key head. kWhole: heads of 128 or 256 channels.
+// A workgroup has `each` pages (a multiple of 64) of a row, from first_row on, and key head. kWhole: heads of 128 or 256 channels.
 template <bool kWhole>
-__global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int each) {
+__global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int first_row, int each) {
     extern __shared__ float queries[];  // [group][dim]
     const int kv_heads = a.pool.kv_heads, dim = a.pool.dim, group = a.heads / kv_heads;
-    const int row = (int)(blockIdx.x / (unsigned)kv_heads), head = (int)(blockIdx.x % (unsigned)kv_heads), tid = threadIdx.x;
+    const int row = first_row + (int)(blockIdx.x / (unsigned)kv_heads), head = (int)(blockIdx.x % (unsigned)kv_heads), tid = threadIdx.x;
     const float* q = a.q + ((size_t)row * a.heads + (size_t)head * group) * dim;
     for (int i = tid; i < group * dim; i += 256) queries[i] = q[i];
     __syncthreads();
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int each) {
     if (at.r < 0 || at.place < 0) return;
     const int pages = min(at.place / a.pool.page, a.batch.width), from = (int)blockIdx.y * each;
     if (pages < a.top || from >= pages) return;  // all of them are taken
-    uint64_t* out = (uint64_t*)a.fits + ((size_t)row * kv_heads + head) * a.batch.width;
+    uint64_t* out = (uint64_t*)a.fits + (size_t)blockIdx.x * a.batch.width;
     const int part = tid & 3;
     for (int p = from + (tid >> 2); p < min(pages, from + each); p += 64) {
         const int page = page_at(a, at.r, p);
@@ -78,19 +78,19 @@ __global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int each) {
 
 constexpr int kBins = 2048, kHeld = 8;  // kHeld: fits a thread keeps in registers
 
-__global__ __launch_bounds__(256) void choose_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) void choose_kernel(AttendArgs a, int first_row) {
     __shared__ int bins[kBins];
     __shared__ int waves[8];
     __shared__ uint32_t differ[8];
     __shared__ int bin_s, left_s;
     const int kv_heads = a.pool.kv_heads, tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const int row = (int)(blockIdx.x / (unsigned)kv_heads), head = (int)(blockIdx.x % (unsigned)kv_heads);
+    const int row = first_row + (int)(blockIdx.x / (unsigned)kv_heads), head = (int)(blockIdx.x % (unsigned)kv_heads);
     const KvRowPlace at = kv_row_place(a.batch, row, a.batch.most);
     if (head == 0 && tid == 0) a.where[row] = at.r;
     if (at.r < 0) return;
     const int own = at.place < 0 ? -1 : at.place / a.pool.page;
     const int pages = own < 0 ? 0 : min(own, a.batch.width), need = a.top - 1;
-    const uint64_t* fits = (const uint64_t*)a.fits + ((size_t)row * kv_heads + head) * a.batch.width;
+    const uint64_t* fits = (const uint64_t*)a.fits + (size_t)blockIdx.x * a.batch.width;
     const bool all = pages <= need;
     // the last fit taken: those above `bound` in the bits from `shift` on, and of those equal to it there the first `left`
     uint64_t bound = 0;
@@ -217,23 +217,37 @@ __global__ __launch_bounds__(256) void choose_kernel(AttendArgs a) {
 
 }  // namespace
 
+// Rows whose fits are kept at a time: all, but no more than kFitBytes of them where that is more than one row (4096 rows of eight key heads
+// over tables of 2048 pages would be 537 MB; in four turns of 134 MB they take as long, 5.3 ms with the attention over 16 pages each).
+int attend_fit_rows(const AttendArgs& a) {
+    constexpr size_t kFitBytes = 128u << 20;
+    if (a.top == 1 || a.batch.width < a.top) return 0;  // a row's own page alone, or all of them
+    const size_t row = (size_t)a.pool.kv_heads * a.batch.width * sizeof(double), rows = kFitBytes / row;
+    return rows >= (size_t)a.batch.rows ? a.batch.rows : rows ? (int)rows : 1;
+}
+
 hipError_t launch_select_pages(const AttendArgs& a, hipStream_t st) {
-    const int group = a.heads / a.pool.kv_heads;
-    const unsigned rows = (unsigned)a.batch.rows * (unsigned)a.pool.kv_heads;
-    if (a.batch.width >= a.top && a.top > 1) {
-        // 64 pages a workgroup, more where that gives more workgroups than the chip holds at a time
-        int each = 64;
-        while (each < 512 && (int64_t)rows * a.batch.width / each > 8192) each *= 2;
-        const dim3 grid(rows, (unsigned)((a.batch.width + each - 1) / each));
-        if (a.pool.dim % 128 == 0)
-            fit_kernel<true><<<grid, 256, (size_t)group * a.pool.dim * 4, st>>>(a, each);
-        else
-            fit_kernel<false><<<grid, 256, (size_t)group * a.pool.dim * 4, st>>>(a, each);
+    const int group = a.heads / a.pool.kv_heads, step = a.fit_rows ? a.fit_rows : a.batch.rows;
+    for (int first = 0; first < a.batch.rows; first += step) {
+        const int count = a.batch.rows - first < step ? a.batch.rows - first : step;
+        const unsigned rows = (unsigned)count * (unsigned)a.pool.kv_heads;
+        if (a.fit_rows) {
+            // 64 pages a workgroup, more where that gives more workgroups than the chip holds at a time
+            int each = 64;
+            while (each < 512 && (int64_t)rows * a.batch.width / each > 8192) each *= 2;
+            const dim3 grid(rows, (unsigned)((a.batch.width + each - 1) / each));
+            if (a.pool.dim % 128 == 0)
+                fit_kernel<true><<<grid, 256, (size_t)group * a.pool.dim * 4, st>>>(a, first, each);
+            else
+                fit_kernel<false><<<grid, 256, (size_t)group * a.pool.dim * 4, st>>>(a, first, each);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        choose_kernel<<<rows, 256, 0, st>>>(a, first);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    choose_kernel<<<rows, 256, 0, st>>>(a);
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace ovfq

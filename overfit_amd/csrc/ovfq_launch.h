@@ -409,11 +409,13 @@ struct AttendArgs {
     int top;
     int* chosen;  // [rows][kv_heads][top], the request's page numbers in rising order, then -1
     int* where;   // scratch [rows]: the row's request, or -1
-    double* fits;  // scratch [rows][kv_heads][width]
+    double* fits;  // scratch [fit_rows][kv_heads][width]
+    int fit_rows;  // rows whose pages are chosen at a time; 0: no row has a choice
 };
 size_t attend_scratch(const AttendArgs& a);
 hipError_t launch_attend(const AttendArgs& a, hipStream_t st);
 size_t attend_selected_scratch(const AttendArgs& a);  // for parts
+int attend_fit_rows(const AttendArgs& a);
 hipError_t launch_attend_selected(const AttendArgs& a, hipStream_t st);
 
 // GGUF Q8_0 (34-byte blocks) -> int8 quant plane + f32 scale plane.
