@@ -440,7 +440,8 @@ OVFQ_API int ovfq_kv_append(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* bat
  * The host form refuses offsets that do not start at 0, fall or do not end at rows, more rows than max_rows, lengths below a request's rows
  * or past its table, pages outside the cache, and pages that two requests of the call would write. Here a request whose offsets fall or
  * leave the rows has no rows; rows of no request are left as they were; a token before the first, past the table or in a page outside the
- * cache is not stored (its query is turned all the same). Offsets of different requests must not overlap, nor q_out k, v or (without being it) q. */
+ * cache is not stored (its query is turned all the same). Offsets of different requests must not overlap, nor
+ * q_out any input but the q that it is. */
 OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch, const float* k, const float* v, int rows,
                                 const ovfq_rope* rope, const int* positions, const float* q, int heads, float* q_out);
 
@@ -454,7 +455,7 @@ OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch*
  * is left out (its rows of `out` stay as they were), and offsets count as there. Host pointers, synchronous. */
 OVFQ_API int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
                          float scale, int window, float* out);
-/* As ovfq_attend, with device pointers (enqueued on the context's stream); out must not overlap q. */
+/* As ovfq_attend, with device pointers (enqueued on the context's stream); out must not overlap an input. */
 OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
                              float scale, int window, float* out);
 
@@ -468,7 +469,7 @@ OVFQ_API int ovfq_attend_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_bat
 #define OVFQ_MAX_TOP_PAGES 4096
 OVFQ_API int ovfq_attend_selected(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
                                   int heads, float scale, int top_pages, float* out, int* pages);
-/* As ovfq_attend_selected, with device pointers (enqueued on the context's stream); out must not overlap q. */
+/* As ovfq_attend_selected, with device pointers (enqueued on the context's stream); neither out nor pages may overlap an input or each other. */
 OVFQ_API int ovfq_attend_selected_dev(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows,
                                       int heads, float scale, int top_pages, float* out, int* pages);
 

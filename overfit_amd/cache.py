@@ -157,8 +157,15 @@ def _rows_of(x, width, name):
 
 
 def _overlap(a, b):
-    """Whether two planes of fp32 values share memory."""
+    """Whether two planes of 32-bit values share memory."""
     return a is not None and b is not None and a.ptr < b.ptr + 4 * b.size and b.ptr < a.ptr + 4 * a.size
+
+
+def _apart(name, written, **others):
+    """Refuses an output that shares memory with what the call reads or writes besides."""
+    for other, b in others.items():
+        if _overlap(written, b):
+            raise OverfitArgumentError(f"{name} overlaps {other}")
 
 
 def _batch(row_offsets, lengths, tables, max_rows):
@@ -215,10 +222,9 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
     elif q_out is not None:
         raise OverfitArgumentNullError("q_out without q")
     yb = _sized(as_buf(q_out, np.float32, "q_out", allow_none=True), rows * heads * cache.head_dim, "q_out")
+    ob, lb, tb = side
+    _apart("q_out", yb, k=kb, v=vb, q=None if yb is not None and yb.ptr == qb.ptr else qb, row_offsets=ob, lengths=lb, tables=tb)
     side += [kb, vb, qb, yb]
-    for name, b in (("k", kb), ("v", vb), ("q", qb)):
-        if _overlap(yb, b) and not (b is qb and yb.ptr == qb.ptr):
-            raise OverfitArgumentError(f"q_out overlaps {name}")
     rs = pb = None
     if rope is not None:
         if not isinstance(rope, Rope):
@@ -235,6 +241,7 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
         xb = _sized(as_buf(rope.pair_axes, np.int32, "pair_axes", allow_none=True), fb.size, "pair_axes")
         if pb is None and xb is not None:
             axes = _lib.MAX_ROPE_AXES  # every axis has the token's place
+        _apart("q_out", yb, inv_freq=fb, positions=pb, pair_axes=xb)
         side += [fb, pb, xb]
         rs = _lib.RopeStruct(2 * fb.size, Rope.STYLES[rope.style], axes, rope.scale, fb.ptr, _ptr(xb))
     elif positions is not None:
@@ -268,18 +275,19 @@ def _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max
         raise OverfitArgumentOutOfRangeError(f"window ({window}) must not be negative")
     if out is None:
         out = _empty(qb, qb.size).reshape(tuple(q.shape))
-    ob = _sized(as_buf(out, np.float32, "out"), qb.size, "out")
-    if _overlap(ob, qb):
-        raise OverfitArgumentError("out overlaps q")
-    side += [qb, ob]
+    yb = _sized(as_buf(out, np.float32, "out"), qb.size, "out")
+    ob, lb, tb = side
+    _apart("out", yb, q=qb, row_offsets=ob, lengths=lb, tables=tb)
+    side += [qb, yb]
     args = (ctypes.byref(batch), qb.ptr, rows, heads, scale)
     if top is None:
-        return _call(cache, ctx, "ovfq_attend", side, (*args, window, ob.ptr), batch), out
+        return _call(cache, ctx, "ovfq_attend", side, (*args, window, yb.ptr), batch), out
     if not 1 <= top <= _lib.MAX_TOP_PAGES:
         raise OverfitArgumentOutOfRangeError(f"top_pages ({top}) must be in [1, {_lib.MAX_TOP_PAGES}]")
     pb = _sized(as_buf(pages, np.int32, "pages", allow_none=True), rows * cache.kv_heads * top, "pages")
+    _apart("pages", pb, q=qb, out=yb, row_offsets=ob, lengths=lb, tables=tb)
     side.append(pb)
-    return _call(cache, ctx, "ovfq_attend_selected", side, (*args, top, ob.ptr, _ptr(pb)), batch), out
+    return _call(cache, ctx, "ovfq_attend_selected", side, (*args, top, yb.ptr, _ptr(pb)), batch), out
 
 
 def attend(cache, q, row_offsets, lengths, tables, out=None, scale=None, window=0, max_rows=0):

@@ -1944,10 +1944,15 @@ static int check_kv_call(const ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_b
     return OVFQ_OK;
 }
 
-// Planes of floats that a kernel reads and writes at once must be apart.
-static bool overlap(const float* a, size_t a_bytes, const float* b, size_t b_bytes) {
+// What a kernel reads and writes at once must be apart.
+static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+static bool overlap_batch(const void* a, size_t a_bytes, const ovfq_kv_batch* b) {
+    const size_t n = (size_t)b->requests;
+    return overlap(a, a_bytes, b->row_offsets, (n + 1) * 4) || overlap(a, a_bytes, b->lengths, n * 4) ||
+           overlap(a, a_bytes, b->tables, n * b->table_width * 4);
 }
 
 static int check_heads(const ovfq_kv* kv, int rows, int heads) {
@@ -2005,6 +2010,9 @@ static int kv_append_impl(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch* batch
         if (overlap(q_out, query_bytes, k, key_bytes) || overlap(q_out, query_bytes, v, key_bytes) ||
             (q_out != q && overlap(q_out, query_bytes, q, query_bytes)))
             return fail(OVFQ_ERR_SIZE, "q_out overlaps k, v or, without being it, q");
+        if (overlap_batch(q_out, query_bytes, batch) || overlap(q_out, query_bytes, positions, R * rope->axes * 4) ||
+            overlap(q_out, query_bytes, rope->inv_freq, half * 4) || overlap(q_out, query_bytes, rope->pair_axes, half * 4))
+            return fail(OVFQ_ERR_SIZE, "q_out overlaps the batch's arrays, positions or the rope's");
     }
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
@@ -2088,7 +2096,10 @@ static int attend_impl(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* ba
     const size_t R = (size_t)rows, Q = (size_t)batch->requests, plane = R * heads * p.dim * 4, list = R * p.kv_heads * top * 4;
     if (!host && (rc_align(q) || rc_align(out) || rc_align(pages)))
         return fail(OVFQ_ERR_SIZE, "device pointers must be 4-byte aligned");
-    if (!host && overlap(out, plane, q, plane)) return fail(OVFQ_ERR_SIZE, "out overlaps q");
+    if (!host && (overlap(out, plane, q, plane) || overlap_batch(out, plane, batch)))
+        return fail(OVFQ_ERR_SIZE, "out overlaps q or the batch's arrays");
+    if (!host && (overlap(pages, list, q, plane) || overlap(pages, list, out, plane) || overlap_batch(pages, list, batch)))
+        return fail(OVFQ_ERR_SIZE, "pages overlap q, out or the batch's arrays");
     std::lock_guard<std::mutex> lk(ctx->mu);
     HIP_TRY(hipSetDevice(ctx->device));
     const void* in[4] = {batch->row_offsets, batch->lengths, batch->tables, q};
