@@ -156,6 +156,21 @@ def _rows_of(x, width, name):
     return x.size // width
 
 
+def _query_rows(q, qb, rows, requests, dim):
+    """Rows of a plane of queries: the given number, or its first axis ([rows][heads * dim] or [rows][heads][dim]); a plane of one axis is one
+    row's, so of one request."""
+    axes = len(q.shape)
+    if rows is None:
+        if axes == 1 and requests > 1:
+            raise OverfitArgumentError(f"q of one axis beside {requests} requests: give rows")
+        if axes > 3 or (axes == 3 and q.shape[2] != dim):
+            raise OverfitArgumentError(f"q of shape {tuple(q.shape)} is neither [rows][heads * {dim}] nor [rows][heads][{dim}]: give rows")
+        rows = int(q.shape[0]) if axes > 1 else 1
+    if rows <= 0 or qb.size == 0 or qb.size % (rows * dim):
+        raise OverfitArgumentError(f"q has {qb.size} elements, not whole heads of {dim} for each of {rows} rows")
+    return rows
+
+
 def _overlap(a, b):
     """Whether two planes of 32-bit values share memory."""
     return a is not None and b is not None and a.ptr < b.ptr + 4 * b.size and b.ptr < a.ptr + 4 * a.size
@@ -193,7 +208,7 @@ def _call(cache, ctx, name, side, args, keep):
     return BoundCall(ctx, fn, (ctx.handle, cache.handle, *args), (cache, side, keep))
 
 
-def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows, ctx=None):
+def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows, rows=None, ctx=None):
     batch, side = _batch(row_offsets, lengths, tables, max_rows)
     kb, vb = as_buf(k, np.float32, "k", allow_none=True), as_buf(v, np.float32, "v", allow_none=True)
     qb = as_buf(q, np.float32, "q", allow_none=True)
@@ -201,19 +216,18 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
         raise OverfitArgumentNullError("k and v go together")
     if kb is None and qb is None:
         raise OverfitArgumentNullError("k, v and q are None")
-    rows = 0
     if kb is not None:
-        rows = _rows_of(kb, cache.kv_heads * cache.head_dim, "k")
+        of_keys = _rows_of(kb, cache.kv_heads * cache.head_dim, "k")
         if vb.size != kb.size:
             raise OverfitArgumentError(f"k has {kb.size} elements, v {vb.size}")
+        if rows not in (None, of_keys):
+            raise OverfitArgumentError(f"k has {of_keys} rows, not {rows}")
+        rows = of_keys
     heads = 0
     if qb is not None:
         if rope is None:
             raise OverfitArgumentNullError("q without a rope")
-        if not rows:
-            rows = int(q.shape[0]) if len(q.shape) > 1 else 1
-        if rows <= 0 or qb.size == 0 or qb.size % (rows * cache.head_dim):
-            raise OverfitArgumentError(f"q has {qb.size} elements, not whole heads of {cache.head_dim} for each of {rows} rows")
+        rows = _query_rows(q, qb, rows, batch.requests, cache.head_dim)
         heads = qb.size // (rows * cache.head_dim)
         if heads % cache.kv_heads:
             raise OverfitArgumentError(f"heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
@@ -250,21 +264,20 @@ def _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, posi
     return _call(cache, ctx, "ovfq_kv_append", side, args, (batch, rs)), q_out
 
 
-def kv_append(cache, k, v, row_offsets, lengths, tables, q=None, q_out=None, rope=None, positions=None, max_rows=0):
+def kv_append(cache, k, v, row_offsets, lengths, tables, q=None, q_out=None, rope=None, positions=None, max_rows=0, rows=None):
     """New tokens into the cache (ovfq_kv_append[_dev]): k and v [rows][kv_heads * head_dim], k turned by its position and both rounded to
     the cache's type; q [rows][heads * head_dim] turned likewise. k and v may be None together (queries only). positions
-    [axes][rows] (int32): each token's place in its request if None. Returns the turned queries (None without q)."""
-    call, q_out = _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows)
+    [axes][rows] (int32): each token's place in its request if None. rows: of k, or of q alone as attend takes it. Returns the turned queries
+    (None without q)."""
+    call, q_out = _append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows, rows)
     call()
     return q_out
 
 
-def _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, top, pages, ctx=None):
+def _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, top, pages, rows=None, ctx=None):
     batch, side = _batch(row_offsets, lengths, tables, max_rows)
     qb = as_buf(q, np.float32, "q")
-    rows = int(q.shape[0]) if len(q.shape) > 1 else 1
-    if rows <= 0 or qb.size == 0 or qb.size % (rows * cache.head_dim):
-        raise OverfitArgumentError(f"q has {qb.size} elements, not whole heads of {cache.head_dim} for each of {rows} rows")
+    rows = _query_rows(q, qb, rows, batch.requests, cache.head_dim)
     heads = qb.size // (rows * cache.head_dim)
     if heads % cache.kv_heads:
         raise OverfitArgumentError(f"heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
@@ -290,18 +303,19 @@ def _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max
     return _call(cache, ctx, "ovfq_attend_selected", side, (*args, top, yb.ptr, _ptr(pb)), batch), out
 
 
-def attend(cache, q, row_offsets, lengths, tables, out=None, scale=None, window=0, max_rows=0):
-    """Attention of each request's new tokens, already appended, over its pages (ovfq_attend[_dev]): q [rows][heads * head_dim], causal,
-    over the last `window` tokens of each row (0: all). scale: 1 / sqrt(head_dim) if None. max_rows bounds every request's rows (0: not
-    known), which sizes the launches: give 1 for a decode step. Returns the output, laid out as q."""
-    call, out = _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, None, None)
+def attend(cache, q, row_offsets, lengths, tables, out=None, scale=None, window=0, max_rows=0, rows=None):
+    """Attention of each request's new tokens, already appended, over its pages (ovfq_attend[_dev]): q [rows][heads * head_dim] or
+    [rows][heads][head_dim] (laid out otherwise: `rows` says how many there are; without it a plane of one axis is one row), causal, over
+    the last `window` tokens of each row (0: all). scale: 1 / sqrt(head_dim) if None. max_rows bounds every request's rows (0: not known),
+    which sizes the launches: give 1 for a decode step. Returns the output, laid out as q."""
+    call, out = _attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, None, None, rows)
     call()
     return out
 
 
-def attend_selected(cache, q, row_offsets, lengths, tables, top_pages, out=None, pages=None, scale=None, max_rows=0):
+def attend_selected(cache, q, row_offsets, lengths, tables, top_pages, out=None, pages=None, scale=None, max_rows=0, rows=None):
     """The same over top_pages pages for each row and key head (ovfq_attend_selected[_dev]): its own and the full pages before it whose mean
     key fits its queries best. The cache keeps sums. pages [rows][kv_heads][top_pages] (int32) receives them if given."""
-    call, out = _attend_call(cache, q, row_offsets, lengths, tables, out, scale, 0, max_rows, top_pages, pages)
+    call, out = _attend_call(cache, q, row_offsets, lengths, tables, out, scale, 0, max_rows, top_pages, pages, rows)
     call()
     return out

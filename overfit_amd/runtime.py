@@ -185,29 +185,30 @@ class Context:
         return _device_call(_verify_call(logits, vocab, row_offsets, draft_tokens, accept_uniforms, final_uniforms,
                                          draft_probs, temperature, accepted, tokens, self)[0])
 
-    def bind_kv_append_dev(self, cache, k, v, row_offsets, lengths, tables, q=None, q_out=None, rope=None, positions=None, max_rows=0):
+    def bind_kv_append_dev(self, cache, k, v, row_offsets, lengths, tables, q=None, q_out=None, rope=None, positions=None, max_rows=0,
+                           rows=None):
         """`cache.kv_append` on device tensors with its arguments converted once (see bind_multi_dev); q_out is given beside q."""
         from .cache import _append_call
 
         if q is not None and q_out is None:
             raise ValueError("a prepared call needs its outputs")
-        return _device_call(_append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows, self)[0])
+        return _device_call(_append_call(cache, k, v, row_offsets, lengths, tables, q, q_out, rope, positions, max_rows, rows, self)[0])
 
-    def bind_attend_dev(self, cache, q, row_offsets, lengths, tables, out, scale=None, window=0, max_rows=0):
+    def bind_attend_dev(self, cache, q, row_offsets, lengths, tables, out, scale=None, window=0, max_rows=0, rows=None):
         """`cache.attend` on device tensors with its arguments converted once; out is given."""
         from .cache import _attend_call
 
         if out is None:
             raise ValueError("a prepared call needs its outputs")
-        return _device_call(_attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, None, None, self)[0])
+        return _device_call(_attend_call(cache, q, row_offsets, lengths, tables, out, scale, window, max_rows, None, None, rows, self)[0])
 
-    def bind_attend_selected_dev(self, cache, q, row_offsets, lengths, tables, top_pages, out, pages=None, scale=None, max_rows=0):
+    def bind_attend_selected_dev(self, cache, q, row_offsets, lengths, tables, top_pages, out, pages=None, scale=None, max_rows=0, rows=None):
         """`cache.attend_selected` on device tensors with its arguments converted once; out is given."""
         from .cache import _attend_call
 
         if out is None:
             raise ValueError("a prepared call needs its outputs")
-        return _device_call(_attend_call(cache, q, row_offsets, lengths, tables, out, scale, 0, max_rows, top_pages, pages, self)[0])
+        return _device_call(_attend_call(cache, q, row_offsets, lengths, tables, out, scale, 0, max_rows, top_pages, pages, rows, self)[0])
 
     def project_multi_prequantized_dev(self, weights, q, s, b, ys, biases=None, rows=1):
         n = len(weights)
