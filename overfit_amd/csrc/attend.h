@@ -402,6 +402,9 @@ __device__ __forceinline__ u32x4 value_operand(int tile, Load load) {
     }
 }
 
+// The first token that a row at `last` sees; before the first token it sees none, whatever this says.
+__device__ __forceinline__ int first_seen(int last, int window) { return window ? max(max(last, 0) - window + 1, 0) : 0; }
+
 // How a launch cuts its work. A request of `least` to `most` columns has tiles of `cols` columns (2^cols_log2), and a tile's blocks are
 // cut into pieces of the same size, none of fewer blocks than least_blocks. `target` is the number of workgroups that the chip holds at
 // a time, for each key head. Fewer tiles are cut into the smallest pieces that still are no more than that: a workgroup more is a round

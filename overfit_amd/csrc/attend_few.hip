@@ -74,12 +74,12 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
         const int qh = head * cut.group + (c - i * cut.group), last = w.place + i;
         typename Att::Row row;
         Att::fetch(row, a.q + ((size_t)(w.first_row + i) * a.heads + qh) * pool.dim, i < w.rows, pool.dim);
-        att.column(t, i < w.rows, a.window ? max(last - a.window + 1, 0) : 0, last);
+        att.column(t, i < w.rows, first_seen(last, a.window), last);
         att.query(t, row, i < w.rows, pool.dim, a.scale * kLog2e);
     }
     const int first_last = w.place + w.col0 / cut.group;  // the tile's rows see up to first_last .. last_last
     const int last_last = w.place + min(w.rows - 1, (w.col0 + 16 * kCols - 1) / cut.group);
-    const int last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+    const int last_low = first_seen(last_last, a.window);
 
     const int* table = b.tables + (size_t)w.r * b.width;
     BlockWalk walk;

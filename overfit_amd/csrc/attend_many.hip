@@ -59,17 +59,17 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
 #pragma unroll
     for (int t = 0; t < kCols; t++) {
         const int i = (wave_col + 16 * t + col) / cut.group, last = w.place + i;
-        att.column(t, i < w.rows, a.window ? max(last - a.window + 1, 0) : 0, last);
+        att.column(t, i < w.rows, first_seen(last, a.window), last);
         att.query(t, rows[t], i < w.rows, pool.dim, a.scale * kLog2e);
     }
     // what the wave's rows see
     const int i0 = wave_col / cut.group, i1 = min(w.rows - 1, (wave_col + 16 * kCols - 1) / cut.group);
     const bool live = i0 < w.rows;
     const int first_last = w.place + i0, last_last = w.place + i1;
-    const int first_low = a.window ? max(first_last - a.window + 1, 0) : 0, last_low = a.window ? max(last_last - a.window + 1, 0) : 0;
+    const int first_low = first_seen(first_last, a.window), last_low = first_seen(last_last, a.window);
     // and the least that a column of the tile sees
     const int tile_last = w.place + w.col0 / cut.group;
-    const int tile_low = a.window ? max(w.place + min(w.rows - 1, (w.col0 + 64 * kCols - 1) / cut.group) - a.window + 1, 0) : 0;
+    const int tile_low = first_seen(w.place + min(w.rows - 1, (w.col0 + 64 * kCols - 1) / cut.group), a.window);
 
     for (int i = 0; i < blocks; i++) {
         const int next = i + 1 < blocks ? walk.page(i + 1) : -1;

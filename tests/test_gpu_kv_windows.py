@@ -1,0 +1,25 @@
+"""Windows of any length over requests that are shorter than their rows."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+ov = pytest.importorskip("overfit_amd")
+from kvdata import Requests, case  # noqa: E402
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 40, 1 << 30, 1000])
+@pytest.mark.parametrize("rows,length,most", [(60, 45, 0), (60, 20, 60), (9, 5, 0), (9, 5, 9), (400, 300, 0)])
+def test_windows_longer_than_what_is_there(window, rows, length, most):
+    """A row whose place would be before the first token sees none of them, the others all up to theirs: as without a window."""
+    case("window", window, rows, length, most)
+    rng = np.random.default_rng(61)
+    req = Requests(ov, rng, "f16", 2, 64, 32, [rows], [0]).fill()
+    q = req.t(rng.standard_normal((rows, 256)).astype(np.float32))
+    off, _, tables = req.batch()
+    lengths = req.t(np.array([length], np.int32))
+    want = ov.attend(req.cache, q, off, lengths, tables, max_rows=most)
+    got = ov.attend(req.cache, q, off, lengths, tables, window=window, max_rows=most)
+    assert not want[:rows - length].any() and want[rows - length:].abs().sum(1).min() > 0
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
