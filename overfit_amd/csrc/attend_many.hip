@@ -151,14 +151,15 @@ __global__ __launch_bounds__(1024) void attend_plan_kernel(KvPool pool, KvBatch 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     float sum = 0.0f;
     int tiles = 0, longest = 0;
+    constexpr int kMostTiles = 1 << 24;  // more than a launch has room for: offsets that overlap may give any number, past 32 bits as well
     for (int r = tid; r < b.requests; r += 1024) {
         const CutRequest q = cut_load(c, pool, b, r);
         sum += q.sum;
-        tiles += q.tiles;
+        tiles = min(tiles + q.tiles, kMostTiles);
         longest = max(longest, q.blocks);
     }
     sum = wave_sum(sum);
-    tiles = wave_sum(tiles);
+    tiles = min(wave_sum(tiles), kMostTiles);
     longest = wave_max(longest);
     if (lane == 0) {
         sums[wave] = sum;
