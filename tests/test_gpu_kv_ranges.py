@@ -140,6 +140,36 @@ def test_finite_scales_that_rows_see(which, value, rows, context, token):
                 check(got[row, at], without[row, at], err_without[row, at], (row, h), whole=False)
 
 
+@pytest.mark.parametrize("value", [np.inf, 3e38])
+@pytest.mark.parametrize("rows,context,token", [(4, 60, 61), (4, 60, 3), (60, 10, 40), (60, 100, 131), (1, 2000, 900)])
+def test_scores_past_fp32(value, rows, context, token):
+    """A key's scale that makes its scores infinite: above all others the row is no number, below it is what is left without the token.
+    A score is one as a power of two: past 2^128 / log2(e)."""
+    rng = np.random.default_rng(23)
+    req = Requests(ov, rng, "i8", 2, 64, 32, [rows], [context]).fill()
+    q = rng.standard_normal((rows, 4 * 64)).astype(np.float32)
+    put(req, 0, token, 0, value)
+    got = ov.attend(req.cache, req.t(q), *req.batch()).cpu().numpy()
+    without, err = attention(req, q, 4, keep=lambda row, a, seen: seen != token)
+    plain, err_plain = attention(req, q, 4)
+    quants, v = quantised(req.k[0])[0], as_stored(req.v[0], "i8")
+    for row in range(rows):
+        for h in range(4):
+            at = slice(h * 64, (h + 1) * 64)
+            if row < max(token - context, 0):
+                check(got[row, at], plain[row, at], err_plain[row, at], (row, h), whole=False)
+                continue
+            score = quants[token, h // 2].astype(np.float64) @ q[row, at]
+            size = abs(score) * value / 8 * math.log2(math.e) / 2.0 ** 128
+            assert abs(score) > 0.1 and not 0.99 < size < 1.01
+            if score > 0 and size < 1:
+                check(got[row, at], v[token, h // 2], np.abs(v[token, h // 2]) * 2.0 ** -20, (row, h), whole=False)
+            elif score > 0:
+                assert np.isnan(got[row, at]).all()
+            else:
+                check(got[row, at], without[row, at], err[row, at], (row, h), whole=False)
+
+
 @pytest.mark.parametrize("type_", ["f16", "bf16", "i8"])
 @pytest.mark.parametrize("rows", [1, 60])
 def test_a_query_with_one_large_channel(type_, rows):
