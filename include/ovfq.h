@@ -450,9 +450,11 @@ OVFQ_API int ovfq_kv_append_dev(ovfq_ctx* ctx, ovfq_kv* kv, const ovfq_kv_batch*
  *   out[m][h] = sum over tokens j, p - window < j <= p (window 0: 0 <= j <= p), of softmax(scale q[m][h] . k_j) v_j
  * heads is a multiple of kv_heads. A channel of q enters the products to 2^-23 of its row's largest one, a probability to 2^-22 of itself
  * or 2^-34 of the row's largest (OVFQ_TYPE_I8: of the largest after each is multiplied by its value's scale); sums are fp32. Keys are
- * below 2^118 and scores fit fp32; values may have any size, in OVFQ_TYPE_BF16 caches beyond 2^116 in up to 4096 tokens of like weight. Tokens in pages outside the cache count as hidden; a row that sees no token gives 0. What is not finite stays in the rows
+ * below 2^118 and scores times log2(e) fit fp32; values may have any size, in OVFQ_TYPE_BF16 caches beyond 2^116 in up to 4096 tokens of
+ * like weight. Tokens in pages outside the cache count as hidden; a row that sees no token gives 0. What is not finite stays in the rows
  * that see it. The host form refuses what ovfq_kv_append does, but for shared pages; in the other a request of more than max_rows rows
- * is left out (its rows of `out` stay as they were), and offsets count as there. Host pointers, synchronous. */
+ * is left out (its rows of `out` stay as they were), and offsets count as there. The context's scratch holds partial outputs, of up to
+ * 250 MB whatever the rows and lengths (500 past 512 key heads). Host pointers, synchronous. */
 OVFQ_API int ovfq_attend(ovfq_ctx* ctx, const ovfq_kv* kv, const ovfq_kv_batch* batch, const float* q, int rows, int heads,
                          float scale, int window, float* out);
 /* As ovfq_attend, with device pointers (enqueued on the context's stream); out must not overlap an input. */

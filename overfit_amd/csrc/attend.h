@@ -18,7 +18,8 @@
 // reference, so that the product fits fp32); what enters the second product is p scale / e, with a power of two e kept for the column
 // that puts the largest p scale so far between 2^10 and 2^15. Both move with the column's reference, so a large scale of little weight
 // takes nothing from the others. (Against the largest scale seen, whatever its weight, a token of 2^36 times the others' scales and no
-// weight made zeros of the rows that saw it.)
+// weight made zeros of the rows that saw it. What the largest product costs: a prompt of 4096 rows 312 -> 323 us, 60 drafted rows 84.0 ->
+// 84.7. A bound of it, checked with the reference, spilled registers: 419 and 503.)
 //
 // Masks: a hidden token's score is -inf whatever its key holds. A hidden token's value meets a probability of zero, which would still
 // make NaN of what is not finite, so blocks with a mask look at their values first: what is not finite is noted for the columns that see
@@ -329,7 +330,7 @@ struct Attention {
     }
 
     // Notes which columns see values that are not finite: ones in their places times ones for the tokens seen.
-    template <int kUnrollNotes, class Value>
+    template <class Value>
     __device__ __forceinline__ void note_bad(int first, Value value) {
         constexpr uint32_t kOne = kType == kKvBf16 ? 0x3f80u : 0x3c00u;
         const int mine = first + ((threadIdx.x >> 4) & 3) * 4;
@@ -342,7 +343,7 @@ struct Attention {
                 seen[i >> 1] |= j <= lim[t] && j >= low[t] ? kOne << (16 * (i & 1)) : 0u;
             }
             uint64_t found = 0;
-#pragma unroll kUnrollNotes
+#pragma unroll 1
             for (int d = 0; d < kTiles; d++) {
                 u32x4 a = not_finite<kType>(value(d));
 #pragma unroll

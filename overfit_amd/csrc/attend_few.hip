@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256, kDp <= 128 ? 2 : 1) void attend_few_kernel(Att
                         bool any = false;
                         for (int k = 0; k < kLoads; k++) any = any | any_not_finite<kType>(*(const u32x4*)(at + kPlane + k * 1024));
                         if (__ballot(any)) {
-                            att.template note_bad<1>(now.first, value);
+                            att.note_bad(now.first, value);
                             for (int k = 0; k < kLoads; k++) {
                                 u32x4* v = (u32x4*)(place + kPlane + k * 1024 + lane * 16);
                                 *v = finite_part<kType>(*v);

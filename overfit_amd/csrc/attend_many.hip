@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a, Cut c
                 bool any = false;
                 for (int k = threadIdx.x * 16; k < kPlane; k += 4096) any = any | any_not_finite<kType>(*(const u32x4*)(values + k));
                 if (__syncthreads_or(any)) {
-                    att.template note_bad<1>(first, [&](int tile) { return *(const u32x4*)(values + tile * 1024 + lane * 16); });
+                    att.note_bad(first, [&](int tile) { return *(const u32x4*)(values + tile * 1024 + lane * 16); });
                     __syncthreads();
                     for (int k = threadIdx.x * 16; k < kPlane; k += 4096) *(u32x4*)(values + k) = finite_part<kType>(*(const u32x4*)(values + k));
                     __syncthreads();
@@ -203,16 +203,23 @@ constexpr int kItems = 512;  // two workgroups a CU: registers and LDS
 // (single rows of 256 tokens: 65 requests 28.5 us with it and 25.9 without, 130 40.2 / 41.6, 300 73.9 / 93.1, 4096 835 / 4883).
 constexpr int kPlanned = 128;
 
+// A piece has at least so many blocks (8; with 4 and 16: one row over 1500 tokens 12.7 us, 12.2, 14.2; 64 rows over 2000 23.9, 24.3, 32.2; a
+// prompt of 512 rows 26.2, 26.9, 29.7), and where there are tiles enough, one is cut if it is longer than so many times a workgroup's mean
+// share: beside tiles of many columns 1.5 (with 1.0 and 2.5: a prompt of 2048 rows 95 us, 116, 105), of few 2 (with 1.5 and 3: 100 single
+// rows over 100 to 16 k tokens 325, 332, 373).
+constexpr int kLeastBlocks = 8;
+constexpr float kSlackMany = 1.5f, kSlackFew = 2.0f;
+
 struct Plan {
     Cut cut;
-    bool few, split;
+    bool split;
     unsigned items, tiles;  // most of a key head
 };
 
 // Which kernels a call takes: the few-column one where no request has more columns than it takes; else the other one, and the first
 // beside it for the requests that it takes if the rows behind the longest request's are that few for each (a decode step with a chunk of a
-// prompt in it: 512 rows over 8 k beside 31 single ones 341 us, all of them in the many-column kernel 457, where they waste three
-// waves of four). A launch for nothing costs 13 us with its join, so prompts alone have one.
+// prompt in it: 512 rows over 8 k beside 31 single ones 344 us, all of them in the many-column kernel 457, where they waste three
+// waves of four). A launch for nothing costs 6 to 8 us with its join, so prompts alone have one.
 struct Kinds {
     bool few, many;
 };
@@ -226,7 +233,6 @@ Plan plan_attend(const AttendArgs& a, bool few) {
     const Kinds kinds = kinds_of(a);
     const int group = a.heads / a.pool.kv_heads, requests = a.batch.requests < a.batch.rows ? a.batch.requests : a.batch.rows;
     Plan p{};
-    p.few = few;
     p.split = true;
     int64_t most = (int64_t)a.batch.most * group;
     if (few && most > few_columns(a)) most = few_columns(a);
@@ -234,7 +240,7 @@ Plan plan_attend(const AttendArgs& a, bool few) {
     const int64_t usual = kinds.many ? (int64_t)(a.batch.rows - a.batch.most) * group / (requests > 1 ? requests - 1 : 1) : most;
     const int log2 = few ? (usual <= 16 ? 4 : 5) : a.pool.dp <= 128 ? 7 : 6;
     const int least = !few && kinds.few ? few_columns(a) + 1 : 1;
-    p.cut = Cut{log2, least, (int)most, ceil_div(kItems, a.pool.kv_heads), 8, few ? 2.0f : 1.5f, a.window, group, 0, 0, 0};
+    p.cut = Cut{log2, least, (int)most, ceil_div(kItems, a.pool.kv_heads), kLeastBlocks, few ? kSlackFew : kSlackMany, a.window, group, 0, 0, 0};
     p.tiles = (unsigned)(few ? requests * ceil_div(most, 1 << log2) : (((int64_t)a.batch.rows * group) >> log2) + requests);
     // Pieces are no longer than the mean by more than `slack`, and the sum of the tiles' lengths that it comes from is half of their number
     // times the longest at least: so many pieces at most, and so many of tiles that are cut.
@@ -318,16 +324,15 @@ hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
 
 namespace {
 
-// A row's pages in pieces of so many blocks that all rows and key heads give about kItems workgroups (at least 8 blocks each).
+// A row's pages in pieces of so many blocks that all rows and key heads give about kItems workgroups (at least kLeastBlocks each).
 Plan plan_selected(const AttendArgs& a) {
     const int group = a.heads / a.pool.kv_heads, tiles = (group + 15) / 16;
     const int64_t blocks = (int64_t)a.top * (a.pool.page / kKvBlock), all = (int64_t)a.batch.rows * a.pool.kv_heads * tiles;
     int64_t pieces = kItems / all;
-    if (pieces > blocks / 8) pieces = blocks / 8;
+    if (pieces > blocks / kLeastBlocks) pieces = blocks / kLeastBlocks;
     if (pieces < 1) pieces = 1;
     const int each = ceil_div(blocks, pieces);
     Plan p{};
-    p.few = true;
     p.cut = Cut{4, 1, 16, ceil_div(blocks, each), each, 1.0f, 0, group, 0, 0, 0};
     p.split = p.cut.target > 1;
     p.tiles = (unsigned)(a.batch.rows * tiles);

@@ -352,7 +352,7 @@ struct VerifyArgs {
 };
 hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t st);
 
-// A paged cache of keys and values (kv_append.hip, attend.hip, attend_select.hip). Its unit is the block: kKvBlock consecutive tokens
+// A paged cache of keys and values (kv_append.hip, attend_few.hip, attend_many.hip, attend_select.hip). Its unit is the block: kKvBlock consecutive tokens
 // of one key head, keys and values in MFMA operand order (kv_cache.h).
 constexpr int kKvBlock = 32;
 struct KvPool {
