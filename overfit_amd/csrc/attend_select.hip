@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int first_row, i
     const int part = tid & 3;
     for (int p = from + (tid >> 2); p < min(pages, from + each); p += 64) {
         const int page = page_at(a, at.r, p);
-        double best = -__builtin_inf();
+        double best = __builtin_nan("");
         if (page >= 0) {
             const float* s = a.pool.sums + ((size_t)page * kv_heads + head) * dim;
             for (int g0 = 0; g0 < group; g0 += 4) {
@@ -68,11 +68,12 @@ __global__ __launch_bounds__(256) void fit_kernel(AttendArgs a, int first_row, i
                 for (int g = 0; g < 4; g++) {
                     fit[g] += __shfl_xor(fit[g], 1, 64);
                     fit[g] += __shfl_xor(fit[g], 2, 64);
-                    best = fit[g] > best ? fit[g] : best;  // (one that is no number fits least)
+                    best = fit[g] > best || best != best ? fit[g] : best;
                 }
             }
         }
-        if (part == 0) out[p] = page >= 0 ? ordered(best + 0.0) : 0;
+        // (one that is no number fits least: minus infinity is ordered far above 1)
+        if (part == 0) out[p] = page < 0 ? 0 : best != best ? 1 : ordered(best + 0.0);
     }
 }
 

@@ -124,3 +124,19 @@ def test_the_widest_groups(heads, dim):
     assert np.array_equal(got.cpu().numpy(), want)
     o, err = attention(req, q, heads, keep=lambda row, a, seen: np.isin(seen // 32, want[row, a]))
     check(out, o, err)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [1, 5])
+def test_no_number_comes_behind_the_lowest(dim, heads):
+    """Of a page that fits by minus infinity and a lower one whose fit is no number, the first is taken."""
+    rng = np.random.default_rng(5)
+    req = Requests(ov, rng, "f16", 1, dim, 32, [1], [320], sums=True)
+    req.k[0][40, 0, 3] = np.nan
+    req.k[0][100, 0, 3] = -np.inf
+    req.fill()
+    q = np.abs(rng.standard_normal((1, heads * dim))).astype(np.float32)
+    for top, want in ((9, [0, 2, 4, 5, 6, 7, 8, 9, 10]), (10, [0, 2, 3, 4, 5, 6, 7, 8, 9, 10]), (11, list(range(11)))):
+        pages = torch.full((1, 1, top), -9, dtype=torch.int32, device=DEV)
+        ov.attend_selected(req.cache, req.t(q), *req.batch(), top, pages=pages)
+        assert pages.cpu().numpy()[0, 0].tolist() == want
